@@ -313,6 +313,143 @@ int pl_prefill_split_run(const void* q, int64_t q_stride_t, int64_t q_stride_h,
                          int dtype, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Trees of drafted tokens over the paged cache                              */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * A step of tree-speculative decoding: the target model runs a small tree of
+ * drafted tokens per request at once (pl_tree_plan once per step, pl_tree_run
+ * once per layer), pl_tree_accept walks the tree along the target's picks, and
+ * pl_tree_commit moves the accepted path's K/V together.  No counterpart in the
+ * reference, which decodes one token per row and step.
+ *
+ * Request r's tree tokens are rows qo_indptr[r] .. qo_indptr[r+1] of the packed
+ * arrays, T_r = their number, node i the i-th of them.  They are the LAST T_r
+ * positions of its kv_len_r tokens (pages kv_indices[kv_indptr[r] ..], the last
+ * one holding kv_last_page_len[r]), the P_r = kv_len_r - T_r before them the
+ * committed ones: the caller appends their K/V before it attends.
+ */
+
+/*
+ * Bytes of the plan buffer, and of the scratch of one pl_tree_run.  tokens: all
+ * tree tokens of the batch, the length of q; max_tree: at least every T_r;
+ * indices_capacity: at least every num_indices that is planned into the buffer.
+ * 0 for sizes that pl_tree_plan refuses.
+ */
+size_t pl_tree_plan_size(int batch, int tokens, int max_tree,
+                         int indices_capacity, int num_qo_heads,
+                         int num_kv_heads, int head_dim);
+size_t pl_tree_workspace_size(int batch, int tokens, int max_tree,
+                              int num_qo_heads, int num_kv_heads,
+                              int head_dim);
+
+/*
+ * Plan of one step for all its layers, made on the device: nothing is read
+ * back, and a captured plan follows the tables as they are at each replay.  It
+ * copies the tables (they may change afterwards), packs the masks and cuts the
+ * work.
+ *
+ * The trees are given by one of
+ *   tree_parents [tokens]: node i's parent, an earlier node of its request or
+ *     -1; a node attends itself, its ancestors and the committed tokens;
+ *   tree_mask [tokens][mask_ld >= max_tree] bytes: node i attends node j of
+ *     its request where tree_mask[i][j] is not 0, and the committed tokens.
+ * A row that attends nothing gets o = 0 and lse = -inf.
+ *
+ * Tables are device arrays; entries outside their range are clamped (T_r to
+ * max_tree, a parent that is not an earlier node to -1).  plan: 16-byte
+ * aligned, at least pl_tree_plan_size bytes; it must be zeroed once before its
+ * first use.  parts: 0, or into how many parts the longest kv range is cut
+ * (1 .. 128; fewer where that many items do not fit).  batch: up to 4096.
+ */
+int pl_tree_plan(const int32_t* qo_indptr, const int32_t* kv_indptr,
+                 const int32_t* kv_indices, int num_indices,
+                 const int32_t* kv_last_page_len, int batch, int tokens,
+                 int max_tree, const int32_t* tree_parents,
+                 const uint8_t* tree_mask, int64_t mask_ld, int num_qo_heads,
+                 int num_kv_heads, int head_dim, int page_size, int parts,
+                 int indices_capacity, void* plan, size_t plan_bytes,
+                 void* stream);
+
+/*
+ * Attention of the planned trees:
+ *   o[t, hq] = softmax(q[t, hq] . K_r[:, hq / g]^T * sm_scale, masked) . V_r
+ * q and o are [tokens, num_qo_heads, head_dim] with strides (stride_t,
+ * stride_h, 1), lse (nullable) [tokens, num_qo_heads] fp32, natural log; caches
+ * are addressed as in pl_decode_run, page ids outside [0, num_pages) clamped
+ * into the pool.  q, caches and o share `dtype` (F16 or BF16); accumulation is
+ * fp32.  head_dim: 64, 128 or 256.  page_size: 1 .. 65536; pages of a multiple
+ * of 16 tokens take the scalar-addressed path.  q and cache strides must be
+ * multiples of 8 elements, o's of 4, q, the caches, the plan and the workspace
+ * 16-byte aligned and o 8-byte aligned.
+ *
+ * K and V of masked positions may hold anything, infinities and NaN included.
+ * An infinity or NaN in V that a row attends makes that output infinite or NaN.
+ *
+ * batch, tokens, max_tree, indices_capacity, heads, head_dim and page_size are
+ * the plan's: a run with others does nothing.  workspace holds partial results
+ * during the call: calls that may run at the same time need one each.  The plan
+ * is only read.
+ */
+int pl_tree_run(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                const void* k_cache, const void* v_cache, int64_t page_stride,
+                int64_t token_stride, int64_t head_stride, int64_t num_pages,
+                void* o, int64_t o_stride_t, int64_t o_stride_h, float* lse,
+                int batch, int tokens, int max_tree, int num_qo_heads,
+                int num_kv_heads, int head_dim, int page_size, float sm_scale,
+                int dtype, const void* plan, size_t plan_bytes,
+                int indices_capacity, void* workspace, size_t workspace_bytes,
+                void* stream);
+
+/*
+ * The path of each tree that the target's greedy picks follow.  Node 0 is the
+ * root, whose token is decided already; from node i the path goes on to the
+ * lowest-numbered child (a later node whose parent is i) whose tokens[] is
+ * picks[i], the target's pick after node i.  Arrays are [num_tokens].
+ *   path [batch][max_path]: the nodes, then -1
+ *   count [batch]: their number (0 for a request without nodes)
+ *   kept [batch][max_path]: picks[] along the path, then -1 -- the tokens the
+ *     step decodes; the last of them has no K/V yet
+ * A path longer than max_path is cut there.
+ */
+int pl_tree_accept(const int64_t* tokens, const int32_t* parents,
+                   const int64_t* picks, const int32_t* qo_indptr, int batch,
+                   int num_tokens, int max_path, int32_t* path, int32_t* count,
+                   int64_t* kept, void* stream);
+
+/*
+ * K/V of position P_r + path[r][k] moved to position P_r + k, for k < count[r],
+ * in each of num_layers layers (layer_stride elements apart; page, token and
+ * head strides as in pl_decode_run): the accepted path then stands behind the
+ * committed tokens, and the request's new length is P_r + count[r].  The tables
+ * are those of the tree's plan.  Paths ascend (path[r][k] >= k): an entry
+ * outside [k, T_r) ends the path.  Moves from or to pages outside [0,
+ * num_pages) are skipped.  Positions that the path leaves keep what they hold.
+ */
+int pl_tree_commit(void* k_cache, void* v_cache, int64_t layer_stride,
+                   int64_t page_stride, int64_t token_stride,
+                   int64_t head_stride, int num_layers, int64_t num_pages,
+                   const int32_t* qo_indptr, const int32_t* kv_indptr,
+                   const int32_t* kv_indices, int num_indices,
+                   const int32_t* kv_last_page_len, const int32_t* path,
+                   const int32_t* count, int batch, int max_path,
+                   int num_kv_heads, int head_dim, int page_size, int dtype,
+                   void* stream);
+
+/*
+ * Page dst_h[i] of a pool made a copy of page src_h[i], i < n, in each of
+ * num_layers layers.  A page is page_elements contiguous elements (K and V
+ * together), pages page_stride and layers layer_stride elements apart.  A
+ * source may be named more than once; a page that is written must not be
+ * written twice nor be a source (PL_ERR_INVALID, and nothing is copied).  The
+ * lists are read before the call returns.
+ */
+int pl_kv_copy_pages(void* cache, int64_t layer_stride, int64_t page_stride,
+                     int64_t page_elements, int num_layers, int64_t num_pages,
+                     const int32_t* src_h, const int32_t* dst_h, int n,
+                     int dtype, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Fused element-wise ops of the decode layer                                */
 /* ------------------------------------------------------------------------ */
 

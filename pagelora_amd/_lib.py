@@ -245,6 +245,54 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             _i32, _vp,                   # dtype, stream
         ],
     ),
+    "pl_tree_plan_size": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "pl_tree_workspace_size": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32]),
+    "pl_tree_plan": (
+        _i32,
+        [
+            _vp, _vp, _vp, _i32, _vp,    # qo_indptr, kv_indptr, kv_indices, their number, last_page_len
+            _i32, _i32, _i32,            # batch, tokens, max_tree
+            _vp, _vp, _i64,              # tree_parents, tree_mask, mask_ld
+            _i32, _i32, _i32, _i32,      # hq, hkv, head_dim, page_size
+            _i32, _i32, _vp, _sz, _vp,   # parts, indices_capacity, plan, bytes, stream
+        ],
+    ),
+    "pl_tree_run": (
+        _i32,
+        [
+            _vp, _i64, _i64,             # q, strides
+            _vp, _vp, _i64, _i64, _i64,  # k/v cache, page/token/head strides
+            _i64,                        # num_pages
+            _vp, _i64, _i64, _vp,        # o, strides, lse
+            _i32, _i32, _i32,            # batch, tokens, max_tree
+            _i32, _i32, _i32, _i32,      # hq, hkv, head_dim, page_size
+            _f32, _i32,                  # sm_scale, dtype
+            _vp, _sz, _i32,              # plan, bytes, indices_capacity
+            _vp, _sz, _vp,               # workspace, bytes, stream
+        ],
+    ),
+    "pl_tree_accept": (
+        _i32,
+        [
+            _vp, _vp, _vp, _vp,          # tokens, parents, picks, qo_indptr
+            _i32, _i32, _i32,            # batch, num_tokens, max_path
+            _vp, _vp, _vp, _vp,          # path, count, kept, stream
+        ],
+    ),
+    "pl_tree_commit": (
+        _i32,
+        [
+            _vp, _vp, _i64, _i64, _i64, _i64,  # caches, layer/page/token/head strides
+            _i32, _i64,                        # num_layers, num_pages
+            _vp, _vp, _vp, _i32, _vp,          # qo_indptr, kv_indptr, kv_indices, their number, last_page_len
+            _vp, _vp, _i32, _i32,              # path, count, batch, max_path
+            _i32, _i32, _i32, _i32, _vp,       # hkv, head_dim, page_size, dtype, stream
+        ],
+    ),
+    "pl_kv_copy_pages": (
+        _i32,
+        [_vp, _i64, _i64, _i64, _i32, _i64, _vp, _vp, _i32, _i32, _vp],
+    ),
     "pl_rmsnorm": (_i32, [_vp, _i64, _vp, _vp, _i64, _i32, _i32, _f32, _i32, _vp]),
     "pl_add_rmsnorm_lora": (
         _i32,
@@ -427,3 +475,11 @@ def stream_handle(device=None) -> int:
     import torch
 
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def on_device(device):
+    """Context in which ``device`` is the current one, as a launch on a stream of it needs."""
+
+    import torch
+
+    return torch.cuda.device(device)

@@ -755,6 +755,208 @@ class PagedDecodeAttention:
         _lib.check(status, "pl_prefill_run")
         return out
 
+    # --------------------------------------------------------------- trees
+    def plan_tree(
+        self,
+        *,
+        qo_indptr: torch.Tensor,
+        paged_kv_indptr: torch.Tensor,
+        paged_kv_indices: torch.Tensor,
+        paged_kv_last_page_len: torch.Tensor,
+        tree_parents: torch.Tensor | None = None,
+        tree_mask: torch.Tensor | None = None,
+        max_tree: int | None = None,
+        parts: int = 0,
+    ) -> None:
+        """Plan the attention of trees of drafted tokens, for all layers of a step.
+
+        Request r owns rows ``qo_indptr[r] .. qo_indptr[r+1]`` of the packed
+        queries: the nodes of its tree, and the last positions of its paged
+        sequence.  Every node attends the request's tokens before the tree, and
+        of the tree itself and its ancestors by ``tree_parents`` (int32
+        [tokens]: an earlier node of the same request, or -1), or the nodes j
+        with ``tree_mask[i, j]`` (bool or uint8 [tokens, >= max_tree]).
+
+        Host tables are validated and uploaded.  Device tables are trusted (the
+        kernels clamp every index into its buffer) and may be planned inside a
+        capture; ``max_tree`` then bounds the nodes of a tree (default: all
+        tokens).  A captured :meth:`run_tree` replays on the plan that
+        ``plan_tree`` made last for the same sizes
+        (:meth:`tree_graph_signature`).  ``parts`` > 0 fixes into how many parts
+        the longest sequence is cut.  Plans and runs of one backend are ordered
+        by the caller; the reference has no counterpart.
+        """
+
+        tables = (qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len)
+        if any(t.dim() != 1 for t in tables):
+            raise ValueError("tree tables must be 1-D")
+        batch = paged_kv_last_page_len.numel()
+        if qo_indptr.numel() != batch + 1 or paged_kv_indptr.numel() != batch + 1:
+            raise ValueError("qo_indptr and paged_kv_indptr must have batch + 1 entries")
+        if (tree_parents is None) == (tree_mask is None):
+            raise ValueError("give tree_parents or tree_mask, and not both")
+        tree = tree_mask if tree_parents is None else tree_parents
+        if tree_parents is not None and tree.dim() != 1:
+            raise ValueError("tree_parents must be 1-D")
+        if tree_mask is not None and (tree.dim() != 2 or tree.dtype not in (torch.bool, torch.uint8)):
+            raise ValueError("tree_mask must be a 2-D bool or uint8 tensor")
+        for t in tables if tree_parents is None else (*tables, tree):
+            if t.dtype != torch.int32:
+                raise ValueError("tree tables must be int32")
+        tokens = tree.shape[0]
+        kinds = {t.device.type for t in (*tables, tree)}
+        if len(kinds) > 1:
+            raise ValueError("tree tables must be all on the host or all on the device")
+        host = kinds == {"cpu"}
+        max_page = None
+        if host:
+            max_page, widest = self._validate_host_trees(*tables, tree_parents, tokens)
+            if max_tree is not None and widest > max_tree:
+                raise ValueError(f"a tree of {widest} nodes exceeds max_tree {max_tree}")
+            max_tree = widest if max_tree is None else int(max_tree)
+        max_tree = tokens if max_tree is None else min(int(max_tree), tokens)
+        if max_tree < min(1, tokens):
+            raise ValueError("max_tree must be >= 1")
+        if tree_mask is not None and tree.shape[1] < max_tree:
+            raise ValueError(f"tree_mask has {tree.shape[1]} columns for trees of up to {max_tree} nodes")
+        if self.device.type != "cuda":
+            raise RuntimeError("PagedDecodeAttention.plan_tree needs a ROCm device")
+
+        with _lib.on_device(self.device):
+            if host:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("plan_tree with host tables uploads them and cannot be captured")
+                if tree_parents is not None:
+                    *tables, tree = _upload_int32((*tables, tree), self.device)
+                else:
+                    tables = _upload_int32(tables, self.device)
+                    tree = tree.contiguous().to(self.device)
+            else:
+                if any(not self._here(t) for t in (*tables, tree)):
+                    raise ValueError(f"tree tables must be on {self.device}")
+                tables = [t.contiguous() for t in tables]
+                tree = tree.contiguous()
+            num_indices = tables[2].numel()
+            capacity = max(16, self.max_pages, 1 << max(0, num_indices - 1).bit_length())
+            sizes = (batch, tokens, max_tree)
+            heads = (self.num_qo_heads, self.num_kv_heads, self.head_dim)
+            plan_bytes = self._lib.pl_tree_plan_size(*sizes, capacity, *heads)
+            if plan_bytes == 0:
+                _lib.check(_lib.PL_ERR_UNSUPPORTED, "pl_tree_plan_size")
+            buffer = self._tree_buffer(plan_bytes)
+            stream = torch.cuda.current_stream(self.device)
+            parents_ptr, mask_ptr, mask_ld = (tree.data_ptr(), None, 0) if tree_parents is not None else (
+                None, tree.data_ptr(), tree.stride(0))
+            _lib.check(self._lib.pl_tree_plan(
+                tables[0].data_ptr(), tables[1].data_ptr(), tables[2].data_ptr(), num_indices, tables[3].data_ptr(),
+                *sizes, parents_ptr, mask_ptr, mask_ld, *heads, self.page_size, int(parts), capacity,
+                buffer.data_ptr(), buffer.numel(), stream.cuda_stream), "pl_tree_plan")
+            captured = torch.cuda.is_current_stream_capturing()
+            self._tree_plan = {
+                "sizes": sizes,
+                "tokens": tokens,
+                "capacity": capacity,
+                "buffer": buffer,
+                "workspace_bytes": self._lib.pl_tree_workspace_size(*sizes, *heads),
+                "max_page": max_page,
+                "stream": stream.cuda_stream,
+                "ready": None if captured else stream.record_event(),
+            }
+
+    def _here(self, t: torch.Tensor) -> bool:
+        index = torch.cuda.current_device() if self.device.index is None else self.device.index
+        return t.device.type == "cuda" and t.device.index == index
+
+    def _tree_buffer(self, nbytes: int) -> torch.Tensor:
+        """The plan buffer of a size class.  One per class lives as long as the
+        backend: captured runs read it."""
+        buffers = self.__dict__.setdefault("_tree_buffers", {})
+        size = 1 << (nbytes - 1).bit_length()
+        if size not in buffers:
+            # zeros: no header of an earlier owner of the memory
+            buffers[size] = torch.zeros(size, dtype=torch.uint8, device=self.device)
+        return buffers[size]
+
+    def _validate_host_trees(self, qo_indptr, kv_indptr, kv_indices, kv_last, parents, tokens) -> tuple[int, int]:
+        """Check host tables of trees; returns (largest page id or -1, nodes of the widest tree)."""
+        max_page = _validate_host_table(kv_indptr, kv_indices, kv_last, self.page_size)
+        qo, kv = qo_indptr.long(), kv_indptr.long()
+        trees = qo.diff()
+        if int(qo[0]) != 0 or bool((trees < 0).any()):
+            raise ValueError("qo_indptr must start at 0 and be non-decreasing")
+        if int(qo[-1]) != tokens:
+            raise ValueError(f"qo_indptr ends at {int(qo[-1])}, but the trees have {tokens} nodes")
+        pages = kv.diff()
+        lens = torch.where(pages > 0, (pages - 1) * self.page_size + kv_last, 0)
+        if bool((trees > lens).any()):
+            r = int((trees > lens).nonzero()[0])
+            raise ValueError(f"request {r}: a tree of {int(trees[r])} nodes exceeds its {int(lens[r])} tokens")
+        if trees.numel() and int(lens.max()) > 2**30:
+            raise ValueError("sequences of more than 2^30 tokens are not supported")
+        if parents is not None and tokens:
+            node = torch.arange(tokens) - torch.repeat_interleave(qo[:-1], trees)
+            if bool(((parents < -1) | (parents >= node)).any()):
+                raise ValueError("tree_parents must be earlier nodes of the same request, or -1")
+        return max_page, int(trees.max()) if trees.numel() else 0
+
+    def tree_graph_signature(self):
+        """Everything a captured run_tree bakes in; sequence lengths are not
+        part of it."""
+        plan = getattr(self, "_tree_plan", None) or {}
+        buffer = plan.get("buffer")
+        return (id(self), plan.get("sizes"), plan.get("capacity"), buffer.data_ptr() if buffer is not None else None)
+
+    def run_tree(self, q: torch.Tensor, paged_kv_cache_layer) -> torch.Tensor:
+        """One layer's attention of the planned trees: packed ``q`` [tokens, Hq, D],
+        returns the same shape."""
+        return self.run_tree_into(q, paged_kv_cache_layer, torch.empty(q.shape, dtype=q.dtype, device=q.device))
+
+    def run_tree_into(self, q: torch.Tensor, paged_kv_cache_layer, out: torch.Tensor,
+                      lse: torch.Tensor | None = None) -> torch.Tensor:
+        """Writes ``out`` ([tokens, Hq, D], head_dim contiguous) and optionally
+        ``lse`` ([tokens, Hq] fp32, natural log) for packed ``q``."""
+
+        plan = getattr(self, "_tree_plan", None)
+        if plan is None:
+            raise RuntimeError("plan_tree must be called before run_tree")
+        if q.dim() != 3 or tuple(q.shape[1:]) != (self.num_qo_heads, self.head_dim):
+            raise ValueError(f"q must be [tokens, {self.num_qo_heads}, {self.head_dim}], got {tuple(q.shape)}")
+        if q.shape[0] != plan["tokens"]:
+            raise ValueError(f"q has {q.shape[0]} tokens but the plan has {plan['tokens']}")
+        if tuple(out.shape) != tuple(q.shape) or out.dtype != q.dtype or q.stride(2) != 1 or out.stride(2) != 1:
+            raise ValueError("q and out must match in shape/dtype with a contiguous head_dim")
+        k, v, page_stride, token_stride, head_stride, num_pages = _cache_geometry(
+            paged_kv_cache_layer, self.num_kv_heads, self.head_dim, self.page_size
+        )
+        if k.dtype != q.dtype:
+            raise ValueError(f"q dtype {q.dtype} != KV cache dtype {k.dtype}")
+        if plan["max_page"] is not None and plan["max_page"] >= num_pages:
+            raise ValueError(f"page id {plan['max_page']} is outside the {num_pages}-page KV pool")
+        if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != tuple(q.shape[:2])
+                                or not lse.is_contiguous()):
+            raise ValueError("lse must be a contiguous fp32 [tokens, Hq] tensor")
+        if not all(self._here(t) for t in (q, k, v, out) + ((lse,) if lse is not None else ())):
+            raise RuntimeError(f"run_tree needs tensors on the backend's device {self.device}")
+        with _lib.on_device(q.device):
+            stream = torch.cuda.current_stream(q.device)
+            if stream.cuda_stream != plan["stream"] and plan["ready"] is not None \
+                    and not torch.cuda.is_current_stream_capturing():
+                stream.wait_event(plan["ready"])
+            # per call, from torch's allocator: calls on other streams and graphs share nothing
+            ws = torch.empty(plan["workspace_bytes"], dtype=torch.uint8, device=q.device)
+            status = self._lib.pl_tree_run(
+                q.data_ptr(), q.stride(0), q.stride(1),
+                k.data_ptr(), v.data_ptr(), page_stride, token_stride, head_stride,
+                num_pages,
+                out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr() if lse is not None else None,
+                *plan["sizes"], self.num_qo_heads, self.num_kv_heads, self.head_dim, self.page_size,
+                self.sm_scale, _lib.dtype_code(q.dtype),
+                plan["buffer"].data_ptr(), plan["buffer"].numel(), plan["capacity"],
+                ws.data_ptr(), ws.numel(), stream.cuda_stream,
+            )
+            _lib.check(status, "pl_tree_run")
+        return out
+
 
 # The reference's class name, for drop-in imports.
 FlashInferAttentionBackend = PagedDecodeAttention

@@ -46,6 +46,7 @@ FILE_FLAGS = {
     "paged_prefill.hip": _MFMA_VGPR,
     "paged_prefill_split.hip": _MFMA_VGPR,
     "lora.hip": _MFMA_VGPR,
+    "tree_attention.hip": _MFMA_VGPR,
     "wide_gemm.hip": _MFMA_VGPR,
 }
 

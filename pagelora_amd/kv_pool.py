@@ -16,16 +16,57 @@ part of every decode graph key, so the next step recaptures once.
 
 Requests own page spans (``KVBlockSpan``); rows may share prefix pages
 (``paged_kvcache_manager.py:324-333``), which are read-only to decode.
+
+Requests can also be forked, cut back and packed together.  A fork shares the
+full pages of its own with its origin, counted, and gets a copy of the page
+they would both write to; a page goes back to the free list with its last
+holder.  The copies run on the device, in all layers at once.
 """
 
 from __future__ import annotations
 
 from dataclasses import dataclass, field
+from typing import Sequence
 
 import numpy as np
 import torch
 
+from . import _lib
 from .page_table import KVBlockSpan, pack_rows
+
+
+def kv_copy_pages(cache: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -> None:
+    """Make page ``dst[i]`` a copy of page ``src[i]`` in every layer (``pl_kv_copy_pages``).
+
+    ``cache``: the pool [layers, P, 2, page, Hkv, D], or one layer of it, its
+    pages contiguous.  Page ids are host integers.  A source may be listed more
+    than once; a page that is written must not be written twice nor be a
+    source.  Enqueued on the current stream; the lists are read at once.
+    """
+
+    if cache.dim() == 5:
+        cache = cache.unsqueeze(0)
+    if cache.dim() != 6 or cache.shape[2] != 2:
+        raise ValueError(f"cache must be [layers, P, 2, page, Hkv, D] or a layer of it, got {tuple(cache.shape)}")
+    src, dst = (np.asarray(x).reshape(-1) for x in (src, dst))
+    if src.size != dst.size:
+        raise ValueError(f"{src.size} source pages but {dst.size} destination pages")
+    if src.size == 0:
+        return
+    if src.dtype.kind not in "iu" or dst.dtype.kind not in "iu":
+        raise ValueError("page ids must be integers")
+    if min(src.min(), dst.min()) < 0 or max(src.max(), dst.max()) >= cache.shape[1]:
+        raise ValueError(f"page ids must be in [0, {cache.shape[1]})")
+    if cache.device.type != "cuda":
+        raise RuntimeError("kv_copy_pages needs a cache on a ROCm device")
+    if not cache[0, 0].is_contiguous():
+        raise ValueError("the pages of the KV cache must be contiguous")
+    src, dst = (np.ascontiguousarray(x, dtype=np.int32) for x in (src, dst))
+    with _lib.on_device(cache.device):
+        _lib.check(_lib.load().pl_kv_copy_pages(
+            cache.data_ptr(), cache.stride(0), cache.stride(1), cache[0, 0].numel(), cache.shape[0], cache.shape[1],
+            src.ctypes.data, dst.ctypes.data, src.size, _lib.dtype_code(cache.dtype),
+            _lib.stream_handle(cache.device)), "pl_kv_copy_pages")
 
 
 class PageAllocator:
@@ -36,12 +77,16 @@ class PageAllocator:
     runs append their (discarded) K/V into.  ``grow(required_pages)``, when
     given, is called when the free list runs short; it returns the new
     capacity, whose pages join the free list (lowest ids handed out first).
+
+    An allocated page has one holder; :meth:`share` adds one, :meth:`free`
+    takes one away, and the last one's free returns the page to the list.
     """
 
     def __init__(self, capacity: int, grow=None) -> None:
         self.capacity = int(capacity)
         self._free = list(range(self.capacity - 1, 0, -1))
         self._grow = grow
+        self._more: dict[int, int] = {}  # holders of a page beyond the first
 
     @property
     def free_pages(self) -> int:
@@ -57,8 +102,31 @@ class PageAllocator:
         out = [self._free.pop() for _ in range(n)]
         return out
 
+    def share(self, pages) -> None:
+        """One holder more for each of these allocated pages."""
+        for p in pages:
+            self._more[int(p)] = self._more.get(int(p), 0) + 1
+
+    def holders(self, page: int) -> int:
+        """How many hold an allocated page."""
+        return 1 + self._more.get(int(page), 0)
+
     def free(self, pages) -> None:
-        self._free.extend(int(p) for p in pages)
+        for p in map(int, pages):
+            more = self._more.get(p, 0)
+            if more == 0:
+                self._free.append(p)
+            elif more == 1:
+                del self._more[p]
+            else:
+                self._more[p] = more - 1
+
+    def move(self, moved: dict[int, int]) -> None:
+        """Allocated pages ``moved`` (page -> free page) take those ids; the
+        free list hands out the lowest ids first again."""
+        free = set(self._free) - set(moved.values()) | set(moved)
+        self._free = sorted(free, reverse=True)
+        self._more = {moved.get(p, p): n for p, n in self._more.items()}
 
 
 @dataclass
@@ -161,6 +229,76 @@ class PagedKVPool:
     def release(self, request: Request) -> None:
         self.allocator.free(request.own_pages)
         request.own_pages = []
+
+    def copy_pages(self, src: Sequence[int], dst: Sequence[int]) -> None:
+        """Page ``dst[i]`` becomes a copy of page ``src[i]`` in every layer (:func:`kv_copy_pages`)."""
+        kv_copy_pages(self.cache, src, dst)
+
+    def fork(self, requests: Sequence[Request]) -> list[Request]:
+        """A continuation of its own for each request (listed n times: n of
+        them), with the same tokens so far.  Full pages are shared, a partial
+        last page is copied: one launch for all of them, in stream order."""
+        partial = [r.length % self.page_size > 0 and r.length > r.prefix_len for r in requests]
+        full = [max(0, r.length - r.prefix_len) // self.page_size for r in requests]
+        src = [r.own_pages[n] for r, n, cut in zip(requests, full, partial) if cut]
+        dst = self.allocator.allocate(len(src))
+        try:
+            self.copy_pages(src, dst)
+        except Exception:
+            self.allocator.free(dst)
+            raise
+        copies = iter(dst)
+        forks = []
+        for r, n, cut in zip(requests, full, partial):
+            pages = r.own_pages[:n]
+            self.allocator.share(pages)
+            forks.append(Request(list(r.prefix_pages), r.prefix_len, pages + ([next(copies)] if cut else []), r.length))
+        return forks
+
+    def truncate(self, request: Request, length: int) -> None:
+        """Cut the request back to its first ``length`` tokens: the pages behind
+        them are freed, and a last page that is now partial and has other
+        holders is replaced by a copy, since the request will write to it."""
+        if not request.prefix_len <= length <= request.length:
+            raise ValueError(f"length {length} is outside [{request.prefix_len}, {request.length}], the request's "
+                             "own tokens")
+        keep = -(-(length - request.prefix_len) // self.page_size)
+        last = request.own_pages[keep - 1] if keep and length % self.page_size else None
+        pages = request.own_pages[:keep]
+        if last is not None and self.allocator.holders(last) > 1:
+            copy = self.allocator.allocate(1)
+            try:
+                self.copy_pages([last], copy)
+            except Exception:
+                self.allocator.free(copy)
+                raise
+            self.allocator.free([last])
+            pages[-1:] = copy
+        self.allocator.free(request.own_pages[keep:])
+        request.own_pages = pages
+        request.length = length
+
+    def compact(self, requests: Sequence[Request]) -> dict[int, int]:
+        """Move the requests' pages to the lowest free ids; returns the moves (old id -> new id).
+
+        ``requests`` names every request that lists a page of theirs, as its own
+        or as a prefix: all their lists are rewritten.  A page with a holder
+        that is not among them stays.  Page tables made before hold the old ids:
+        plan again, and let no step run on the old ones in between."""
+        requests = list({id(r): r for r in requests}.values())
+        held: dict[int, int] = {}
+        for r in requests:
+            for p in r.own_pages:
+                held[p] = held.get(p, 0) + 1
+        pages = sorted((p for p, n in held.items() if n == self.allocator.holders(p)), reverse=True)
+        moved = {p: f for p, f in zip(pages, sorted(self.allocator._free)) if f < p}
+        if moved:
+            self.copy_pages(list(moved), list(moved.values()))
+            self.allocator.move(moved)
+            for r in requests:
+                r.own_pages = [moved.get(p, p) for p in r.own_pages]
+                r.prefix_pages = [moved.get(p, p) for p in r.prefix_pages]
+        return moved
 
     def tables(self, requests) -> tuple[np.ndarray, np.ndarray, np.ndarray]:
         """int32 (indptr, indices, last_page_len) for the batch."""
