@@ -359,15 +359,15 @@ size_t pl_tree_workspace_size(int batch, int tokens, int max_tree,
  * Tables are device arrays; entries outside their range are clamped (T_r to
  * max_tree, a parent that is not an earlier node to -1).  plan: 16-byte
  * aligned, at least pl_tree_plan_size bytes; it must be zeroed once before its
- * first use.  parts: 0, or into how many parts the longest kv range is cut
- * (1 .. 128; fewer where that many items do not fit).  batch: up to 4096.
+ * first use.  min_share: the kv tiles of all row blocks are dealt out in equal shares;
+ * the least size of a share in tiles (0: any).  batch: up to 4096.
  */
 int pl_tree_plan(const int32_t* qo_indptr, const int32_t* kv_indptr,
                  const int32_t* kv_indices, int num_indices,
                  const int32_t* kv_last_page_len, int batch, int tokens,
                  int max_tree, const int32_t* tree_parents,
                  const uint8_t* tree_mask, int64_t mask_ld, int num_qo_heads,
-                 int num_kv_heads, int head_dim, int page_size, int parts,
+                 int num_kv_heads, int head_dim, int page_size, int min_share,
                  int indices_capacity, void* plan, size_t plan_bytes,
                  void* stream);
 

@@ -254,7 +254,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             _i32, _i32, _i32,            # batch, tokens, max_tree
             _vp, _vp, _i64,              # tree_parents, tree_mask, mask_ld
             _i32, _i32, _i32, _i32,      # hq, hkv, head_dim, page_size
-            _i32, _i32, _vp, _sz, _vp,   # parts, indices_capacity, plan, bytes, stream
+            _i32, _i32, _vp, _sz, _vp,   # min_share, indices_capacity, plan, bytes, stream
         ],
     ),
     "pl_tree_run": (

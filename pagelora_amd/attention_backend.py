@@ -766,7 +766,7 @@ class PagedDecodeAttention:
         tree_parents: torch.Tensor | None = None,
         tree_mask: torch.Tensor | None = None,
         max_tree: int | None = None,
-        parts: int = 0,
+        min_share: int = 0,
     ) -> None:
         """Plan the attention of trees of drafted tokens, for all layers of a step.
 
@@ -782,9 +782,9 @@ class PagedDecodeAttention:
         capture; ``max_tree`` then bounds the nodes of a tree (default: all
         tokens).  A captured :meth:`run_tree` replays on the plan that
         ``plan_tree`` made last for the same sizes
-        (:meth:`tree_graph_signature`).  ``parts`` > 0 fixes into how many parts
-        the longest sequence is cut.  Plans and runs of one backend are ordered
-        by the caller; the reference has no counterpart.
+        (:meth:`tree_graph_signature`).  ``min_share`` > 0 keeps a workgroup's
+        share of the kv tiles from being less.  Plans and runs of one backend
+        are ordered by the caller; the reference has no counterpart.
         """
 
         tables = (qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len)
@@ -849,7 +849,7 @@ class PagedDecodeAttention:
                 None, tree.data_ptr(), tree.stride(0))
             _lib.check(self._lib.pl_tree_plan(
                 tables[0].data_ptr(), tables[1].data_ptr(), tables[2].data_ptr(), num_indices, tables[3].data_ptr(),
-                *sizes, parents_ptr, mask_ptr, mask_ld, *heads, self.page_size, int(parts), capacity,
+                *sizes, parents_ptr, mask_ptr, mask_ld, *heads, self.page_size, int(min_share), capacity,
                 buffer.data_ptr(), buffer.numel(), stream.cuda_stream), "pl_tree_plan")
             captured = torch.cuda.is_current_stream_capturing()
             self._tree_plan = {

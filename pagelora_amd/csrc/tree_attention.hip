@@ -9,16 +9,24 @@
 // o = 0 and lse = -inf.
 //
 // plan_kernel (once per step, for all layers) checks the tables, cuts the work
-// and packs the masks into 64-bit words.  A work item is R rows (tree token,
-// head of the GQA group) of a request over a range of kv tiles; one workgroup
-// takes one item for one kv head.  Its waves share the rows and take 32 tokens
-// of a tile each, in LDS buffers of their own that are filled straight from the
-// pages while the block before is worked on: no wave waits for another until
-// the item ends.  Few rows then cost few instructions per byte, and one pass
-// over the cache serves all rows.  S^T = K Q^T keeps a query per lane; the
-// probabilities are the B operand of O^T += V^T P^T as they lie, and V comes
-// out of LDS transposed.  The waves' states meet in LDS at the item's end, and
-// the parts of rows whose range was cut in merge_kernel, in order.
+// and packs the masks into 64-bit words.  A row block is up to 64 rows (tree
+// token, head of the GQA group) of a request.  The kv tiles of all row blocks,
+// one after another, are dealt out in equal shares to as many slots as the chip
+// holds workgroups (per kv head), so that all of them end together however
+// ragged the batch is; a workgroup takes what its share holds in turn.  Where a
+// request has several row blocks, its kv range is cut into chunks of a share and
+// a chunk's row blocks follow one another: neighbouring slots read the same
+// pages at the same time, and find them in the L2.
+//
+// A tile is four blocks (two at head_dim 256) of 32 tokens.  A wave, or two of 32
+// rows each, works on a block of every tile, in LDS buffers of its own that are
+// filled straight from the pages while the block before is worked on, and waits
+// for no other block's waves until the row block ends.  Few rows then cost few
+// instructions per byte, and one pass over the cache serves all rows of a block.
+// S^T = K Q^T keeps a query per lane; the probabilities are the B operand of
+// O^T += V^T P^T as they lie, and V comes out of LDS transposed.  The blocks'
+// states meet in LDS at the row block's end, and the parts of row blocks that
+// several slots share in merge_kernel, in order.
 #include <algorithm>
 #include <type_traits>
 
@@ -30,9 +38,9 @@ namespace tree {
 constexpr int kWave = 64;
 constexpr int kBlock = 32;        // kv tokens of a wave per tile
 constexpr int kMaxRequests = 4096;
+constexpr int kMaxLen = 1 << 30;
 constexpr int kMagic = 0x54524545;
-constexpr int kPlanThreads = 1024;
-constexpr int kCandidates = 128;  // split counts of the longest range that the plan weighs
+constexpr int kPlanThreads = 256;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -45,61 +53,72 @@ typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 // What a plan was made for, then what it holds.
 struct Header {
   int32_t magic, batch, tokens, max_tree, indices_capacity, hq, hkv, head_dim, page_size;
-  int32_t num_items, num_blocks, pad[5];
+  int32_t num_requests, num_slots, num_shared, pad[2];
+  int64_t share;  // tiles of a slot
 };
 static_assert(sizeof(Header) == 64, "the plan's header");
+// A request with nodes.  Its work is tiles x blocks (row blocks), from `base` of
+// all work on: chunk after chunk of its tiles, of a chunk row block after row
+// block.  The first `longer` chunks have chunk_len + 1 tiles, the others
+// chunk_len; where there are several, none is less than a share.
 struct Request {
-  int32_t q_begin, tree, page_begin, kv_len;
+  int32_t q_begin, tree, page_begin, kv_len, blocks, chunks, chunk_len, longer, index, pad;
+  int64_t base;
 };
-// R rows of a request: its parts are the items slot, slot + step, ...
-struct RowBlock {
-  int32_t request, row0, slot, step, parts, pad[3];
+// A place in the work: of a row block (`block`) in a chunk, after `tile` tiles of
+// it.  Of a row block that slots share: the slots of its one chunk, times two,
+// and whether the first one's second partial result is of it.
+struct Place {
+  Request rq;
+  int32_t chunk, block, tile, parts;
 };
-struct Item {
-  int32_t request, row0, tile_begin, tile_end, parts, pad[3];
-};
+static_assert(sizeof(Place) == 64, "one load");
 
 // ------------------------------------------------------- sizes and layout ---
-inline int waves_of(int head_dim) { return head_dim == 256 ? 2 : 4; }
-inline int tile_of(int head_dim) { return kBlock * waves_of(head_dim); }
+// Rows of a row block: as few as the widest tree needs.
+constexpr int rows_of(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+// Waves of a block: their rows' outputs and queries stay in registers.
+constexpr int ranks_of(int rows) { return rows == 64 ? 2 : 1; }
+// Blocks of a tile: two buffers of their K and V fill 128 KiB of LDS (64 at head_dim 64).
+constexpr int blocks_of(int head_dim) { return head_dim == 256 ? 2 : 4; }
+constexpr int tile_of(int head_dim) { return kBlock * blocks_of(head_dim); }
+constexpr int threads_of(int rows, int head_dim) { return kWave * ranks_of(rows) * blocks_of(head_dim); }
 
-// 16-row columns a wave holds: as few as the widest tree needs, at most 4 (2 at
-// head_dim 256, by its accumulators).
-inline int cols_of(int64_t max_tree, int g, int head_dim) {
-  const int64_t rows = max_tree * g;
-  const int most = head_dim == 256 ? 2 : 4;
-  return std::min(most, rows <= 16 ? 1 : (rows <= 32 ? 2 : 4));
+// Workgroups per kv head that run at once: one per CU by their LDS (two at
+// head_dim 64, where 64 rows' registers allow one again).
+inline int slots_of(int rows, int hkv, int head_dim) {
+  return std::max(1, (head_dim == 64 && rows < 64 ? 512 : 256) / hkv);
 }
 
-// Workgroups per kv head that run at once: one per CU by their LDS, two at head_dim 64.
-inline int slots_of(int hkv, int head_dim) { return std::max(1, (head_dim == 64 ? 512 : 256) / hkv); }
-
 struct Layout {
-  int rows, slots, max_blocks, max_items, mask_words;
-  size_t requests, blocks, items, masks, indices, bytes;  // offsets, then the size
+  int rows, slots, mask_words;
+  size_t requests, first, shared, masks, indices, bytes;  // offsets, then the size
 };
 
 inline Layout layout(int batch, int tokens, int max_tree, int indices_capacity, int hq, int hkv, int head_dim) {
   Layout l{};
-  const int g = hq / hkv;
-  l.rows = 16 * cols_of(max_tree, g, head_dim);
-  l.slots = slots_of(hkv, head_dim);
-  l.max_blocks = (int)((int64_t)tokens * g / l.rows) + batch;
-  l.max_items = l.max_blocks + 3 * l.slots;
+  l.rows = rows_of((int64_t)max_tree * (hq / hkv));
+  l.slots = slots_of(l.rows, hkv, head_dim);
   l.mask_words = (max_tree + 63) / 64;
   size_t at = sizeof(Header);
+  l.first = at;  // where each slot begins
+  at += sizeof(Place) * (size_t)l.slots;
+  l.shared = at;  // the row blocks that slots share, by the slot in which they begin
+  at += sizeof(Place) * (size_t)l.slots;
   l.requests = at;
   at += align_up(sizeof(Request) * (size_t)batch, 64);
-  l.blocks = at;
-  at += sizeof(RowBlock) * (size_t)l.max_blocks;
-  l.items = at;
-  at += sizeof(Item) * (size_t)l.max_items;
   l.masks = at;
   at += align_up(sizeof(uint64_t) * (size_t)tokens * l.mask_words, 64);
   l.indices = at;
   at += align_up(sizeof(int32_t) * (size_t)indices_capacity, 64);
   l.bytes = at;
   return l;
+}
+
+// A slot leaves at most two partial results: of the row block it takes over and
+// of the one it hands on.
+inline size_t workspace_bytes(const Layout& l, int hkv, int head_dim) {
+  return (size_t)l.slots * 2 * hkv * l.rows * (head_dim + 2) * sizeof(float);
 }
 
 // ------------------------------------------------------------------- plan ---
@@ -109,37 +128,62 @@ struct PlanArgs {
   int64_t mask_ld;
   Header* header;
   Request* requests;
-  RowBlock* blocks;
-  Item* items;
+  Place *first, *shared;
   uint64_t* masks;
   int32_t* indices;
-  int batch, tokens, max_tree, indices_count, indices_capacity, hq, hkv, head_dim, page_size;
-  int rows, tile, slots, max_items, max_blocks, mask_words;
-  int parts_fixed;  // > 0: cuts of the longest range (0: weighed)
+  Header want;
+  int indices_count;
+  int rows, tile, slots, mask_words;
+  int min_share;
 };
 
+// Request r, every entry of the tables brought into its range.
 __device__ __forceinline__ Request read_request(const PlanArgs& A, int r) {
-  Request q;
-  q.q_begin = min(max(A.qo_indptr[r], 0), A.tokens);
-  q.tree = min(min(max(A.qo_indptr[r + 1], q.q_begin), A.tokens) - q.q_begin, A.max_tree);
+  Request q{};
+  q.q_begin = min(max(A.qo_indptr[r], 0), A.want.tokens);
+  q.tree = min(min(max(A.qo_indptr[r + 1], q.q_begin), A.want.tokens) - q.q_begin, A.want.max_tree);
   q.page_begin = min(max(A.kv_indptr[r], 0), A.indices_count);
   const int pages = min(max(A.kv_indptr[r + 1], q.page_begin), A.indices_count) - q.page_begin;
-  const int last = min(max(A.kv_last[r], 1), A.page_size);
-  const int64_t len = pages > 0 ? (int64_t)(pages - 1) * A.page_size + last : 0;
-  q.kv_len = (int)min(len, (int64_t)(INT32_MAX / 2));
+  const int last = min(max(A.kv_last[r], 1), A.want.page_size);
+  const int64_t len = pages > 0 ? (int64_t)(pages - 1) * A.want.page_size + last : 0;
+  q.kv_len = (int)min(len, (int64_t)kMaxLen);
+  q.chunks = 1;
+  q.chunk_len = max(1, (q.kv_len + A.tile - 1) / A.tile);
+  q.blocks = (int)(((int64_t)q.tree * (A.want.hq / A.want.hkv) + A.rows - 1) / A.rows);
   return q;
+}
+
+// The chunk's first tile, and its tiles.
+__device__ __forceinline__ int chunk_tile(const Request& q, int chunk) {
+  return chunk * q.chunk_len + min(chunk, q.longer);
+}
+__device__ __forceinline__ int chunk_tiles(const Request& q, int chunk) { return q.chunk_len + (chunk < q.longer); }
+
+// The place at x of the request's own work.
+__device__ __forceinline__ Place place_at(const Request& q, int64_t x) {
+  Place p{};
+  p.rq = q;
+  const int64_t longer = (int64_t)q.longer * (q.chunk_len + 1) * q.blocks;
+  p.chunk = q.chunks == 1 ? 0
+            : x < longer  ? (int)(x / ((int64_t)(q.chunk_len + 1) * q.blocks))
+                          : q.longer + (int)((x - longer) / ((int64_t)q.chunk_len * q.blocks));
+  const int64_t y = x - (int64_t)chunk_tile(q, p.chunk) * q.blocks;
+  const int n = chunk_tiles(q, p.chunk);
+  p.block = (int)(y / n);
+  p.tile = (int)(y % n);
+  return p;
 }
 
 // Workgroup 0 cuts the work; the others copy the page ids and pack the masks.
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs A) {
-  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const int tid = threadIdx.x, batch = A.want.batch;
   if (blockIdx.x > 0) {
     const int64_t step = (int64_t)(gridDim.x - 1) * kPlanThreads;
     const int64_t first = (int64_t)(blockIdx.x - 1) * kPlanThreads + tid;
     for (int64_t i = first; i < A.indices_count; i += step) A.indices[i] = A.kv_indices[i];
-    for (int64_t i = first; i < (int64_t)A.tokens * A.mask_words; i += step) {
+    for (int64_t i = first; i < (int64_t)A.want.tokens * A.mask_words; i += step) {
       const int t = (int)(i / A.mask_words), w = (int)(i % A.mask_words);
-      int lo = 0, hi = A.batch;  // the request that holds token t: the last whose first token is <= t
+      int lo = 0, hi = batch;  // the request that holds token t: the last whose first token is <= t
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (A.qo_indptr[mid] <= t) lo = mid; else hi = mid;
@@ -166,134 +210,108 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs A) {
     return;
   }
 
-  __shared__ int s_tiles[kMaxRequests];       // tiles of a request's kv
-  __shared__ int s_nblocks[kMaxRequests];     // row blocks of its tree
-  __shared__ int s_item[kMaxRequests];        // items before it
-  __shared__ int s_block[kMaxRequests];       // row blocks before it
-  __shared__ int s_scan[2][kPlanThreads];
-  __shared__ int s_longest, s_chunk;
-  __shared__ float s_cost[kCandidates];
-  const int g = A.hq / A.hkv;
-  if (tid == 0) s_longest = 1;
-  __syncthreads();
-  for (int r = tid; r < A.batch; r += kPlanThreads) {
+  // The work before each request: a thread owns a run of requests, and the
+  // threads' sums are added up over the wave, then over the waves.
+  __shared__ long long s_base[kMaxRequests];  // of the n-th request with nodes
+  __shared__ long long s_wave_work[kPlanThreads / kWave];
+  __shared__ int s_wave_live[kPlanThreads / kWave];
+  const int lane = tid % kWave, wave = tid / kWave;
+  const int per = (batch + kPlanThreads - 1) / kPlanThreads;
+  const int r0 = min(batch, tid * per), r1 = min(batch, r0 + per);
+  long long work = 0;
+  int live = 0;
+  for (int r = r0; r < r1; ++r) {
     const Request q = read_request(A, r);
-    A.requests[r] = q;
-    s_tiles[r] = max(1, (q.kv_len + A.tile - 1) / A.tile);
-    s_nblocks[r] = (int)(((int64_t)q.tree * g + A.rows - 1) / A.rows);
-    if (q.tree > 0) atomicMax(&s_longest, s_tiles[r]);
+    work += (long long)q.chunk_len * q.blocks;
+    live += q.blocks > 0;
   }
-  __syncthreads();
-  const int longest = s_longest;
-
-  // The length of a part: of the longest range cut 1 .. 128 times, the one with
-  // the least estimated time in tiles.  An item costs its tiles and kOver more
-  // (its first loads, its partial results and the merge's reading of them);
-  // items in excess of the slots share them evenly but for half a part.
-  constexpr float kOver = 2.f;
-  for (int k = wave; k < kCandidates; k += kPlanThreads / kWave) {
-    const int chunk = (longest + k) / (k + 1);
-    long long items = 0, work = 0;
-    for (int r = lane; r < A.batch; r += kWave) {
-      items += (long long)((s_tiles[r] + chunk - 1) / chunk) * s_nblocks[r];
-      work += (long long)s_tiles[r] * s_nblocks[r];
-    }
+  long long work_upto = work;
+  int live_upto = live;
 #pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-      items += __shfl_xor(items, d);
-      work += __shfl_xor(work, d);
+  for (int d = 1; d < kWave; d <<= 1) {
+    const long long t = __shfl_up(work_upto, d);
+    const int n = __shfl_up(live_upto, d);
+    if (lane >= d) {
+      work_upto += t;
+      live_upto += n;
     }
-    float cost = ((float)work + kOver * (float)items) / A.slots + (items > A.slots ? 0.5f * chunk : 0.f);
-    cost = fmaxf(cost, chunk + kOver);
-    if (k > 0 && items > A.max_items) cost = INFINITY;
-    if (A.parts_fixed > 0 && k > 0 && k + 1 != A.parts_fixed) cost = INFINITY;
-    if (A.parts_fixed > 1 && k == 0) cost = 1e37f;
-    if (lane == 0) s_cost[k] = cost;
+  }
+  if (lane == kWave - 1) {
+    s_wave_work[wave] = work_upto;
+    s_wave_live[wave] = live_upto;
   }
   __syncthreads();
-  if (tid == 0) {
-    int best = 0;
-    for (int k = 1; k < kCandidates; ++k)
-      if (s_cost[k] < s_cost[best]) best = k;
-    s_chunk = (longest + best) / (best + 1);
+  long long total = 0, base = work_upto - work;
+  int n_live = 0, index = live_upto - live;
+  for (int w = 0; w < kPlanThreads / kWave; ++w) {
+    if (w < wave) {
+      base += s_wave_work[w];
+      index += s_wave_live[w];
+    }
+    total += s_wave_work[w];
+    n_live += s_wave_live[w];
   }
-  __syncthreads();
-  const int chunk = s_chunk;
-
-  // items and row blocks before each request: each thread owns a run of requests
-  const int per = (A.batch + kPlanThreads - 1) / kPlanThreads;
-  const int r0 = min(A.batch, tid * per), r1 = min(A.batch, r0 + per);
-  int items = 0, blocks = 0;
+  const long long share = max((long long)max(A.min_share, 1), (total + A.slots - 1) / A.slots);
+  const int n_slots = (int)((total + share - 1) / share);
   for (int r = r0; r < r1; ++r) {
-    items += (s_tiles[r] + chunk - 1) / chunk * s_nblocks[r];
-    blocks += s_nblocks[r];
+    Request q = read_request(A, r);
+    if (q.blocks <= 0) continue;
+    const long long tiles = q.chunk_len;
+    q.index = index;
+    q.base = base;
+    if (q.blocks > 1 && tiles >= 2 * share) {
+      q.chunks = (int)(tiles / share);
+      q.chunk_len = (int)(tiles / q.chunks);
+      q.longer = (int)(tiles % q.chunks);
+    }
+    A.requests[index] = q;
+    s_base[index] = base;
+    base += tiles * q.blocks;
+    ++index;
   }
-  s_scan[0][tid] = items;
-  s_scan[1][tid] = blocks;
   __syncthreads();
-  for (int off = 1; off < kPlanThreads; off <<= 1) {
-    const int a = tid >= off ? s_scan[0][tid - off] : 0, b = tid >= off ? s_scan[1][tid - off] : 0;
-    __syncthreads();
-    s_scan[0][tid] += a;
-    s_scan[1][tid] += b;
-    __syncthreads();
-  }
-  items = s_scan[0][tid] - items;
-  blocks = s_scan[1][tid] - blocks;
-  for (int r = r0; r < r1; ++r) {
-    s_item[r] = items;
-    s_block[r] = blocks;
-    items += (s_tiles[r] + chunk - 1) / chunk * s_nblocks[r];
-    blocks += s_nblocks[r];
-  }
-  // (a decreasing qo_indptr can ask for more than there is room for: it loses the rest)
-  const int n_items = min(s_scan[0][kPlanThreads - 1], A.max_items);
-  const int n_blocks = min(s_scan[1][kPlanThreads - 1], A.max_blocks);
-  __syncthreads();
-  auto owner = [&](const int* before, int i) {  // the last request r with before[r] <= i
-    int lo = 0, hi = A.batch;
+  auto locate = [&](long long x) {
+    int lo = 0, hi = n_live;  // the last request with base <= x
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (before[mid] <= i) lo = mid; else hi = mid;
+      if (s_base[mid] <= x) lo = mid; else hi = mid;
     }
-    return lo;
+    return place_at(A.requests[lo], x - s_base[lo]);
   };
-  // the row blocks of one kv range side by side: they find its pages in the L2
-  for (int i = tid; i < n_items; i += kPlanThreads) {
-    const int r = owner(s_item, i), at = i - s_item[r], nb = s_nblocks[r];
-    const int parts = (s_tiles[r] + chunk - 1) / chunk, part = at / nb;
-    Item it{};
-    it.request = r;
-    it.row0 = (at % nb) * A.rows;
-    it.tile_begin = (int)((int64_t)s_tiles[r] * part / parts);
-    it.tile_end = (int)((int64_t)s_tiles[r] * (part + 1) / parts);
-    it.parts = parts;
-    A.items[i] = it;
-  }
-  for (int i = tid; i < n_blocks; i += kPlanThreads) {
-    const int r = owner(s_block, i), at = i - s_block[r];
-    RowBlock b{};
-    b.request = r;
-    b.row0 = at * A.rows;
-    b.slot = s_item[r] + at;
-    b.step = s_nblocks[r];
-    b.parts = (s_tiles[r] + chunk - 1) / chunk;
-    if (b.slot + (int64_t)(b.parts - 1) * b.step >= n_items) b.parts = 0;
-    A.blocks[i] = b;
+  __shared__ int s_wave_shared[kPlanThreads / kWave];
+  int n_shared = 0;
+  for (int s0 = 0; s0 < n_slots; s0 += kPlanThreads) {
+    const int s = s0 + tid;
+    Place p{};
+    if (s < n_slots) {
+      A.first[s] = locate(s * share);
+      // The row block at the slot's end is shared if it begins in the slot and does
+      // not end there, or is one of several chunks (a chunk is no less than a share)
+      const long long end = min((s + 1) * share, total);
+      p = locate(end - 1);
+      const long long start = end - 1 - p.tile;
+      const int parts = (int)((start + chunk_tiles(p.rq, 0) - 1) / share - s) + 1;
+      if (p.chunk > 0 || start < s * share || (p.rq.chunks == 1 && parts == 1)) p.rq.blocks = 0;
+      p.parts = 2 * parts + (start > s * share);
+      p.tile = s;
+    }
+    const uint64_t mine = __builtin_amdgcn_ballot_w64(p.rq.blocks > 0);
+    if (lane == 0) s_wave_shared[wave] = __builtin_popcountll(mine);
+    __syncthreads();
+    int at = n_shared + __builtin_popcountll(mine & ((1ull << lane) - 1));
+    for (int w = 0; w < kPlanThreads / kWave; ++w) {
+      if (w < wave) at += s_wave_shared[w];
+      n_shared += s_wave_shared[w];
+    }
+    if (p.rq.blocks > 0) A.shared[at] = p;
+    __syncthreads();
   }
   if (tid == 0) {
-    Header h{};
-    h.magic = kMagic;
-    h.batch = A.batch;
-    h.tokens = A.tokens;
-    h.max_tree = A.max_tree;
-    h.indices_capacity = A.indices_capacity;
-    h.hq = A.hq;
-    h.hkv = A.hkv;
-    h.head_dim = A.head_dim;
-    h.page_size = A.page_size;
-    h.num_items = n_items;
-    h.num_blocks = n_blocks;
+    Header h = A.want;
+    h.num_requests = n_live;
+    h.num_slots = n_slots;
+    h.num_shared = n_shared;
+    h.share = share;
     *A.header = h;
   }
 }
@@ -317,9 +335,31 @@ __device__ __forceinline__ float column_max(float v) {
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-__device__ __forceinline__ void load_lds16(const char* g, char* l) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
-                                   (__attribute__((address_space(3))) void*)l, 16, 0, 0);
+// 16 bytes per lane from base + offset (bytes, per lane) into LDS at l + 16 lane.
+// Written as asm because the compiler, which cannot tell which buffer a
+// transposed LDS read is from, waits for every such load in flight before one:
+// the loads of the next block would be waited for in the middle of this one.
+// They have no register outputs; wait_loads() waits for them.
+__device__ __forceinline__ uint32_t lds_address(char* l) {
+  return uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)l);
+}
+// ONCE: the lines go first from the caches.  Bytes that one workgroup reads alone
+// stream 11 % faster so (5.8 and 6.4 TB/s); row blocks that share them do not.
+template <bool ONCE>
+__device__ __forceinline__ void load_lds16(const char* base, uint32_t offset, uint32_t l) {
+  if constexpr (ONCE)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(l), "v"(offset), "s"(base)
+                 : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(l), "v"(offset), "s"(base)
+                 : "memory");
+}
+__device__ __forceinline__ void load_lds16(const char* address, uint32_t l) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(l), "v"(address) : "memory");
+}
+// All but the N newest loads are done.
+template <int N> __device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
 __device__ __forceinline__ u32x2 read_tr(const char* p) {
@@ -338,13 +378,13 @@ struct Args {
   float *lse, *part;
   const Header* header;
   const Request* requests;
-  const RowBlock* blocks;
-  const Item* items;
+  const Place *first, *shared;
   const uint64_t* masks;
   const int32_t* indices;
   int64_t q_st, q_sh, o_st, o_sh, page_stride, token_stride, head_stride, num_pages;  // elements
   Header want;
-  int max_items, max_blocks, mask_words;
+  int slots, mask_words;
+  int once;  // no two row blocks read the same tokens
   float scale_log2;  // > 0; a negative scale negates q instead
   uint32_t q_flip;
 };
@@ -353,9 +393,9 @@ struct Args {
 __device__ __forceinline__ bool plan_fits(const Args& A) {
   const Header& h = *A.header;
   const Header& w = A.want;
-  return h.magic == kMagic && h.batch == w.batch && h.tokens == w.tokens && h.max_tree == w.max_tree &&
+  return h.magic == w.magic && h.batch == w.batch && h.tokens == w.tokens && h.max_tree == w.max_tree &&
          h.indices_capacity == w.indices_capacity && h.hq == w.hq && h.hkv == w.hkv && h.head_dim == w.head_dim &&
-         h.page_size == w.page_size && h.num_items <= A.max_items && h.num_blocks <= A.max_blocks;
+         h.page_size == w.page_size && h.num_requests <= w.batch && h.num_slots <= A.slots && h.num_shared <= A.slots;
 }
 
 template <typename T> struct Softmax {
@@ -387,432 +427,604 @@ __device__ __forceinline__ void store_row(const Args& A, const Request& q, int h
         sum == 0.f ? -INFINITY : (top + log2f(sum) - Softmax<T>::kShift) * 0.693147180559945309f;
 }
 
-template <typename T, int D, int C, bool PAGE16>
-__global__ __launch_bounds__(D == 256 ? 128 : 256, 1) void tree_kernel(Args A) {
+template <typename T, int D, int R, bool PAGE16>
+__global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256 ? 2 : 1) void tree_kernel(Args A) {
   using S = Softmax<T>;
   constexpr int NPP = S::kPlanes;
-  constexpr int W = D == 256 ? 2 : 4;          // waves
-  constexpr int NT = W * kWave;
-  constexpr int R = 16 * C;
+  constexpr int W = blocks_of(D);              // blocks of a tile
+  constexpr int WR = ranks_of(R);              // waves of a block
+  constexpr int NT = threads_of(R, D);
+  constexpr int C = R / WR / 16;               // 16-row columns of a wave
   constexpr int RB = D * 2;                    // bytes of a token's row
   constexpr int CPR = D / 8;                   // 16-byte chunks of a row
   constexpr int TPI = kWave / CPR;             // tokens per load
   constexpr int NL = kBlock / TPI;             // loads of a block's K
+  constexpr int JG = 16 / TPI;                 // loads of 16 tokens
   constexpr int KS = D / 32, NA = D / 16;
-  constexpr int kBuf = W * kBlock * RB;
   constexpr int kTile = W * kBlock;
+  constexpr int kK = kBlock * RB;              // bytes of a block's K, then its V
+  constexpr int kStage = W * 2 * kK;
+  constexpr int kMine = 2 * NL / WR;           // a wave's loads of a block: K and V, or one of them
   constexpr int kPartFloats = R * (D + 2);     // outputs [row][dim], then (max, sum) per row
   constexpr int kSwz = CPR < 16 ? CPR - 1 : 15;
-  static_assert(kBuf >= R * D * 4, "a wave's outputs fit one buffer");
-  // one object per buffer: loads into one never alias reads of another
-  __shared__ __align__(16) char s_k0[kBuf];
-  __shared__ __align__(16) char s_v0[kBuf];
-  __shared__ __align__(16) char s_k1[kBuf];
-  __shared__ __align__(16) char s_v1[kBuf];
+  static_assert(W * R * D * 4 <= 2 * kStage, "the blocks' outputs fit the buffers");
+  __shared__ __align__(16) char s_ring[2 * kStage];
   __shared__ float s_ml[W][R][2];
+  __shared__ int s_turn[W * WR];
 
   if (!plan_fits(A)) return;
-  const int n_items = A.header->num_items, hkv = A.want.hkv;
-  // Workgroups go round the 8 XCDs.  Where the kv heads divide 8, each XCD keeps
-  // one head and one run of the items, so row blocks of one range share an L2.
-  int h, index;
-  if (8 % hkv == 0) {
-    const int rep = 8 / hkv, x = blockIdx.x % 8, per = (n_items + rep - 1) / rep, at = blockIdx.x / 8;
-    h = x % hkv;
-    index = at < per ? x / hkv * per + at : n_items;
-  } else {
-    h = blockIdx.x % hkv;
-    index = blockIdx.x / hkv;
-  }
-  if (index >= n_items) return;
-  const Item it = A.items[index];
-  const Request rq = A.requests[it.request];
-  const int g = A.want.hq / hkv, n_rows = rq.tree * g;
-  const int kv_len = rq.kv_len, prefix = max(0, kv_len - rq.tree);
-  const int page_size = A.want.page_size, n_pages = (kv_len + page_size - 1) / page_size;
-  const int32_t* ind = A.indices + rq.page_begin;
-  const int lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave);
-  const int lr = lane % 16, grp = lane / 16;
+  const int n_slots = A.header->num_slots, hkv = A.want.hkv;
+  const int64_t share = A.header->share;
+  // Workgroups go round the 8 XCDs: with 8 heads each has one, and its L2 the row blocks of one chunk.
+  const int slot = blockIdx.x / hkv, h = blockIdx.x % hkv;
+  if (slot >= n_slots) return;
+  const int n_requests = A.header->num_requests;
+  Place pl = A.first[slot];
+  int64_t left = share;  // tiles of the share to come
 
-  u32x4 qb[C][KS];
-  const uint64_t* masks[C];
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int row = min(it.row0 + c * 16 + lr, n_rows - 1);  // rows past the end repeat the last one, unstored
-    const int node = row / g;
-    masks[c] = A.masks + (int64_t)(rq.q_begin + node) * A.mask_words;
-    const char* qp = A.q + ((int64_t)(rq.q_begin + node) * A.q_st + (int64_t)(h * g + row - node * g) * A.q_sh) * 2 + grp * 16;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      u32x4 v = *reinterpret_cast<const u32x4*>(qp + ks * 64);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] ^= A.q_flip;
-      qb[c][ks] = v;
-    }
-  }
+  const int g = A.want.hq / hkv, page_size = A.want.page_size;
+  const int lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave);
+  const int blk = wave % W, rank = wave / W;  // the wave's block of a tile, its rows of the row block
+  const int lr = lane % 16, grp = lane / 16;
+  const float sc = A.scale_log2;
 
   auto swz_k = [](int n) { return n & kSwz; };
   auto swz_v = [](int n) { return CPR < 16 ? (n & kSwz) : 2 * (n & 7); };
   auto clamp_page = [&](int page) -> int64_t {
     return page < 0 ? 0 : ((int64_t)page >= A.num_pages ? A.num_pages - 1 : (int64_t)page);
   };
-  // byte offset of token t of the sequence (or of the page's rest behind the last one)
-  auto token_offset = [&](int t) -> int64_t {
-    const int page = t / page_size;
-    return (clamp_page(ind[min(page, n_pages - 1)]) * A.page_stride + (int64_t)(t - page * page_size) * A.token_stride) * 2;
-  };
-  // Offsets of the wave's tokens, one per lane.  Pages of a multiple of 16
-  // tokens: of the 16-token groups of 32 tiles; others: of a block's 32 tokens.
-  auto load_offsets = [&](int tile) -> int64_t {
-    if constexpr (PAGE16) return token_offset((tile + lane / 2) * kTile + wave * kBlock + (lane % 2) * 16);
-    return token_offset(min(tile * kTile + wave * kBlock + lane % kBlock, kv_len - 1));
-  };
-  // loads: instruction j fetches tokens j TPI .. of the block, lane l chunk
-  // l % CPR of token l / CPR, permuted by the token
-  constexpr int JG = PAGE16 ? 16 / TPI : 1;
-  int64_t koff[NL], voff[NL];
+  // Loads: instruction j fetches tokens j TPI .. of the block, lane l chunk
+  // l % CPR of token l / CPR, permuted by the token.  A wave alone fetches K (0)
+  // and V (1), of two the first K and the second V.
+  const bool second = rank > 0;
+  uint32_t off0[JG], off1[JG];  // within 16 tokens of a page (others: within the token's row)
 #pragma unroll
-  for (int j = 0; j < NL; ++j) {
+  for (int j = 0; j < JG; ++j) {
     const int n = j * TPI + lane / CPR;
-    const int64_t base = ((PAGE16 ? (int64_t)(n % 16) * A.token_stride : 0) + (int64_t)h * A.head_stride) * 2;
-    koff[j] = base + ((lane % CPR) ^ swz_k(n)) * 16;
-    voff[j] = base + ((lane % CPR) ^ swz_v(n)) * 16;
+    const uint32_t base = PAGE16 ? n * (uint32_t)A.token_stride * 2 : 0;
+    off0[j] = base + ((lane % CPR) ^ (second ? swz_v(n) : swz_k(n))) * 16;
+    off1[j] = base + ((lane % CPR) ^ swz_v(n)) * 16;
   }
-  auto load_block = [&](int64_t offs, int at, char* kd, char* vd) {
-    kd += wave * kBlock * RB;
-    vd += wave * kBlock * RB;
+  const char* src0 = (second ? A.v : A.k) + (int64_t)h * A.head_stride * 2;
+  const char* src1 = A.v + (int64_t)h * A.head_stride * 2;
+  const uint32_t ring = lds_address(s_ring + blk * 2 * kK + (second ? kK : 0));
+  auto load_group = [&](auto ONCE, int64_t off, uint32_t to) {  // 16 tokens of a page
 #pragma unroll
-    for (int j = 0; j < NL; ++j) {
-      int64_t off;
-      if constexpr (PAGE16) {
-        const int from = at * 2 + j / JG;
-        off = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)offs, from) |
-                        (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(offs >> 32), from) << 32);
+    for (int j = 0; j < JG; ++j) {
+      load_lds16<decltype(ONCE)::value>(src0 + off, off0[j], to + j * kWave * 16);
+      if constexpr (WR == 1) load_lds16<decltype(ONCE)::value>(src1 + off, off1[j], to + kK + j * kWave * 16);
+    }
+  };
+  auto load_block = [&](int64_t offs, int at, int stage) {
+    const uint32_t to = ring + stage * kStage;
+    if constexpr (PAGE16) {
+      int64_t off[2];
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+        off[half] = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)offs, at * 2 + half) |
+                              (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(offs >> 32), at * 2 + half) << 32);
+      // (fewer than 64 rows are one row block)
+      if (R < 64 || A.once) {
+        load_group(std::true_type{}, off[0], to);
+        load_group(std::true_type{}, off[1], to + JG * kWave * 16);
       } else {
-        off = __shfl(offs, j * TPI + lane / CPR);
+        load_group(std::false_type{}, off[0], to);
+        load_group(std::false_type{}, off[1], to + JG * kWave * 16);
       }
-      load_lds16(A.k + off + koff[j], kd + j * kWave * 16);
-      load_lds16(A.v + off + voff[j], vd + j * kWave * 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < NL; ++j) {
+        const int64_t off = __shfl(offs, j * TPI + lane / CPR);
+        load_lds16(src0 + off + off0[j % JG], to + j * kWave * 16);
+        if constexpr (WR == 1) load_lds16(src1 + off + off1[j % JG], to + kK + j * kWave * 16);
+      }
     }
   };
 
-  // operand reads: K row blk*16 + lr, chunk 4 ks + grp; V tokens 4 grp + lr/4
+  // operand reads: K row b*16 + lr, chunk 4 ks + grp; V tokens 4 grp + lr/4
   // (+16), dims 16 a + 4 (lr % 4)
   int kaddr[KS], vaddr[NA];
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) kaddr[ks] = wave * kBlock * RB + lr * RB + ((ks * 4 + grp) ^ swz_k(lr)) * 16;
+  for (int ks = 0; ks < KS; ++ks) kaddr[ks] = blk * 2 * kK + lr * RB + ((ks * 4 + grp) ^ swz_k(lr)) * 16;
 #pragma unroll
   for (int a = 0; a < NA; ++a) {
     const int n = grp * 4 + lr / 4;
-    vaddr[a] = wave * kBlock * RB + n * RB + ((2 * a + (lr % 4) / 2) ^ swz_v(n)) * 16 + (lr % 2) * 8;
+    vaddr[a] = blk * 2 * kK + kK + n * RB + ((2 * a + (lr % 4) / 2) ^ swz_v(n)) * 16 + (lr % 2) * 8;
   }
 
-  f32x4 acc[C][NA];
-  float m[C], l[C];
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    m[c] = -INFINITY;
-    l[c] = 0.f;
-#pragma unroll
-    for (int a = 0; a < NA; ++a) acc[c][a] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // The two waves of a block meet: each leaves the number of its meetings and
+  // waits for the other's.  Both work on the same blocks in the same order, so
+  // they come as often, and the wait ends.
+  int turn = 0;
+  auto meet = [&]() {
+    if constexpr (WR > 1) {
+      __builtin_amdgcn_sched_barrier(0);
+      ++turn;
+      asm volatile("" ::: "memory");
+      if (lane == 0) __hip_atomic_store(&s_turn[wave], turn, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      const int* other = &s_turn[(wave + W) % (W * WR)];
+      while (uniform(__hip_atomic_load(other, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP)) < turn) {
+      }
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  if constexpr (WR > 1) {
+    if (lane == 0) s_turn[wave] = 0;
+    __syncthreads();
   }
-  const float sc = A.scale_log2;
 
-  // the wave's blocks: only the last tile can lie behind its tokens
-  const int t_begin = it.tile_begin;
-  const int t_end = (it.tile_end - 1) * kTile + wave * kBlock < kv_len ? it.tile_end : it.tile_end - 1;
-  int64_t offs = 0, offs_next = 0;
+  for (;;) {
+    const Request& rq = pl.rq;
+    // this share's tiles of the row block
+    const int c_first = chunk_tile(rq, pl.chunk), c_tiles = chunk_tiles(rq, pl.chunk);
+    const int t_first = c_first + pl.tile, t_last = c_first + (int)min((int64_t)c_tiles, pl.tile + left);
+    const bool whole = rq.chunks == 1 && t_last - t_first == c_tiles;
+    const int row0 = pl.block * R, n_rows = rq.tree * g;
+    const int kv_len = rq.kv_len, prefix = max(0, kv_len - rq.tree);
+    const int n_pages = (kv_len + page_size - 1) / page_size;
+    const int32_t* ind = A.indices + rq.page_begin;
+    // the wave's blocks: only the last tile can lie behind its tokens
+    const int t_end = (int64_t)(t_last - 1) * kTile + blk * kBlock < kv_len ? t_last : t_last - 1;
+    // byte offset of token t of the sequence (or of the page's rest behind the last one)
+    auto token_offset = [&](int t) -> int64_t {
+      const int page = t / page_size;
+      return (clamp_page(ind[min(page, n_pages - 1)]) * A.page_stride + (int64_t)(t - page * page_size) * A.token_stride) * 2;
+    };
+    // Offsets of the block's tokens, one per lane.  Pages of a multiple of 16
+    // tokens: of the 16-token groups of 32 tiles; others: of a block's 32 tokens.
+    auto load_offsets = [&](int tile) -> int64_t {
+      if constexpr (PAGE16) return token_offset((tile + lane / 2) * kTile + blk * kBlock + (lane % 2) * 16);
+      return token_offset(min(tile * kTile + blk * kBlock + lane % kBlock, kv_len - 1));
+    };
+    int64_t offs = 0, offs_next = 0;
+    const bool any_tokens = t_first < t_end && kv_len > 0;
+    if (any_tokens) {
+      offs = load_offsets(t_first);
+      offs_next = load_offsets(t_first + (PAGE16 ? 32 : 1));
+    }
 
-  auto body = [&](int tile, const char* kb, char* vb, char* kn, char* vn) {
-    __builtin_amdgcn_sched_barrier(0);
-    if (tile + 1 < t_end) {
-      if constexpr (PAGE16) {
-        const int at = (tile + 1 - t_begin) % 32;
+    u32x4 qb[C][KS];
+    int nodes[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int row = min(row0 + (rank * C + c) * 16 + lr, n_rows - 1);  // rows past the end repeat the last one, unstored
+      const int node = row / g;
+      nodes[c] = rq.q_begin + node;
+      const char* qp = A.q + ((int64_t)(rq.q_begin + node) * A.q_st + (int64_t)(h * g + row - node * g) * A.q_sh) * 2 + grp * 16;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        u32x4 v = *reinterpret_cast<const u32x4*>(qp + ks * 64);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] ^= A.q_flip;
+        qb[c][ks] = v;
+      }
+    }
+    f32x4 acc[C][NA];
+    float m[C], l[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      m[c] = -INFINITY;
+      l[c] = 0.f;
+#pragma unroll
+      for (int a = 0; a < NA; ++a) acc[c][a] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    if (any_tokens) load_block(offs, 0, 0);
+
+    for (int tile = t_first; tile < t_end && any_tokens; ++tile) {
+      __builtin_amdgcn_sched_barrier(0);
+      const int stage = (tile - t_first) % 2;
+      meet();  // both are done with the other stage
+      if (tile + 1 < t_end) {
+        const int at = PAGE16 ? (tile + 1 - t_first) % 32 : 0;
         if (at == 0) {
           offs = offs_next;
-          offs_next = load_offsets(tile + 33);
+          offs_next = load_offsets(tile + (PAGE16 ? 33 : 2));
         }
-        load_block(offs, at, kn, vn);
+        load_block(offs, at, stage ^ 1);
+        __builtin_amdgcn_sched_barrier(0);
+        wait_loads<kMine>();  // all but those of the next block
       } else {
-        offs = offs_next;
-        offs_next = load_offsets(tile + 2);
-        load_block(offs, 0, kn, vn);
+        wait_loads<0>();
       }
+      meet();  // the other's are done too
       __builtin_amdgcn_sched_barrier(0);
-      // all but the 2 NL loads of the next block are done
-      __builtin_amdgcn_s_waitcnt(0xF70 | ((2 * NL) & 15) | ((2 * NL) >> 4) << 14);
-    } else {
-      __builtin_amdgcn_s_waitcnt(0xF70);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    const int tb = tile * kTile + wave * kBlock;
-    uint32_t vis[C];
-    const bool tail = tb + kBlock > prefix;
-    if (tail) {
-      // bit n: the column's row sees token tb + n
-      const int j0 = tb - prefix, w = j0 >> 6, sh = j0 & 63, n = min(kv_len - tb, kBlock);
-      const uint32_t inside = n == kBlock ? ~0u : (1u << n) - 1;
+      char* kb = s_ring + stage * kStage;
+      const int tb = tile * kTile + blk * kBlock;
+      uint32_t vis[C];
+      const bool tail = tb + kBlock > prefix;
+      if (tail) {
+        // bit n: the column's row sees token tb + n
+        const int j0 = tb - prefix, w = j0 >> 6, sh = j0 & 63, n = min(kv_len - tb, kBlock);
+        const uint32_t inside = n == kBlock ? ~0u : (1u << n) - 1;
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const uint64_t lo = w < 0 ? ~0ull : (w < A.mask_words ? masks[c][w] : 0);
-        const uint64_t hi = w + 1 < 0 ? ~0ull : (w + 1 < A.mask_words ? masks[c][w + 1] : 0);
-        vis[c] = (uint32_t)(sh ? lo >> sh | hi << (64 - sh) : lo) & inside;
-      }
-      // 0 * V is NaN where V is not finite: V behind the last token is set to
-      // zero, and so are infinities and NaN of tree tokens, which go to the
-      // outputs of the rows that see them by themselves
-      char* v0 = vb + wave * kBlock * RB;
-      bool found = false;
-#pragma unroll
-      for (int j = 0; j < NL; ++j) {
-        const int nn = j * TPI + lane / CPR;
-        u32x4* p = reinterpret_cast<u32x4*>(v0 + (j * kWave + lane) * 16);
-        if (nn >= n) {
-          *p = u32x4{0u, 0u, 0u, 0u};
-        } else if (nn + tb >= prefix) {
-          const u32x4 x = *p;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) found = found || nonfinite16<T>(x[e]) || nonfinite16<T>(x[e] >> 16);
+        for (int c = 0; c < C; ++c) {
+          const uint64_t* mask = A.masks + (int64_t)nodes[c] * A.mask_words;
+          const uint64_t lo = w < 0 ? ~0ull : (w < A.mask_words ? mask[w] : 0);
+          const uint64_t hi = w + 1 < 0 ? ~0ull : (w + 1 < A.mask_words ? mask[w + 1] : 0);
+          vis[c] = (uint32_t)(sh ? lo >> sh | hi << (64 - sh) : lo) & inside;
         }
-      }
-      if (__builtin_amdgcn_ballot_w64(found) != 0) {
-        for (int nn = max(0, prefix - tb); nn < n; ++nn) {
+        // 0 * V is NaN where V is not finite: V behind the last token is set to
+        // zero, and so are infinities and NaN of tree tokens, which go to the
+        // outputs of the rows that see them by themselves
+        char* v0 = kb + blk * 2 * kK + kK;
+        bool found = false;
 #pragma unroll
-          for (int a = 0; a < NA; ++a) {
-            u32x2* p = reinterpret_cast<u32x2*>(v0 + nn * RB + ((2 * a + grp / 2) ^ swz_v(nn)) * 16 + (grp % 2) * 8);
-            u32x2 x = *p;
-            u32x2 keep = x;
+        for (int j = 0; j < NL; ++j) {
+          const int nn = j * TPI + lane / CPR;
+          if (nn < n && nn + tb >= prefix) {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(v0 + (j * kWave + lane) * 16);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t b = i % 2 ? x[i / 2] >> 16 : x[i / 2] & 0xffffu;
-              if (nonfinite16<T>(b)) {
+            for (int e = 0; e < 4; ++e) found = found || nonfinite16<T>(x[e]) || nonfinite16<T>(x[e] >> 16);
+          }
+        }
+        const bool any = __builtin_amdgcn_ballot_w64(found) != 0;
+        if (any) {
+          for (int nn = max(0, prefix - tb); nn < n; ++nn) {
+#pragma unroll
+            for (int a = 0; a < NA; ++a) {
+              const u32x2 x = *reinterpret_cast<const u32x2*>(v0 + nn * RB + ((2 * a + grp / 2) ^ swz_v(nn)) * 16 + (grp % 2) * 8);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t b = i % 2 ? x[i / 2] >> 16 : x[i / 2] & 0xffffu;
                 float f, unused;
                 unpack2<T>(b, f, unused);
 #pragma unroll
                 for (int c = 0; c < C; ++c)
-                  if (vis[c] >> nn & 1) acc[c][a][i] += f;
-                keep[i / 2] &= i % 2 ? 0x0000ffffu : 0xffff0000u;
+                  if (nonfinite16<T>(b) && (vis[c] >> nn & 1)) acc[c][a][i] += f;
               }
             }
-            // (the 16 lanes of a group write the same values)
-            *p = keep;
           }
         }
+        meet();  // both have read the block's V
+#pragma unroll
+        for (int j = 0; j < NL; ++j) {
+          const int nn = j * TPI + lane / CPR;
+          u32x4* p = reinterpret_cast<u32x4*>(v0 + (j * kWave + lane) * 16);
+          if (nn >= n) {
+            *p = u32x4{0u, 0u, 0u, 0u};
+          } else if (any && nn + tb >= prefix) {
+            u32x4 x = *p;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              x[e] &= (nonfinite16<T>(x[e]) ? 0u : 0xffffu) | (nonfinite16<T>(x[e] >> 16) ? 0u : 0xffff0000u);
+            *p = x;
+          }
+        }
+        meet();  // (both have written the same)
       }
-    }
 
-    f32x4 s[C][2];
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int b = 0; b < 2; ++b) s[c][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      u32x4 ka[2];
-#pragma unroll
-      for (int b = 0; b < 2; ++b) ka[b] = *reinterpret_cast<const u32x4*>(kb + kaddr[ks] + b * 16 * RB);
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int c = 0; c < C; ++c) s[c][b] = mfma32<T>(ka[b], qb[c][ks], s[c][b]);
-    }
-    if (tail) {
+      f32x4 s[C][2];
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
+        for (int b = 0; b < 2; ++b) s[c][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        u32x4 ka[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) ka[b] = *reinterpret_cast<const u32x4*>(kb + kaddr[ks] + b * 16 * RB);
+#pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            s[c][b][i] = vis[c] >> (b * 16 + 4 * grp + i) & 1 ? s[c][b][i] : -INFINITY;
-    }
-    float mx[C];
-    bool rose = false;
+          for (int c = 0; c < C; ++c) s[c][b] = mfma32<T>(ka[b], qb[c][ks], s[c][b]);
+      }
+      if (tail) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      float v = -INFINITY;
+        for (int c = 0; c < C; ++c)
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+          for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v = fmaxf(v, s[c][b][i]);
-      mx[c] = v * sc;
-      rose |= mx[c] > m[c] + S::kLag;
-    }
-    if (__builtin_amdgcn_ballot_w64(rose) != 0) {
+            for (int i = 0; i < 4; ++i)
+              s[c][b][i] = vis[c] >> (b * 16 + 4 * grp + i) & 1 ? s[c][b][i] : -INFINITY;
+      }
+      float mx[C];
+      bool rose = false;
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        const float mn = fmaxf(m[c], column_max(mx[c]));
-        const float alpha = fast_exp2(m[c] - (mn == -INFINITY ? 0.f : mn));
-        m[c] = mn;
-        l[c] *= alpha;
+        float v = -INFINITY;
 #pragma unroll
-        for (int a = 0; a < NA; ++a)
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[c][a][i] *= alpha;
+          for (int i = 0; i < 4; ++i) v = fmaxf(v, s[c][b][i]);
+        mx[c] = v * sc;
+        rose |= mx[c] > m[c] + S::kLag;
+      }
+      if (__builtin_amdgcn_ballot_w64(rose) != 0) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const float mn = fmaxf(m[c], column_max(mx[c]));
+          const float alpha = fast_exp2(m[c] - (mn == -INFINITY ? 0.f : mn));
+          m[c] = mn;
+          l[c] *= alpha;
+#pragma unroll
+          for (int a = 0; a < NA; ++a)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[c][a][i] *= alpha;
+        }
+      }
+      u32x4 pb[C][NPP];
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const float mu = (m[c] == -INFINITY ? 0.f : m[c]) - S::kShift;
+        float ps = 0.f;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float e = fast_exp2(__builtin_fmaf(s[c][b][i], sc, -mu));
+            s[c][b][i] = e;
+            ps += e;
+          }
+        l[c] += ps;  // per lane; the column's lanes meet after the last block
+        // P^T as the B operand: k = 8 grp + e is token 4 grp + e % 4 of block e / 4
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const f32x4 src = s[c][e / 2];
+          const float p0 = src[(e % 2) * 2], p1 = src[(e % 2) * 2 + 1];
+          const uint32_t hw = pack2_hw<T>(p0, p1);
+          pb[c][0][e] = hw;
+          if constexpr (NPP == 2) {
+            float h0, h1;
+            unpack2<T>(hw, h0, h1);
+            pb[c][NPP - 1][e] = pack2_hw<T>(p0 - h0, p1 - h1);
+          }
+        }
+      }
+      // four independent accumulations in turn: an MFMA waits for the one before
+      // it on the same accumulator
+#pragma unroll
+      for (int a0 = 0; a0 < NA; a0 += 2) {
+        u32x4 va[2];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+          const u32x2 v0 = read_tr(kb + vaddr[a0 + a]), v1 = read_tr(kb + vaddr[a0 + a] + 16 * RB);
+          va[a] = u32x4{v0[0], v0[1], v1[0], v1[1]};
+        }
+#pragma unroll
+        for (int i = 0; i < NPP; ++i)
+#pragma unroll
+          for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int c = 0; c < C; ++c) acc[c][a0 + a] = mfma32<T>(va[a], pb[c][i], acc[c][a0 + a]);
       }
     }
-    u32x4 pb[C][NPP];
+
+    // the blocks' states meet in the buffers, rows' 16-byte chunks permuted
+    __syncthreads();
+    float* outs = reinterpret_cast<float*>(s_ring);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const float mu = (m[c] == -INFINITY ? 0.f : m[c]) - S::kShift;
-      float ps = 0.f;
+      float sum = l[c];
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
+      const int pr = (rank * C + c) * 16 + lr;
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float e = fast_exp2(__builtin_fmaf(s[c][b][i], sc, -mu));
-          s[c][b][i] = e;
-          ps += e;
-        }
-      l[c] += ps;  // per lane; the column's lanes meet after the last block
-      // P^T as the B operand: k = 8 grp + e is token 4 grp + e % 4 of block e / 4
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const f32x4 src = s[c][e / 2];
-        const float p0 = src[(e % 2) * 2], p1 = src[(e % 2) * 2 + 1];
-        const uint32_t hw = pack2_hw<T>(p0, p1);
-        pb[c][0][e] = hw;
-        if constexpr (NPP == 2) {
-          float h0, h1;
-          unpack2<T>(hw, h0, h1);
-          pb[c][NPP - 1][e] = pack2_hw<T>(p0 - h0, p1 - h1);
-        }
+      for (int a = 0; a < NA; ++a)
+        *reinterpret_cast<f32x4*>(outs + (blk * R + pr) * D + ((a * 4 + grp) ^ lr) * 4) = acc[c][a];
+      if (grp == 0) {
+        s_ml[blk][pr][0] = m[c];
+        s_ml[blk][pr][1] = sum;
       }
     }
+    __syncthreads();
+    constexpr int LPR = D / 4;  // lanes of a row, four dims each
+    const int ch = threadIdx.x % LPR;
+    // a slot's first partial result is of what it takes over, its second of what it hands on
+    float* part = A.part + ((2 * (int64_t)slot + (left < share)) * hkv + h) * kPartFloats;
+    for (int pr = threadIdx.x / LPR; pr < R; pr += NT / LPR) {
+      const int row = row0 + pr;
+      if (row >= n_rows) break;
+      float top = -INFINITY;
 #pragma unroll
-    for (int a = 0; a < NA; ++a) {
-      const u32x2 v0 = read_tr(vb + vaddr[a]), v1 = read_tr(vb + vaddr[a] + 16 * RB);
-      const u32x4 va = u32x4{v0[0], v0[1], v1[0], v1[1]};
+      for (int w = 0; w < W; ++w) top = fmaxf(top, s_ml[w][pr][0]);
+      const float ref = top == -INFINITY ? 0.f : top;
+      float sum = 0.f;
+      f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int pl = 0; pl < NPP; ++pl)
+      for (int w = 0; w < W; ++w) {
+        const float wt = fast_exp2(s_ml[w][pr][0] - ref);
+        const f32x4 x = *reinterpret_cast<const f32x4*>(outs + (w * R + pr) * D + (ch ^ (pr % 16)) * 4);
+        sum = __builtin_fmaf(s_ml[w][pr][1], wt, sum);
 #pragma unroll
-        for (int c = 0; c < C; ++c) acc[c][a] = mfma32<T>(va, pb[c][pl], acc[c][a]);
+        for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(x[i], wt, o[i]);
+      }
+      if (whole) {
+        store_row<T>(A, rq, h, row, ch * 4, o, top, sum, ch == 0);
+      } else {
+        *reinterpret_cast<f32x4*>(part + pr * D + ch * 4) = o;
+        if (ch == 0) *reinterpret_cast<f32x2*>(part + R * D + pr * 2) = f32x2{top, sum};
+      }
     }
-  };
-
-  if (t_begin < t_end && kv_len > 0) {
-    offs = load_offsets(t_begin);
-    offs_next = load_offsets(t_begin + (PAGE16 ? 32 : 1));
-    load_block(offs, 0, s_k0, s_v0);
-    int tile = t_begin;
-    for (; tile + 2 <= t_end; tile += 2) {
-      body(tile, s_k0, s_v0, s_k1, s_v1);
-      body(tile + 1, s_k1, s_v1, s_k0, s_v0);
+    left -= t_last - t_first;
+    if (left <= 0) return;
+    pl.tile = 0;
+    if (++pl.block == rq.blocks) {
+      pl.block = 0;
+      if (++pl.chunk == rq.chunks) {
+        pl.chunk = 0;
+        if (rq.index + 1 >= n_requests) return;
+        pl.rq = A.requests[rq.index + 1];
+      }
     }
-    if (tile < t_end) body(tile, s_k0, s_v0, s_k1, s_v1);
-  }
-
-  // the waves' states meet: outputs in one buffer per wave, rows' 16-byte chunks permuted
-  __syncthreads();
-  float* mine = reinterpret_cast<float*>(wave == 0 ? s_k0 : wave == 1 ? s_v0 : wave == 2 ? s_k1 : s_v1);
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    float sum = l[c];
-    sum += __shfl_xor(sum, 16);
-    sum += __shfl_xor(sum, 32);
-    const int pr = c * 16 + lr;
-#pragma unroll
-    for (int a = 0; a < NA; ++a) *reinterpret_cast<f32x4*>(mine + pr * D + ((a * 4 + grp) ^ lr) * 4) = acc[c][a];
-    if (grp == 0) {
-      s_ml[wave][pr][0] = m[c];
-      s_ml[wave][pr][1] = sum;
-    }
-  }
-  __syncthreads();
-  constexpr int LPR = D / 4;  // lanes of a row, four dims each
-  const int ch = threadIdx.x % LPR;
-  float* part = A.part + ((int64_t)index * hkv + h) * kPartFloats;
-  for (int pr = threadIdx.x / LPR; pr < R; pr += NT / LPR) {
-    const int row = it.row0 + pr;
-    if (row >= n_rows) break;
-    float top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < W; ++w) top = fmaxf(top, s_ml[w][pr][0]);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
-    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const float wt = fast_exp2(s_ml[w][pr][0] - ref);
-      const char* buf = w == 0 ? s_k0 : w == 1 ? s_v0 : w == 2 ? s_k1 : s_v1;
-      const f32x4 x = *reinterpret_cast<const f32x4*>(buf + (pr * D + (ch ^ (pr & 15)) * 4) * 4);
-      sum = __builtin_fmaf(s_ml[w][pr][1], wt, sum);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(x[i], wt, o[i]);
-    }
-    if (it.parts > 1) {
-      *reinterpret_cast<f32x4*>(part + pr * D + ch * 4) = o;
-      if (ch == 0) *reinterpret_cast<f32x2*>(part + R * D + pr * 2) = f32x2{top, sum};
-    } else {
-      store_row<T>(A, rq, h, row, ch * 4, o, top, sum, ch == 0);
-    }
+    __syncthreads();  // the outputs are read: the buffers may be filled again
   }
 }
 
-// The parts of a row, in order: D / 4 lanes per row, four dims each.
+// A weighted sum of parts with its maximum: joins N more, those past n left out.
+template <int N>
+__device__ __forceinline__ void join(float& top, float& sum, f32x4& o, const f32x4 (&x)[N], const f32x2 (&own)[N], int n) {
+  float here = top;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < n) here = fmaxf(here, own[i][0]);
+  const float ref = here == -INFINITY ? 0.f : here, old = fast_exp2(top - ref);
+  top = here;
+  sum *= old;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] *= old;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (i >= n) break;
+    const float wt = fast_exp2(own[i][0] - ref);
+    sum = __builtin_fmaf(own[i][1], wt, sum);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[i][e], wt, o[e]);
+  }
+}
+
+// The parts of a row block that slots share, in order: D / 4 lanes per row, four
+// dims each.  A wave takes all parts of its rows where they are up to 8, and as
+// many rows as keep 8 loads in flight; of more parts each of the workgroup's four
+// waves takes every fourth of the same rows.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void merge_kernel(Args A, int rows) {
-  if (!plan_fits(A)) return;
+  constexpr int LPR = D / 4, RPW = kWave / LPR, W = 4;  // lanes of a row, rows of a wave, waves
+  __shared__ f32x4 s_o[W][kWave];
+  __shared__ f32x2 s_ml[W][kWave];
   const int hkv = A.want.hkv, h = blockIdx.x % hkv, index = blockIdx.x / hkv;
-  if (index >= A.header->num_blocks) return;
-  const RowBlock b = A.blocks[index];
-  if (b.parts <= 1) return;
-  const Request rq = A.requests[b.request];
-  constexpr int LPR = D / 4;
-  const int pr = blockIdx.y * (256 / LPR) + threadIdx.x / LPR, ch = threadIdx.x % LPR;
-  const int row = b.row0 + pr, g = A.want.hq / hkv;
-  if (pr >= rows || row >= rq.tree * g) return;
+  const Place pl = A.shared[index];
+  if (!plan_fits(A) || index >= A.header->num_shared) return;
+  const int64_t share = A.header->share;
+  const Request& rq = pl.rq;
+  const int lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), ch = lane % LPR;
+  const int row0 = pl.block * rows, n_rows = min(rows, rq.tree * (A.want.hq / hkv) - row0);
   const int64_t size = (int64_t)rows * (D + 2);
-  const float* p = A.part + ((int64_t)b.slot * hkv + h) * size;
-  const int64_t step = (int64_t)b.step * hkv * size;
-  const float* ml = p + rows * D + pr * 2;
-  float top = -INFINITY;
-  for (int i = 0; i < b.parts; ++i) top = fmaxf(top, ml[i * step]);
-  const float ref = top == -INFINITY ? 0.f : top;
-  float sum = 0.f;
-  f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-  for (int i = 0; i < b.parts; ++i) {
-    const f32x2 own = *reinterpret_cast<const f32x2*>(ml + i * step);
-    const f32x4 x = *reinterpret_cast<const f32x4*>(p + i * step + pr * D + ch * 4);
-    const float wt = fast_exp2(own[0] - ref);
-    sum = __builtin_fmaf(own[1], wt, sum);
+  // One of several chunks lies in up to three slots: candidate i is slot i % 3 of
+  // chunk i / 3's.
+  const int candidates = rq.chunks > 1 ? rq.chunks * 3 : pl.parts / 2;
+  auto part_at = [&](int i) -> int {  // the candidate's partial result, or -1
+    if (i >= candidates) return -1;
+    if (rq.chunks == 1) return 2 * (pl.tile + i) + (i == 0 ? pl.parts % 2 : 0);
+    const int chunk = i / 3, t0 = chunk_tile(rq, chunk), n = chunk_tiles(rq, chunk);
+    const int64_t start = rq.base + (int64_t)t0 * rq.blocks + (int64_t)pl.block * n;
+    const int64_t s = start / share + i % 3;
+    return s * share < start + n ? (int)(2 * s + (start > s * share)) : -1;
+  };
+  // the next N live parts' results
+  auto take = [&](auto& p, int part, uint64_t& live) {
+    constexpr int N = sizeof(p) / sizeof(p[0]);
+    int n = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[e], wt, o[e]);
+    for (int i = 0; i < N; ++i) {
+      const int from = live ? __builtin_ctzll(live) : 0;
+      if (live) n = i + 1;
+      p[i] = live ? A.part + ((int64_t)__builtin_amdgcn_readlane(part, from) * hkv + h) * size : p[0];
+      live &= live - 1;
+    }
+    return n;
+  };
+
+  const int all = part_at(lane);
+  uint64_t live = __builtin_amdgcn_ballot_w64(all >= 0);
+  if (candidates <= kWave && __builtin_popcountll(live) <= 8) {
+    auto rows_at_once = [&](auto P_) {
+      constexpr int P = decltype(P_)::value, G = 8 / P;
+      const float* p[P];
+      const int n = take(p, all, live);
+      for (int r0 = (blockIdx.y * W + wave) * RPW * G; r0 < n_rows; r0 += gridDim.y * W * RPW * G) {
+        f32x4 x[G][P];
+        f32x2 own[G][P];
+#pragma unroll
+        for (int k = 0; k < G; ++k) {
+          const int pr = min(r0 + k * RPW + lane / LPR, n_rows - 1);
+#pragma unroll
+          for (int i = 0; i < P; ++i) {
+            x[k][i] = *reinterpret_cast<const f32x4*>(p[i] + pr * D + ch * 4);
+            own[k][i] = *reinterpret_cast<const f32x2*>(p[i] + rows * D + pr * 2);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < G; ++k) {
+          const int pr = r0 + k * RPW + lane / LPR;
+          float top = -INFINITY, sum = 0.f;
+          f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+          join(top, sum, o, x[k], own[k], n);
+          if (pr < n_rows) store_row<T>(A, rq, h, row0 + pr, ch * 4, o, top, sum, ch == 0);
+        }
+      }
+    };
+    const int n = __builtin_popcountll(live);
+    if (n <= 2) rows_at_once(std::integral_constant<int, 2>{});
+    else if (n <= 4) rows_at_once(std::integral_constant<int, 4>{});
+    else rows_at_once(std::integral_constant<int, 8>{});
+    return;
   }
-  store_row<T>(A, rq, h, row, ch * 4, o, top, sum, ch == 0);
+  for (int r0 = blockIdx.y * RPW; r0 < n_rows; r0 += gridDim.y * RPW) {
+    const int pr = min(r0 + lane / LPR, n_rows - 1);
+    float top = -INFINITY, sum = 0.f;
+    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i0 = 0; i0 < candidates; i0 += kWave * W) {
+      const int mine = part_at(i0 + lane * W + wave);
+      live = __builtin_amdgcn_ballot_w64(mine >= 0);
+      while (live) {
+        const float* p[8];
+        const int n = take(p, mine, live);
+        f32x4 x[8];
+        f32x2 own[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (i >= n) break;
+          x[i] = *reinterpret_cast<const f32x4*>(p[i] + pr * D + ch * 4);
+          own[i] = *reinterpret_cast<const f32x2*>(p[i] + rows * D + pr * 2);
+        }
+        join(top, sum, o, x, own, n);
+      }
+    }
+    s_o[wave][lane] = o;
+    s_ml[wave][lane] = f32x2{top, sum};
+    __syncthreads();
+    if (wave == 0) {
+      f32x4 x[W];
+      f32x2 own[W];
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        x[w] = s_o[w][lane];
+        own[w] = s_ml[w][lane];
+      }
+      top = -INFINITY;
+      sum = 0.f;
+      o = f32x4{0.f, 0.f, 0.f, 0.f};
+      join(top, sum, o, x, own, W);
+      if (r0 + lane / LPR < n_rows) store_row<T>(A, rq, h, row0 + pr, ch * 4, o, top, sum, ch == 0);
+    }
+    __syncthreads();
+  }
 }
 
-template <typename T, int D, int C>
+template <typename T, int D, int R>
 int launch(const Args& a, const Layout& l, hipStream_t s) {
   const int hkv = a.want.hkv;
-  const int64_t grid = 8 % hkv == 0 ? 8ll * ((l.max_items + 8 / hkv - 1) / (8 / hkv)) : (int64_t)l.max_items * hkv;
-  constexpr int threads = D == 256 ? 128 : 256;
-  if (a.want.page_size % 16 == 0)
-    hipLaunchKernelGGL((tree_kernel<T, D, C, true>), dim3((unsigned)grid), dim3(threads), 0, s, a);
+  const int64_t grid = ((int64_t)l.slots * hkv + 7) / 8 * 8;
+  // (32-bit offsets within 16 tokens)
+  if (a.want.page_size % 16 == 0 && a.token_stride >= 0 && a.token_stride < (1 << 26))
+    hipLaunchKernelGGL((tree_kernel<T, D, R, true>), dim3((unsigned)grid), dim3(threads_of(R, D)), 0, s, a);
   else
-    hipLaunchKernelGGL((tree_kernel<T, D, C, false>), dim3((unsigned)grid), dim3(threads), 0, s, a);
+    hipLaunchKernelGGL((tree_kernel<T, D, R, false>), dim3((unsigned)grid), dim3(threads_of(R, D)), 0, s, a);
   PL_LAUNCH_CHECK("tree_kernel");
-  const int per = 256 / (D / 4);
-  hipLaunchKernelGGL((merge_kernel<T, D>), dim3((unsigned)(l.max_blocks * hkv), (l.rows + per - 1) / per), dim3(256), 0,
-                     s, a, l.rows);
+  // A slot's end falls into one row block.  A workgroup for every few rows, and
+  // fewer where row blocks are many: 2,048 empty ones take 5 us.
+  const int g = a.want.hq / hkv, blocks = (int)(((int64_t)a.want.max_tree * g + R - 1) / R);
+  const int shared = (int)std::min<int64_t>(l.slots, (int64_t)a.want.batch * blocks);
+  const int rows = kWave / (D / 4), across = std::max(1, std::min(R / rows, 512 / (shared * hkv)));
+  hipLaunchKernelGGL((merge_kernel<T, D>), dim3((unsigned)(shared * hkv), across), dim3(256), 0, s, a, R);
   PL_LAUNCH_CHECK("tree merge_kernel");
   return ok();
 }
 
 template <typename T, int D>
-int launch_cols(const Args& a, const Layout& l, hipStream_t s) {
-  if (l.rows == 16) return launch<T, D, 1>(a, l, s);
-  if (l.rows == 32) return launch<T, D, 2>(a, l, s);
-  if constexpr (D != 256) return launch<T, D, 4>(a, l, s);
-  return fail(PL_ERR_UNSUPPORTED, "tree rows %d", l.rows);
+int launch_rows(const Args& a, const Layout& l, hipStream_t s) {
+  if (l.rows == 16) return launch<T, D, 16>(a, l, s);
+  if (l.rows == 32) return launch<T, D, 32>(a, l, s);
+  return launch<T, D, 64>(a, l, s);
 }
 
 template <typename T>
 int launch_dim(const Args& a, const Layout& l, hipStream_t s) {
   switch (a.want.head_dim) {
-    case 64: return launch_cols<T, 64>(a, l, s);
-    case 128: return launch_cols<T, 128>(a, l, s);
-    default: return launch_cols<T, 256>(a, l, s);
+    case 64: return launch_rows<T, 64>(a, l, s);
+    case 128: return launch_rows<T, 128>(a, l, s);
+    default: return launch_rows<T, 256>(a, l, s);
   }
 }
 
@@ -836,6 +1048,21 @@ inline int check_sizes(int batch, int tokens, int max_tree, int indices_capacity
   return PL_OK;
 }
 
+inline Header wanted(int batch, int tokens, int max_tree, int indices_capacity, int hq, int hkv, int head_dim,
+                     int page_size) {
+  Header h{};
+  h.magic = kMagic;
+  h.batch = batch;
+  h.tokens = tokens;
+  h.max_tree = max_tree;
+  h.indices_capacity = indices_capacity;
+  h.hq = hq;
+  h.hkv = hkv;
+  h.head_dim = head_dim;
+  h.page_size = page_size;
+  return h;
+}
+
 }  // namespace tree
 }  // namespace pl
 
@@ -852,13 +1079,13 @@ extern "C" size_t pl_tree_workspace_size(int batch, int tokens, int max_tree, in
                                          int head_dim) {
   if (check_sizes(batch, tokens, max_tree, 0, num_qo_heads, num_kv_heads, head_dim, 1) != PL_OK) return 0;
   const Layout l = layout(batch, tokens, max_tree, 0, num_qo_heads, num_kv_heads, head_dim);
-  return (size_t)l.max_items * num_kv_heads * l.rows * (head_dim + 2) * sizeof(float);
+  return workspace_bytes(l, num_kv_heads, head_dim);
 }
 
 extern "C" int pl_tree_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices,
                             int num_indices, const int32_t* kv_last_page_len, int batch, int tokens, int max_tree,
                             const int32_t* tree_parents, const uint8_t* tree_mask, int64_t mask_ld, int num_qo_heads,
-                            int num_kv_heads, int head_dim, int page_size, int parts, int indices_capacity, void* plan,
+                            int num_kv_heads, int head_dim, int page_size, int min_share, int indices_capacity, void* plan,
                             size_t plan_bytes, void* stream) {
   if (int st = check_sizes(batch, tokens, max_tree, indices_capacity, num_qo_heads, num_kv_heads, head_dim, page_size))
     return st;
@@ -871,8 +1098,7 @@ extern "C" int pl_tree_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, 
   if (!tree_parents == !tree_mask) return fail(PL_ERR_INVALID, "give tree_parents or tree_mask, and not both");
   if (tree_mask && mask_ld < max_tree)
     return fail(PL_ERR_INVALID, "mask_ld (%lld) must be at least max_tree (%d)", (long long)mask_ld, max_tree);
-  if (parts < 0 || parts > kCandidates)
-    return fail(PL_ERR_INVALID, "parts must be in [0, %d] (got %d)", kCandidates, parts);
+  if (min_share < 0) return fail(PL_ERR_INVALID, "min_share must be >= 0 (got %d)", min_share);
   if ((uintptr_t)plan % 16) return fail(PL_ERR_INVALID, "plan must be 16-byte aligned");
   const Layout l = layout(batch, tokens, max_tree, indices_capacity, num_qo_heads, num_kv_heads, head_dim);
   if (plan_bytes < l.bytes) return fail(PL_ERR_WORKSPACE, "tree plan of %zu bytes < %zu needed", plan_bytes, l.bytes);
@@ -887,26 +1113,17 @@ extern "C" int pl_tree_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, 
   a.mask_ld = mask_ld;
   a.header = (Header*)base;
   a.requests = (Request*)(base + l.requests);
-  a.blocks = (RowBlock*)(base + l.blocks);
-  a.items = (Item*)(base + l.items);
+  a.first = (Place*)(base + l.first);
+  a.shared = (Place*)(base + l.shared);
   a.masks = (uint64_t*)(base + l.masks);
   a.indices = (int32_t*)(base + l.indices);
-  a.batch = batch;
-  a.tokens = tokens;
-  a.max_tree = max_tree;
+  a.want = wanted(batch, tokens, max_tree, indices_capacity, num_qo_heads, num_kv_heads, head_dim, page_size);
   a.indices_count = num_indices;
-  a.indices_capacity = indices_capacity;
-  a.hq = num_qo_heads;
-  a.hkv = num_kv_heads;
-  a.head_dim = head_dim;
-  a.page_size = page_size;
   a.rows = l.rows;
   a.tile = tile_of(head_dim);
   a.slots = l.slots;
-  a.max_items = l.max_items;
-  a.max_blocks = l.max_blocks;
   a.mask_words = l.mask_words;
-  a.parts_fixed = parts;
+  a.min_share = min_share;
   const int64_t side = std::max<int64_t>(num_indices, (int64_t)tokens * l.mask_words);
   const int grid = 1 + (int)std::min<int64_t>(255, (side + kPlanThreads - 1) / kPlanThreads);
   hipLaunchKernelGGL(plan_kernel, dim3(grid), dim3(kPlanThreads), 0, (hipStream_t)stream, a);
@@ -919,7 +1136,7 @@ extern "C" int pl_tree_run(const void* q, int64_t q_stride_t, int64_t q_stride_h
                            int64_t num_pages, void* o, int64_t o_stride_t, int64_t o_stride_h, float* lse, int batch,
                            int tokens, int max_tree, int num_qo_heads, int num_kv_heads, int head_dim, int page_size,
                            float sm_scale, int dtype, const void* plan, size_t plan_bytes, int indices_capacity,
-                           void* workspace, size_t workspace_bytes, void* stream) {
+                           void* workspace, size_t workspace_size, void* stream) {
   if (int st = check_sizes(batch, tokens, max_tree, indices_capacity, num_qo_heads, num_kv_heads, head_dim, page_size))
     return st;
   if (dtype != PL_DTYPE_BF16 && dtype != PL_DTYPE_F16)
@@ -938,9 +1155,9 @@ extern "C" int pl_tree_run(const void* q, int64_t q_stride_t, int64_t q_stride_h
   if ((uintptr_t)o % 8) return fail(PL_ERR_INVALID, "o must be 8-byte aligned");
   const Layout l = layout(batch, tokens, max_tree, indices_capacity, num_qo_heads, num_kv_heads, head_dim);
   if (plan_bytes < l.bytes) return fail(PL_ERR_WORKSPACE, "tree plan of %zu bytes < %zu needed", plan_bytes, l.bytes);
-  const size_t need = (size_t)l.max_items * num_kv_heads * l.rows * (head_dim + 2) * sizeof(float);
-  if (workspace_bytes < need)
-    return fail(PL_ERR_WORKSPACE, "tree workspace of %zu bytes < %zu needed", workspace_bytes, need);
+  const size_t need = workspace_bytes(l, num_kv_heads, head_dim);
+  if (workspace_size < need)
+    return fail(PL_ERR_WORKSPACE, "tree workspace of %zu bytes < %zu needed", workspace_size, need);
   const char* base = (const char*)plan;
   Args a{};
   a.q = (const char*)q;
@@ -951,8 +1168,8 @@ extern "C" int pl_tree_run(const void* q, int64_t q_stride_t, int64_t q_stride_h
   a.part = (float*)workspace;
   a.header = (const Header*)base;
   a.requests = (const Request*)(base + l.requests);
-  a.blocks = (const RowBlock*)(base + l.blocks);
-  a.items = (const Item*)(base + l.items);
+  a.first = (const Place*)(base + l.first);
+  a.shared = (const Place*)(base + l.shared);
   a.masks = (const uint64_t*)(base + l.masks);
   a.indices = (const int32_t*)(base + l.indices);
   a.q_st = q_stride_t;
@@ -963,17 +1180,10 @@ extern "C" int pl_tree_run(const void* q, int64_t q_stride_t, int64_t q_stride_h
   a.token_stride = token_stride;
   a.head_stride = head_stride;
   a.num_pages = num_pages;
-  a.want.batch = batch;
-  a.want.tokens = tokens;
-  a.want.max_tree = max_tree;
-  a.want.indices_capacity = indices_capacity;
-  a.want.hq = num_qo_heads;
-  a.want.hkv = num_kv_heads;
-  a.want.head_dim = head_dim;
-  a.want.page_size = page_size;
-  a.max_items = l.max_items;
-  a.max_blocks = l.max_blocks;
+  a.want = wanted(batch, tokens, max_tree, indices_capacity, num_qo_heads, num_kv_heads, head_dim, page_size);
+  a.slots = l.slots;
   a.mask_words = l.mask_words;
+  a.once = (int64_t)max_tree * (num_qo_heads / num_kv_heads) <= l.rows;
   // the kernel takes maxima before scaling: a positive scale (a zero one as
   // one far below any score's rounding), the sign moved into q
   const float s2 = sm_scale * 1.44269504088896340736f;

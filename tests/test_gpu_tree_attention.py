@@ -120,12 +120,12 @@ def test_page_sizes(gpu_device, page_size, dtype):
     check(case, out, lse, dtype)
 
 
-@pytest.mark.parametrize("parts", [0, 1, 2, 7, 128])
+@pytest.mark.parametrize("min_share", [0, 2, 3, 1000])
 @pytest.mark.parametrize("kv_len", [31, 127, 128, 129, 1000, 5000])
-def test_split_ranges(gpu_device, parts, kv_len):
-    """The kv range cut into parts, at the edges of blocks and tiles."""
+def test_split_ranges(gpu_device, min_share, kv_len):
+    """The kv range cut into shares of several sizes, at the edges of blocks and tiles."""
     case = tree_case([9, 2], [kv_len, 50], 8, 2, 128, 16, BF16, gpu_device, seed=kv_len)
-    out, lse = run(case, 8, 2, 128, 16, gpu_device, parts=parts)
+    out, lse = run(case, 8, 2, 128, 16, gpu_device, min_share=min_share)
     check(case, out, lse)
 
 
@@ -299,6 +299,34 @@ def test_matches_causal_prefill_on_a_chain(gpu_device):
     be.plan_tree(**tables(case), tree_parents=case["parents"])
     b = be.run_tree(case["q"], case["cache"]).float()
     assert ((a - b).abs() <= 2.0**-7 * a.abs() + 1e-4).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+@pytest.mark.parametrize("n", [2, 9, 17, 60, 130, 300])
+def test_row_blocks_of_every_size(gpu_device, head_dim, n, dtype):
+    """16 to 256 rows of a row block, several per request, shares that begin and end inside them."""
+    case = tree_case([n, 3, n // 2], [n + 1500, 3, 900], 2, 1, head_dim, 16, dtype, gpu_device, seed=n)
+    out, lse = run(case, 2, 1, head_dim, 16, gpu_device)
+    check(case, out, lse, dtype)
+    out, lse = run(case, 2, 1, head_dim, 16, gpu_device, min_share=5)
+    check(case, out, lse, dtype)
+
+
+@pytest.mark.parametrize("n", [20, 50, 120, 250])
+def test_row_blocks_of_every_size_masked_values(gpu_device, n):
+    """Infinities and NaN in nodes, for each number of waves per block."""
+    for bad in (float("nan"), float("inf")):
+        case = tree_case([n], [n + 45], 1, 1, 128, 16, BF16, gpu_device, seed=n)
+        ip, ind = case["indptr"].tolist(), case["indices"].tolist()
+        for j in (3, n // 2, n - 1):
+            case["cache_host"][ind[ip[0] + (45 + j) // 16], :, (45 + j) % 16] = bad
+        case["cache"] = case["cache_host"].to(gpu_device)
+        out, _ = run(case, 1, 1, 128, 16, gpu_device)
+        touched = case["sees"][0][:, [3, n // 2, n - 1]].any(axis=1)
+        got, ref = out.double().cpu().numpy(), oracle(case)[0]
+        assert np.isfinite(got[~touched]).all() and not np.isfinite(got[touched]).any()
+        assert (np.abs(got - ref)[~touched] <= 2.0**-7 * np.abs(ref[~touched]) + 0.01).all()
 
 
 def test_many_requests(gpu_device):

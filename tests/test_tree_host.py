@@ -53,7 +53,7 @@ def test_plan_tree_needs_a_device():
 
 def plan(**kw):
     a = dict(qo=PTR, kv=PTR, ind=PTR, n=3, last=PTR, batch=2, tokens=3, max_tree=2, parents=PTR, mask=None, ld=0, hq=4,
-             hkv=2, d=64, page=16, parts=0, cap=16, buf=PTR, size=1 << 30, stream=None)
+             hkv=2, d=64, page=16, share=0, cap=16, buf=PTR, size=1 << 30, stream=None)
     return _lib.load().pl_tree_plan(*{**a, **kw}.values())
 
 
@@ -61,7 +61,7 @@ def plan(**kw):
     (dict(batch=-1), 1), (dict(tokens=-1), 1), (dict(hkv=3), 1), (dict(hkv=0), 1), (dict(d=96), 2), (dict(page=0), 1),
     (dict(page=65537), 1), (dict(batch=4097), 2), (dict(max_tree=4), 1), (dict(tokens=1 << 27, hq=4), 2), (dict(n=17), 1),
     (dict(n=-1), 1), (dict(qo=None), 1), (dict(buf=None), 1), (dict(ind=None), 1), (dict(mask=PTR, ld=4), 1),
-    (dict(parents=None), 1), (dict(parents=None, mask=PTR, ld=1), 1), (dict(parts=-1), 1), (dict(parts=129), 1),
+    (dict(parents=None), 1), (dict(parents=None, mask=PTR, ld=1), 1), (dict(share=-1), 1),
     (dict(buf=PTR + 8), 1), (dict(size=64), 3),
 ])
 def test_pl_tree_plan_refuses(kw, status):
@@ -94,9 +94,9 @@ def test_pl_tree_run_of_nothing():
 
 def test_sizes_hold_what_is_planned():
     lib = _lib.load()
-    # header, requests, masks and indices at the least; partial results of 3 slots a head
-    assert lib.pl_tree_plan_size(64, 1024, 16, 40000, 32, 8, 128) >= 64 + 64 * 16 + 1024 * 8 + 40000 * 4
-    assert lib.pl_tree_workspace_size(1, 8, 8, 32, 8, 128) >= 3 * 32 * 8 * 32 * 130 * 4
+    # header, masks and indices at the least; two partial results of each of 256 slots
+    assert lib.pl_tree_plan_size(64, 1024, 16, 40000, 32, 8, 128) >= 64 + 1024 * 8 + 40000 * 4
+    assert lib.pl_tree_workspace_size(1, 8, 8, 32, 8, 128) >= 2 * 256 * 32 * 130 * 4
     assert lib.pl_tree_plan_size(1, 8, 8, 16, 32, 8, 96) == 0 and lib.pl_tree_workspace_size(1, 8, 9, 32, 8, 128) == 0
 
 
