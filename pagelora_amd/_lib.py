@@ -6,6 +6,7 @@ or torch fallback behind any entry point of this package.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
 from pathlib import Path
@@ -477,9 +478,22 @@ def stream_handle(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def on_device(device):
-    """Context in which ``device`` is the current one, as a launch on a stream of it needs."""
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def on_device(index: int):
+    """Context in which CUDA device ``index`` is the current one, as a launch on a stream of it needs."""
 
     import torch
 
-    return torch.cuda.device(device)
+    return _NO_GUARD if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+
+def raw_stream(index: int) -> int:
+    """:func:`stream_handle` for a device index, without a Stream object where torch has the call (0.1 us, not 1.8)."""
+
+    import torch
+
+    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return get(index) if get is not None else torch.cuda.current_stream(index).cuda_stream

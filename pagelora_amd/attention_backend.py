@@ -152,6 +152,23 @@ def _cache_geometry(cache, num_kv_heads: int, head_dim: int, page_size: int):
     return cache[:, 0], cache[:, 1], cache.stride(0), cache.stride(2), cache.stride(3), cache.shape[0]
 
 
+def _cache_pointers(cache, num_kv_heads: int, head_dim: int, page_size: int):
+    """:func:`_cache_geometry` as numbers, without views of the cache: (K and V
+    addresses, page/token/head stride, num_pages, dtype, device index)."""
+
+    if isinstance(cache, (tuple, list)):
+        k, v, page_stride, token_stride, head_stride, num_pages = _cache_geometry(cache, num_kv_heads, head_dim,
+                                                                                  page_size)
+        device = k.get_device() if k.get_device() == v.get_device() else -1
+        return k.data_ptr(), v.data_ptr(), page_stride, token_stride, head_stride, num_pages, k.dtype, device
+    shape = cache.shape
+    if len(shape) != 5 or shape[1:] != (2, page_size, num_kv_heads, head_dim) or cache.stride(4) != 1:
+        _cache_geometry(cache, num_kv_heads, head_dim, page_size)  # says what is wrong
+    strides, k_ptr = cache.stride(), cache.data_ptr()
+    return (k_ptr, k_ptr + strides[1] * cache.element_size(), strides[0], strides[2], strides[3], shape[0],
+            cache.dtype, cache.get_device())
+
+
 class PagedDecodeAttention:
     """gfx950 paged decode attention with the FlashInferAttentionBackend surface.
 
@@ -822,7 +839,8 @@ class PagedDecodeAttention:
         if self.device.type != "cuda":
             raise RuntimeError("PagedDecodeAttention.plan_tree needs a ROCm device")
 
-        with _lib.on_device(self.device):
+        index = self._device_index()
+        with _lib.on_device(index):
             if host:
                 if torch.cuda.is_current_stream_capturing():
                     raise RuntimeError("plan_tree with host tables uploads them and cannot be captured")
@@ -832,7 +850,7 @@ class PagedDecodeAttention:
                     tables = _upload_int32(tables, self.device)
                     tree = tree.contiguous().to(self.device)
             else:
-                if any(not self._here(t) for t in (*tables, tree)):
+                if any(t.get_device() != index for t in (*tables, tree)):
                     raise ValueError(f"tree tables must be on {self.device}")
                 tables = [t.contiguous() for t in tables]
                 tree = tree.contiguous()
@@ -853,19 +871,20 @@ class PagedDecodeAttention:
                 buffer.data_ptr(), buffer.numel(), stream.cuda_stream), "pl_tree_plan")
             captured = torch.cuda.is_current_stream_capturing()
             self._tree_plan = {
+                "device": index,
                 "sizes": sizes,
                 "tokens": tokens,
                 "capacity": capacity,
                 "buffer": buffer,
+                "buffer_args": (buffer.data_ptr(), buffer.numel()),
                 "workspace_bytes": self._lib.pl_tree_workspace_size(*sizes, *heads),
                 "max_page": max_page,
                 "stream": stream.cuda_stream,
                 "ready": None if captured else stream.record_event(),
             }
 
-    def _here(self, t: torch.Tensor) -> bool:
-        index = torch.cuda.current_device() if self.device.index is None else self.device.index
-        return t.device.type == "cuda" and t.device.index == index
+    def _device_index(self) -> int:
+        return self.workspace_buffer.get_device()
 
     def _tree_buffer(self, nbytes: int) -> torch.Tensor:
         """The plan buffer of a size class.  One per class lives as long as the
@@ -919,40 +938,42 @@ class PagedDecodeAttention:
         plan = getattr(self, "_tree_plan", None)
         if plan is None:
             raise RuntimeError("plan_tree must be called before run_tree")
-        if q.dim() != 3 or tuple(q.shape[1:]) != (self.num_qo_heads, self.head_dim):
-            raise ValueError(f"q must be [tokens, {self.num_qo_heads}, {self.head_dim}], got {tuple(q.shape)}")
-        if q.shape[0] != plan["tokens"]:
-            raise ValueError(f"q has {q.shape[0]} tokens but the plan has {plan['tokens']}")
-        if tuple(out.shape) != tuple(q.shape) or out.dtype != q.dtype or q.stride(2) != 1 or out.stride(2) != 1:
+        shape, dtype, device = q.shape, q.dtype, plan["device"]
+        if len(shape) != 3 or shape[1] != self.num_qo_heads or shape[2] != self.head_dim:
+            raise ValueError(f"q must be [tokens, {self.num_qo_heads}, {self.head_dim}], got {tuple(shape)}")
+        if shape[0] != plan["tokens"]:
+            raise ValueError(f"q has {shape[0]} tokens but the plan has {plan['tokens']}")
+        qs, os_ = q.stride(), out.stride()
+        if out.shape != shape or out.dtype != dtype or qs[2] != 1 or os_[2] != 1:
             raise ValueError("q and out must match in shape/dtype with a contiguous head_dim")
-        k, v, page_stride, token_stride, head_stride, num_pages = _cache_geometry(
+        k_ptr, v_ptr, page_stride, token_stride, head_stride, num_pages, kv_dtype, kv_device = _cache_pointers(
             paged_kv_cache_layer, self.num_kv_heads, self.head_dim, self.page_size
         )
-        if k.dtype != q.dtype:
-            raise ValueError(f"q dtype {q.dtype} != KV cache dtype {k.dtype}")
+        if kv_dtype != dtype:
+            raise ValueError(f"q dtype {dtype} != KV cache dtype {kv_dtype}")
         if plan["max_page"] is not None and plan["max_page"] >= num_pages:
             raise ValueError(f"page id {plan['max_page']} is outside the {num_pages}-page KV pool")
-        if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != tuple(q.shape[:2])
-                                or not lse.is_contiguous()):
+        if lse is not None and (lse.dtype != torch.float32 or lse.shape != shape[:2] or not lse.is_contiguous()):
             raise ValueError("lse must be a contiguous fp32 [tokens, Hq] tensor")
-        if not all(self._here(t) for t in (q, k, v, out) + ((lse,) if lse is not None else ())):
+        if (q.get_device() != device or out.get_device() != device or kv_device != device
+                or (lse is not None and lse.get_device() != device)):
             raise RuntimeError(f"run_tree needs tensors on the backend's device {self.device}")
-        with _lib.on_device(q.device):
-            stream = torch.cuda.current_stream(q.device)
-            if stream.cuda_stream != plan["stream"] and plan["ready"] is not None \
+        with _lib.on_device(device):
+            stream = _lib.raw_stream(device)
+            if stream != plan["stream"] and plan["ready"] is not None \
                     and not torch.cuda.is_current_stream_capturing():
-                stream.wait_event(plan["ready"])
+                torch.cuda.current_stream(device).wait_event(plan["ready"])
             # per call, from torch's allocator: calls on other streams and graphs share nothing
-            ws = torch.empty(plan["workspace_bytes"], dtype=torch.uint8, device=q.device)
+            nbytes = plan["workspace_bytes"]
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
             status = self._lib.pl_tree_run(
-                q.data_ptr(), q.stride(0), q.stride(1),
-                k.data_ptr(), v.data_ptr(), page_stride, token_stride, head_stride,
+                q.data_ptr(), qs[0], qs[1],
+                k_ptr, v_ptr, page_stride, token_stride, head_stride,
                 num_pages,
-                out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr() if lse is not None else None,
+                out.data_ptr(), os_[0], os_[1], lse.data_ptr() if lse is not None else None,
                 *plan["sizes"], self.num_qo_heads, self.num_kv_heads, self.head_dim, self.page_size,
-                self.sm_scale, _lib.dtype_code(q.dtype),
-                plan["buffer"].data_ptr(), plan["buffer"].numel(), plan["capacity"],
-                ws.data_ptr(), ws.numel(), stream.cuda_stream,
+                self.sm_scale, _lib.dtype_code(dtype),
+                *plan["buffer_args"], plan["capacity"], ws.data_ptr(), nbytes, stream,
             )
             _lib.check(status, "pl_tree_run")
         return out

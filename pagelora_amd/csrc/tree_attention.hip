@@ -53,21 +53,24 @@ typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 // What a plan was made for, then what it holds.
 struct Header {
   int32_t magic, batch, tokens, max_tree, indices_capacity, hq, hkv, head_dim, page_size;
-  int32_t num_requests, num_slots, num_shared, pad[2];
+  int32_t num_requests, num_slots, num_shared, chunk_per_slot, pad;
   int64_t share;  // tiles of a slot
 };
 static_assert(sizeof(Header) == 64, "the plan's header");
 // A request with nodes.  Its work is tiles x blocks (row blocks), from `base` of
 // all work on: chunk after chunk of its tiles, of a chunk row block after row
-// block.  The first `longer` chunks have chunk_len + 1 tiles, the others
-// chunk_len; where there are several, none is less than a share.
+// block.  The first `longer` chunks have chunk_len + 1 tiles, the others chunk_len.
+// Either every chunk of a row block is a slot's (`base` and all work then count
+// those), or only requests of several row blocks have several chunks, none less
+// than a share.
 struct Request {
   int32_t q_begin, tree, page_begin, kv_len, blocks, chunks, chunk_len, longer, index, pad;
   int64_t base;
 };
 // A place in the work: of a row block (`block`) in a chunk, after `tile` tiles of
-// it.  Of a row block that slots share: the slots of its one chunk, times two,
-// and whether the first one's second partial result is of it.
+// it.  Of a row block that slots share: in `tile` the slot of its first part, in
+// `parts` the slots of its one chunk, times two, and whether the first one's
+// second partial result is of it.
 struct Place {
   Request rq;
   int32_t chunk, block, tile, parts;
@@ -159,10 +162,15 @@ __device__ __forceinline__ int chunk_tile(const Request& q, int chunk) {
 }
 __device__ __forceinline__ int chunk_tiles(const Request& q, int chunk) { return q.chunk_len + (chunk < q.longer); }
 
-// The place at x of the request's own work.
-__device__ __forceinline__ Place place_at(const Request& q, int64_t x) {
+// The place at x of the request's own work; `single`: the x-th chunk of a row block.
+__device__ __forceinline__ Place place_at(const Request& q, int64_t x, bool single) {
   Place p{};
   p.rq = q;
+  if (single) {
+    p.chunk = (int)(x / q.blocks);
+    p.block = (int)(x % q.blocks);
+    return p;
+  }
   const int64_t longer = (int64_t)q.longer * (q.chunk_len + 1) * q.blocks;
   p.chunk = q.chunks == 1 ? 0
             : x < longer  ? (int)(x / ((int64_t)(q.chunk_len + 1) * q.blocks))
@@ -213,104 +221,114 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs A) {
   // The work before each request: a thread owns a run of requests, and the
   // threads' sums are added up over the wave, then over the waves.
   __shared__ long long s_base[kMaxRequests];  // of the n-th request with nodes
-  __shared__ long long s_wave_work[kPlanThreads / kWave];
-  __shared__ int s_wave_live[kPlanThreads / kWave];
+  __shared__ long long s_wave[kPlanThreads / kWave];
   const int lane = tid % kWave, wave = tid / kWave;
   const int per = (batch + kPlanThreads - 1) / kPlanThreads;
   const int r0 = min(batch, tid * per), r1 = min(batch, r0 + per);
-  long long work = 0;
-  int live = 0;
+  // sums over all threads, and those before this one
+  auto scan = [&](long long& before, long long& total, long long v) {
+    long long upto = v;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+      const long long t = __shfl_up(upto, d);
+      if (lane >= d) upto += t;
+    }
+    if (lane == kWave - 1) s_wave[wave] = upto;
+    __syncthreads();
+    before = upto - v;
+    total = 0;
+    for (int w = 0; w < kPlanThreads / kWave; ++w) {
+      if (w < wave) before += s_wave[w];
+      total += s_wave[w];
+    }
+    __syncthreads();
+  };
+  long long work = 0, live = 0;
   for (int r = r0; r < r1; ++r) {
     const Request q = read_request(A, r);
     work += (long long)q.chunk_len * q.blocks;
     live += q.blocks > 0;
   }
-  long long work_upto = work;
-  int live_upto = live;
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const long long t = __shfl_up(work_upto, d);
-    const int n = __shfl_up(live_upto, d);
-    if (lane >= d) {
-      work_upto += t;
-      live_upto += n;
+  long long base, index, total, n_live;
+  scan(base, total, work);
+  scan(index, n_live, live);
+  long long share = max((long long)max(A.min_share, 1), (total + A.slots - 1) / A.slots);
+  // A slot for every chunk of a row block saves the slots that would work on two:
+  // taken where the chunks so need no more than an eighth longer.
+  bool single = false;
+  for (int i = 0; i < 4 && !single; ++i) {
+    const long long at = share + share * i / 24;
+    long long chunks = 0, before, all;
+    for (int r = r0; r < r1; ++r) {
+      const Request q = read_request(A, r);
+      chunks += (q.chunk_len + at - 1) / at * q.blocks;
+    }
+    scan(before, all, chunks);
+    if (all <= A.slots) {
+      single = true;
+      share = at;
+      base = before;
+      total = all;
     }
   }
-  if (lane == kWave - 1) {
-    s_wave_work[wave] = work_upto;
-    s_wave_live[wave] = live_upto;
-  }
-  __syncthreads();
-  long long total = 0, base = work_upto - work;
-  int n_live = 0, index = live_upto - live;
-  for (int w = 0; w < kPlanThreads / kWave; ++w) {
-    if (w < wave) {
-      base += s_wave_work[w];
-      index += s_wave_live[w];
-    }
-    total += s_wave_work[w];
-    n_live += s_wave_live[w];
-  }
-  const long long share = max((long long)max(A.min_share, 1), (total + A.slots - 1) / A.slots);
-  const int n_slots = (int)((total + share - 1) / share);
+  const int n_slots = (int)(single ? total : (total + share - 1) / share);
   for (int r = r0; r < r1; ++r) {
     Request q = read_request(A, r);
     if (q.blocks <= 0) continue;
     const long long tiles = q.chunk_len;
-    q.index = index;
+    const long long chunks = single ? (tiles + share - 1) / share : q.blocks > 1 ? max(1ll, tiles / share) : 1;
+    q.index = (int)index;
     q.base = base;
-    if (q.blocks > 1 && tiles >= 2 * share) {
-      q.chunks = (int)(tiles / share);
-      q.chunk_len = (int)(tiles / q.chunks);
-      q.longer = (int)(tiles % q.chunks);
-    }
+    q.chunks = (int)chunks;
+    q.chunk_len = (int)(tiles / chunks);
+    q.longer = (int)(tiles % chunks);
     A.requests[index] = q;
     s_base[index] = base;
-    base += tiles * q.blocks;
+    base += (single ? chunks : tiles) * q.blocks;
     ++index;
   }
   __syncthreads();
   auto locate = [&](long long x) {
-    int lo = 0, hi = n_live;  // the last request with base <= x
+    int lo = 0, hi = (int)n_live;  // the last request with base <= x
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (s_base[mid] <= x) lo = mid; else hi = mid;
     }
-    return place_at(A.requests[lo], x - s_base[lo]);
+    return place_at(A.requests[lo], x - s_base[lo], single);
   };
-  __shared__ int s_wave_shared[kPlanThreads / kWave];
-  int n_shared = 0;
+  long long n_shared = 0;
   for (int s0 = 0; s0 < n_slots; s0 += kPlanThreads) {
     const int s = s0 + tid;
     Place p{};
     if (s < n_slots) {
-      A.first[s] = locate(s * share);
-      // The row block at the slot's end is shared if it begins in the slot and does
-      // not end there, or is one of several chunks (a chunk is no less than a share)
-      const long long end = min((s + 1) * share, total);
-      p = locate(end - 1);
-      const long long start = end - 1 - p.tile;
-      const int parts = (int)((start + chunk_tiles(p.rq, 0) - 1) / share - s) + 1;
-      if (p.chunk > 0 || start < s * share || (p.rq.chunks == 1 && parts == 1)) p.rq.blocks = 0;
-      p.parts = 2 * parts + (start > s * share);
+      p = locate(single ? s : s * share);
+      A.first[s] = p;
+      if (single) {
+        if (p.chunk > 0 || p.rq.chunks == 1) p.rq.blocks = 0;
+      } else {
+        // The row block at the slot's end is shared if it begins in the slot and does
+        // not end there, or is one of several chunks (a chunk is no less than a share)
+        const long long end = min((s + 1) * share, total);
+        p = locate(end - 1);
+        const long long start = end - 1 - p.tile;
+        const int parts = (int)((start + chunk_tiles(p.rq, 0) - 1) / share - s) + 1;
+        if (p.chunk > 0 || start < s * share || (p.rq.chunks == 1 && parts == 1)) p.rq.blocks = 0;
+        p.parts = 2 * parts + (start > s * share);
+      }
       p.tile = s;
     }
-    const uint64_t mine = __builtin_amdgcn_ballot_w64(p.rq.blocks > 0);
-    if (lane == 0) s_wave_shared[wave] = __builtin_popcountll(mine);
-    __syncthreads();
-    int at = n_shared + __builtin_popcountll(mine & ((1ull << lane) - 1));
-    for (int w = 0; w < kPlanThreads / kWave; ++w) {
-      if (w < wave) at += s_wave_shared[w];
-      n_shared += s_wave_shared[w];
-    }
+    long long before, all;
+    scan(before, all, p.rq.blocks > 0);
+    const long long at = n_shared + before;
+    n_shared += all;
     if (p.rq.blocks > 0) A.shared[at] = p;
-    __syncthreads();
   }
   if (tid == 0) {
     Header h = A.want;
-    h.num_requests = n_live;
+    h.num_requests = (int)n_live;
     h.num_slots = n_slots;
-    h.num_shared = n_shared;
+    h.num_shared = (int)n_shared;
+    h.chunk_per_slot = single;
     h.share = share;
     *A.header = h;
   }
@@ -414,10 +432,10 @@ template <typename T> struct Softmax {
 
 // Finishes a row: its four dims by one lane, and the row's lse by lane `first`.
 template <typename T>
-__device__ __forceinline__ void store_row(const Args& A, const Request& q, int h, int row, int dim, f32x4 o, float top,
+__device__ __forceinline__ void store_row(const Args& A, int q_begin, int h, int row, int dim, f32x4 o, float top,
                                           float sum, bool first) {
   const int g = A.want.hq / A.want.hkv, node = row / g;
-  const int64_t token = q.q_begin + node;
+  const int64_t token = q_begin + node;
   const int head = h * g + row - node * g;
   const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
   T* op = (T*)A.o + token * A.o_st + (int64_t)head * A.o_sh + dim;
@@ -455,16 +473,23 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
   if (!plan_fits(A)) return;
   const int n_slots = A.header->num_slots, hkv = A.want.hkv;
   const int64_t share = A.header->share;
-  // Workgroups go round the 8 XCDs: with 8 heads each has one, and its L2 the row blocks of one chunk.
-  const int slot = blockIdx.x / hkv, h = blockIdx.x % hkv;
-  if (slot >= n_slots) return;
+  // Workgroups go round the 8 XCDs.  Where the heads divide 8 an XCD has one head
+  // and a run of the slots, so that the row blocks of a chunk share an L2.
+  const int runs = 8 % hkv == 0 ? 8 / hkv : 1, per = (n_slots + runs - 1) / runs;
+  const int at = blockIdx.x / (runs * hkv), h = blockIdx.x % hkv;
+  const int slot = (int)(blockIdx.x / hkv) % runs * per + at;
+  if (at >= per || slot >= n_slots) return;
+  const bool single = A.header->chunk_per_slot;
   const int n_requests = A.header->num_requests;
   Place pl = A.first[slot];
   int64_t left = share;  // tiles of the share to come
 
   const int g = A.want.hq / hkv, page_size = A.want.page_size;
   const int lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave);
-  const int blk = wave % W, rank = wave / W;  // the wave's block of a tile, its rows of the row block
+  // The wave's block of a tile, its rows of the row block.  Two waves of a block
+  // are on two SIMDs, each beside one of another block: one's softmax then runs
+  // beside the other's matrix instructions.
+  const int blk = wave / WR, rank = wave % WR;
   const int lr = lane % 16, grp = lane / 16;
   const float sc = A.scale_log2;
 
@@ -542,7 +567,7 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
       ++turn;
       asm volatile("" ::: "memory");
       if (lane == 0) __hip_atomic_store(&s_turn[wave], turn, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-      const int* other = &s_turn[(wave + W) % (W * WR)];
+      const int* other = &s_turn[wave ^ 1];
       while (uniform(__hip_atomic_load(other, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP)) < turn) {
       }
       asm volatile("" ::: "memory");
@@ -554,52 +579,90 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
     __syncthreads();
   }
 
-  for (;;) {
-    const Request& rq = pl.rq;
-    // this share's tiles of the row block
-    const int c_first = chunk_tile(rq, pl.chunk), c_tiles = chunk_tiles(rq, pl.chunk);
-    const int t_first = c_first + pl.tile, t_last = c_first + (int)min((int64_t)c_tiles, pl.tile + left);
-    const bool whole = rq.chunks == 1 && t_last - t_first == c_tiles;
-    const int row0 = pl.block * R, n_rows = rq.tree * g;
-    const int kv_len = rq.kv_len, prefix = max(0, kv_len - rq.tree);
-    const int n_pages = (kv_len + page_size - 1) / page_size;
-    const int32_t* ind = A.indices + rq.page_begin;
-    // the wave's blocks: only the last tile can lie behind its tokens
-    const int t_end = (int64_t)(t_last - 1) * kTile + blk * kBlock < kv_len ? t_last : t_last - 1;
-    // byte offset of token t of the sequence (or of the page's rest behind the last one)
-    auto token_offset = [&](int t) -> int64_t {
-      const int page = t / page_size;
-      return (clamp_page(ind[min(page, n_pages - 1)]) * A.page_stride + (int64_t)(t - page * page_size) * A.token_stride) * 2;
-    };
-    // Offsets of the block's tokens, one per lane.  Pages of a multiple of 16
-    // tokens: of the 16-token groups of 32 tiles; others: of a block's 32 tokens.
-    auto load_offsets = [&](int tile) -> int64_t {
-      if constexpr (PAGE16) return token_offset((tile + lane / 2) * kTile + blk * kBlock + (lane % 2) * 16);
-      return token_offset(min(tile * kTile + blk * kBlock + lane % kBlock, kv_len - 1));
-    };
-    int64_t offs = 0, offs_next = 0;
-    const bool any_tokens = t_first < t_end && kv_len > 0;
-    if (any_tokens) {
-      offs = load_offsets(t_first);
-      offs_next = load_offsets(t_first + (PAGE16 ? 32 : 1));
-    }
+  // What the share holds of a row block.
+  struct Segment {
+    int q_begin, page_begin, row0, n_rows, kv_len, prefix, n_pages, t_first, t_last, t_end;
+    bool whole, second;
+  };
+  auto segment_at = [&](const Place& p) {
+    const Request& rq = p.rq;
+    Segment g_;
+    const int c_first = chunk_tile(rq, p.chunk), c_tiles = chunk_tiles(rq, p.chunk);
+    g_.q_begin = rq.q_begin;
+    g_.page_begin = rq.page_begin;
+    g_.row0 = p.block * R;
+    g_.n_rows = rq.tree * g;
+    g_.kv_len = rq.kv_len;
+    g_.prefix = max(0, rq.kv_len - rq.tree);
+    g_.n_pages = (rq.kv_len + page_size - 1) / page_size;
+    g_.t_first = c_first + p.tile;
+    g_.t_last = c_first + (single ? c_tiles : (int)min((int64_t)c_tiles, p.tile + left));
+    // the block's tokens: only the last tile can lie behind them
+    g_.t_end = rq.kv_len <= 0 ? g_.t_first
+               : (int64_t)(g_.t_last - 1) * kTile + blk * kBlock < rq.kv_len ? g_.t_last : g_.t_last - 1;
+    g_.whole = rq.chunks == 1 && g_.t_last - g_.t_first == c_tiles;
+    // a slot's first partial result is of what it takes over, its second of what it hands on
+    g_.second = left < share;
+    return g_;
+  };
 
-    u32x4 qb[C][KS];
-    int nodes[C];
+  // Page ids are asked for long before their use: `id` is in flight, `rest` the
+  // byte offset within the page.
+  struct Offset {
+    int id;
+    int64_t rest;
+  };
+  // Of the block's tokens, one per lane.  Pages of a multiple of 16 tokens: of the
+  // 16-token groups of 32 tiles; others: of a block's 32 tokens.  Behind the last
+  // token it is the rest of the last page.
+  auto ask_offsets = [&](const Segment& e, int tile) {
+    const int t = PAGE16 ? (tile + lane / 2) * kTile + blk * kBlock + (lane % 2) * 16
+                         : min(tile * kTile + blk * kBlock + lane % kBlock, e.kv_len - 1);
+    const int page = t / page_size;
+    return Offset{A.indices[e.page_begin + min(page, e.n_pages - 1)], (int64_t)(t - page * page_size) * A.token_stride};
+  };
+  auto offsets = [&](const Offset& o) -> int64_t { return (clamp_page(o.id) * A.page_stride + o.rest) * 2; };
+
+  u32x4 qb[C][KS];
+  Offset ask0{}, ask1{};
+  auto ask = [&](const Segment& e) {  // queries and page ids
+    if (e.t_first < e.t_end) {
+      ask0 = ask_offsets(e, e.t_first);
+      ask1 = ask_offsets(e, e.t_first + (PAGE16 ? 32 : 1));
+    }
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int row = min(row0 + (rank * C + c) * 16 + lr, n_rows - 1);  // rows past the end repeat the last one, unstored
+      const int row = min(e.row0 + (rank * C + c) * 16 + lr, e.n_rows - 1);  // rows past the end repeat the last one, unstored
       const int node = row / g;
-      nodes[c] = rq.q_begin + node;
-      const char* qp = A.q + ((int64_t)(rq.q_begin + node) * A.q_st + (int64_t)(h * g + row - node * g) * A.q_sh) * 2 + grp * 16;
+      const char* qp = A.q + ((int64_t)(e.q_begin + node) * A.q_st + (int64_t)(h * g + row - node * g) * A.q_sh) * 2 + grp * 16;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        u32x4 v = *reinterpret_cast<const u32x4*>(qp + ks * 64);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] ^= A.q_flip;
-        qb[c][ks] = v;
+      for (int ks = 0; ks < KS; ++ks) qb[c][ks] = *reinterpret_cast<const u32x4*>(qp + ks * 64);
+    }
+  };
+
+  Segment e = segment_at(pl);
+  ask(e);
+  for (;;) {
+    // the place behind this row block
+    left -= e.t_last - e.t_first;
+    bool more = !single && left > 0;
+    pl.tile = 0;
+    if (more && ++pl.block == pl.rq.blocks) {
+      pl.block = 0;
+      if (++pl.chunk == pl.rq.chunks) {
+        pl.chunk = 0;
+        more = pl.rq.index + 1 < n_requests;
+        if (more) pl.rq = A.requests[pl.rq.index + 1];
       }
     }
+    const int kv_len = e.kv_len, prefix = e.prefix, t_first = e.t_first, t_end = e.t_end;
+    int64_t offs = offsets(ask0);
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) qb[c][ks][i] ^= A.q_flip;
     f32x4 acc[C][NA];
     float m[C], l[C];
 #pragma unroll
@@ -609,17 +672,17 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
 #pragma unroll
       for (int a = 0; a < NA; ++a) acc[c][a] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    if (any_tokens) load_block(offs, 0, 0);
+    if (t_first < t_end) load_block(offs, 0, 0);
 
-    for (int tile = t_first; tile < t_end && any_tokens; ++tile) {
+    for (int tile = t_first; tile < t_end; ++tile) {
       __builtin_amdgcn_sched_barrier(0);
       const int stage = (tile - t_first) % 2;
       meet();  // both are done with the other stage
       if (tile + 1 < t_end) {
         const int at = PAGE16 ? (tile + 1 - t_first) % 32 : 0;
         if (at == 0) {
-          offs = offs_next;
-          offs_next = load_offsets(tile + (PAGE16 ? 33 : 2));
+          offs = offsets(ask1);
+          ask1 = ask_offsets(e, tile + (PAGE16 ? 33 : 2));
         }
         load_block(offs, at, stage ^ 1);
         __builtin_amdgcn_sched_barrier(0);
@@ -639,7 +702,8 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
         const uint32_t inside = n == kBlock ? ~0u : (1u << n) - 1;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-          const uint64_t* mask = A.masks + (int64_t)nodes[c] * A.mask_words;
+          const int row = min(e.row0 + (rank * C + c) * 16 + lr, e.n_rows - 1);
+          const uint64_t* mask = A.masks + (int64_t)(e.q_begin + row / g) * A.mask_words;
           const uint64_t lo = w < 0 ? ~0ull : (w < A.mask_words ? mask[w] : 0);
           const uint64_t hi = w + 1 < 0 ? ~0ull : (w + 1 < A.mask_words ? mask[w + 1] : 0);
           vis[c] = (uint32_t)(sh ? lo >> sh | hi << (64 - sh) : lo) & inside;
@@ -790,6 +854,12 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
       }
     }
 
+    // the next row block's queries and page ids come while this one's states meet
+    const Segment was = e;
+    if (more) {
+      e = segment_at(pl);
+      ask(e);
+    }
     // the blocks' states meet in the buffers, rows' 16-byte chunks permuted
     __syncthreads();
     float* outs = reinterpret_cast<float*>(s_ring);
@@ -810,11 +880,10 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
     __syncthreads();
     constexpr int LPR = D / 4;  // lanes of a row, four dims each
     const int ch = threadIdx.x % LPR;
-    // a slot's first partial result is of what it takes over, its second of what it hands on
-    float* part = A.part + ((2 * (int64_t)slot + (left < share)) * hkv + h) * kPartFloats;
+    float* part = A.part + ((2 * (int64_t)slot + was.second) * hkv + h) * kPartFloats;
     for (int pr = threadIdx.x / LPR; pr < R; pr += NT / LPR) {
-      const int row = row0 + pr;
-      if (row >= n_rows) break;
+      const int row = was.row0 + pr;
+      if (row >= was.n_rows) break;
       float top = -INFINITY;
 #pragma unroll
       for (int w = 0; w < W; ++w) top = fmaxf(top, s_ml[w][pr][0]);
@@ -829,24 +898,14 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(x[i], wt, o[i]);
       }
-      if (whole) {
-        store_row<T>(A, rq, h, row, ch * 4, o, top, sum, ch == 0);
+      if (was.whole) {
+        store_row<T>(A, was.q_begin, h, row, ch * 4, o, top, sum, ch == 0);
       } else {
         *reinterpret_cast<f32x4*>(part + pr * D + ch * 4) = o;
         if (ch == 0) *reinterpret_cast<f32x2*>(part + R * D + pr * 2) = f32x2{top, sum};
       }
     }
-    left -= t_last - t_first;
-    if (left <= 0) return;
-    pl.tile = 0;
-    if (++pl.block == rq.blocks) {
-      pl.block = 0;
-      if (++pl.chunk == rq.chunks) {
-        pl.chunk = 0;
-        if (rq.index + 1 >= n_requests) return;
-        pl.rq = A.requests[rq.index + 1];
-      }
-    }
+    if (!more) return;
     __syncthreads();  // the outputs are read: the buffers may be filled again
   }
 }
@@ -892,9 +951,11 @@ __global__ __launch_bounds__(256) void merge_kernel(Args A, int rows) {
   const int64_t size = (int64_t)rows * (D + 2);
   // One of several chunks lies in up to three slots: candidate i is slot i % 3 of
   // chunk i / 3's.
-  const int candidates = rq.chunks > 1 ? rq.chunks * 3 : pl.parts / 2;
+  const bool single = A.header->chunk_per_slot;
+  const int candidates = single ? rq.chunks : rq.chunks > 1 ? rq.chunks * 3 : pl.parts / 2;
   auto part_at = [&](int i) -> int {  // the candidate's partial result, or -1
     if (i >= candidates) return -1;
+    if (single) return 2 * (pl.tile + i * rq.blocks);
     if (rq.chunks == 1) return 2 * (pl.tile + i) + (i == 0 ? pl.parts % 2 : 0);
     const int chunk = i / 3, t0 = chunk_tile(rq, chunk), n = chunk_tiles(rq, chunk);
     const int64_t start = rq.base + (int64_t)t0 * rq.blocks + (int64_t)pl.block * n;
@@ -940,7 +1001,7 @@ __global__ __launch_bounds__(256) void merge_kernel(Args A, int rows) {
           float top = -INFINITY, sum = 0.f;
           f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
           join(top, sum, o, x[k], own[k], n);
-          if (pr < n_rows) store_row<T>(A, rq, h, row0 + pr, ch * 4, o, top, sum, ch == 0);
+          if (pr < n_rows) store_row<T>(A, rq.q_begin, h, row0 + pr, ch * 4, o, top, sum, ch == 0);
         }
       }
     };
@@ -986,7 +1047,7 @@ __global__ __launch_bounds__(256) void merge_kernel(Args A, int rows) {
       sum = 0.f;
       o = f32x4{0.f, 0.f, 0.f, 0.f};
       join(top, sum, o, x, own, W);
-      if (r0 + lane / LPR < n_rows) store_row<T>(A, rq, h, row0 + pr, ch * 4, o, top, sum, ch == 0);
+      if (r0 + lane / LPR < n_rows) store_row<T>(A, rq.q_begin, h, row0 + pr, ch * 4, o, top, sum, ch == 0);
     }
     __syncthreads();
   }

@@ -25,6 +25,8 @@ holder.  The copies run on the device, in all layers at once.
 
 from __future__ import annotations
 
+import math
+from array import array
 from dataclasses import dataclass, field
 from typing import Sequence
 
@@ -44,29 +46,30 @@ def kv_copy_pages(cache: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -
     source.  Enqueued on the current stream; the lists are read at once.
     """
 
-    if cache.dim() == 5:
-        cache = cache.unsqueeze(0)
-    if cache.dim() != 6 or cache.shape[2] != 2:
+    shape, strides = cache.shape, cache.stride()
+    if len(shape) == 5:
+        shape, strides = (1, *shape), (0, *strides)
+    if len(shape) != 6 or shape[2] != 2:
         raise ValueError(f"cache must be [layers, P, 2, page, Hkv, D] or a layer of it, got {tuple(cache.shape)}")
-    src, dst = (np.asarray(x).reshape(-1) for x in (src, dst))
-    if src.size != dst.size:
-        raise ValueError(f"{src.size} source pages but {dst.size} destination pages")
-    if src.size == 0:
+    try:
+        src, dst = array("i", src), array("i", dst)
+    except (TypeError, OverflowError):
+        raise ValueError("page ids must be integers of 32 bits") from None
+    if len(src) != len(dst):
+        raise ValueError(f"{len(src)} source pages but {len(dst)} destination pages")
+    if not src:
         return
-    if src.dtype.kind not in "iu" or dst.dtype.kind not in "iu":
-        raise ValueError("page ids must be integers")
-    if min(src.min(), dst.min()) < 0 or max(src.max(), dst.max()) >= cache.shape[1]:
-        raise ValueError(f"page ids must be in [0, {cache.shape[1]})")
-    if cache.device.type != "cuda":
+    device = cache.get_device()
+    if device < 0:
         raise RuntimeError("kv_copy_pages needs a cache on a ROCm device")
-    if not cache[0, 0].is_contiguous():
+    page = math.prod(shape[2:])
+    if strides[2:] != (page // 2, shape[4] * shape[5], shape[5], 1):
         raise ValueError("the pages of the KV cache must be contiguous")
-    src, dst = (np.ascontiguousarray(x, dtype=np.int32) for x in (src, dst))
-    with _lib.on_device(cache.device):
+    with _lib.on_device(device):
         _lib.check(_lib.load().pl_kv_copy_pages(
-            cache.data_ptr(), cache.stride(0), cache.stride(1), cache[0, 0].numel(), cache.shape[0], cache.shape[1],
-            src.ctypes.data, dst.ctypes.data, src.size, _lib.dtype_code(cache.dtype),
-            _lib.stream_handle(cache.device)), "pl_kv_copy_pages")
+            cache.data_ptr(), strides[0], strides[1], page, shape[0], shape[1], src.buffer_info()[0],
+            dst.buffer_info()[0], len(src), _lib.dtype_code(cache.dtype), _lib.raw_stream(device)),
+            "pl_kv_copy_pages")
 
 
 class PageAllocator:

@@ -31,18 +31,15 @@ class AcceptedTree:
     tokens: torch.Tensor  # int64 [B, max_path]: the target's picks along it, then -1
 
 
-def _device_1d(t: torch.Tensor, name: str, dtype: torch.dtype, numel: int | None = None) -> None:
-    if t.device.type != "cuda":
-        raise RuntimeError(f"{name} must be on a ROCm device")
+def _vector(t: torch.Tensor, name: str, dtype: torch.dtype, numel: int, device: int) -> int:
+    """The address of a contiguous 1-D tensor of ``numel`` elements on device ``device``."""
+    if t.get_device() != device:
+        raise RuntimeError(f"{name} must be on the same ROCm device as the others")
     if t.dtype != dtype or t.dim() != 1 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous 1-D {dtype} tensor")
-    if numel is not None and t.numel() != numel:
+    if t.numel() != numel:
         raise ValueError(f"{name} must have {numel} entries, got {t.numel()}")
-
-
-def _same_device(*tensors: torch.Tensor) -> None:
-    if len({t.device for t in tensors}) > 1:
-        raise ValueError("all tensors must be on the same device")
+    return t.data_ptr()
 
 
 def accept_tree(tokens: torch.Tensor, parents: torch.Tensor, picks: torch.Tensor, qo_indptr: torch.Tensor, *,
@@ -58,18 +55,19 @@ def accept_tree(tokens: torch.Tensor, parents: torch.Tensor, picks: torch.Tensor
     the target's own pick after the last of them.  ``out``: tensors to write to.
     """
 
-    if parents.dim() != 1 or qo_indptr.dim() != 1 or qo_indptr.numel() < 1:
-        raise ValueError("parents and qo_indptr must be 1-D, qo_indptr with batch + 1 entries")
-    n, batch = parents.numel(), qo_indptr.numel() - 1
-    _device_1d(tokens, "tokens", torch.int64, n)
-    _device_1d(parents, "parents", torch.int32)
-    _device_1d(picks, "picks", torch.int64, n)
-    _device_1d(qo_indptr, "qo_indptr", torch.int32)
+    n, batch, device = parents.numel(), qo_indptr.numel() - 1, tokens.get_device()
+    if device < 0:
+        raise RuntimeError("accept_tree needs tensors on a ROCm device")
+    if batch < 0:
+        raise ValueError("qo_indptr must have batch + 1 entries")
     max_path = int(max_path)
     if max_path < 1:
         raise ValueError("max_path must be >= 1")
-    dev = tokens.device
+    args = (_vector(tokens, "tokens", torch.int64, n, device), _vector(parents, "parents", torch.int32, n, device),
+            _vector(picks, "picks", torch.int64, n, device),
+            _vector(qo_indptr, "qo_indptr", torch.int32, batch + 1, device))
     if out is None:
+        dev = tokens.device
         out = AcceptedTree(torch.empty((batch, max_path), dtype=torch.int32, device=dev),
                            torch.empty(batch, dtype=torch.int32, device=dev),
                            torch.empty((batch, max_path), dtype=torch.int64, device=dev))
@@ -77,14 +75,11 @@ def accept_tree(tokens: torch.Tensor, parents: torch.Tensor, picks: torch.Tensor
         for name, t, dtype, shape in (("path", out.path, torch.int32, (batch, max_path)),
                                       ("count", out.count, torch.int32, (batch,)),
                                       ("tokens", out.tokens, torch.int64, (batch, max_path))):
-            if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
-                raise ValueError(f"out.{name} must be a contiguous {dtype} tensor of shape {shape}")
-    _same_device(tokens, parents, picks, qo_indptr, out.path, out.count, out.tokens)
-    with _lib.on_device(dev):
-        _lib.check(_lib.load().pl_tree_accept(
-            tokens.data_ptr(), parents.data_ptr(), picks.data_ptr(), qo_indptr.data_ptr(), batch, n, max_path,
-            out.path.data_ptr(), out.count.data_ptr(), out.tokens.data_ptr(), _lib.stream_handle(dev)),
-            "pl_tree_accept")
+            if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != device:
+                raise ValueError(f"out.{name} must be a contiguous {dtype} tensor of shape {shape} on the same device")
+    with _lib.on_device(device):
+        _lib.check(_lib.load().pl_tree_accept(*args, batch, n, max_path, out.path.data_ptr(), out.count.data_ptr(),
+                                              out.tokens.data_ptr(), _lib.raw_stream(device)), "pl_tree_accept")
     return out
 
 
@@ -102,32 +97,35 @@ def commit_tree(cache: torch.Tensor, path: torch.Tensor, count: torch.Tensor, *,
     Pages that two requests of the batch share are not written safely.
     """
 
-    if cache.dim() == 5:
-        cache = cache.unsqueeze(0)
-    if cache.dim() != 6 or cache.shape[2] != 2:
+    shape, strides = cache.shape, cache.stride()
+    if len(shape) == 5:
+        shape, strides = (1, *shape), (0, *strides)
+    if len(shape) != 6 or shape[2] != 2:
         raise ValueError(f"cache must be [layers, P, 2, page, Hkv, D] or a layer of it, got {tuple(cache.shape)}")
-    if cache.device.type != "cuda":
+    device = cache.get_device()
+    if device < 0:
         raise RuntimeError("commit_tree needs a cache on a ROCm device")
-    if cache.stride(5) != 1:
+    if strides[5] != 1:
         raise ValueError("head_dim must be contiguous in the KV cache")
-    layers, num_pages, _, page_size, hkv, head_dim = cache.shape
-    if qo_indptr.dim() != 1 or qo_indptr.numel() < 1:
-        raise ValueError("qo_indptr must be 1-D with batch + 1 entries")
+    layers, num_pages, _, page_size, hkv, head_dim = shape
     batch = qo_indptr.numel() - 1
-    _device_1d(qo_indptr, "qo_indptr", torch.int32)
-    _device_1d(paged_kv_indptr, "paged_kv_indptr", torch.int32, batch + 1)
-    _device_1d(paged_kv_indices, "paged_kv_indices", torch.int32)
-    _device_1d(paged_kv_last_page_len, "paged_kv_last_page_len", torch.int32, batch)
-    _device_1d(count, "count", torch.int32, batch)
+    if batch < 0:
+        raise ValueError("qo_indptr must have batch + 1 entries")
+    num_indices = paged_kv_indices.numel()
+    tables = (_vector(qo_indptr, "qo_indptr", torch.int32, batch + 1, device),
+              _vector(paged_kv_indptr, "paged_kv_indptr", torch.int32, batch + 1, device),
+              _vector(paged_kv_indices, "paged_kv_indices", torch.int32, num_indices, device), num_indices,
+              _vector(paged_kv_last_page_len, "paged_kv_last_page_len", torch.int32, batch, device))
     if path.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != batch or not path.is_contiguous():
         raise ValueError(f"path must be a contiguous int32 [{batch}, max_path] tensor")
-    _same_device(cache, path, count, qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len)
+    if path.get_device() != device:
+        raise RuntimeError("path must be on the same ROCm device as the others")
+    counts = _vector(count, "count", torch.int32, batch, device)
     if path.shape[1] == 0 or num_pages == 0:
         return
-    with _lib.on_device(cache.device):
+    base = cache.data_ptr()
+    with _lib.on_device(device):
         _lib.check(_lib.load().pl_tree_commit(
-            cache.data_ptr(), cache[:, :, 1].data_ptr(), cache.stride(0), cache.stride(1), cache.stride(3),
-            cache.stride(4), layers, num_pages, qo_indptr.data_ptr(), paged_kv_indptr.data_ptr(),
-            paged_kv_indices.data_ptr(), paged_kv_indices.numel(), paged_kv_last_page_len.data_ptr(), path.data_ptr(),
-            count.data_ptr(), batch, path.shape[1], hkv, head_dim, page_size, _lib.dtype_code(cache.dtype),
-            _lib.stream_handle(cache.device)), "pl_tree_commit")
+            base, base + strides[2] * cache.element_size(), strides[0], strides[1], strides[3], strides[4], layers,
+            num_pages, *tables, path.data_ptr(), counts, batch, path.shape[1], hkv, head_dim, page_size,
+            _lib.dtype_code(cache.dtype), _lib.raw_stream(device)), "pl_tree_commit")

@@ -67,7 +67,7 @@ def test_refusals(gpu_device):
     cache = random_cache(2, 8, 16, 2, 64, torch.bfloat16, gpu_device)
     before = cache.clone()
     for src, dst, what in (([1], [1], "also a source"), ([1, 2], [3, 3], "written twice"), ([1, 2], [2, 3], "also a source"),
-                           ([8], [1], "page ids"), ([1], [-1], "page ids"), ([1, 2], [3], "destination"),
+                           ([8], [1], "outside the 8-page"), ([1], [-1], "outside the 8-page"), ([1], [2**40], "integers"), ([1, 2], [3], "destination"),
                            ([1.0], [2.0], "integers")):
         with pytest.raises(ValueError, match=what):
             kv_copy_pages(cache, src, dst)

@@ -178,6 +178,8 @@ def test_refusals(gpu_device):
         accept_tree(d[0], d[1], d[2][:1], d[3], max_path=2)
     with pytest.raises(RuntimeError, match="ROCm device"):
         accept_tree(d[0].cpu(), *d[1:], max_path=2)
+    with pytest.raises(RuntimeError, match="same ROCm device"):
+        accept_tree(d[0], d[1], d[2].cpu(), d[3], max_path=2)
     out = accept_tree(*d, max_path=2)
     with pytest.raises(ValueError, match="out.path"):
         accept_tree(*d, max_path=3, out=out)
