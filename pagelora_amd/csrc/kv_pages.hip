@@ -33,10 +33,10 @@ __global__ __launch_bounds__(kThreads) void copy_kernel(Args A) {
   u32x4 x[kLoads];
 #pragma unroll
   for (int i = 0; i < kLoads; ++i)
-    if (at + i * kThreads * 16 < A.page_bytes) x[i] = *reinterpret_cast<const u32x4*>(from + at + i * kThreads * 16);
+    if (at + i * kThreads * 16 < A.page_bytes) x[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(from + at + i * kThreads * 16));
 #pragma unroll
   for (int i = 0; i < kLoads; ++i)
-    if (at + i * kThreads * 16 < A.page_bytes) *reinterpret_cast<u32x4*>(to + at + i * kThreads * 16) = x[i];
+    if (at + i * kThreads * 16 < A.page_bytes) __builtin_nontemporal_store(x[i], reinterpret_cast<u32x4*>(to + at + i * kThreads * 16));
 }
 
 }  // namespace pages

@@ -470,18 +470,22 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
   __shared__ float s_ml[W][R][2];
   __shared__ int s_turn[W * WR];
 
+  const int hkv = A.want.hkv, h = blockIdx.x % hkv;
+  // Workgroups go round the 8 XCDs.  Where the heads divide 8 and row blocks share
+  // their pages, an XCD has one head and a run of the slots, so that the row blocks
+  // of a chunk share an L2.
+  int slot = blockIdx.x / hkv;
+  if (!A.once && 8 % hkv == 0) {
+    const int runs = 8 / hkv, per = (A.header->num_slots + runs - 1) / runs, at = slot / runs;
+    slot = at < per ? slot % runs * per + at : A.slots;
+  }
+  // (asked for before the checks: one latency for both)
+  Place pl = A.first[min(slot, A.slots - 1)];
   if (!plan_fits(A)) return;
-  const int n_slots = A.header->num_slots, hkv = A.want.hkv;
   const int64_t share = A.header->share;
-  // Workgroups go round the 8 XCDs.  Where the heads divide 8 an XCD has one head
-  // and a run of the slots, so that the row blocks of a chunk share an L2.
-  const int runs = 8 % hkv == 0 ? 8 / hkv : 1, per = (n_slots + runs - 1) / runs;
-  const int at = blockIdx.x / (runs * hkv), h = blockIdx.x % hkv;
-  const int slot = (int)(blockIdx.x / hkv) % runs * per + at;
-  if (at >= per || slot >= n_slots) return;
+  if (slot >= A.header->num_slots) return;
   const bool single = A.header->chunk_per_slot;
   const int n_requests = A.header->num_requests;
-  Place pl = A.first[slot];
   int64_t left = share;  // tiles of the share to come
 
   const int g = A.want.hq / hkv, page_size = A.want.page_size;
@@ -625,7 +629,8 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
 
   u32x4 qb[C][KS];
   Offset ask0{}, ask1{};
-  auto ask = [&](const Segment& e) {  // queries and page ids
+  uint64_t mask0[C];  // the rows' masks where they are one word
+  auto ask = [&](const Segment& e) {  // queries, masks and page ids
     if (e.t_first < e.t_end) {
       ask0 = ask_offsets(e, e.t_first);
       ask1 = ask_offsets(e, e.t_first + (PAGE16 ? 32 : 1));
@@ -634,6 +639,7 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
     for (int c = 0; c < C; ++c) {
       const int row = min(e.row0 + (rank * C + c) * 16 + lr, e.n_rows - 1);  // rows past the end repeat the last one, unstored
       const int node = row / g;
+      mask0[c] = A.masks[(int64_t)(e.q_begin + node) * A.mask_words];
       const char* qp = A.q + ((int64_t)(e.q_begin + node) * A.q_st + (int64_t)(h * g + row - node * g) * A.q_sh) * 2 + grp * 16;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) qb[c][ks] = *reinterpret_cast<const u32x4*>(qp + ks * 64);
@@ -702,10 +708,13 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
         const uint32_t inside = n == kBlock ? ~0u : (1u << n) - 1;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-          const int row = min(e.row0 + (rank * C + c) * 16 + lr, e.n_rows - 1);
-          const uint64_t* mask = A.masks + (int64_t)(e.q_begin + row / g) * A.mask_words;
-          const uint64_t lo = w < 0 ? ~0ull : (w < A.mask_words ? mask[w] : 0);
-          const uint64_t hi = w + 1 < 0 ? ~0ull : (w + 1 < A.mask_words ? mask[w + 1] : 0);
+          uint64_t lo = w < 0 ? ~0ull : (w == 0 ? mask0[c] : 0), hi = w + 1 < 0 ? ~0ull : (w + 1 == 0 ? mask0[c] : 0);
+          if (A.mask_words > 1) {
+            const int row = min(e.row0 + (rank * C + c) * 16 + lr, e.n_rows - 1);
+            const uint64_t* mask = A.masks + (int64_t)(e.q_begin + row / g) * A.mask_words;
+            if (w > 0 && w < A.mask_words) lo = mask[w];
+            if (w >= 0 && w + 1 < A.mask_words) hi = mask[w + 1];
+          }
           vis[c] = (uint32_t)(sh ? lo >> sh | hi << (64 - sh) : lo) & inside;
         }
         // 0 * V is NaN where V is not finite: V behind the last token is set to

@@ -20,6 +20,8 @@ namespace commit {
 constexpr int kWave = 64;
 constexpr int kThreads = 256;
 
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
 __global__ __launch_bounds__(kWave) void accept_kernel(const int64_t* __restrict__ tokens,
                                                        const int32_t* __restrict__ parents,
                                                        const int64_t* __restrict__ picks,
@@ -81,15 +83,16 @@ struct Args {
   char* v;
   int64_t layer_stride, page_stride, token_stride, head_stride, num_pages;  // bytes; pages
   const int32_t *qo_indptr, *kv_indptr, *kv_indices, *kv_last, *path, *count;
-  int batch, layers, num_indices, max_path, page_size;
+  int batch, layers, layers_each, num_indices, max_path, page_size;
   int row_chunks, head_chunks;  // 16-byte chunks of a token's K row, of one head
 };
 
-// A workgroup: 256 chunks of one request's token rows (K, then V) in one layer.
+// A workgroup: 256 chunks of one request's token rows (K, then V) in some layers.
 __global__ __launch_bounds__(kThreads) void commit_kernel(Args A) {
   __shared__ int64_t s_src[kWave], s_dst[kWave];
   __shared__ int s_live;
-  const int r = blockIdx.y, layer = blockIdx.z;
+  const int r = blockIdx.y, layer0 = blockIdx.z * A.layers_each;
+  const int layers = min(A.layers - layer0, A.layers_each);
   const int begin = uniform(A.kv_indptr[r]), pages = min(uniform(A.kv_indptr[r + 1]), A.num_indices) - begin;
   const int count = min(uniform(A.count[r]), A.max_path);
   if (begin < 0 || pages <= 0 || count <= 0) return;
@@ -100,7 +103,7 @@ __global__ __launch_bounds__(kThreads) void commit_kernel(Args A) {
   const int chunk = blockIdx.x * kThreads + threadIdx.x;
   const bool on = chunk < 2 * A.row_chunks;
   const int c = chunk % A.row_chunks;
-  char* row = (chunk < A.row_chunks ? A.k : A.v) + (int64_t)layer * A.layer_stride +
+  char* row = (chunk < A.row_chunks ? A.k : A.v) + (int64_t)layer0 * A.layer_stride +
               (int64_t)(c / A.head_chunks) * A.head_stride + (int64_t)(c % A.head_chunks) * 16;
   auto slot = [&](int64_t pos) -> int64_t {  // byte offset, -1 outside the pool
     const int64_t page = pos / A.page_size;
@@ -121,17 +124,26 @@ __global__ __launch_bounds__(kThreads) void commit_kernel(Args A) {
     __syncthreads();
     const int live = s_live;
     if (on) {
-      // eight loads, then their stores: a token's slot is no source of a later one
+      // The loads of eight tokens in two layers, then their stores: a token's slot
+      // is no source of a later one.
       for (int i0 = 0; i0 < live; i0 += 8) {
-        uint4 x[8];
+        for (int l0 = 0; l0 < layers; l0 += 2) {
+          u32x4 x[2][8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i0 + i < live && s_src[i0 + i] >= 0 && s_dst[i0 + i] >= 0)
-            x[i] = *reinterpret_cast<const uint4*>(row + s_src[i0 + i]);
+          for (int l = 0; l < 2; ++l)
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i0 + i < live && s_src[i0 + i] >= 0 && s_dst[i0 + i] >= 0)
-            *reinterpret_cast<uint4*>(row + s_dst[i0 + i]) = x[i];
+            for (int i = 0; i < 8; ++i)
+              if (l0 + l < layers && i0 + i < live && s_src[i0 + i] >= 0 && s_dst[i0 + i] >= 0)
+                x[l][i] = __builtin_nontemporal_load(
+                    reinterpret_cast<const u32x4*>(row + (l0 + l) * A.layer_stride + s_src[i0 + i]));
+#pragma unroll
+          for (int l = 0; l < 2; ++l)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (l0 + l < layers && i0 + i < live && s_src[i0 + i] >= 0 && s_dst[i0 + i] >= 0)
+                __builtin_nontemporal_store(
+                    x[l][i], reinterpret_cast<u32x4*>(row + (l0 + l) * A.layer_stride + s_dst[i0 + i]));
+        }
       }
     }
     if (live < kWave) return;
@@ -204,7 +216,11 @@ extern "C" int pl_tree_commit(void* k_cache, void* v_cache, int64_t layer_stride
   a.page_size = page_size;
   a.head_chunks = head_dim / per;
   a.row_chunks = num_kv_heads * a.head_chunks;
-  const dim3 grid((2 * a.row_chunks + commit::kThreads - 1) / commit::kThreads, batch, num_layers);
+  // Enough workgroups to fill the chip, and no more: each first looks up its request's slots.
+  const int across = (2 * a.row_chunks + commit::kThreads - 1) / commit::kThreads;
+  const int64_t each = ((int64_t)across * batch * num_layers + 2047) / 2048;
+  a.layers_each = (int)(each < num_layers ? each : num_layers);
+  const dim3 grid(across, batch, (num_layers + a.layers_each - 1) / a.layers_each);
   hipLaunchKernelGGL(commit::commit_kernel, grid, dim3(commit::kThreads), 0, (hipStream_t)stream, a);
   PL_LAUNCH_CHECK("tree commit_kernel");
   return ok();
