@@ -417,17 +417,19 @@ __device__ __forceinline__ bool plan_fits(const Args& A) {
 }
 
 template <typename T> struct Softmax {
-  static constexpr bool kTwo = std::is_same<T, bf16_t>::value;
-  // bf16 probabilities enter the product as two planes, hi + lo, so they carry
-  // 16 bits; fp16's one plane carries its 11.
-  static constexpr int kPlanes = kTwo ? 2 : 1;
+  static constexpr bool kBf16 = std::is_same<T, bf16_t>::value;
+  // Probabilities enter the product as two planes, hi + lo, of the cache's type:
+  // they carry 16 bits (bf16) or 22 (fp16), as a decode step's do, and a draft is
+  // verified by what decoding would give.  One plane saves a third of the matrix
+  // instructions: 1 x 64 nodes behind 32768 80 -> 75 us, 64 x 16 behind 8192 none.
+  static constexpr int kPlanes = 2;
   // A column's running maximum follows only scores more than kLag above it,
-  // which takes the rescale out of the steady state.  One fp16 plane is exact
-  // for the largest probability only where that is a power of two: no lag.
-  static constexpr float kLag = kTwo ? 8.f : 0.f;
+  // which takes the rescale out of the steady state.
+  static constexpr float kLag = kBf16 ? 8.f : 1.f;
   // Probabilities are held 2^kShift times as large: fp16 ends at 2^-24, and
-  // 32768 tokens of 2^-25 are no small part of a row.  2^14 keeps them to 2^-38.
-  static constexpr float kShift = kTwo ? 0.f : 14.f;
+  // 32768 tokens of 2^-25 are no small part of a row.  2^14 keeps them to 2^-38,
+  // and the largest, 2^15 with the lag, below fp16's 65504.
+  static constexpr float kShift = kBf16 ? 0.f : 14.f;
 };
 
 // Finishes a row: its four dims by one lane, and the row's lse by lane `first`.

@@ -1,8 +1,8 @@
 """Attention of drafted trees (plan_tree / run_tree) against the float64 oracle.
 
 Tolerance of an output element, from the kernel's arithmetic: half a step of
-the storage type for the store; for the weights the rounding of p (2^-17 in
-bf16's two planes, 2^-11 in fp16's one), twice the error of a score (fp32 sums
+the storage type for the store; for the weights the rounding of p to two planes
+(2^-17 and less), twice the error of a score (fp32 sums
 of D products, and an exponent below 2^5) and of the sums over the tokens, all
 times the largest |v| that the row attends.
 """
@@ -69,7 +69,7 @@ def check(case, out, lse=None, dtype=BF16):
     cache, q = case["cache_host"].double().numpy(), case["q_host"].double().numpy()
     d = q.shape[2]
     got = out.double().cpu().numpy()
-    half, p_err = (2.0**-8, 2.0**-17) if dtype == BF16 else (2.0**-11, 2.0**-11)
+    half, p_err = 2.0**-8 if dtype == BF16 else 2.0**-11, 2.0**-17
     for r, n in enumerate(case["trees"]):
         if n == 0:
             continue
