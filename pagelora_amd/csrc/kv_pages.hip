@@ -60,27 +60,33 @@ extern "C" int pl_kv_copy_pages(void* cache, int64_t layer_stride, int64_t page_
     return fail(PL_ERR_INVALID, "pages of %lld elements overlap at a stride of %lld", (long long)page_elements,
                 (long long)page_stride);
   if ((uintptr_t)cache % 16) return fail(PL_ERR_INVALID, "cache must be 16-byte aligned");
-  const int64_t pieces = (page_elements * eb + pages::kBytes - 1) / pages::kBytes;
-  if (num_layers > 65535 || pieces * pages::kPairs > INT32_MAX)
+  // a launch has less than 2^32 threads per dimension
+  const int64_t pieces = page_elements > (1ll << 40) ? 1 << 24 : (page_elements * eb + pages::kBytes - 1) / pages::kBytes;
+  if (num_layers > 65535 || pieces * pages::kPairs >= (1 << 24))
     return fail(PL_ERR_UNSUPPORTED, "%d layers or pages of %lld elements are too many", num_layers,
                 (long long)page_elements);
-  try {
-    // 1: some copy reads the page, 2: one writes it
-    std::vector<uint8_t> role((size_t)num_pages, 0);
-    for (int i = 0; i < n; ++i) {
-      if (src_h[i] < 0 || src_h[i] >= num_pages || dst_h[i] < 0 || dst_h[i] >= num_pages)
-        return fail(PL_ERR_INVALID, "copy %d: page %d to page %d is outside the %lld-page pool", i, src_h[i], dst_h[i],
-                    (long long)num_pages);
-      role[src_h[i]] |= 1;
+  for (int i = 0; i < n; ++i)
+    if (src_h[i] < 0 || src_h[i] >= num_pages || dst_h[i] < 0 || dst_h[i] >= num_pages)
+      return fail(PL_ERR_INVALID, "copy %d: page %d to page %d is outside the %lld-page pool", i, src_h[i], dst_h[i],
+                  (long long)num_pages);
+  auto clash = [&](int i, bool source) {
+    return fail(PL_ERR_INVALID, "copy %d: page %d is %s", i, dst_h[i], source ? "also a source" : "written twice");
+  };
+  if ((int64_t)n * n <= num_pages) {
+    for (int i = 0; i < n; ++i)
+      for (int j = 0; j < n; ++j)
+        if (dst_h[i] == src_h[j] || (j < i && dst_h[i] == dst_h[j])) return clash(i, dst_h[i] == src_h[j]);
+  } else {
+    try {
+      std::vector<uint8_t> role((size_t)num_pages, 0);  // 1: some copy reads the page, 2: one writes it
+      for (int i = 0; i < n; ++i) role[src_h[i]] = 1;
+      for (int i = 0; i < n; ++i) {
+        if (role[dst_h[i]]) return clash(i, role[dst_h[i]] == 1);
+        role[dst_h[i]] = 2;
+      }
+    } catch (...) {
+      return fail(PL_ERR_INVALID, "no host memory to check the copies of a %lld-page pool", (long long)num_pages);
     }
-    for (int i = 0; i < n; ++i) {
-      if (role[dst_h[i]])
-        return fail(PL_ERR_INVALID, "copy %d: page %d is %s", i, dst_h[i],
-                    role[dst_h[i]] & 1 ? "also a source" : "written twice");
-      role[dst_h[i]] = 2;
-    }
-  } catch (...) {
-    return fail(PL_ERR_INVALID, "no host memory to check the copies of a %lld-page pool", (long long)num_pages);
   }
   pages::Args a{};
   a.cache = (char*)cache;

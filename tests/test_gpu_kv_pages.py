@@ -77,6 +77,11 @@ def test_refusals(gpu_device):
         kv_copy_pages(cache[0, 0], [1], [2])
     with pytest.raises(NotImplementedError):
         kv_copy_pages(cache.double(), [1], [2])
+    many = list(range(1, 60))
+    big = random_cache(1, 130, 1, 1, 8, torch.bfloat16, gpu_device)
+    for dst, what in ((many, "also a source"), ([60 + i // 2 for i in range(59)], "written twice")):
+        with pytest.raises(ValueError, match=what):
+            kv_copy_pages(big, many, dst)
     kv_copy_pages(cache, [], [])
     torch.cuda.synchronize()
     assert torch.equal(cache, before)

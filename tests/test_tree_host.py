@@ -1,5 +1,7 @@
 """What plan_tree and the tree's C entries refuse before any launch (host checks only; pointers are never read)."""
 
+import ctypes
+
 import pytest
 import torch
 
@@ -123,3 +125,10 @@ def test_pl_tree_commit_refuses():
         assert commit(**kw) == _lib.PL_ERR_INVALID and _lib.last_error()
     assert commit(dtype=7) == _lib.PL_ERR_UNSUPPORTED and commit(batch=65536) == _lib.PL_ERR_UNSUPPORTED
     assert commit(batch=0, qo=None) == 0 and commit(layers=0, k=None) == 0
+
+
+def test_pl_kv_copy_pages_refuses():
+    src, dst = (ctypes.c_int32 * 1)(1), (ctypes.c_int32 * 1)(2)
+    for layers, elements, stride in ((65536, 1024, 1024), (1, 1 << 29, 1 << 29), (1, 1 << 50, 1 << 50)):
+        assert _lib.load().pl_kv_copy_pages(PTR, 0, stride, elements, layers, 9, ctypes.addressof(src),
+                                            ctypes.addressof(dst), 1, 2, None) == _lib.PL_ERR_UNSUPPORTED
