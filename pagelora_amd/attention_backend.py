@@ -238,6 +238,9 @@ class PagedDecodeAttention:
         self._decode_graph_buffers: tuple[torch.Tensor, torch.Tensor, torch.Tensor] | None = None
         self._decode_host_uploads: deque = deque()
         self._plan: dict | None = None
+        self._tree_plan: dict | None = None
+        self._tree_buffers: dict[int, torch.Tensor] = {}  # by size class
+        self._tree_kept: dict[tuple, torch.Tensor] = {}   # by sizes: those that captured graphs use
 
     # ------------------------------------------------------------ planning
     def plan_decode(
@@ -861,18 +864,20 @@ class PagedDecodeAttention:
             plan_bytes = self._lib.pl_tree_plan_size(*sizes, capacity, *heads)
             if plan_bytes == 0:
                 _lib.check(_lib.PL_ERR_UNSUPPORTED, "pl_tree_plan_size")
-            buffer = self._tree_buffer(plan_bytes)
+            captured = torch.cuda.is_current_stream_capturing()
+            buffer = self._tree_buffer(plan_bytes, (sizes, capacity), captured)
             stream = torch.cuda.current_stream(self.device)
             parents_ptr, mask_ptr, mask_ld = (tree.data_ptr(), None, 0) if tree_parents is not None else (
-                None, tree.data_ptr(), tree.stride(0))
+                None, tree.data_ptr(), tree.shape[1])
             _lib.check(self._lib.pl_tree_plan(
                 tables[0].data_ptr(), tables[1].data_ptr(), tables[2].data_ptr(), num_indices, tables[3].data_ptr(),
                 *sizes, parents_ptr, mask_ptr, mask_ld, *heads, self.page_size, int(min_share), capacity,
                 buffer.data_ptr(), buffer.numel(), stream.cuda_stream), "pl_tree_plan")
-            captured = torch.cuda.is_current_stream_capturing()
             self._tree_plan = {
                 "device": index,
                 "sizes": sizes,
+                "bytes": plan_bytes,
+                "kept": captured,
                 "tokens": tokens,
                 "capacity": capacity,
                 "buffer": buffer,
@@ -886,15 +891,21 @@ class PagedDecodeAttention:
     def _device_index(self) -> int:
         return self.workspace_buffer.get_device()
 
-    def _tree_buffer(self, nbytes: int) -> torch.Tensor:
-        """The plan buffer of a size class.  One per class lives as long as the
-        backend: captured runs read it."""
-        buffers = self.__dict__.setdefault("_tree_buffers", {})
+    def _tree_buffer(self, nbytes: int, key, keep: bool) -> torch.Tensor:
+        """The plan buffer of the sizes ``key``: one that plans of a size class
+        share, or with ``keep`` (a capture reads or writes it) one that no plan
+        of other sizes is made in from now on.  All live as long as the backend."""
+        kept, shared = self._tree_kept, self._tree_buffers
+        if key in kept:
+            return kept[key]
         size = 1 << (nbytes - 1).bit_length()
-        if size not in buffers:
+        if size not in shared:
             # zeros: no header of an earlier owner of the memory
-            buffers[size] = torch.zeros(size, dtype=torch.uint8, device=self.device)
-        return buffers[size]
+            shared[size] = torch.zeros(size, dtype=torch.uint8, device=self.device)
+        if keep:
+            kept[key] = shared.pop(size)
+            return kept[key]
+        return shared[size]
 
     def _validate_host_trees(self, qo_indptr, kv_indptr, kv_indices, kv_last, parents, tokens) -> tuple[int, int]:
         """Check host tables of trees; returns (largest page id or -1, nodes of the widest tree)."""
@@ -921,7 +932,7 @@ class PagedDecodeAttention:
     def tree_graph_signature(self):
         """Everything a captured run_tree bakes in; sequence lengths are not
         part of it."""
-        plan = getattr(self, "_tree_plan", None) or {}
+        plan = self._tree_plan or {}
         buffer = plan.get("buffer")
         return (id(self), plan.get("sizes"), plan.get("capacity"), buffer.data_ptr() if buffer is not None else None)
 
@@ -935,7 +946,7 @@ class PagedDecodeAttention:
         """Writes ``out`` ([tokens, Hq, D], head_dim contiguous) and optionally
         ``lse`` ([tokens, Hq] fp32, natural log) for packed ``q``."""
 
-        plan = getattr(self, "_tree_plan", None)
+        plan = self._tree_plan
         if plan is None:
             raise RuntimeError("plan_tree must be called before run_tree")
         shape, dtype, device = q.shape, q.dtype, plan["device"]
@@ -960,6 +971,9 @@ class PagedDecodeAttention:
             raise RuntimeError(f"run_tree needs tensors on the backend's device {self.device}")
         with _lib.on_device(device):
             stream = _lib.raw_stream(device)
+            if not plan["kept"] and torch.cuda.is_current_stream_capturing():
+                self._tree_buffer(plan["bytes"], (plan["sizes"], plan["capacity"]), True)
+                plan["kept"] = True
             if stream != plan["stream"] and plan["ready"] is not None \
                     and not torch.cuda.is_current_stream_capturing():
                 torch.cuda.current_stream(device).wait_event(plan["ready"])

@@ -367,13 +367,13 @@ template <bool ONCE>
 __device__ __forceinline__ void load_lds16(const char* base, uint32_t offset, uint32_t l) {
   if constexpr (ONCE)
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(l), "v"(offset), "s"(base)
-                 : "memory");
+                 : "memory", "m0");
   else
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(l), "v"(offset), "s"(base)
-                 : "memory");
+                 : "memory", "m0");
 }
 __device__ __forceinline__ void load_lds16(const char* address, uint32_t l) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(l), "v"(address) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(l), "v"(address) : "memory", "m0");
 }
 // All but the N newest loads are done.
 template <int N> __device__ __forceinline__ void wait_loads() {
@@ -1017,6 +1017,7 @@ __global__ __launch_bounds__(256) void merge_kernel(Args A, int rows) {
       }
     };
     const int n = __builtin_popcountll(live);
+    if (n == 0) return;
     if (n <= 2) rows_at_once(std::integral_constant<int, 2>{});
     else if (n <= 4) rows_at_once(std::integral_constant<int, 4>{});
     else rows_at_once(std::integral_constant<int, 8>{});

@@ -329,6 +329,23 @@ def test_row_blocks_of_every_size_masked_values(gpu_device, n):
         assert (np.abs(got - ref)[~touched] <= 2.0**-7 * np.abs(ref[~touched]) + 0.01).all()
 
 
+@pytest.mark.parametrize("kv_len,tree", [(40000, 3), (70000, 2), (70000, 40)])
+def test_one_long_sequence_in_very_many_parts(gpu_device, kv_len, tree):
+    """One kv head: its rows come together from more than 64 and more than 256 parts."""
+    case = tree_case([tree], [kv_len], 1, 1, 64, 16, BF16, gpu_device, seed=tree)
+    out, lse = run(case, 1, 1, 64, 16, gpu_device)
+    check(case, out, lse)
+
+
+@pytest.mark.parametrize("long,small", [(30000, 250), (3000, 250), (9000, 40), (2000, 300)])
+def test_long_wide_trees_among_many_small_ones(gpu_device, long, small):
+    """Shares that hold several requests, chunks of row blocks that slots share."""
+    trees, lens = [40] + [1] * small + [33], [long] + [3 + i % 120 for i in range(small)] + [long // 2]
+    case = tree_case(trees, lens, 4, 1, 64, 16, F16, gpu_device, seed=small)
+    out, lse = run(case, 4, 1, 64, 16, gpu_device)
+    check(case, out, lse, F16)
+
+
 def test_many_requests(gpu_device):
     """More requests than slots, empty ones among them."""
     rng = np.random.default_rng(2)
@@ -436,6 +453,60 @@ def test_two_captured_runs_of_other_sizes(gpu_device):
             g.replay()
             torch.cuda.synchronize()
             check(c, out)
+
+
+def test_captured_run_keeps_its_plan(gpu_device):
+    """Plans of other sizes that need as many bytes, made after the capture, leave the graph's plan alone."""
+    a, b = (tree_case([n], [70], 8, 2, 128, 16, BF16, gpu_device, seed=n) for n in (4, 5))
+    be = backend(8, 2, 128, 16, gpu_device)
+    be.plan_tree(**tables(a), tree_parents=a["parents"])
+    signature = be.tree_graph_signature()
+    out = be.run_tree(a["q"], a["cache"])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        be.run_tree_into(a["q"], a["cache"], out)
+    for _ in range(3):
+        be.plan_tree(**tables(b), tree_parents=b["parents"])
+        check(b, be.run_tree(b["q"], b["cache"]))
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        check(a, out)
+    be.plan_tree(**tables(a), tree_parents=a["parents"])
+    assert be.tree_graph_signature() == signature
+
+
+def test_batches_without_nodes(gpu_device):
+    """No request, or requests without nodes: nothing runs, nothing is written."""
+    be = backend(8, 2, 128, 16, gpu_device)
+    cache = torch.zeros((3, 2, 16, 2, 128), dtype=BF16, device=gpu_device)
+    none = torch.zeros(0, dtype=torch.int32)
+    for qo, kv, ind, last in (([0], [0], none, none), ([0, 0, 0], [0, 1, 1], torch.tensor([2], dtype=torch.int32),
+                                                     torch.tensor([7, 0], dtype=torch.int32))):
+        for dev in ("cpu", gpu_device):
+            t = {"qo_indptr": torch.tensor(qo, dtype=torch.int32), "paged_kv_indptr": torch.tensor(kv, dtype=torch.int32),
+                 "paged_kv_indices": ind, "paged_kv_last_page_len": last, "tree_parents": none}
+            be.plan_tree(**{k: v.to(dev) for k, v in t.items()})
+            q = torch.zeros((0, 8, 128), dtype=BF16, device=gpu_device)
+            assert be.run_tree(q, cache).shape == q.shape
+    torch.cuda.synchronize()
+
+
+def test_masks_in_any_order(gpu_device):
+    """A mask whose rows are not rows of memory, on the host and on the device."""
+    for n in (1, 9):
+        case = tree_case([n], [n + 40], 4, 2, 64, 16, F16, gpu_device, seed=n)
+        mask = torch.from_numpy(case["sees"][0].copy())
+        be = backend(4, 2, 64, 16, gpu_device)
+        for dev in ("cpu", gpu_device):
+            room = torch.ones((mask.shape[1] + 3, n), dtype=torch.bool, device=dev)
+            view = room.t()
+            view[:, :n] = mask.to(dev)
+            be.plan_tree(**tables(case, dev), tree_mask=view)
+            out = be.run_tree(case["q"], case["cache"])
+            torch.cuda.synchronize()
+            check(case, out, None, F16)
 
 
 def test_same_bits_twice(gpu_device):
