@@ -10,6 +10,8 @@ Modules (each function cites the reference file:line it follows):
   page_table    span -> (indptr, indices, last_page_len) packing, pure Python
   lora          no-merge LoRA delta: per-module, packed (A concat, block-diag B),
                 multi-adapter, and the merged-weight comparator (float64 numpy)
+  tree          attention, acceptance and commit of drafted trees (float64 numpy;
+                the formulas alone: the reference has no counterpart)
 
 Pinning (what each function is checked against, in tests/test_oracle_*.py):
   page_table    the reference's own test vectors (tests/golden/reference_vectors.json)

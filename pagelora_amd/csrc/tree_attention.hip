@@ -27,6 +27,20 @@
 // O^T += V^T P^T as they lie, and V comes out of LDS transposed.  The blocks'
 // states meet in LDS at the row block's end, and the parts of row blocks that
 // several slots share in merge_kernel, in order.
+//
+// Measured (head_dim 128, GQA 4 unless said otherwise; tree_kernel + merge_kernel):
+//   1 x 8 nodes behind 2048     10 + 4 us: dependent round trips (the place, the
+//                               page ids, the pages) and two launches
+//   1 x 64 behind 32768         73 + 5 us, 0.71 PFLOP/s: four row blocks of the same
+//                               pages, matrix and vector issue.  Without loads the
+//                               tiles take 52 us, 21 of them MFMAs at their full rate
+//   23 ragged, up to 4099, GQA 7  41 + 8 us: the starts of ~3 row blocks per slot
+//   8 x 32 behind 4096, no GQA, fp16  92 + 5 us, 5.8 TB/s: HBM (6.4 without any arithmetic)
+//   64 x 16 behind 2048 .. 8192  255 + 7 us, 5.3 TB/s: HBM, and the row blocks' starts
+// Tried and slower: 128 and 256 rows per row block, which read a page once for all
+// (80 - 91 us instead of 78 at 1 x 64); the next block's scores beside this one's
+// softmax in one wave (no faster at 1 x 64, 59 - 70 us instead of 55 at 23 requests:
+// registers spill and every row block computes one block of scores more).
 #include <algorithm>
 #include <type_traits>
 
@@ -189,6 +203,8 @@ __device__ __forceinline__ Place place_at(const Request& q, int64_t x, bool sing
 }
 
 // Workgroup 0 cuts the work; the others copy the page ids and pack the masks.
+// Bound by workgroup 0's dependent loads and scans: 6 us at one request, 12 at 64,
+// once per step.
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs A) {
   const int tid = threadIdx.x, batch = A.want.batch;
   if (blockIdx.x > 0) {
@@ -964,7 +980,7 @@ __device__ __forceinline__ void join(float& top, float& sum, f32x4& o, const f32
 // The parts of a row block that slots share, in order: D / 4 lanes per row, four
 // dims each.  A wave takes all parts of its rows where they are up to 8, and as
 // many rows as keep 8 loads in flight; of more parts each of the workgroup's four
-// waves takes every fourth of the same rows.
+// waves takes every fourth of the same rows.  Bound by latency: 4 - 8 us.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void merge_kernel(Args A, int rows) {
   constexpr int LPR = D / 4, RPW = kWave / LPR, W = 4;  // lanes of a row, rows of a wave, waves

@@ -6,12 +6,15 @@
 // pick after i.  The kept tokens are the picks along the path: the children's
 // own tokens, then the pick after the last node.  One wave per request; a tree
 // of up to 64 nodes lies one node per lane, and a step is two lane reads and a
-// ballot.  Bound by latency: the loads, and a launch.
+// ballot.  Bound by latency, the loads and a launch: 1.7 us for one tree of 8
+// nodes, 3.3 for 256 of up to 64.
 //
 // commit_kernel: slot(P + k) <- slot(P + path[k]) for the tokens of an accepted
 // path, in every layer, P the committed tokens before the tree.  path[k] >= k,
 // so no token is overwritten before it is read if a thread takes its bytes of
-// all tokens in order.  Bound by latency at few requests, by HBM at many.
+// all tokens in order.  Bound by latency at few requests (4.8 us for one with 4
+// tokens in 36 layers), by HBM at many, in rows of 2 KiB in no order: 64 requests'
+// 1 .. 8 tokens in 36 layers, 58 MB, 18 us, 3.2 TB/s.
 #include "pl_common.h"
 
 namespace pl {
