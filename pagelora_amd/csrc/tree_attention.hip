@@ -29,18 +29,21 @@
 // several slots share in merge_kernel, in order.
 //
 // Measured (head_dim 128, GQA 4 unless said otherwise; tree_kernel + merge_kernel):
-//   1 x 8 nodes behind 2048     10 + 4 us: dependent round trips (the place, the
+//   1 x 8 nodes behind 2048     8 + 4 us: dependent round trips (the place, the
 //                               page ids, the pages) and two launches
 //   1 x 64 behind 32768         73 + 5 us, 0.71 PFLOP/s: four row blocks of the same
 //                               pages, matrix and vector issue.  Without loads the
 //                               tiles take 52 us, 21 of them MFMAs at their full rate
-//   23 ragged, up to 4099, GQA 7  41 + 8 us: the starts of ~3 row blocks per slot
-//   8 x 32 behind 4096, no GQA, fp16  92 + 5 us, 5.8 TB/s: HBM (6.4 without any arithmetic)
+//   23 ragged, up to 4099, GQA 7  40 + 8 us: 12 tiles and the starts and
+//                               ends of ~3 row blocks per slot
+//   8 x 32 behind 4096, no GQA, fp16  91 + 5 us, 5.9 TB/s: HBM (6.4 without any arithmetic)
 //   64 x 16 behind 2048 .. 8192  255 + 7 us, 5.3 TB/s: HBM, and the row blocks' starts
+//   640 x 16 behind 112         167 us in all: ~7 us per row block of one tile
 // Tried and slower: 128 and 256 rows per row block, which read a page once for all
 // (80 - 91 us instead of 78 at 1 x 64); the next block's scores beside this one's
 // softmax in one wave (no faster at 1 x 64, 59 - 70 us instead of 55 at 23 requests:
-// registers spill and every row block computes one block of scores more).
+// registers spill and every row block computes one block of scores more); the next
+// row block's first loads while this one's states meet in half of the LDS (no faster).
 #include <algorithm>
 #include <type_traits>
 
@@ -67,6 +70,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
 // What a plan was made for, then what it holds.
 struct Header {
@@ -463,11 +467,22 @@ template <typename T> struct Softmax {
   static constexpr float kShift = kBf16 ? 0.f : 14.f;
 };
 
+// x / g: the product with 2^32 / g rounded up is the quotient or one more.
+struct Group {
+  uint32_t g, inverse;
+  __device__ __forceinline__ explicit Group(int g_) : g(g_), inverse(0xffffffffu / g + 1) {}
+  __device__ __forceinline__ int of(int x) const {
+    if (g == 1) return x;
+    const uint32_t n = __umulhi((uint32_t)x, inverse);
+    return (int)(n - (n * g > (uint32_t)x));
+  }
+};
+
 // Finishes a row: its four dims by one lane, and the row's lse by lane `first`.
 template <typename T>
-__device__ __forceinline__ void store_row(const Args& A, int q_begin, int h, int row, int dim, f32x4 o, float top,
-                                          float sum, bool first) {
-  const int g = A.want.hq / A.want.hkv, node = row / g;
+__device__ __forceinline__ void store_row(const Args& A, const Group& group, int q_begin, int h, int row, int dim,
+                                          f32x4 o, float top, float sum, bool first) {
+  const int g = group.g, node = group.of(row);
   const int64_t token = q_begin + node;
   const int head = h * g + row - node * g;
   const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
@@ -476,6 +491,28 @@ __device__ __forceinline__ void store_row(const Args& A, int q_begin, int h, int
   if (A.lse && first)
     A.lse[token * A.want.hq + head] =
         sum == 0.f ? -INFINITY : (top + log2f(sum) - Softmax<T>::kShift) * 0.693147180559945309f;
+}
+
+// A weighted sum of parts with its maximum: joins N more, those past n left out.
+template <int N>
+__device__ __forceinline__ void join(float& top, float& sum, f32x4& o, const f32x4 (&x)[N], const f32x2 (&own)[N], int n) {
+  float here = top;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < n) here = fmaxf(here, own[i][0]);
+  const float ref = here == -INFINITY ? 0.f : here, old = fast_exp2(top - ref);
+  top = here;
+  sum *= old;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] *= old;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (i >= n) break;
+    const float wt = fast_exp2(own[i][0] - ref);
+    sum = __builtin_fmaf(own[i][1], wt, sum);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[i][e], wt, o[e]);
+  }
 }
 
 template <typename T, int D, int R, bool PAGE16>
@@ -523,6 +560,7 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
   int64_t left = share;  // tiles of the share to come
 
   const int g = A.want.hq / hkv, page_size = A.want.page_size;
+  const Group group(g);
   const int lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave);
   // The wave's block of a tile, its rows of the row block.  Two waves of a block
   // are on two SIMDs, each beside one of another block: one's softmax then runs
@@ -674,7 +712,7 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int row = min(e.row0 + (rank * C + c) * 16 + lr, e.n_rows - 1);  // rows past the end repeat the last one, unstored
-      const int node = row / g;
+      const int node = group.of(row);
       mask0[c] = A.masks[(int64_t)(e.q_begin + node) * A.mask_words];
       const char* qp = A.q + ((int64_t)(e.q_begin + node) * A.q_st + (int64_t)(h * g + row - node * g) * A.q_sh) * 2 + grp * 16;
 #pragma unroll
@@ -747,7 +785,7 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
           uint64_t lo = w < 0 ? ~0ull : (w == 0 ? mask0[c] : 0), hi = w + 1 < 0 ? ~0ull : (w + 1 == 0 ? mask0[c] : 0);
           if (A.mask_words > 1) {
             const int row = min(e.row0 + (rank * C + c) * 16 + lr, e.n_rows - 1);
-            const uint64_t* mask = A.masks + (int64_t)(e.q_begin + row / g) * A.mask_words;
+            const uint64_t* mask = A.masks + (int64_t)(e.q_begin + group.of(row)) * A.mask_words;
             if (w > 0 && w < A.mask_words) lo = mask[w];
             if (w >= 0 && w + 1 < A.mask_words) hi = mask[w + 1];
           }
@@ -755,18 +793,25 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
         }
         // 0 * V is NaN where V is not finite: V behind the last token is set to
         // zero, and so are infinities and NaN of tree tokens, which go to the
-        // outputs of the rows that see them by themselves
+        // outputs of the rows that see them by themselves.  (Looked for in two
+        // halves of V: all of it at once spills registers.)
         char* v0 = kb + blk * 2 * kK + kK;
-        bool found = false;
+        u16x2 top2 = {0, 0};  // the largest magnitudes: not finite from infinity on
 #pragma unroll
-        for (int j = 0; j < NL; ++j) {
-          const int nn = j * TPI + lane / CPR;
-          if (nn < n && nn + tb >= prefix) {
-            const u32x4 x = *reinterpret_cast<const u32x4*>(v0 + (j * kWave + lane) * 16);
+        for (int j0 = 0; j0 < NL; j0 += 4) {
+          u32x4 x[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) found = found || nonfinite16<T>(x[e]) || nonfinite16<T>(x[e] >> 16);
+          for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const u32x4*>(v0 + ((j0 + j) * kWave + lane) * 16);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int nn = (j0 + j) * TPI + lane / CPR;
+            const uint32_t tree = nn < n && nn + tb >= prefix ? 0x7fff7fffu : 0u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top2 = __builtin_elementwise_max(top2, __builtin_bit_cast(u16x2, x[j][i] & tree));
           }
         }
+        constexpr int kInf = std::is_same<T, bf16_t>::value ? 0x7f80 : 0x7c00;
+        const bool found = top2[0] >= kInf || top2[1] >= kInf;
         const bool any = __builtin_amdgcn_ballot_w64(found) != 0;
         if (any) {
           for (int nn = max(0, prefix - tb); nn < n; ++nn) {
@@ -785,22 +830,24 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
             }
           }
         }
-        meet();  // both have read the block's V
+        if (any || n < kBlock) {
+          meet();  // both have read the block's V
 #pragma unroll
-        for (int j = 0; j < NL; ++j) {
-          const int nn = j * TPI + lane / CPR;
-          u32x4* p = reinterpret_cast<u32x4*>(v0 + (j * kWave + lane) * 16);
-          if (nn >= n) {
-            *p = u32x4{0u, 0u, 0u, 0u};
-          } else if (any && nn + tb >= prefix) {
-            u32x4 x = *p;
+          for (int j = 0; j < NL; ++j) {
+            const int nn = j * TPI + lane / CPR;
+            u32x4* p = reinterpret_cast<u32x4*>(v0 + (j * kWave + lane) * 16);
+            if (nn >= n) {
+              *p = u32x4{0u, 0u, 0u, 0u};
+            } else if (any && nn + tb >= prefix) {
+              u32x4 x = *p;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              x[e] &= (nonfinite16<T>(x[e]) ? 0u : 0xffffu) | (nonfinite16<T>(x[e] >> 16) ? 0u : 0xffff0000u);
-            *p = x;
+              for (int e = 0; e < 4; ++e)
+                x[e] &= (nonfinite16<T>(x[e]) ? 0u : 0xffffu) | (nonfinite16<T>(x[e] >> 16) ? 0u : 0xffff0000u);
+              *p = x;
+            }
           }
+          meet();  // (both have written the same)
         }
-        meet();  // (both have written the same)
       }
 
       f32x4 s[C][2];
@@ -926,25 +973,22 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
     constexpr int LPR = D / 4;  // lanes of a row, four dims each
     const int ch = threadIdx.x % LPR;
     float* part = A.part + ((2 * (int64_t)slot + was.second) * hkv + h) * kPartFloats;
-    for (int pr = threadIdx.x / LPR; pr < R; pr += NT / LPR) {
-      const int row = was.row0 + pr;
-      if (row >= was.n_rows) break;
-      float top = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < W; ++w) top = fmaxf(top, s_ml[w][pr][0]);
-      const float ref = top == -INFINITY ? 0.f : top;
-      float sum = 0.f;
-      f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int r0 = 0; r0 < R; r0 += NT / LPR) {
+      const int pr = r0 + threadIdx.x / LPR, row = was.row0 + pr;
+      f32x4 x[W];
+      f32x2 own[W];
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        const float wt = fast_exp2(s_ml[w][pr][0] - ref);
-        const f32x4 x = *reinterpret_cast<const f32x4*>(outs + (w * R + pr) * D + (ch ^ (pr % 16)) * 4);
-        sum = __builtin_fmaf(s_ml[w][pr][1], wt, sum);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(x[i], wt, o[i]);
+        own[w] = f32x2{s_ml[w][pr][0], s_ml[w][pr][1]};
+        x[w] = *reinterpret_cast<const f32x4*>(outs + (w * R + pr) * D + (ch ^ (pr % 16)) * 4);
       }
+      float top = -INFINITY, sum = 0.f;
+      f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+      join(top, sum, o, x, own, W);
+      if (row >= was.n_rows) continue;
       if (was.whole) {
-        store_row<T>(A, was.q_begin, h, row, ch * 4, o, top, sum, ch == 0);
+        store_row<T>(A, group, was.q_begin, h, row, ch * 4, o, top, sum, ch == 0);
       } else {
         *reinterpret_cast<f32x4*>(part + pr * D + ch * 4) = o;
         if (ch == 0) *reinterpret_cast<f32x2*>(part + R * D + pr * 2) = f32x2{top, sum};
@@ -952,28 +996,6 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
     }
     if (!more) return;
     __syncthreads();  // the outputs are read: the buffers may be filled again
-  }
-}
-
-// A weighted sum of parts with its maximum: joins N more, those past n left out.
-template <int N>
-__device__ __forceinline__ void join(float& top, float& sum, f32x4& o, const f32x4 (&x)[N], const f32x2 (&own)[N], int n) {
-  float here = top;
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (i < n) here = fmaxf(here, own[i][0]);
-  const float ref = here == -INFINITY ? 0.f : here, old = fast_exp2(top - ref);
-  top = here;
-  sum *= old;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) o[e] *= old;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    if (i >= n) break;
-    const float wt = fast_exp2(own[i][0] - ref);
-    sum = __builtin_fmaf(own[i][1], wt, sum);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[i][e], wt, o[e]);
   }
 }
 
@@ -994,6 +1016,7 @@ __global__ __launch_bounds__(256) void merge_kernel(Args A, int rows) {
   const int lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), ch = lane % LPR;
   const int row0 = pl.block * rows, n_rows = min(rows, rq.tree * (A.want.hq / hkv) - row0);
   const int64_t size = (int64_t)rows * (D + 2);
+  const Group group(A.want.hq / A.want.hkv);
   // One of several chunks lies in up to three slots: candidate i is slot i % 3 of
   // chunk i / 3's.
   const bool single = A.header->chunk_per_slot;
@@ -1046,7 +1069,7 @@ __global__ __launch_bounds__(256) void merge_kernel(Args A, int rows) {
           float top = -INFINITY, sum = 0.f;
           f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
           join(top, sum, o, x[k], own[k], n);
-          if (pr < n_rows) store_row<T>(A, rq.q_begin, h, row0 + pr, ch * 4, o, top, sum, ch == 0);
+          if (pr < n_rows) store_row<T>(A, group, rq.q_begin, h, row0 + pr, ch * 4, o, top, sum, ch == 0);
         }
       }
     };
@@ -1093,7 +1116,7 @@ __global__ __launch_bounds__(256) void merge_kernel(Args A, int rows) {
       sum = 0.f;
       o = f32x4{0.f, 0.f, 0.f, 0.f};
       join(top, sum, o, x, own, W);
-      if (r0 + lane / LPR < n_rows) store_row<T>(A, rq.q_begin, h, row0 + pr, ch * 4, o, top, sum, ch == 0);
+      if (r0 + lane / LPR < n_rows) store_row<T>(A, group, rq.q_begin, h, row0 + pr, ch * 4, o, top, sum, ch == 0);
     }
     __syncthreads();
   }
