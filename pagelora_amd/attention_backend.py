@@ -939,7 +939,7 @@ class PagedDecodeAttention:
     def run_tree(self, q: torch.Tensor, paged_kv_cache_layer) -> torch.Tensor:
         """One layer's attention of the planned trees: packed ``q`` [tokens, Hq, D],
         returns the same shape."""
-        return self.run_tree_into(q, paged_kv_cache_layer, torch.empty(q.shape, dtype=q.dtype, device=q.device))
+        return self.run_tree_into(q, paged_kv_cache_layer, torch.empty_like(q, memory_format=torch.contiguous_format))
 
     def run_tree_into(self, q: torch.Tensor, paged_kv_cache_layer, out: torch.Tensor,
                       lse: torch.Tensor | None = None) -> torch.Tensor:
