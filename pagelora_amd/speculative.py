@@ -67,10 +67,8 @@ def accept_tree(tokens: torch.Tensor, parents: torch.Tensor, picks: torch.Tensor
             _vector(picks, "picks", torch.int64, n, device),
             _vector(qo_indptr, "qo_indptr", torch.int32, batch + 1, device))
     if out is None:
-        dev = tokens.device
-        out = AcceptedTree(torch.empty((batch, max_path), dtype=torch.int32, device=dev),
-                           torch.empty(batch, dtype=torch.int32, device=dev),
-                           torch.empty((batch, max_path), dtype=torch.int64, device=dev))
+        out = AcceptedTree(parents.new_empty((batch, max_path)), parents.new_empty(batch),
+                           tokens.new_empty((batch, max_path)))
     else:
         for name, t, dtype, shape in (("path", out.path, torch.int32, (batch, max_path)),
                                       ("count", out.count, torch.int32, (batch,)),
