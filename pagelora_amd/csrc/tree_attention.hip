@@ -425,6 +425,22 @@ template <typename T> __device__ __forceinline__ bool nonfinite16(uint32_t v) {
   return (v & e) == e;
 }
 
+// A plane of two floats, bf16 cut towards zero, fp16 rounded to nearest; what it
+// leaves stays in them.
+template <typename T> __device__ __forceinline__ uint32_t plane(float& a, float& b);
+template <> __device__ __forceinline__ uint32_t plane<bf16_t>(float& a, float& b) {
+  const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+  a -= __uint_as_float(x & 0xffff0000u);
+  b -= __uint_as_float(y & 0xffff0000u);
+  return __builtin_amdgcn_perm(y, x, 0x07060302u);
+}
+template <> __device__ __forceinline__ uint32_t plane<f16_t>(float& a, float& b) {
+  const uint32_t w = pack2_hw<f16_t>(a, b);
+  a -= h_lo(w);
+  b -= h_hi(w);
+  return w;
+}
+
 struct Args {
   const char *q, *k, *v;
   char* o;
@@ -453,11 +469,14 @@ __device__ __forceinline__ bool plan_fits(const Args& A) {
 
 template <typename T> struct Softmax {
   static constexpr bool kBf16 = std::is_same<T, bf16_t>::value;
-  // Probabilities enter the product as two planes, hi + lo, of the cache's type:
-  // they carry 16 bits (bf16) or 22 (fp16), as a decode step's do, and a draft is
-  // verified by what decoding would give.  One plane saves a third of the matrix
-  // instructions: 1 x 64 nodes behind 32768 80 -> 75 us, 64 x 16 behind 8192 none.
-  static constexpr int kPlanes = 2;
+  // Probabilities enter the product as planes of the cache's type, each what the
+  // one before left: three of bf16 hold the value's 24 bits, two of fp16, the first
+  // rounded to nearest, all but the last of them.  So drafts are verified with the
+  // precision of a decode step.  Two planes of bf16 leave 2^-17, 2.3e-2 of terms that
+  // cancel to 2^-12 of themselves (three: 2.5e-3, the output's rounding).  bf16, two
+  // planes -> three: 1 x 64 nodes behind 32768 81 -> 91 us, 23 ragged requests
+  // 49 -> 54, 64 x 16 behind 8192 261 -> 269.
+  static constexpr int kPlanes = kBf16 ? 3 : 2;
   // A column's running maximum follows only scores more than kLag above it,
   // which takes the rescale out of the steady state.
   static constexpr float kLag = kBf16 ? 8.f : 1.f;
@@ -917,14 +936,9 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const f32x4 src = s[c][e / 2];
-          const float p0 = src[(e % 2) * 2], p1 = src[(e % 2) * 2 + 1];
-          const uint32_t hw = pack2_hw<T>(p0, p1);
-          pb[c][0][e] = hw;
-          if constexpr (NPP == 2) {
-            float h0, h1;
-            unpack2<T>(hw, h0, h1);
-            pb[c][NPP - 1][e] = pack2_hw<T>(p0 - h0, p1 - h1);
-          }
+          float p0 = src[(e % 2) * 2], p1 = src[(e % 2) * 2 + 1];
+#pragma unroll
+          for (int n = 0; n < NPP; ++n) pb[c][n][e] = plane<T>(p0, p1);
         }
       }
       // four independent accumulations in turn: an MFMA waits for the one before
