@@ -384,7 +384,9 @@ int pl_tree_plan(const int32_t* qo_indptr, const int32_t* kv_indptr,
  * 16-byte aligned and o 8-byte aligned.
  *
  * K and V of masked positions may hold anything, infinities and NaN included.
- * An infinity or NaN in V that a row attends makes that output infinite or NaN.
+ * An infinity in V that a row attends makes that output this infinity, however
+ * small its weight; NaN, infinities of both signs, and an infinity at a position
+ * whose K is not finite either make it NaN.
  *
  * batch, tokens, max_tree, indices_capacity, heads, head_dim and page_size are
  * the plan's: a run with others does nothing.  workspace holds partial results

@@ -512,7 +512,11 @@ __device__ __forceinline__ void store_row(const Args& A, const Group& group, int
         sum == 0.f ? -INFINITY : (top + log2f(sum) - Softmax<T>::kShift) * 0.693147180559945309f;
 }
 
-// A weighted sum of parts with its maximum: joins N more, those past n left out.
+__device__ __forceinline__ bool nonfinite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
+
+// A weighted sum of parts with its maximum: joins N more, those past n left out.  A
+// weight is above 0, also where fp32 has it as 0: then 0 times a part's infinity is
+// put right.
 template <int N>
 __device__ __forceinline__ void join(float& top, float& sum, f32x4& o, const f32x4 (&x)[N], const f32x2 (&own)[N], int n) {
   float here = top;
@@ -520,6 +524,7 @@ __device__ __forceinline__ void join(float& top, float& sum, f32x4& o, const f32
   for (int i = 0; i < N; ++i)
     if (i < n) here = fmaxf(here, own[i][0]);
   const float ref = here == -INFINITY ? 0.f : here, old = fast_exp2(top - ref);
+  const f32x4 before = o;
   top = here;
   sum *= old;
 #pragma unroll
@@ -531,6 +536,17 @@ __device__ __forceinline__ void join(float& top, float& sum, f32x4& o, const f32
     sum = __builtin_fmaf(own[i][1], wt, sum);
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[i][e], wt, o[e]);
+  }
+  const float all = (o[0] + o[1]) + (o[2] + o[3]);
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(all != all) != 0, 0)) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float f = nonfinite(before[e]) ? before[e] : 0.f;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i < n && nonfinite(x[i][e])) f += x[i][e];
+      if (f != 0.f) o[e] = f;
+    }
   }
 }
 
@@ -739,6 +755,75 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
     }
   };
 
+  // The infinities and NaN in V of the block's tokens, to the outputs of the rows that
+  // see them: a weight is above 0, however small, unless K is infinite too.  Outputs
+  // that are NaN by other causes stay so.
+  auto restore_nonfinite = [&](const Segment& e, f32x4 (&acc)[C][NA], const float (&l)[C]) {
+    constexpr uint32_t kNan = 0x7fc00001u;  // a NaN from here
+    int ln = lane;
+    asm volatile("" : "+v"(ln));  // (nothing of this is worked out ahead, in registers)
+    bool live[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      float sum = l[c];
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
+      live[c] = sum == sum;
+    }
+    auto row_of = [&](const char* cache, int t) {
+      const int page = t / page_size;
+      return cache + (clamp_page(A.indices[e.page_begin + page]) * A.page_stride + (int64_t)(t - page * page_size) * A.token_stride +
+                      (int64_t)h * A.head_stride) * 2;
+    };
+    auto any_nonfinite = [&](const char* p) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+      bool is = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) is |= nonfinite16<T>(x[i]) || nonfinite16<T>(x[i] >> 16);
+      return is;
+    };
+#pragma unroll 1
+    for (int tile = e.t_first; tile < e.t_end; ++tile) {
+      const int tb = tile * kTile + blk * kBlock, n = min(e.kv_len - tb, kBlock);
+      uint32_t found = 0;  // tokens of the block
+#pragma unroll 1
+      for (int j = 0; j < NL; ++j) {
+        const int nn = j * TPI + ln / CPR;
+        uint64_t at = __builtin_amdgcn_ballot_w64(nn < n && any_nonfinite(row_of(A.v, tb + min(nn, n - 1)) + ln % CPR * 16));
+        for (; at; at &= at - 1) found |= 1u << (j * TPI + __builtin_ctzll(at) / CPR);
+      }
+#pragma unroll 1
+      for (; found; found &= found - 1) {
+        const int t = tb + __builtin_ctz(found), node = t - e.prefix;
+        const bool no_weight = __builtin_amdgcn_ballot_w64(any_nonfinite(row_of(A.k, t) + ln % CPR * 16)) != 0;
+        bool sees[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const int row = min(e.row0 + (rank * C + c) * 16 + ln % 16, e.n_rows - 1);
+          const uint64_t* mask = A.masks + (int64_t)(e.q_begin + group.of(row)) * A.mask_words;
+          sees[c] = live[c] && (node < 0 || (node / 64 < A.mask_words && (mask[node / 64] >> (node % 64) & 1)));
+        }
+        const char* v = row_of(A.v, t) + ln / 16 * 8;
+#pragma unroll
+        for (int a = 0; a < NA; ++a) {
+          const u32x2 x = *reinterpret_cast<const u32x2*>(v + a * 32);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t b = i % 2 ? x[i / 2] >> 16 : x[i / 2] & 0xffffu;
+            float f, unused;
+            unpack2<T>(b, f, unused);
+            if (no_weight) f = __uint_as_float(kNan);
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+              const float o = acc[c][a][i], sum = o != o && __float_as_uint(o) != kNan ? f : o + f;
+              if (nonfinite16<T>(b) && sees[c]) acc[c][a][i] = sum == sum ? sum : __uint_as_float(kNan);
+            }
+          }
+        }
+      }
+    }
+  };
+
   Segment e = segment_at(pl);
   ask(e);
   for (;;) {
@@ -771,6 +856,7 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
 #pragma unroll
       for (int a = 0; a < NA; ++a) acc[c][a] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    bool bad = false;  // infinities and NaN were taken out of V
     if (t_first < t_end) load_block(offs, 0, 0);
 
     for (int tile = t_first; tile < t_end; ++tile) {
@@ -811,8 +897,8 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
           vis[c] = (uint32_t)(sh ? lo >> sh | hi << (64 - sh) : lo) & inside;
         }
         // 0 * V is NaN where V is not finite: V behind the last token is set to
-        // zero, and so are infinities and NaN of tree tokens, which go to the
-        // outputs of the rows that see them by themselves.  (Looked for in two
+        // zero, and so are infinities and NaN of nodes, which rows may not see
+        // (restore_nonfinite gives them to the rows that do).  (Looked for in two
         // halves of V: all of it at once spills registers.)
         char* v0 = kb + blk * 2 * kK + kK;
         u16x2 top2 = {0, 0};  // the largest magnitudes: not finite from infinity on
@@ -832,23 +918,7 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
         constexpr int kInf = std::is_same<T, bf16_t>::value ? 0x7f80 : 0x7c00;
         const bool found = top2[0] >= kInf || top2[1] >= kInf;
         const bool any = __builtin_amdgcn_ballot_w64(found) != 0;
-        if (any) {
-          for (int nn = max(0, prefix - tb); nn < n; ++nn) {
-#pragma unroll
-            for (int a = 0; a < NA; ++a) {
-              const u32x2 x = *reinterpret_cast<const u32x2*>(v0 + nn * RB + ((2 * a + grp / 2) ^ swz_v(nn)) * 16 + (grp % 2) * 8);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const uint32_t b = i % 2 ? x[i / 2] >> 16 : x[i / 2] & 0xffffu;
-                float f, unused;
-                unpack2<T>(b, f, unused);
-#pragma unroll
-                for (int c = 0; c < C; ++c)
-                  if (nonfinite16<T>(b) && (vis[c] >> nn & 1)) acc[c][a][i] += f;
-              }
-            }
-          }
-        }
+        bad |= any;
         if (any || n < kBlock) {
           meet();  // both have read the block's V
 #pragma unroll
@@ -960,6 +1030,16 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
       }
     }
 
+    // An infinity times a plane of a probability that is 0 is NaN too: looked at again.
+    float all = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int a = 0; a < NA; ++a)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) all += acc[c][a][i];
+    bad |= __builtin_amdgcn_ballot_w64(all != all) != 0;
+    if (__builtin_expect(bad, 0)) restore_nonfinite(e, acc, l);
     // the next row block's queries and page ids come while this one's states meet
     const Segment was = e;
     if (more) {

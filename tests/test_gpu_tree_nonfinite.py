@@ -1,0 +1,95 @@
+"""Infinities in V that a row of a tree sees: the definition's infinity, wherever the work is cut."""
+
+import numpy as np
+import pytest
+import torch
+
+from tests.test_gpu_tree_attention import backend, oracle, tables, tree_case
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16 = torch.bfloat16, torch.float16
+INF = float("inf")
+
+
+def slot(case, pos, page_size=16):
+    return case["indices"].tolist()[case["indptr"].tolist()[0] + pos // page_size], pos % page_size
+
+
+def compare(case, got, dtype):
+    """Infinities with their sign and NaN (both signs in one dim) where the definition has them; the rest within the
+    output's rounding and 1e-3, which weights off by 2^-13 make of values of up to 5 (theirs are off by less)."""
+    ref = oracle(case)[0]
+    got = got.double().cpu().numpy()
+    assert (np.isnan(got) == np.isnan(ref)).all()
+    inf = np.isinf(ref)
+    assert inf.any() and (got[inf] == ref[inf]).all() and not np.isinf(got[~inf]).any()
+    live = np.isfinite(ref)
+    assert (np.abs(got - ref)[live] <= torch.finfo(dtype).eps / 2 * np.abs(ref[live]) + 1e-3).all()
+
+
+def run(case, heads, head_dim, device, **kw):
+    be = backend(*heads, head_dim, 16, device)
+    be.plan_tree(**tables(case), tree_parents=case["parents"], **kw)
+    out = be.run_tree(case["q"], case["cache"])
+    torch.cuda.synchronize()
+    return out
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads,head_dim", [((1, 1), 128), ((4, 1), 128), ((4, 1), 64), ((4, 1), 256)])
+@pytest.mark.parametrize("tree,prefix", [(4, 0), (4, 44), (20, 44), (30, 700), (70, 1500)])
+@pytest.mark.parametrize("where", ["node", "committed", "both"])
+def test_infinite_v(gpu_device, dtype, heads, head_dim, tree, prefix, where):
+    """In nodes and in committed tokens, both signs, in the first block of a wave and in later ones, 16 to 64 rows of a
+    row block, every kv range cut in several ways."""
+    if where != "node" and not prefix:
+        pytest.skip("no committed token")
+    case = tree_case([tree], [prefix + tree], *heads, head_dim, 16, dtype, gpu_device, seed=tree + prefix)
+    at = ([prefix, prefix + tree // 2, prefix + tree - 1] if where != "committed" else []) + \
+         ([0, prefix // 2, prefix - 1] if where != "node" else [])
+    for n, pos in enumerate(at):
+        page, off = slot(case, pos)
+        case["cache_host"][page, 1, off, 0, 5 + n] = INF
+        case["cache_host"][page, 1, off, 0, 30 + n] = -INF
+        case["cache_host"][page, 1, off, 0, 50] = INF if n % 2 else -INF
+    case["cache"] = case["cache_host"].to(gpu_device)
+    for share in (0, 1, 3):
+        compare(case, run(case, heads, head_dim, gpu_device, min_share=share), dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+@pytest.mark.parametrize("tree", [1, 20, 64])
+@pytest.mark.parametrize("far", [60.0, 190.0])
+@pytest.mark.parametrize("high", [0, 210, 399])
+def test_infinite_v_far_below_the_maximum(gpu_device, dtype, head_dim, tree, far, high):
+    """The infinite V lies in tokens whose score is `far` (in e's) below the row's maximum, before and after it, a
+    weight of e^-190 among them, which fp32 does not hold: still an infinity, however the range is cut."""
+    case = tree_case([tree], [400 + tree], 1, 1, head_dim, 16, dtype, gpu_device, seed=tree)
+    q, cache = torch.zeros_like(case["q_host"]), torch.nan_to_num(case["cache_host"])
+    q[:, :, 0] = 4.0
+    cache[:, 0] = 0.0
+    page, off = slot(case, high)
+    cache[page, 0, off, 0, 0] = far * head_dim**0.5 / 4
+    for n, pos in enumerate((5, 130, 300, 398)):
+        page, off = slot(case, pos)
+        cache[page, 1, off, 0, 9 + n] = -INF
+    case.update(q_host=q, cache_host=cache, q=q.to(gpu_device), cache=cache.to(gpu_device))
+    for share in (0, 1, 2):
+        compare(case, run(case, (1, 1), head_dim, gpu_device, min_share=share), dtype)
+
+
+def test_an_infinite_v_leaves_other_requests_and_rows_their_bits(gpu_device):
+    """Rows that do not see it, of its own request and of others in the same workgroup, come out as without it."""
+    trees, lens = [24] + [3] * 40, [200] + [20 + i for i in range(40)]
+    case = tree_case(trees, lens, 2, 1, 64, 16, BF16, gpu_device, seed=4)
+    clean = run(case, (2, 1), 64, gpu_device)
+    page, off = slot(case, 176 + 7)
+    case["cache"][page, 1, off, 0, 3] = INF
+    got = run(case, (2, 1), 64, gpu_device)
+    sees = torch.from_numpy(case["sees"][0][:, 7].copy()).to(gpu_device)
+    assert torch.equal(got[24:], clean[24:]) and torch.equal(got[:24][~sees], clean[:24][~sees])
+    assert (got[:24][sees][:, :, 3] == INF).all()
+    rest = torch.arange(64, device=gpu_device) != 3
+    assert torch.equal(got[:24][sees][:, :, rest], clean[:24][sees][:, :, rest])
