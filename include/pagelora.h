@@ -356,8 +356,10 @@ size_t pl_tree_workspace_size(int batch, int tokens, int max_tree,
  *     its request where tree_mask[i][j] is not 0, and the committed tokens.
  * A row that attends nothing gets o = 0 and lse = -inf.
  *
- * Tables are device arrays; entries outside their range are clamped (T_r to
- * max_tree, a parent that is not an earlier node to -1).  plan: 16-byte
+ * Tables are device arrays; entries outside their range are clamped (a parent
+ * that is not an earlier node to -1).  Of a tree of more than max_tree nodes the
+ * first max_tree are worked on; o and lse of the others, and of rows behind the
+ * last request, stay as they are.  plan: 16-byte
  * aligned, at least pl_tree_plan_size bytes; it must be zeroed once before its
  * first use.  min_share: the kv tiles of all row blocks are dealt out in equal shares;
  * the least size of a share in tiles (0: any).  batch: up to 4096.

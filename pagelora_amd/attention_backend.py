@@ -800,9 +800,10 @@ class PagedDecodeAttention:
         Host tables are validated and uploaded.  Device tables are trusted (the
         kernels clamp every index into its buffer) and may be planned inside a
         capture; ``max_tree`` then bounds the nodes of a tree (default: all
-        tokens).  A captured :meth:`run_tree` replays on the plan that
-        ``plan_tree`` made last for the same sizes
-        (:meth:`tree_graph_signature`).  ``min_share`` > 0 keeps a workgroup's
+        tokens; of a tree that has more, the first ``max_tree`` are attended).
+        A captured :meth:`run_tree` replays on the plan that ``plan_tree`` made
+        last for the same sizes (:meth:`tree_graph_signature`).
+        ``min_share`` > 0 keeps a workgroup's
         share of the kv tiles from being less.  Plans and runs of one backend
         are ordered by the caller; the reference has no counterpart.
         """
@@ -938,13 +939,15 @@ class PagedDecodeAttention:
 
     def run_tree(self, q: torch.Tensor, paged_kv_cache_layer) -> torch.Tensor:
         """One layer's attention of the planned trees: packed ``q`` [tokens, Hq, D],
-        returns the same shape."""
+        returns the same shape.  Rows that no tree of the plan holds (behind the last
+        request, past ``max_tree`` in one) are not written: they hold anything."""
         return self.run_tree_into(q, paged_kv_cache_layer, torch.empty_like(q, memory_format=torch.contiguous_format))
 
     def run_tree_into(self, q: torch.Tensor, paged_kv_cache_layer, out: torch.Tensor,
                       lse: torch.Tensor | None = None) -> torch.Tensor:
         """Writes ``out`` ([tokens, Hq, D], head_dim contiguous) and optionally
-        ``lse`` ([tokens, Hq] fp32, natural log) for packed ``q``."""
+        ``lse`` ([tokens, Hq] fp32, natural log) for packed ``q``; rows that no
+        tree of the plan holds stay as they are."""
 
         plan = self._tree_plan
         if plan is None:

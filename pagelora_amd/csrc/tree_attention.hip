@@ -79,7 +79,7 @@ struct Header {
   int64_t share;  // tiles of a slot
 };
 static_assert(sizeof(Header) == 64, "the plan's header");
-// A request with nodes.  Its work is tiles x blocks (row blocks), from `base` of
+// A request with nodes: `prefix` tokens before them, `tree` of them worked on.  Its work is tiles x blocks (row blocks), from `base` of
 // all work on: chunk after chunk of its tiles, of a chunk row block after row
 // block.  The first `setup` tiles are none and stand for what a row block costs
 // beside its tiles.  The first `longer` chunks have chunk_len + 1 tiles, the others
@@ -88,7 +88,7 @@ static_assert(sizeof(Header) == 64, "the plan's header");
 // those), or only requests of several row blocks have several chunks, none less
 // than a share.
 struct Request {
-  int32_t q_begin, tree, page_begin, kv_len, blocks, chunks, chunk_len, longer, index, pad;
+  int32_t q_begin, tree, prefix, page_begin, kv_len, blocks, chunks, chunk_len, longer, index;
   int64_t base;
 };
 // A place in the work: of a row block (`block`) in a chunk, after `tile` tiles of
@@ -168,12 +168,14 @@ struct PlanArgs {
 __device__ __forceinline__ Request read_request(const PlanArgs& A, int r) {
   Request q{};
   q.q_begin = min(max(A.qo_indptr[r], 0), A.want.tokens);
-  q.tree = min(min(max(A.qo_indptr[r + 1], q.q_begin), A.want.tokens) - q.q_begin, A.want.max_tree);
+  const int nodes = min(max(A.qo_indptr[r + 1], q.q_begin), A.want.tokens) - q.q_begin;
+  q.tree = min(nodes, A.want.max_tree);  // the first of them
   q.page_begin = min(max(A.kv_indptr[r], 0), A.indices_count);
   const int pages = min(max(A.kv_indptr[r + 1], q.page_begin), A.indices_count) - q.page_begin;
   const int last = min(max(A.kv_last[r], 1), A.want.page_size);
   const int64_t len = pages > 0 ? (int64_t)(pages - 1) * A.want.page_size + last : 0;
   q.kv_len = (int)min(len, (int64_t)kMaxLen);
+  q.prefix = max(0, q.kv_len - nodes);
   q.chunks = 1;
   q.chunk_len = max(1, (q.kv_len + A.tile - 1) / A.tile);
   q.blocks = (int)(((int64_t)q.tree * (A.want.hq / A.want.hkv) + A.rows - 1) / A.rows);
@@ -704,7 +706,7 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
     g_.row0 = p.block * R;
     g_.n_rows = rq.tree * g;
     g_.kv_len = rq.kv_len;
-    g_.prefix = max(0, rq.kv_len - rq.tree);
+    g_.prefix = rq.prefix;
     g_.n_pages = (rq.kv_len + page_size - 1) / page_size;
     const int upto = single ? c_tiles : (int)min((int64_t)c_tiles, p.tile + left);
     g_.units = upto - p.tile;
