@@ -360,8 +360,8 @@ size_t pl_tree_workspace_size(int batch, int tokens, int max_tree,
  * that is not an earlier node to -1).  Of a tree of more than max_tree nodes the
  * first max_tree are worked on; o and lse of the others, and of rows behind the
  * last request, stay as they are.  plan: 16-byte
- * aligned, at least pl_tree_plan_size bytes; it must be zeroed once before its
- * first use.  min_share: the kv tiles of all row blocks are dealt out in equal shares;
+ * aligned, at least pl_tree_plan_size bytes; zeroed once where a run may come
+ * before its first plan.  min_share: the kv tiles of all row blocks are dealt out in equal shares;
  * the least size of a share in tiles (0: any).  batch: up to 4096.
  */
 int pl_tree_plan(const int32_t* qo_indptr, const int32_t* kv_indptr,

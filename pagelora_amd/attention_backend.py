@@ -239,8 +239,7 @@ class PagedDecodeAttention:
         self._decode_host_uploads: deque = deque()
         self._plan: dict | None = None
         self._tree_plan: dict | None = None
-        self._tree_buffers: dict[int, torch.Tensor] = {}  # by size class
-        self._tree_kept: dict[tuple, torch.Tensor] = {}   # by sizes: those that captured graphs use
+        self._tree_kept: dict[tuple, dict] = {}  # by sizes: the last plan in a buffer that captured graphs use
 
     # ------------------------------------------------------------ planning
     def plan_decode(
@@ -804,8 +803,10 @@ class PagedDecodeAttention:
         A captured :meth:`run_tree` replays on the plan that ``plan_tree`` made
         last for the same sizes (:meth:`tree_graph_signature`).
         ``min_share`` > 0 keeps a workgroup's
-        share of the kv tiles from being less.  Plans and runs of one backend
-        are ordered by the caller; the reference has no counterpart.
+        share of the kv tiles from being less.  Runs on any stream read the plan
+        that was made before the call, also where another plan is made while
+        they wait; replays are ordered with the plans by the caller.  The
+        reference has no counterpart.
         """
 
         tables = (qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len)
@@ -866,47 +867,50 @@ class PagedDecodeAttention:
             if plan_bytes == 0:
                 _lib.check(_lib.PL_ERR_UNSUPPORTED, "pl_tree_plan_size")
             captured = torch.cuda.is_current_stream_capturing()
-            buffer = self._tree_buffer(plan_bytes, (sizes, capacity), captured)
             stream = torch.cuda.current_stream(self.device)
+            streams = {stream.cuda_stream: stream}
+            kept = self._tree_kept.get((sizes, capacity))
+            if kept is None:
+                buffer = torch.empty(plan_bytes, dtype=torch.uint8, device=self.device)
+            else:
+                buffer = kept["buffer"]
+                streams = {**kept["streams"], **streams}
+                if not captured:  # what runs on other streams is done with the plan that the buffer holds
+                    for raw, other in streams.items():
+                        if raw != stream.cuda_stream:
+                            stream.wait_stream(other)
+                    streams = {stream.cuda_stream: stream}
             parents_ptr, mask_ptr, mask_ld = (tree.data_ptr(), None, 0) if tree_parents is not None else (
                 None, tree.data_ptr(), tree.shape[1])
             _lib.check(self._lib.pl_tree_plan(
                 tables[0].data_ptr(), tables[1].data_ptr(), tables[2].data_ptr(), num_indices, tables[3].data_ptr(),
                 *sizes, parents_ptr, mask_ptr, mask_ld, *heads, self.page_size, int(min_share), capacity,
                 buffer.data_ptr(), buffer.numel(), stream.cuda_stream), "pl_tree_plan")
-            self._tree_plan = {
+            plan = self._tree_plan = {
                 "device": index,
                 "sizes": sizes,
-                "bytes": plan_bytes,
-                "kept": captured,
+                "kept": False,
                 "tokens": tokens,
                 "capacity": capacity,
                 "buffer": buffer,
                 "buffer_args": (buffer.data_ptr(), buffer.numel()),
                 "workspace_bytes": self._lib.pl_tree_workspace_size(*sizes, *heads),
                 "max_page": max_page,
-                "stream": stream.cuda_stream,
+                "raw_stream": stream.cuda_stream,
                 "ready": None if captured else stream.record_event(),
+                "streams": streams,  # that plan in its buffer or read it
             }
+            if captured or kept is not None:
+                self._keep_tree_plan(plan)
+
+    def _keep_tree_plan(self, plan: dict) -> None:
+        """From now on the plans of these sizes are made in this plan's buffer, which lives as long as the backend: a
+        captured graph reads or writes it."""
+        plan["kept"] = True
+        self._tree_kept[plan["sizes"], plan["capacity"]] = plan
 
     def _device_index(self) -> int:
         return self.workspace_buffer.get_device()
-
-    def _tree_buffer(self, nbytes: int, key, keep: bool) -> torch.Tensor:
-        """The plan buffer of the sizes ``key``: one that plans of a size class
-        share, or with ``keep`` (a capture reads or writes it) one that no plan
-        of other sizes is made in from now on.  All live as long as the backend."""
-        kept, shared = self._tree_kept, self._tree_buffers
-        if key in kept:
-            return kept[key]
-        size = 1 << (nbytes - 1).bit_length()
-        if size not in shared:
-            # zeros: no header of an earlier owner of the memory
-            shared[size] = torch.zeros(size, dtype=torch.uint8, device=self.device)
-        if keep:
-            kept[key] = shared.pop(size)
-            return kept[key]
-        return shared[size]
 
     def _validate_host_trees(self, qo_indptr, kv_indptr, kv_indices, kv_last, parents, tokens) -> tuple[int, int]:
         """Check host tables of trees; returns (largest page id or -1, nodes of the widest tree)."""
@@ -974,12 +978,14 @@ class PagedDecodeAttention:
             raise RuntimeError(f"run_tree needs tensors on the backend's device {self.device}")
         with _lib.on_device(device):
             stream = _lib.raw_stream(device)
-            if not plan["kept"] and torch.cuda.is_current_stream_capturing():
-                self._tree_buffer(plan["bytes"], (plan["sizes"], plan["capacity"]), True)
-                plan["kept"] = True
-            if stream != plan["stream"] and plan["ready"] is not None \
-                    and not torch.cuda.is_current_stream_capturing():
-                torch.cuda.current_stream(device).wait_event(plan["ready"])
+            if (not plan["kept"] or stream not in plan["streams"]) and torch.cuda.is_current_stream_capturing():
+                if not plan["kept"]:
+                    self._keep_tree_plan(plan)
+            elif stream not in plan["streams"]:
+                plan["streams"][stream] = away = torch.cuda.current_stream(device)
+                plan["buffer"].record_stream(away)
+                if plan["ready"] is not None:
+                    away.wait_event(plan["ready"])
             # per call, from torch's allocator: calls on other streams and graphs share nothing
             nbytes = plan["workspace_bytes"]
             ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
