@@ -374,6 +374,23 @@ int pl_tree_plan(const int32_t* qo_indptr, const int32_t* kv_indptr,
                  void* stream);
 
 /*
+ * pl_tree_plan with the page ids copied to memory of their own, `ids` with room
+ * for ids_capacity >= num_indices: the plan buffer is one of indices_capacity 0,
+ * whose size and place no longer go by the sequences' lengths, and a captured
+ * pl_tree_run follows plans of any number of pages.  ids is read by the runs: it
+ * lives as long as the plan is used.
+ */
+int pl_tree_plan_ids(const int32_t* qo_indptr, const int32_t* kv_indptr,
+                     const int32_t* kv_indices, int num_indices,
+                     const int32_t* kv_last_page_len, int batch, int tokens,
+                     int max_tree, const int32_t* tree_parents,
+                     const uint8_t* tree_mask, int64_t mask_ld,
+                     int num_qo_heads, int num_kv_heads, int head_dim,
+                     int page_size, int min_share, int32_t* ids,
+                     int ids_capacity, void* plan, size_t plan_bytes,
+                     void* stream);
+
+/*
  * Attention of the planned trees:
  *   o[t, hq] = softmax(q[t, hq] . K_r[:, hq / g]^T * sm_scale, masked) . V_r
  * q and o are [tokens, num_qo_heads, head_dim] with strides (stride_t,

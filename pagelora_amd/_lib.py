@@ -258,6 +258,16 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             _i32, _i32, _vp, _sz, _vp,   # min_share, indices_capacity, plan, bytes, stream
         ],
     ),
+    "pl_tree_plan_ids": (
+        _i32,
+        [
+            _vp, _vp, _vp, _i32, _vp,    # qo_indptr, kv_indptr, kv_indices, their number, last_page_len
+            _i32, _i32, _i32,            # batch, tokens, max_tree
+            _vp, _vp, _i64,              # tree_parents, tree_mask, mask_ld
+            _i32, _i32, _i32, _i32,      # hq, hkv, head_dim, page_size
+            _i32, _vp, _i32, _vp, _sz, _vp,  # min_share, ids, ids_capacity, plan, bytes, stream
+        ],
+    ),
     "pl_tree_run": (
         _i32,
         [

@@ -801,10 +801,12 @@ class PagedDecodeAttention:
         capture; ``max_tree`` then bounds the nodes of a tree (default: all
         tokens; of a tree that has more, the first ``max_tree`` are attended).
         A captured :meth:`run_tree` replays on the plan that ``plan_tree`` made
-        last for the same sizes (:meth:`tree_graph_signature`).
-        ``min_share`` > 0 keeps a workgroup's
-        share of the kv tiles from being less.  Runs on any stream read the plan
-        that was made before the call, also where another plan is made while
+        last for the same sizes (:meth:`tree_graph_signature`: requests, nodes,
+        ``max_tree``), whatever its sequences' lengths; a replayed ``plan_tree``
+        counts as made then.  The backend keeps a plan buffer for each sizes that
+        were captured.  ``min_share`` > 0 keeps a workgroup's share of the kv
+        tiles from being less.  Runs on any stream read the plan that was made
+        before the call, also where another plan is made while
         they wait; replays are ordered with the plans by the caller.  The
         reference has no counterpart.
         """
@@ -860,20 +862,24 @@ class PagedDecodeAttention:
                 tables = [t.contiguous() for t in tables]
                 tree = tree.contiguous()
             num_indices = tables[2].numel()
-            capacity = max(16, self.max_pages, 1 << max(0, num_indices - 1).bit_length())
             sizes = (batch, tokens, max_tree)
             heads = (self.num_qo_heads, self.num_kv_heads, self.head_dim)
-            plan_bytes = self._lib.pl_tree_plan_size(*sizes, capacity, *heads)
+            plan_bytes = self._lib.pl_tree_plan_size(*sizes, 0, *heads)
             if plan_bytes == 0:
                 _lib.check(_lib.PL_ERR_UNSUPPORTED, "pl_tree_plan_size")
             captured = torch.cuda.is_current_stream_capturing()
             stream = torch.cuda.current_stream(self.device)
             streams = {stream.cuda_stream: stream}
-            kept = self._tree_kept.get((sizes, capacity))
-            if kept is None:
-                buffer = torch.empty(plan_bytes, dtype=torch.uint8, device=self.device)
+            kept = self._tree_kept.get(sizes)
+            if kept is None:  # the plan, then the page ids
+                buffer = torch.empty(plan_bytes + 4 * num_indices, dtype=torch.uint8, device=self.device)
+                ids = buffer[plan_bytes:].view(torch.int32)
+                held = [buffer]
             else:
-                buffer = kept["buffer"]
+                buffer, ids, held = kept["buffer"], kept["ids"], kept["held"]
+                if ids.numel() < num_indices:  # (graphs may read or write the former ones)
+                    ids = torch.empty(1 << (num_indices - 1).bit_length(), dtype=torch.int32, device=self.device)
+                    held.append(ids)
                 streams = {**kept["streams"], **streams}
                 if not captured:  # what runs on other streams is done with the plan that the buffer holds
                     for raw, other in streams.items():
@@ -882,18 +888,19 @@ class PagedDecodeAttention:
                     streams = {stream.cuda_stream: stream}
             parents_ptr, mask_ptr, mask_ld = (tree.data_ptr(), None, 0) if tree_parents is not None else (
                 None, tree.data_ptr(), tree.shape[1])
-            _lib.check(self._lib.pl_tree_plan(
+            _lib.check(self._lib.pl_tree_plan_ids(
                 tables[0].data_ptr(), tables[1].data_ptr(), tables[2].data_ptr(), num_indices, tables[3].data_ptr(),
-                *sizes, parents_ptr, mask_ptr, mask_ld, *heads, self.page_size, int(min_share), capacity,
-                buffer.data_ptr(), buffer.numel(), stream.cuda_stream), "pl_tree_plan")
+                *sizes, parents_ptr, mask_ptr, mask_ld, *heads, self.page_size, int(min_share), ids.data_ptr(),
+                ids.numel(), buffer.data_ptr(), plan_bytes, stream.cuda_stream), "pl_tree_plan_ids")
             plan = self._tree_plan = {
                 "device": index,
                 "sizes": sizes,
                 "kept": False,
                 "tokens": tokens,
-                "capacity": capacity,
                 "buffer": buffer,
-                "buffer_args": (buffer.data_ptr(), buffer.numel()),
+                "buffer_args": (buffer.data_ptr(), plan_bytes),
+                "ids": ids,
+                "held": held,  # all memory that it and the plans before it in this buffer read
                 "workspace_bytes": self._lib.pl_tree_workspace_size(*sizes, *heads),
                 "max_page": max_page,
                 "raw_stream": stream.cuda_stream,
@@ -904,10 +911,10 @@ class PagedDecodeAttention:
                 self._keep_tree_plan(plan)
 
     def _keep_tree_plan(self, plan: dict) -> None:
-        """From now on the plans of these sizes are made in this plan's buffer, which lives as long as the backend: a
-        captured graph reads or writes it."""
+        """From now on the plans of these sizes, of any number of pages, are made in this plan's buffer, which lives as
+        long as the backend: a captured graph reads or writes it."""
         plan["kept"] = True
-        self._tree_kept[plan["sizes"], plan["capacity"]] = plan
+        self._tree_kept[plan["sizes"]] = plan
 
     def _device_index(self) -> int:
         return self.workspace_buffer.get_device()
@@ -939,7 +946,7 @@ class PagedDecodeAttention:
         part of it."""
         plan = self._tree_plan or {}
         buffer = plan.get("buffer")
-        return (id(self), plan.get("sizes"), plan.get("capacity"), buffer.data_ptr() if buffer is not None else None)
+        return (id(self), plan.get("sizes"), buffer.data_ptr() if buffer is not None else None)
 
     def run_tree(self, q: torch.Tensor, paged_kv_cache_layer) -> torch.Tensor:
         """One layer's attention of the planned trees: packed ``q`` [tokens, Hq, D],
@@ -983,7 +990,8 @@ class PagedDecodeAttention:
                     self._keep_tree_plan(plan)
             elif stream not in plan["streams"]:
                 plan["streams"][stream] = away = torch.cuda.current_stream(device)
-                plan["buffer"].record_stream(away)
+                for memory in plan["held"]:
+                    memory.record_stream(away)
                 if plan["ready"] is not None:
                     away.wait_event(plan["ready"])
             # per call, from torch's allocator: calls on other streams and graphs share nothing
@@ -996,7 +1004,7 @@ class PagedDecodeAttention:
                 out.data_ptr(), os_[0], os_[1], lse.data_ptr() if lse is not None else None,
                 *plan["sizes"], self.num_qo_heads, self.num_kv_heads, self.head_dim, self.page_size,
                 self.sm_scale, _lib.dtype_code(dtype),
-                *plan["buffer_args"], plan["capacity"], ws.data_ptr(), nbytes, stream,
+                *plan["buffer_args"], 0, ws.data_ptr(), nbytes, stream,
             )
             _lib.check(status, "pl_tree_run")
         return out

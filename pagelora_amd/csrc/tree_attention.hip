@@ -73,12 +73,13 @@ typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
 // What a plan was made for, then what it holds.
-struct Header {
+struct alignas(64) Header {
   int32_t magic, batch, tokens, max_tree, indices_capacity, hq, hkv, head_dim, page_size;
   int32_t num_requests, num_slots, num_shared, chunk_per_slot, setup;
-  int64_t share;  // tiles of a slot
+  int64_t share;     // tiles of a slot
+  uint64_t indices;  // the address of the page ids: in the plan or apart from it
 };
-static_assert(sizeof(Header) == 64, "the plan's header");
+static_assert(sizeof(Header) == 128, "the plan's header");
 // A request with nodes: `prefix` tokens before them, `tree` of them worked on.  Its work is tiles x blocks (row blocks), from `base` of
 // all work on: chunk after chunk of its tiles, of a chunk row block after row
 // block.  The first `setup` tiles are none and stand for what a row block costs
@@ -367,6 +368,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs A) {
     h.chunk_per_slot = single;
     h.setup = setup;
     h.share = share;
+    h.indices = (uint64_t)A.indices;
     *A.header = h;
   }
 }
@@ -451,7 +453,6 @@ struct Args {
   const Request* requests;
   const Place *first, *shared;
   const uint64_t* masks;
-  const int32_t* indices;
   int64_t q_st, q_sh, o_st, o_sh, page_stride, token_stride, head_stride, num_pages;  // elements
   Header want;
   int slots, mask_words;
@@ -593,6 +594,7 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
   if (slot >= A.header->num_slots) return;
   const bool single = A.header->chunk_per_slot;
   const int setup = A.header->setup;
+  const int32_t* indices = gptr<const int32_t*>(A.header->indices);
   const int n_requests = A.header->num_requests;
   int64_t left = share;  // tiles of the share to come
 
@@ -734,7 +736,7 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
     const int t = PAGE16 ? (tile + lane / 2) * kTile + blk * kBlock + (lane % 2) * 16
                          : min(tile * kTile + blk * kBlock + lane % kBlock, e.kv_len - 1);
     const int page = t / page_size;
-    return Offset{A.indices[e.page_begin + min(page, e.n_pages - 1)], (int64_t)(t - page * page_size) * A.token_stride};
+    return Offset{indices[e.page_begin + min(page, e.n_pages - 1)], (int64_t)(t - page * page_size) * A.token_stride};
   };
   auto offsets = [&](const Offset& o) -> int64_t { return (clamp_page(o.id) * A.page_stride + o.rest) * 2; };
 
@@ -774,7 +776,7 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
     }
     auto row_of = [&](const char* cache, int t) {
       const int page = t / page_size;
-      return cache + (clamp_page(A.indices[e.page_begin + page]) * A.page_stride + (int64_t)(t - page * page_size) * A.token_stride +
+      return cache + (clamp_page(indices[e.page_begin + page]) * A.page_stride + (int64_t)(t - page * page_size) * A.token_stride +
                       (int64_t)h * A.head_stride) * 2;
     };
     auto any_nonfinite = [&](const char* p) {
@@ -1308,17 +1310,19 @@ extern "C" size_t pl_tree_workspace_size(int batch, int tokens, int max_tree, in
   return workspace_bytes(l, num_kv_heads, head_dim);
 }
 
-extern "C" int pl_tree_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices,
-                            int num_indices, const int32_t* kv_last_page_len, int batch, int tokens, int max_tree,
-                            const int32_t* tree_parents, const uint8_t* tree_mask, int64_t mask_ld, int num_qo_heads,
-                            int num_kv_heads, int head_dim, int page_size, int min_share, int indices_capacity, void* plan,
-                            size_t plan_bytes, void* stream) {
+namespace {
+// `ids`: where the page ids go, or null: behind the rest of the plan, room for indices_capacity.
+int make_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices, int num_indices,
+              const int32_t* kv_last_page_len, int batch, int tokens, int max_tree, const int32_t* tree_parents,
+              const uint8_t* tree_mask, int64_t mask_ld, int num_qo_heads, int num_kv_heads, int head_dim, int page_size,
+              int min_share, int32_t* ids, int ids_capacity, int indices_capacity, void* plan, size_t plan_bytes,
+              void* stream) {
   if (int st = check_sizes(batch, tokens, max_tree, indices_capacity, num_qo_heads, num_kv_heads, head_dim, page_size))
     return st;
   if (batch == 0 || tokens == 0) return ok();
-  if (num_indices < 0 || num_indices > indices_capacity)
-    return fail(PL_ERR_INVALID, "num_indices (%d) must be in [0, indices_capacity = %d]", num_indices,
-                indices_capacity);
+  if (num_indices < 0 || num_indices > ids_capacity)
+    return fail(PL_ERR_INVALID, "num_indices (%d) must be in [0, %s = %d]", num_indices,
+                ids ? "ids_capacity" : "indices_capacity", ids_capacity);
   if (!qo_indptr || !kv_indptr || !kv_last_page_len || !plan || (num_indices > 0 && !kv_indices))
     return fail(PL_ERR_INVALID, "null pointer argument");
   if (!tree_parents == !tree_mask) return fail(PL_ERR_INVALID, "give tree_parents or tree_mask, and not both");
@@ -1342,7 +1346,7 @@ extern "C" int pl_tree_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, 
   a.first = (Place*)(base + l.first);
   a.shared = (Place*)(base + l.shared);
   a.masks = (uint64_t*)(base + l.masks);
-  a.indices = (int32_t*)(base + l.indices);
+  a.indices = ids ? ids : (int32_t*)(base + l.indices);
   a.want = wanted(batch, tokens, max_tree, indices_capacity, num_qo_heads, num_kv_heads, head_dim, page_size);
   a.indices_count = num_indices;
   a.rows = l.rows;
@@ -1355,6 +1359,29 @@ extern "C" int pl_tree_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, 
   hipLaunchKernelGGL(plan_kernel, dim3(grid), dim3(kPlanThreads), 0, (hipStream_t)stream, a);
   PL_LAUNCH_CHECK("tree plan_kernel");
   return ok();
+}
+}  // namespace
+
+extern "C" int pl_tree_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices,
+                            int num_indices, const int32_t* kv_last_page_len, int batch, int tokens, int max_tree,
+                            const int32_t* tree_parents, const uint8_t* tree_mask, int64_t mask_ld, int num_qo_heads,
+                            int num_kv_heads, int head_dim, int page_size, int min_share, int indices_capacity, void* plan,
+                            size_t plan_bytes, void* stream) {
+  return make_plan(qo_indptr, kv_indptr, kv_indices, num_indices, kv_last_page_len, batch, tokens, max_tree, tree_parents,
+                   tree_mask, mask_ld, num_qo_heads, num_kv_heads, head_dim, page_size, min_share, nullptr,
+                   indices_capacity, indices_capacity, plan, plan_bytes, stream);
+}
+
+extern "C" int pl_tree_plan_ids(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices,
+                                int num_indices, const int32_t* kv_last_page_len, int batch, int tokens, int max_tree,
+                                const int32_t* tree_parents, const uint8_t* tree_mask, int64_t mask_ld, int num_qo_heads,
+                                int num_kv_heads, int head_dim, int page_size, int min_share, int32_t* ids,
+                                int ids_capacity, void* plan, size_t plan_bytes, void* stream) {
+  if (num_indices > 0 && !ids) return fail(PL_ERR_INVALID, "null pointer argument");
+  if ((uintptr_t)ids % 4) return fail(PL_ERR_INVALID, "ids must be 4-byte aligned");
+  return make_plan(qo_indptr, kv_indptr, kv_indices, num_indices, kv_last_page_len, batch, tokens, max_tree, tree_parents,
+                   tree_mask, mask_ld, num_qo_heads, num_kv_heads, head_dim, page_size, min_share, ids, ids_capacity, 0,
+                   plan, plan_bytes, stream);
 }
 
 extern "C" int pl_tree_run(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_cache,
@@ -1397,7 +1424,6 @@ extern "C" int pl_tree_run(const void* q, int64_t q_stride_t, int64_t q_stride_h
   a.first = (const Place*)(base + l.first);
   a.shared = (const Place*)(base + l.shared);
   a.masks = (const uint64_t*)(base + l.masks);
-  a.indices = (const int32_t*)(base + l.indices);
   a.q_st = q_stride_t;
   a.q_sh = q_stride_h;
   a.o_st = o_stride_t;

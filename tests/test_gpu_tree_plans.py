@@ -1,4 +1,4 @@
-"""Plans of trees: of fewer nodes than a tree has, and beside runs on other streams."""
+"""Plans of trees: captured runs as their sequences grow, fewer nodes than a tree has, runs on other streams."""
 
 import pytest
 import torch
@@ -6,6 +6,75 @@ import torch
 from tests.test_gpu_tree_attention import BF16, F16, backend, check, oracle, tables, tree_case
 
 pytestmark = pytest.mark.gpu
+
+
+def grown(lens, trees=(6, 9), seed=3):
+    """The same trees behind sequences of other lengths, in pools of one size."""
+    cases = [tree_case(list(trees), [n + trees[0], n // 2 + trees[1]], 8, 2, 128, 16, BF16, "cpu", seed=seed + n)
+             for n in lens]
+    pool = max(c["cache_host"].shape[0] for c in cases)
+    for c in cases:
+        cache = torch.full((pool, *c["cache_host"].shape[1:]), float("nan"), dtype=BF16)
+        cache[: c["cache_host"].shape[0]] = c["cache_host"]
+        c["cache_host"] = cache
+    return cases
+
+
+def test_a_captured_run_follows_its_sequences_past_any_number_of_pages(gpu_device):
+    """The tables list 14 pages when the run is captured, then 17, 40, 300 and 14 again: plans of the same sizes."""
+    cases = grown([100, 130, 400, 3000, 100, 2000])
+    be = backend(8, 2, 128, 16, gpu_device)
+    q, cache = cases[0]["q"].to(gpu_device), cases[0]["cache_host"].to(gpu_device)
+    out = torch.empty_like(q)
+    be.plan_tree(**tables(cases[0]), tree_parents=cases[0]["parents"])
+    be.run_tree_into(q, cache, out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        be.run_tree_into(q, cache, out)
+    signature = be.tree_graph_signature()
+    for n, c in enumerate(cases):
+        q.copy_(c["q_host"])
+        cache.copy_(c["cache_host"])
+        t = tables(c) if n % 2 == 0 else tables(c, gpu_device)
+        be.plan_tree(**t, tree_parents=c["parents"] if n % 2 == 0 else c["parents"].to(gpu_device), max_tree=9)
+        assert be.tree_graph_signature() == signature
+        for _ in range(2):
+            out.fill_(float("nan"))
+            graph.replay()
+            torch.cuda.synchronize()
+            check(c, out)
+        check(c, be.run_tree(q, cache))
+
+
+def test_a_captured_plan_beside_plans_of_more_pages(gpu_device):
+    """A graph of plan and run, replayed after eager plans of the same sizes and more pages: each reads its own page ids."""
+    small, large = grown([40, 3000])
+    be = backend(8, 2, 128, 16, gpu_device)
+    dev = tables(small, gpu_device)
+    parents = small["parents"].to(gpu_device)
+    q, cache = small["q"].to(gpu_device), small["cache_host"].to(gpu_device)
+    out = torch.empty_like(q)
+
+    def step():
+        be.plan_tree(**dev, tree_parents=parents, max_tree=9)
+        be.run_tree_into(q, cache, out)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(3):
+        be.plan_tree(**tables(large), tree_parents=large["parents"], max_tree=9)
+        check(large, be.run_tree(large["q"].to(gpu_device), large["cache_host"].to(gpu_device)))
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        check(small, out)
 
 
 @pytest.mark.parametrize("mask", [False, True])
