@@ -218,8 +218,11 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs A) {
     const int64_t step = (int64_t)(gridDim.x - 1) * kPlanThreads;
     const int64_t first = (int64_t)(blockIdx.x - 1) * kPlanThreads + tid;
     for (int64_t i = first; i < A.indices_count; i += step) A.indices[i] = A.kv_indices[i];
-    for (int64_t i = first; i < (int64_t)A.want.tokens * A.mask_words; i += step) {
-      const int t = (int)(i / A.mask_words), w = (int)(i % A.mask_words);
+    // Given by parents, a thread packs a token's words from the last to the first on
+    // one walk to the root; given by a mask, a thread packs a word.
+    const int words = A.parents ? A.mask_words : 1;
+    for (int64_t i = first; i < (int64_t)A.want.tokens * A.mask_words / words; i += step) {
+      const int t = (int)(i * words / A.mask_words);
       int lo = 0, hi = batch;  // the request that holds token t: the last whose first token is <= t
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -227,22 +230,25 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs A) {
       }
       const Request q = read_request(A, lo);
       const int node = t - q.q_begin;
-      uint64_t bits = 0;
-      if (node >= 0 && node < q.tree) {
-        if (A.parents) {
-          // a parent is an earlier node: the walk ends
-          for (int at = node; at >= 0;) {
-            if (at / 64 == w) bits |= 1ull << (at % 64);
+      const bool on = node >= 0 && node < q.tree;
+      if (A.parents) {
+        int at = on ? node : -1;
+        for (int w = words - 1; w >= 0; --w) {
+          uint64_t bits = 0;
+          while (at >= w * 64) {  // a parent is an earlier node: the walk ends
+            bits |= 1ull << (at % 64);
             const int up = A.parents[q.q_begin + at];
             at = up < at ? up : -1;
           }
-        } else {
-          const uint8_t* m = A.mask + (int64_t)t * A.mask_ld + w * 64;
-          const int n = min(q.tree - w * 64, 64);
-          for (int j = 0; j < n; ++j) bits |= (uint64_t)(m[j] != 0) << j;
+          A.masks[i * words + w] = bits;
         }
+      } else {
+        const int w = (int)(i % A.mask_words), n = on ? min(q.tree - w * 64, 64) : 0;
+        const uint8_t* m = A.mask + (int64_t)t * A.mask_ld + w * 64;
+        uint64_t bits = 0;
+        for (int j = 0; j < n; ++j) bits |= (uint64_t)(m[j] != 0) << j;
+        A.masks[i] = bits;
       }
-      A.masks[i] = bits;
     }
     return;
   }
@@ -1354,7 +1360,7 @@ int make_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t*
   a.slots = l.slots;
   a.mask_words = l.mask_words;
   a.min_share = min_share;
-  const int64_t side = std::max<int64_t>(num_indices, (int64_t)tokens * l.mask_words);
+  const int64_t side = std::max<int64_t>(num_indices, (int64_t)tokens * (tree_parents ? 1 : l.mask_words));
   const int grid = 1 + (int)std::min<int64_t>(255, (side + kPlanThreads - 1) / kPlanThreads);
   hipLaunchKernelGGL(plan_kernel, dim3(grid), dim3(kPlanThreads), 0, (hipStream_t)stream, a);
   PL_LAUNCH_CHECK("tree plan_kernel");

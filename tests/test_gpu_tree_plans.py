@@ -133,3 +133,35 @@ def test_a_plan_made_while_a_run_waits_on_another_stream(gpu_device, kept):
         for out in (*waits, last):
             check(first, out)
         check(second, now)
+
+
+@pytest.mark.parametrize("kind", ["chain", "tree"])
+def test_deep_trees_by_parents_and_by_mask(gpu_device, kind):
+    """Masks of many words, packed on one walk to the root: the same bits as from the mask that says the same."""
+    n = 5000 if kind == "chain" else 3001
+    parents = torch.arange(-1, n - 1) if kind == "chain" else (torch.rand(n, generator=torch.Generator().manual_seed(1))
+                                                               * torch.arange(n)).long()
+    parents[0] = -1
+    sees = torch.zeros((n, n), dtype=torch.bool)
+    for i, up in enumerate(parents.tolist()):
+        if up >= 0:
+            sees[i] = sees[up]
+        sees[i, i] = True
+    length = n + 40
+    pages = -(-length // 16)
+    t = {"qo_indptr": [0, n], "paged_kv_indptr": [0, pages], "paged_kv_indices": list(range(pages))[::-1],
+         "paged_kv_last_page_len": [length - (pages - 1) * 16]}
+    t = {k: torch.tensor(v, dtype=torch.int32) for k, v in t.items()}
+    gen = torch.Generator(device=gpu_device).manual_seed(2)
+    q = torch.randn((n, 2, 64), device=gpu_device, generator=gen).to(F16)
+    cache = torch.randn((pages, 2, 16, 1, 64), device=gpu_device, generator=gen).to(F16)
+    be = backend(2, 1, 64, 16, gpu_device)
+    be.plan_tree(**t, tree_mask=sees)
+    want = be.run_tree(q, cache)
+    be.plan_tree(**t, tree_parents=parents.int())
+    assert torch.equal(be.run_tree(q, cache), want)
+    if kind == "chain":
+        be.plan_prefill(**t)
+        causal = be.run_prefill(q, cache).float()
+        # two roundings to fp16, and weights off by less than 2^-13 for values of up to 5
+        assert ((want.float() - causal).abs() <= 2.0**-10 * causal.abs() + 1e-3).all()
