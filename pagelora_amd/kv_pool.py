@@ -63,7 +63,8 @@ def kv_copy_pages(cache: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -
     if device < 0:
         raise RuntimeError("kv_copy_pages needs a cache on a ROCm device")
     page = math.prod(shape[2:])
-    if strides[2:] != (page // 2, shape[4] * shape[5], shape[5], 1):
+    # (the stride of a dim of one entry says nothing)
+    if any(n > 1 and a != b for n, a, b in zip(shape[2:], strides[2:], (page // 2, shape[4] * shape[5], shape[5], 1))):
         raise ValueError("the pages of the KV cache must be contiguous")
     with _lib.on_device(device):
         _lib.check(_lib.load().pl_kv_copy_pages(
