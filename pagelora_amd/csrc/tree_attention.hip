@@ -768,7 +768,7 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
   // The infinities and NaN in V of the block's tokens, to the outputs of the rows that
   // see them: a weight is above 0, however small, unless K is infinite too.  Outputs
   // that are NaN by other causes stay so.
-  auto restore_nonfinite = [&](const Segment& e, f32x4 (&acc)[C][NA], const float (&l)[C]) {
+  auto restore_nonfinite = [&](const Segment& e, int from, f32x4 (&acc)[C][NA], const float (&l)[C]) {  // from a tile on
     constexpr uint32_t kNan = 0x7fc00001u;  // a NaN from here
     int ln = lane;
     asm volatile("" : "+v"(ln));  // (nothing of this is worked out ahead, in registers)
@@ -793,7 +793,7 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
       return is;
     };
 #pragma unroll 1
-    for (int tile = e.t_first; tile < e.t_end; ++tile) {
+    for (int tile = from; tile < e.t_end; ++tile) {
       const int tb = tile * kTile + blk * kBlock, n = min(e.kv_len - tb, kBlock);
       uint32_t found = 0;  // tokens of the block
 #pragma unroll 1
@@ -1040,7 +1040,7 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
       }
     }
 
-    // An infinity times a plane of a probability that is 0 is NaN too: looked at again.
+    // An infinity of a committed token times a plane of a probability that is 0 is NaN.
     float all = 0.f;
 #pragma unroll
     for (int c = 0; c < C; ++c)
@@ -1048,8 +1048,8 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
       for (int a = 0; a < NA; ++a)
 #pragma unroll
         for (int i = 0; i < 4; ++i) all += acc[c][a][i];
-    bad |= __builtin_amdgcn_ballot_w64(all != all) != 0;
-    if (__builtin_expect(bad, 0)) restore_nonfinite(e, acc, l);
+    const bool nan = __builtin_amdgcn_ballot_w64(all != all) != 0;
+    if (__builtin_expect(bad || nan, 0)) restore_nonfinite(e, nan ? e.t_first : max(e.t_first, e.prefix / kTile), acc, l);
     // the next row block's queries and page ids come while this one's states meet
     const Segment was = e;
     if (more) {

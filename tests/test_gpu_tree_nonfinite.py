@@ -93,3 +93,36 @@ def test_an_infinite_v_leaves_other_requests_and_rows_their_bits(gpu_device):
     assert (got[:24][sees][:, :, 3] == INF).all()
     rest = torch.arange(64, device=gpu_device) != 3
     assert torch.equal(got[:24][sees][:, :, rest], clean[:24][sees][:, :, rest])
+
+
+@pytest.mark.parametrize("page_size", [1, 5, 48])
+@pytest.mark.parametrize("tree,prefix", [(30, 300), (200, 90)])
+def test_infinite_v_in_any_pages_and_wide_trees(gpu_device, page_size, tree, prefix):
+    """Pages that end inside blocks, nodes past the first word of the masks, heads of their own."""
+    case = tree_case([3, tree], [50, prefix + tree], 4, 2, 128, page_size, BF16, gpu_device, seed=tree + page_size)
+    ip, ind = case["indptr"].tolist(), case["indices"].tolist()
+    for n, pos in enumerate((0, prefix - 1, prefix, prefix + 17, prefix + tree - 3)):
+        case["cache_host"][ind[ip[1] + pos // page_size], 1, pos % page_size, n % 2, 4 + n] = -INF
+    case["cache"] = case["cache_host"].to(gpu_device)
+    be = backend(4, 2, 128, page_size, gpu_device)
+    for share in (0, 1):
+        be.plan_tree(**tables(case), tree_parents=case["parents"], min_share=share)
+        compare(case, be.run_tree(case["q"], case["cache"]), BF16)
+
+
+def test_nan_and_infinite_k_stay_nan(gpu_device):
+    """NaN in V, both signs in one dim of a row, V infinite where K is (a weight of exactly 0): NaN in that dim alone."""
+    case = tree_case([5], [300], 1, 1, 64, 16, F16, gpu_device, seed=2)
+    q, cache = case["q_host"].abs(), torch.nan_to_num(case["cache_host"])
+    (p0, o0), (p1, o1), (p2, o2), (p3, o3) = (slot(case, n) for n in (3, 150, 200, 201))
+    cache[p0, 1, o0, 0, 7] = float("nan")
+    cache[p0, 1, o0, 0, 11] = cache[p3, 1, o3, 0, 11] = INF
+    cache[p1, 1, o1, 0, 11] = -INF
+    cache[p2, 0, o2, 0, :] = -INF  # q > 0: a score of -inf
+    cache[p2, 1, o2, 0, 13] = INF
+    cache[p1, 1, o1, 0, 20] = -INF
+    case.update(q_host=q, cache_host=cache, q=q.to(gpu_device), cache=cache.to(gpu_device))
+    for share in (0, 1, 2):
+        got = run(case, (1, 1), 64, gpu_device, min_share=share)
+        compare(case, got, F16)
+        assert torch.isnan(got[:, 0, [7, 11, 13]]).all() and (got[:, 0, 20] == -INF).all()
