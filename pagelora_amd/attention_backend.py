@@ -873,13 +873,14 @@ class PagedDecodeAttention:
             kept = self._tree_kept.get(sizes)
             if kept is None:  # the plan, then the page ids
                 buffer = torch.empty(plan_bytes + 4 * num_indices, dtype=torch.uint8, device=self.device)
-                ids = buffer[plan_bytes:].view(torch.int32)
+                ids = (buffer.data_ptr() + plan_bytes, num_indices)
                 held = [buffer]
             else:
                 buffer, ids, held = kept["buffer"], kept["ids"], kept["held"]
-                if ids.numel() < num_indices:  # (graphs may read or write the former ones)
-                    ids = torch.empty(1 << (num_indices - 1).bit_length(), dtype=torch.int32, device=self.device)
-                    held.append(ids)
+                if ids[1] < num_indices:  # (graphs may read or write the former ones)
+                    room = 1 << (num_indices - 1).bit_length()
+                    held.append(torch.empty(room, dtype=torch.int32, device=self.device))
+                    ids = (held[-1].data_ptr(), room)
                 streams = {**kept["streams"], **streams}
                 if not captured:  # what runs on other streams is done with the plan that the buffer holds
                     for raw, other in streams.items():
@@ -890,8 +891,8 @@ class PagedDecodeAttention:
                 None, tree.data_ptr(), tree.shape[1])
             _lib.check(self._lib.pl_tree_plan_ids(
                 tables[0].data_ptr(), tables[1].data_ptr(), tables[2].data_ptr(), num_indices, tables[3].data_ptr(),
-                *sizes, parents_ptr, mask_ptr, mask_ld, *heads, self.page_size, int(min_share), ids.data_ptr(),
-                ids.numel(), buffer.data_ptr(), plan_bytes, stream.cuda_stream), "pl_tree_plan_ids")
+                *sizes, parents_ptr, mask_ptr, mask_ld, *heads, self.page_size, int(min_share), *ids,
+                buffer.data_ptr(), plan_bytes, stream.cuda_stream), "pl_tree_plan_ids")
             plan = self._tree_plan = {
                 "device": index,
                 "sizes": sizes,
@@ -899,7 +900,7 @@ class PagedDecodeAttention:
                 "tokens": tokens,
                 "buffer": buffer,
                 "buffer_args": (buffer.data_ptr(), plan_bytes),
-                "ids": ids,
+                "ids": ids,    # their place and room
                 "held": held,  # all memory that it and the plans before it in this buffer read
                 "workspace_bytes": self._lib.pl_tree_workspace_size(*sizes, *heads),
                 "max_page": max_page,
