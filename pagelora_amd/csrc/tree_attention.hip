@@ -523,9 +523,7 @@ __device__ __forceinline__ void store_row(const Args& A, const Group& group, int
 
 __device__ __forceinline__ bool nonfinite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
 
-// A weighted sum of parts with its maximum: joins N more, those past n left out.  A
-// weight is above 0, also where fp32 has it as 0: then 0 times a part's infinity is
-// put right.
+// A weighted sum of parts with its maximum: joins N more, those past n left out.
 template <int N>
 __device__ __forceinline__ void join(float& top, float& sum, f32x4& o, const f32x4 (&x)[N], const f32x2 (&own)[N], int n) {
   float here = top;
@@ -533,7 +531,6 @@ __device__ __forceinline__ void join(float& top, float& sum, f32x4& o, const f32
   for (int i = 0; i < N; ++i)
     if (i < n) here = fmaxf(here, own[i][0]);
   const float ref = here == -INFINITY ? 0.f : here, old = fast_exp2(top - ref);
-  const f32x4 before = o;
   top = here;
   sum *= old;
 #pragma unroll
@@ -546,8 +543,19 @@ __device__ __forceinline__ void join(float& top, float& sum, f32x4& o, const f32
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[i][e], wt, o[e]);
   }
+}
+__device__ __forceinline__ bool has_nan(f32x4 o) {  // (or infinities of both signs)
   const float all = (o[0] + o[1]) + (o[2] + o[3]);
-  if (__builtin_expect(__builtin_amdgcn_ballot_w64(all != all) != 0, 0)) {
+  return all != all;
+}
+// The same for parts that may hold infinities: a weight is above 0, also where fp32
+// has it as 0, and 0 times a part's infinity is put right.
+template <int N>
+__device__ __forceinline__ void join_kept(float& top, float& sum, f32x4& o, const f32x4 (&x)[N], const f32x2 (&own)[N],
+                                          int n) {
+  const f32x4 before = o;
+  join(top, sum, o, x, own, n);
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(has_nan(o)) != 0, 0)) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       float f = nonfinite(before[e]) ? before[e] : 0.f;
@@ -583,6 +591,7 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
   __shared__ __align__(16) char s_ring[2 * kStage];
   __shared__ float s_ml[W][R][2];
   __shared__ int s_turn[W * WR];
+  __shared__ int s_bad[W * WR];
 
   const int hkv = A.want.hkv, h = blockIdx.x % hkv;
   // Workgroups go round the 8 XCDs.  Where the heads divide 8 and row blocks share
@@ -765,21 +774,12 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
     }
   };
 
-  // The infinities and NaN in V of the block's tokens, to the outputs of the rows that
-  // see them: a weight is above 0, however small, unless K is infinite too.  Outputs
-  // that are NaN by other causes stay so.
-  auto restore_nonfinite = [&](const Segment& e, int from, f32x4 (&acc)[C][NA], const float (&l)[C]) {  // from a tile on
-    constexpr uint32_t kNan = 0x7fc00001u;  // a NaN from here
-    int ln = lane;
-    asm volatile("" : "+v"(ln));  // (nothing of this is worked out ahead, in registers)
-    bool live[C];
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      float sum = l[c];
-      sum += __shfl_xor(sum, 16);
-      sum += __shfl_xor(sum, 32);
-      live[c] = sum == sum;
-    }
+  // What the thread's rows (four dims each, by passes over the row block) see of the
+  // infinities and NaN in V, from token `from` of the segment on: their outputs, since
+  // a weight is above 0, however small, unless K is infinite too.
+  constexpr int LPR = D / 4;  // lanes of a row, four dims each
+  constexpr int P = R * LPR / NT;
+  auto see_nonfinite = [&](const Segment& e, int from, f32x4 (&seen)[P]) {
     auto row_of = [&](const char* cache, int t) {
       const int page = t / page_size;
       return cache + (clamp_page(indices[e.page_begin + page]) * A.page_stride + (int64_t)(t - page * page_size) * A.token_stride +
@@ -792,42 +792,28 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
       for (int i = 0; i < 4; ++i) is |= nonfinite16<T>(x[i]) || nonfinite16<T>(x[i] >> 16);
       return is;
     };
+    const int end = min(e.t_last * kTile, e.kv_len);
 #pragma unroll 1
-    for (int tile = from; tile < e.t_end; ++tile) {
-      const int tb = tile * kTile + blk * kBlock, n = min(e.kv_len - tb, kBlock);
-      uint32_t found = 0;  // tokens of the block
+    for (int t0 = from; t0 < end; t0 += TPI) {  // tokens of a load
+      const int mine = min(t0 + lane / CPR, end - 1);
+      uint64_t found = __builtin_amdgcn_ballot_w64(t0 + lane / CPR < end && any_nonfinite(row_of(A.v, mine) + lane % CPR * 16));
 #pragma unroll 1
-      for (int j = 0; j < NL; ++j) {
-        const int nn = j * TPI + ln / CPR;
-        uint64_t at = __builtin_amdgcn_ballot_w64(nn < n && any_nonfinite(row_of(A.v, tb + min(nn, n - 1)) + ln % CPR * 16));
-        for (; at; at &= at - 1) found |= 1u << (j * TPI + __builtin_ctzll(at) / CPR);
-      }
-#pragma unroll 1
-      for (; found; found &= found - 1) {
-        const int t = tb + __builtin_ctz(found), node = t - e.prefix;
-        const bool no_weight = __builtin_amdgcn_ballot_w64(any_nonfinite(row_of(A.k, t) + ln % CPR * 16)) != 0;
-        bool sees[C];
+      while (found) {
+        const int i = __builtin_ctzll(found) / CPR, t = t0 + i, node = t - e.prefix;
+        found &= CPR * (i + 1) < 64 ? ~0ull << (CPR * (i + 1)) : 0;
+        const bool no_weight = __builtin_amdgcn_ballot_w64(any_nonfinite(row_of(A.k, t) + lane % CPR * 16)) != 0;
+        const u32x2 x = *reinterpret_cast<const u32x2*>(row_of(A.v, t) + threadIdx.x % LPR * 8);
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-          const int row = min(e.row0 + (rank * C + c) * 16 + ln % 16, e.n_rows - 1);
+        for (int k = 0; k < P; ++k) {
+          const int row = min(e.row0 + k * (NT / LPR) + (int)threadIdx.x / LPR, e.n_rows - 1);
           const uint64_t* mask = A.masks + (int64_t)(e.q_begin + group.of(row)) * A.mask_words;
-          sees[c] = live[c] && (node < 0 || (node / 64 < A.mask_words && (mask[node / 64] >> (node % 64) & 1)));
-        }
-        const char* v = row_of(A.v, t) + ln / 16 * 8;
+          if (node >= 0 && !(node / 64 < A.mask_words && (mask[node / 64] >> (node % 64) & 1))) continue;
 #pragma unroll
-        for (int a = 0; a < NA; ++a) {
-          const u32x2 x = *reinterpret_cast<const u32x2*>(v + a * 32);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t b = i % 2 ? x[i / 2] >> 16 : x[i / 2] & 0xffffu;
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t b = j % 2 ? x[j / 2] >> 16 : x[j / 2] & 0xffffu;
             float f, unused;
             unpack2<T>(b, f, unused);
-            if (no_weight) f = __uint_as_float(kNan);
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-              const float o = acc[c][a][i], sum = o != o && __float_as_uint(o) != kNan ? f : o + f;
-              if (nonfinite16<T>(b) && sees[c]) acc[c][a][i] = sum == sum ? sum : __uint_as_float(kNan);
-            }
+            if (nonfinite16<T>(b)) seen[k][j] += no_weight ? __builtin_nanf("") : f;
           }
         }
       }
@@ -908,7 +894,7 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
         }
         // 0 * V is NaN where V is not finite: V behind the last token is set to
         // zero, and so are infinities and NaN of nodes, which rows may not see
-        // (restore_nonfinite gives them to the rows that do).  (Looked for in two
+        // (see_nonfinite gives them to the rows that do).  (Looked for in two
         // halves of V: all of it at once spills registers.)
         char* v0 = kb + blk * 2 * kK + kK;
         u16x2 top2 = {0, 0};  // the largest magnitudes: not finite from infinity on
@@ -1040,16 +1026,7 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
       }
     }
 
-    // An infinity of a committed token times a plane of a probability that is 0 is NaN.
-    float all = 0.f;
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int a = 0; a < NA; ++a)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) all += acc[c][a][i];
-    const bool nan = __builtin_amdgcn_ballot_w64(all != all) != 0;
-    if (__builtin_expect(bad || nan, 0)) restore_nonfinite(e, nan ? e.t_first : max(e.t_first, e.prefix / kTile), acc, l);
+    if (lane == 0) s_bad[wave] = bad;
     // the next row block's queries and page ids come while this one's states meet
     const Segment was = e;
     if (more) {
@@ -1074,12 +1051,12 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
       }
     }
     __syncthreads();
-    constexpr int LPR = D / 4;  // lanes of a row, four dims each
     const int ch = threadIdx.x % LPR;
     float* part = A.part + ((2 * (int64_t)slot + was.second) * hkv + h) * kPartFloats;
-#pragma unroll
-    for (int r0 = 0; r0 < R; r0 += NT / LPR) {
-      const int pr = r0 + threadIdx.x / LPR, row = was.row0 + pr;
+    // A pass over the row block; `seen` where it is not 0.  Whether there is a NaN:
+    // 0 times an infinity, of a plane of a probability, a rescale or a block's weight.
+    auto finish = [&](int k, const f32x4& seen) {
+      const int pr = k * (NT / LPR) + threadIdx.x / LPR, row = was.row0 + pr;
       f32x4 x[W];
       f32x2 own[W];
 #pragma unroll
@@ -1090,13 +1067,29 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
       float top = -INFINITY, sum = 0.f;
       f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
       join(top, sum, o, x, own, W);
-      if (row >= was.n_rows) continue;
+      const bool nan = has_nan(o);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = seen[i] != 0.f ? seen[i] : o[i];
+      if (row >= was.n_rows) return nan;
       if (was.whole) {
         store_row<T>(A, group, was.q_begin, h, row, ch * 4, o, top, sum, ch == 0);
       } else {
         *reinterpret_cast<f32x4*>(part + pr * D + ch * 4) = o;
         if (ch == 0) *reinterpret_cast<f32x2*>(part + R * D + pr * 2) = f32x2{top, sum};
       }
+      return nan;
+    };
+    bool nan = false;
+#pragma unroll
+    for (int k = 0; k < P; ++k) nan |= finish(k, f32x4{0.f, 0.f, 0.f, 0.f});
+    nan = __builtin_amdgcn_ballot_w64(nan) != 0;
+    if (__builtin_expect(nan || __builtin_amdgcn_ballot_w64(s_bad[lane % (W * WR)] != 0) != 0, 0)) {
+      f32x4 seen[P];
+#pragma unroll
+      for (int k = 0; k < P; ++k) seen[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+      see_nonfinite(was, max(was.t_first * kTile, nan ? 0 : was.prefix / TPI * TPI), seen);
+#pragma unroll
+      for (int k = 0; k < P; ++k) finish(k, seen[k]);
     }
     if (!more) return;
     __syncthreads();  // the outputs are read: the buffers may be filled again
@@ -1172,7 +1165,7 @@ __global__ __launch_bounds__(256) void merge_kernel(Args A, int rows) {
           const int pr = r0 + k * RPW + lane / LPR;
           float top = -INFINITY, sum = 0.f;
           f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-          join(top, sum, o, x[k], own[k], n);
+          join_kept(top, sum, o, x[k], own[k], n);
           if (pr < n_rows) store_row<T>(A, group, rq.q_begin, h, row0 + pr, ch * 4, o, top, sum, ch == 0);
         }
       }
@@ -1202,7 +1195,7 @@ __global__ __launch_bounds__(256) void merge_kernel(Args A, int rows) {
           x[i] = *reinterpret_cast<const f32x4*>(p[i] + pr * D + ch * 4);
           own[i] = *reinterpret_cast<const f32x2*>(p[i] + rows * D + pr * 2);
         }
-        join(top, sum, o, x, own, n);
+        join_kept(top, sum, o, x, own, n);
       }
     }
     s_o[wave][lane] = o;
@@ -1219,7 +1212,7 @@ __global__ __launch_bounds__(256) void merge_kernel(Args A, int rows) {
       top = -INFINITY;
       sum = 0.f;
       o = f32x4{0.f, 0.f, 0.f, 0.f};
-      join(top, sum, o, x, own, W);
+      join_kept(top, sum, o, x, own, W);
       if (r0 + lane / LPR < n_rows) store_row<T>(A, group, rq.q_begin, h, row0 + pr, ch * 4, o, top, sum, ch == 0);
     }
     __syncthreads();
