@@ -28,22 +28,28 @@
 // states meet in LDS at the row block's end, and the parts of row blocks that
 // several slots share in merge_kernel, in order.
 //
-// Measured (head_dim 128, GQA 4 unless said otherwise; tree_kernel + merge_kernel):
-//   1 x 8 nodes behind 2048     8 + 4 us: dependent round trips (the place, the
+// Infinities and NaN in V would spoil the products of rows that do not see them, and
+// 0 times an infinity those of rows that do.  Nodes' are taken out of V in LDS; where
+// they are found, or an output is NaN, the row block's V is looked through once more
+// at its end, and what a row sees of them is its output (see_nonfinite).
+//
+// Measured (head_dim 128, GQA 4, bf16 unless said otherwise; tree_kernel + merge_kernel):
+//   1 x 8 nodes behind 2048     9 + 4 us: dependent round trips (the place, the
 //                               page ids, the pages) and two launches
-//   1 x 64 behind 32768         73 + 5 us, 0.71 PFLOP/s: four row blocks of the same
-//                               pages, matrix and vector issue.  Without loads the
-//                               tiles take 52 us, 21 of them MFMAs at their full rate
-//   23 ragged, up to 4099, GQA 7  40 + 8 us: 12 tiles and the starts and
+//   1 x 64 behind 32768         81 .. 87 + 6 us, 34 GFLOP, 0.4 PFLOP/s: four row blocks of
+//                               the same pages, matrix and vector issue; 2 x as many
+//                               matrix operations with the planes of P
+//   23 ragged, up to 4099, GQA 7  45 + 7 us: 12 tiles and the starts and
 //                               ends of ~3 row blocks per slot
-//   8 x 32 behind 4096, no GQA, fp16  91 + 5 us, 5.9 TB/s: HBM (6.4 without any arithmetic)
-//   64 x 16 behind 2048 .. 8192  255 + 7 us, 5.3 TB/s: HBM, and the row blocks' starts
-//   640 x 16 behind 112         167 us in all: ~7 us per row block of one tile
-// Tried and slower: 128 and 256 rows per row block, which read a page once for all
-// (80 - 91 us instead of 78 at 1 x 64); the next block's scores beside this one's
-// softmax in one wave (no faster at 1 x 64, 59 - 70 us instead of 55 at 23 requests:
-// registers spill and every row block computes one block of scores more); the next
-// row block's first loads while this one's states meet in half of the LDS (no faster).
+//   8 x 32 behind 4096, no GQA, fp16  92 + 5 us, 5.9 TB/s: HBM (6.4 without any arithmetic)
+//   64 x 16 behind 2048 .. 8192  253 .. 270 + 8 us, 5.2 TB/s: HBM, row blocks' starts;
+//                               279 in all with pages of 8 tokens, 285 with pages of 1
+//   640 x 16 behind 112         177 us in all: ~8 us per row block of one tile
+// Tried with two planes of P, and slower: 128 and 256 rows per row block, which read a
+// page once for all (80 - 91 us instead of 78 at 1 x 64); the next block's scores beside
+// this one's softmax in one wave (no faster at 1 x 64, 59 - 70 us instead of 55 at 23
+// requests: registers spill and every row block computes one block of scores more); the
+// next row block's first loads while this one's states meet in half of the LDS (no faster).
 #include <algorithm>
 #include <type_traits>
 
@@ -407,7 +413,10 @@ __device__ __forceinline__ uint32_t lds_address(char* l) {
   return uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)l);
 }
 // ONCE: the lines go first from the caches.  Bytes that one workgroup reads alone
-// stream 11 % faster so (5.8 and 6.4 TB/s); row blocks that share them do not.
+// stream 11 % faster so (5.8 and 6.4 TB/s); a request's row blocks that share them do
+// not.  Requests that share pages (forks) lose nothing by it: 16 x 8 nodes behind 8192
+// shared tokens 58 us with and without, behind 8192 of their own 94 and 106;
+// 64 x 16 behind 4096 shared 149 and 148, of their own 202 and 214.
 template <bool ONCE>
 __device__ __forceinline__ void load_lds16(const char* base, uint32_t offset, uint32_t l) {
   if constexpr (ONCE)
@@ -462,7 +471,7 @@ struct Args {
   int64_t q_st, q_sh, o_st, o_sh, page_stride, token_stride, head_stride, num_pages;  // elements
   Header want;
   int slots, mask_words;
-  int once;  // no two row blocks read the same tokens
+  int once;  // no two row blocks of a request read the same tokens
   float scale_log2;  // > 0; a negative scale negates q instead
   uint32_t q_flip;
 };

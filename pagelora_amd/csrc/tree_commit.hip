@@ -1,20 +1,26 @@
-// What follows a tree's attention (gfx950): the longest path of the tree that
-// the target's picks confirm, and that path's K/V moved together in the cache.
+// What follows a tree's attention (gfx950): the path of the tree that the target's
+// picks follow, and that path's K/V moved together in the cache.
 //
 // accept_kernel: node 0 is the root, whose token is already decided.  From node
 // i the walk goes on to its first child whose drafted token is the target's
-// pick after i.  The kept tokens are the picks along the path: the children's
+// pick after i (of equal drafts beside each other the first, though another may
+// lead further).  The kept tokens are the picks along the path: the children's
 // own tokens, then the pick after the last node.  One wave per request; a tree
 // of up to 64 nodes lies one node per lane, and a step is two lane reads and a
-// ballot.  Bound by latency, the loads and a launch: 1.7 us for one tree of 8
-// nodes, 3.3 for 256 of up to 64.
+// ballot; of more nodes a step is a round trip to the caches.  Bound by latency,
+// the loads and a launch: 1.7 us for one tree of 8 nodes, 3.3 for 256 of up to 64;
+// in a graph 3.9 for one of 64 random nodes and 8.9 for a chain of 64 that is kept
+// whole, 4.9 and 83 for 256 nodes.
 //
 // commit_kernel: slot(P + k) <- slot(P + path[k]) for the tokens of an accepted
 // path, in every layer, P the committed tokens before the tree.  path[k] >= k,
 // so no token is overwritten before it is read if a thread takes its bytes of
 // all tokens in order.  Bound by latency at few requests (4.8 us for one with 4
-// tokens in 36 layers), by HBM at many, in rows of 2 KiB in no order: 64 requests'
-// 1 .. 8 tokens in 36 layers, 58 MB, 18 us, 3.2 TB/s.
+// tokens in 36 layers): a chain of look-ups, then a burst of loads and one of
+// stores, which all workgroups do at once.  64 requests' 1 .. 8 tokens in 36
+// layers, 58 MB, 18 us, 3.2 TB/s; 3 tokens of each, 57 MB, 14 us; 8 of each,
+// 151 MB, 30 us, 5.0 TB/s, and 256 requests' 128 us, 4.7 TB/s.  Whether pages and
+// tokens lie in order makes no difference (30.2 and 30.7 us).
 #include "pl_common.h"
 
 namespace pl {
@@ -86,7 +92,7 @@ struct Args {
   char* v;
   int64_t layer_stride, page_stride, token_stride, head_stride, num_pages;  // bytes; pages
   const int32_t *qo_indptr, *kv_indptr, *kv_indices, *kv_last, *path, *count;
-  int batch, layers, layers_each, num_indices, max_path, page_size;
+  int layers, layers_each, num_indices, max_path, page_size;
   int row_chunks, head_chunks;  // 16-byte chunks of a token's K row, of one head
 };
 
@@ -212,7 +218,6 @@ extern "C" int pl_tree_commit(void* k_cache, void* v_cache, int64_t layer_stride
   a.kv_last = kv_last_page_len;
   a.path = path;
   a.count = count;
-  a.batch = batch;
   a.layers = num_layers;
   a.num_indices = num_indices;
   a.max_path = max_path;

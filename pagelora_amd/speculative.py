@@ -3,8 +3,8 @@
 A drafter proposes a tree of tokens per request; the target model runs its
 nodes in one pass (``PagedDecodeAttention.plan_tree`` / ``run_tree``), each
 node at the position of its depth, and picks a token after every node.  Then
-:func:`accept_tree` keeps the longest path that the picks follow, so that
-greedy decoding emits the tokens it would have emitted one by one, and
+:func:`accept_tree` keeps the path that the picks follow, so that greedy
+decoding emits the tokens it would have emitted one by one, and
 :func:`commit_tree` moves that path's K/V together behind the committed
 tokens.  :meth:`~pagelora_amd.kv_pool.PagedKVPool.truncate` gives back the pages
 that the rest of the tree held.
@@ -50,7 +50,8 @@ def accept_tree(tokens: torch.Tensor, parents: torch.Tensor, picks: torch.Tensor
     pick after each node, ``fused_ops.greedy_argmax`` of the nodes' logits) hold
     the batch's nodes, request r's at ``qo_indptr[r] .. qo_indptr[r+1]``.  Node
     0 of a tree is its root, the token decided by the step before; from node i
-    the path goes on to the lowest-numbered child whose token is ``picks[i]``.
+    the path goes on to the lowest-numbered child whose token is ``picks[i]``
+    (the only one, unless a drafter gives a node two children of one token).
     The result's ``tokens`` are what the step decodes: the accepted drafts, then
     the target's own pick after the last of them.  ``out``: tensors to write to.
     """
