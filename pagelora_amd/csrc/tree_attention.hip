@@ -495,13 +495,15 @@ template <typename T> struct Softmax {
   // planes -> three: 1 x 64 nodes behind 32768 81 -> 91 us, 23 ragged requests
   // 49 -> 54, 64 x 16 behind 8192 261 -> 269.
   static constexpr int kPlanes = kBf16 ? 3 : 2;
-  // A column's running maximum follows only scores more than kLag above it,
-  // which takes the rescale out of the steady state.
+  // A column's running maximum, rounded up to a whole number, follows only scores more
+  // than kLag above it, which takes the rescale out of the steady state and makes it
+  // exact.
   static constexpr float kLag = kBf16 ? 8.f : 1.f;
-  // Probabilities are held 2^kShift times as large: fp16 ends at 2^-24, and
-  // 32768 tokens of 2^-25 are no small part of a row.  2^14 keeps them to 2^-38,
-  // and the largest, 2^15 with the lag, below fp16's 65504.
-  static constexpr float kShift = kBf16 ? 0.f : 14.f;
+  // Probabilities are held 2^kShift times as large.  bf16: with the lag none is above 1,
+  // so that V of any size stays finite.  fp16 ends at 2^-24, and 32768 tokens of 2^-25
+  // are no small part of a row: 2^14 keeps them to 2^-38, and the largest, 2^15 with
+  // the lag, below fp16's 65504.
+  static constexpr float kShift = kBf16 ? -8.f : 14.f;
 };
 
 // x / g: the product with 2^32 / g rounded up is the quotient or one more.
@@ -983,7 +985,7 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
       if (__builtin_amdgcn_ballot_w64(rose) != 0) {
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-          const float mn = fmaxf(m[c], column_max(mx[c]));
+          const float mn = fmaxf(m[c], __builtin_ceilf(column_max(mx[c])));
           const float alpha = fast_exp2(m[c] - (mn == -INFINITY ? 0.f : mn));
           m[c] = mn;
           l[c] *= alpha;
