@@ -226,9 +226,10 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs A) {
     for (int64_t i = first; i < A.indices_count; i += step) A.indices[i] = A.kv_indices[i];
     // Given by parents, a thread packs a token's words from the last to the first on
     // one walk to the root; given by a mask, a thread packs a word.
-    const int words = A.parents ? A.mask_words : 1;
-    for (int64_t i = first; i < (int64_t)A.want.tokens * A.mask_words / words; i += step) {
-      const int t = (int)(i * words / A.mask_words);
+    const int words = A.mask_words;
+    const int64_t items = words == 0 ? 0 : (int64_t)A.want.tokens * (A.parents ? 1 : words);
+    for (int64_t i = first; i < items; i += step) {
+      const int t = (int)(A.parents ? i : i / words);
       int lo = 0, hi = batch;  // the request that holds token t: the last whose first token is <= t
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -249,7 +250,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs A) {
           A.masks[i * words + w] = bits;
         }
       } else {
-        const int w = (int)(i % A.mask_words), n = on ? min(q.tree - w * 64, 64) : 0;
+        const int w = (int)(i % words), n = on ? min(q.tree - w * 64, 64) : 0;
         const uint8_t* m = A.mask + (int64_t)t * A.mask_ld + w * 64;
         uint64_t bits = 0;
         for (int j = 0; j < n; ++j) bits |= (uint64_t)(m[j] != 0) << j;

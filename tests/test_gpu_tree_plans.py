@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+from pagelora_amd import _lib
 from tests.test_gpu_tree_attention import BF16, F16, backend, check, oracle, tables, tree_case
 
 pytestmark = pytest.mark.gpu
@@ -165,3 +166,28 @@ def test_deep_trees_by_parents_and_by_mask(gpu_device, kind):
         causal = be.run_prefill(q, cache).float()
         # two roundings to fp16, and weights off by less than 2^-13 for values of up to 5
         assert ((want.float() - causal).abs() <= 2.0**-10 * causal.abs() + 1e-3).all()
+
+
+def test_a_c_plan_of_no_nodes(gpu_device):
+    """max_tree 0 with tokens, through the C entries: nothing is worked on, by parents and by mask."""
+    lib = _lib.load()
+    case = tree_case([4, 3], [40, 30], 4, 2, 64, 16, F16, gpu_device, seed=1)
+    t = tables(case, gpu_device)
+    dev = {k: v.data_ptr() for k, v in t.items()}
+    parents, mask = case["parents"].to(gpu_device), torch.ones((7, 4), dtype=torch.uint8, device=gpu_device)
+    n, out = t["paged_kv_indices"].numel(), torch.full_like(case["q"], 7.0)
+    size = lib.pl_tree_plan_size(2, 7, 0, n, 4, 2, 64)
+    plan = torch.zeros(size + 64, dtype=torch.uint8, device=gpu_device)
+    plan[size:] = 5
+    stream = _lib.stream_handle(gpu_device)
+    for by in ((parents.data_ptr(), None, 0), (None, mask.data_ptr(), 4)):
+        assert lib.pl_tree_plan(dev["qo_indptr"], dev["paged_kv_indptr"], dev["paged_kv_indices"], n,
+                                dev["paged_kv_last_page_len"], 2, 7, 0, *by, 4, 2, 64, 16, 0, n, plan.data_ptr(), size,
+                                stream) == 0
+        ws = torch.empty(lib.pl_tree_workspace_size(2, 7, 0, 4, 2, 64), dtype=torch.uint8, device=gpu_device)
+        c = case["cache"]
+        assert lib.pl_tree_run(case["q"].data_ptr(), 256, 64, c.data_ptr(), c[:, 1].data_ptr(), c.stride(0), c.stride(2),
+                               c.stride(3), c.shape[0], out.data_ptr(), 256, 64, None, 2, 7, 0, 4, 2, 64, 16, 0.125,
+                               _lib.PL_DTYPE_F16, plan.data_ptr(), size, n, ws.data_ptr(), ws.numel(), stream) == 0
+        torch.cuda.synchronize()
+        assert (out == 7).all() and (plan[size:] == 5).all()
