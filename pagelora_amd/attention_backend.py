@@ -800,6 +800,8 @@ class PagedDecodeAttention:
         kernels clamp every index into its buffer) and may be planned inside a
         capture; ``max_tree`` then bounds the nodes of a tree (default: all
         tokens; of a tree that has more, the first ``max_tree`` are attended).
+        With host tables its default is the widest tree's nodes: give it where
+        runs are captured and trees vary.
         A captured :meth:`run_tree` replays on the plan that ``plan_tree`` made
         last for the same sizes (:meth:`tree_graph_signature`: requests, nodes,
         ``max_tree``), whatever its sequences' lengths; a replayed ``plan_tree``

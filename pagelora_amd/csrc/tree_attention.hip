@@ -86,11 +86,11 @@ struct alignas(64) Header {
   uint64_t indices;  // the address of the page ids: in the plan or apart from it
 };
 static_assert(sizeof(Header) == 128, "the plan's header");
-// A request with nodes: `prefix` tokens before them, `tree` of them worked on.  Its work is tiles x blocks (row blocks), from `base` of
-// all work on: chunk after chunk of its tiles, of a chunk row block after row
-// block.  The first `setup` tiles are none and stand for what a row block costs
-// beside its tiles.  The first `longer` chunks have chunk_len + 1 tiles, the others
-// chunk_len.
+// A request with nodes: `prefix` tokens before them, `tree` of them worked on.  Its
+// work is tiles x blocks (row blocks), from `base` of all work on: chunk after chunk
+// of its tiles, of a chunk row block after row block.  The first `setup` tiles are
+// none and stand for what a row block costs beside its tiles.  The first `longer`
+// chunks have chunk_len + 1 tiles, the others chunk_len.
 // Either every chunk of a row block is a slot's (`base` and all work then count
 // those), or only requests of several row blocks have several chunks, none less
 // than a share.
@@ -796,8 +796,8 @@ __global__ __launch_bounds__(threads_of(R, D), D == 64 || threads_of(R, D) > 256
   auto see_nonfinite = [&](const Segment& e, int from, f32x4 (&seen)[P]) {
     auto row_of = [&](const char* cache, int t) {
       const int page = t / page_size;
-      return cache + (clamp_page(indices[e.page_begin + page]) * A.page_stride + (int64_t)(t - page * page_size) * A.token_stride +
-                      (int64_t)h * A.head_stride) * 2;
+      return cache + (clamp_page(indices[e.page_begin + page]) * A.page_stride +
+                      (int64_t)(t - page * page_size) * A.token_stride + (int64_t)h * A.head_stride) * 2;
     };
     auto any_nonfinite = [&](const char* p) {
       const u32x4 x = *reinterpret_cast<const u32x4*>(p);

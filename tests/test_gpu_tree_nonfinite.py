@@ -38,13 +38,12 @@ def run(case, heads, head_dim, device, **kw):
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("heads,head_dim", [((1, 1), 128), ((4, 1), 128), ((4, 1), 64), ((4, 1), 256)])
-@pytest.mark.parametrize("tree,prefix", [(4, 0), (4, 44), (20, 44), (30, 700), (70, 1500)])
-@pytest.mark.parametrize("where", ["node", "committed", "both"])
+@pytest.mark.parametrize("tree,prefix,where", [(4, 0, "node")] + [
+    (tree, prefix, where) for tree, prefix in ((4, 44), (20, 44), (30, 700), (70, 1500))
+    for where in ("node", "committed", "both")])
 def test_infinite_v(gpu_device, dtype, heads, head_dim, tree, prefix, where):
     """In nodes and in committed tokens, both signs, in the first block of a wave and in later ones, 16 to 64 rows of a
     row block, every kv range cut in several ways."""
-    if where != "node" and not prefix:
-        pytest.skip("no committed token")
     case = tree_case([tree], [prefix + tree], *heads, head_dim, 16, dtype, gpu_device, seed=tree + prefix)
     at = ([prefix, prefix + tree // 2, prefix + tree - 1] if where != "committed" else []) + \
          ([0, prefix // 2, prefix - 1] if where != "node" else [])
