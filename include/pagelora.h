@@ -313,6 +313,113 @@ int pl_prefill_split_run(const void* q, int64_t q_stride_t, int64_t q_stride_h,
                          int dtype, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Long contexts: a 4-bit paged cache, attention under a window with sinks   */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * Tokens into a paged 4-bit KV cache, and back.  No counterpart in the
+ * reference, whose cache has 16 bits.
+ *
+ * A page of one kv head holds page_size * (head_dim / 2 + head_dim / 32) bytes,
+ * codes and then scales.  Each 32 values along head_dim share a scale byte s, a
+ * power of two 2^(s - 127): the least at which the largest magnitude is at most
+ * 6, s in 2 .. 252 (values below fall to 0, values above end at the largest).
+ * A value is an e2m1 code of it (sign, 0 0.5 1 1.5 2 3 4 6), the nearest,
+ * halfway to the one of even mantissa; lower nibble, lower dim.  A group that
+ * holds a NaN or an infinity gets s = 255 and reads back as NaN.
+ *   K: codes [token][head_dim / 2], scales [token][head_dim / 32];
+ *   V: codes [token / 4][d / 8][token % 4][4], scales [token / 4][d / 32][token % 4].
+ *
+ * k, v: [tokens, num_kv_heads, head_dim] bf16 or fp16, strides in elements;
+ * page_stride and head_stride in bytes; all multiples of 16 bytes.  head_dim 64
+ * or 128, page_size a multiple of 8.  Token i lies at (page_id[i], offset[i]);
+ * outside the pool it is dropped by the append and read as NaN.  A place that
+ * one append lists twice holds neither token for certain.
+ */
+int pl_kv4_append(const void* k, const void* v, int64_t k_stride_t,
+                  int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h,
+                  void* k_cache, void* v_cache, int64_t page_stride,
+                  int64_t head_stride, int64_t num_pages, int page_size,
+                  const int64_t* page_id, const int64_t* offset, int tokens,
+                  int num_kv_heads, int head_dim, int dtype, void* stream);
+int pl_kv4_read(const void* k_cache, const void* v_cache, int64_t page_stride,
+                int64_t head_stride, int64_t num_pages, int page_size,
+                const int64_t* page_id, const int64_t* offset, int tokens,
+                int num_kv_heads, int head_dim, void* k, void* v,
+                int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t,
+                int64_t v_stride_h, int dtype, void* stream);
+
+/*
+ * Decode attention of one query per request, at its last position p, which sees
+ * position t <= p where t > p - window (window 0: every one) or t < sinks.
+ *
+ * pl_window_decode_plan cuts the step's work on the device, once for all layers:
+ * nothing is read back, and a captured plan follows the tables as they are at
+ * each replay.  It copies the tables (indices_capacity page ids); entries
+ * outside their range are clamped, page ids to the pool when they are used.
+ * plan: 64-byte aligned, pl_window_decode_plan_size bytes (0: sizes refused).
+ *
+ * pl_window_decode_run attends with it; run with other sizes than its plan's it
+ * does nothing.  kv_bits 16: caches as in pl_decode_run, of q's dtype, strides in
+ * elements.  kv_bits 4: as in pl_kv4_append, page_stride and head_stride in
+ * bytes, token_stride unused.  dtype bf16 or fp16, head_dim 64 or 128; every
+ * stride a multiple of 16 bytes.  lse (nullable): fp32 [batch, num_qo_heads],
+ * natural log.  A request of no tokens gets o = 0, lse = -inf.  What is not seen
+ * may hold anything; an infinite V that is seen is an infinity in the output,
+ * however small its weight.  workspace: pl_window_decode_workspace_size bytes,
+ * one call's at a time.
+ */
+size_t pl_window_decode_plan_size(int batch, int indices_capacity,
+                                  int num_qo_heads, int num_kv_heads);
+size_t pl_window_decode_workspace_size(int batch, int num_qo_heads,
+                                       int num_kv_heads, int head_dim);
+int pl_window_decode_plan(const int32_t* indptr, const int32_t* indices,
+                          int indices_capacity, const int32_t* last_page_len,
+                          int batch, int num_qo_heads, int num_kv_heads,
+                          int page_size, int window, int sinks, void* plan,
+                          size_t plan_bytes, void* stream);
+int pl_window_decode_run(const void* q, int64_t q_stride_b, int64_t q_stride_h,
+                         const void* k_cache, const void* v_cache,
+                         int64_t page_stride, int64_t token_stride,
+                         int64_t head_stride, int64_t num_pages, int kv_bits,
+                         void* o, int64_t o_stride_b, int64_t o_stride_h,
+                         float* lse, int batch, int num_qo_heads,
+                         int num_kv_heads, int head_dim, int page_size,
+                         int window, int sinks, float sm_scale, int dtype,
+                         const void* plan, size_t plan_bytes,
+                         int indices_capacity, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/*
+ * Prefill attention under the same mask: request r's queries, rows
+ * qo_indptr[r] .. qo_indptr[r+1] of q, are its sequence's last positions.  The
+ * plan is made on the host from host tables, and called twice: with items_h null
+ * for the numbers of records, then for the records themselves (eight int32 each,
+ * num_items work items and then num_merges merges), which the caller uploads
+ * together with the tables.  workspace: the plan's bytes (0: may be null).
+ */
+int pl_window_prefill_plan(const int32_t* qo_indptr_h,
+                           const int32_t* kv_indptr_h,
+                           const int32_t* kv_last_page_len_h, int batch,
+                           int num_qo_heads, int num_kv_heads, int head_dim,
+                           int page_size, int window, int sinks,
+                           int32_t* items_h, int max_records, int* num_items_h,
+                           int* num_merges_h, size_t* workspace_bytes_h);
+int pl_window_prefill_run(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                          const void* k_cache, const void* v_cache,
+                          int64_t page_stride, int64_t token_stride,
+                          int64_t head_stride, int64_t num_pages, int kv_bits,
+                          const int32_t* qo_indptr, const int32_t* kv_indptr,
+                          const int32_t* kv_indices,
+                          const int32_t* kv_last_page_len, const int32_t* items,
+                          int num_items, int num_merges, void* o,
+                          int64_t o_stride_t, int64_t o_stride_h, int batch,
+                          int num_qo_heads, int num_kv_heads, int head_dim,
+                          int page_size, int window, int sinks, float sm_scale,
+                          int dtype, void* workspace, size_t workspace_bytes,
+                          size_t plan_workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Trees of drafted tokens over the paged cache                              */
 /* ------------------------------------------------------------------------ */
 

@@ -401,6 +401,73 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                        _vp, _i64, _i32, _vp]),
     "pl_linear_shuffled_add": (_i32, [_vp, _i64, _i32, _i32, _vp, _i32, _vp, _i64, ctypes.POINTER(LoraUp),
                                       ctypes.POINTER(LoraPartials), _vp, _i32, _vp, _i64, _vp, _i64, _i32, _vp]),
+    "pl_kv4_append": (
+        _i32,
+        [
+            _vp, _vp, _i64, _i64, _i64, _i64,  # k, v, strides
+            _vp, _vp, _i64, _i64,              # caches, page/head strides (bytes)
+            _i64, _i32,                        # num_pages, page_size
+            _vp, _vp,                          # page_id, offset
+            _i32, _i32, _i32, _i32, _vp,       # tokens, hkv, head_dim, dtype, stream
+        ],
+    ),
+    "pl_kv4_read": (
+        _i32,
+        [
+            _vp, _vp, _i64, _i64,              # caches, page/head strides (bytes)
+            _i64, _i32,                        # num_pages, page_size
+            _vp, _vp,                          # page_id, offset
+            _i32, _i32, _i32,                  # tokens, hkv, head_dim
+            _vp, _vp, _i64, _i64, _i64, _i64,  # k, v, strides
+            _i32, _vp,                         # dtype, stream
+        ],
+    ),
+    "pl_window_decode_plan_size": (_sz, [_i32, _i32, _i32, _i32]),
+    "pl_window_decode_workspace_size": (_sz, [_i32, _i32, _i32, _i32]),
+    "pl_window_decode_plan": (
+        _i32,
+        [
+            _vp, _vp, _i32, _vp,               # indptr, indices, their number, last_page_len
+            _i32, _i32, _i32, _i32,            # batch, hq, hkv, page_size
+            _i32, _i32, _vp, _sz, _vp,         # window, sinks, plan, bytes, stream
+        ],
+    ),
+    "pl_window_decode_run": (
+        _i32,
+        [
+            _vp, _i64, _i64,                   # q, strides
+            _vp, _vp, _i64, _i64, _i64,        # k/v cache, page/token/head strides
+            _i64, _i32,                        # num_pages, kv_bits
+            _vp, _i64, _i64, _vp,              # o, strides, lse
+            _i32, _i32, _i32, _i32, _i32,      # batch, hq, hkv, head_dim, page_size
+            _i32, _i32, _f32, _i32,            # window, sinks, sm_scale, dtype
+            _vp, _sz, _i32,                    # plan, bytes, indices planned
+            _vp, _sz, _vp,                     # workspace, bytes, stream
+        ],
+    ),
+    "pl_window_prefill_plan": (
+        _i32,
+        [
+            _vp, _vp, _vp, _i32,               # qo_indptr, kv_indptr, last_page_len (host), batch
+            _i32, _i32, _i32, _i32,            # hq, hkv, head_dim, page_size
+            _i32, _i32, _vp, _i32,             # window, sinks, items (host), max_records
+            ctypes.POINTER(_i32), ctypes.POINTER(_i32), ctypes.POINTER(_sz),  # items, merges, workspace bytes
+        ],
+    ),
+    "pl_window_prefill_run": (
+        _i32,
+        [
+            _vp, _i64, _i64,                   # q, strides
+            _vp, _vp, _i64, _i64, _i64,        # k/v cache, page/token/head strides
+            _i64, _i32,                        # num_pages, kv_bits
+            _vp, _vp, _vp, _vp,                # qo_indptr, kv_indptr, kv_indices, last_page_len
+            _vp, _i32, _i32,                   # items, num_items, num_merges
+            _vp, _i64, _i64,                   # o, strides
+            _i32, _i32, _i32, _i32, _i32,      # batch, hq, hkv, head_dim, page_size
+            _i32, _i32, _f32, _i32,            # window, sinks, sm_scale, dtype
+            _vp, _sz, _sz, _vp,                # workspace, bytes, the plan's bytes, stream
+        ],
+    ),
     "pl_lora_workspace_size": (_sz, [_i32, _i32, ctypes.POINTER(LoraModule), _i32]),
     "pl_lora_delta": (
         _i32,

@@ -48,6 +48,8 @@ FILE_FLAGS = {
     "lora.hip": _MFMA_VGPR,
     "tree_attention.hip": _MFMA_VGPR,
     "wide_gemm.hip": _MFMA_VGPR,
+    "window_decode.hip": _MFMA_VGPR,
+    "window_prefill.hip": _MFMA_VGPR,
 }
 
 

@@ -1,0 +1,121 @@
+// What the kernels of windowed attention and of the 4-bit cache share (gfx950):
+// matrix operands, the 4-bit cache's layout and conversion, the planes in which
+// probabilities enter a product, and what a query sees.
+#pragma once
+
+#include <type_traits>
+
+#include "pl_common.h"
+
+namespace pl {
+namespace window {
+
+constexpr int kWave = 64;
+constexpr int kMaxLen = 1 << 30;   // tokens of a sequence
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+
+// ------------------------------------------------------------ products ---
+template <typename T> __device__ __forceinline__ f32x4 mfma32(u32x4 a, u32x4 b, f32x4 c);
+template <> __device__ __forceinline__ f32x4 mfma32<bf16_t>(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                 0, 0);
+}
+template <> __device__ __forceinline__ f32x4 mfma32<f16_t>(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                0);
+}
+
+// The largest of the four lanes l, l ^ 16, l ^ 32, l ^ 48.
+__device__ __forceinline__ float column_max(float v) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// Probabilities are p = 2^(x - mu), mu a constant (kBias) past the running maximum
+// that the row's sums are held at, which follows only scores more than kLag above
+// it.  They enter the product with V in two planes of its type, so that 16 bits of
+// each (bf16) or 22 (fp16) do: off by 2^-15 and 2^-22 of the weight, under the 2^-8
+// and 2^-11 of the output's rounding.  bf16: p <= 2^-24, so that the sums over 2^24
+// tokens of the largest V are finite.  fp16: p <= 2^15, near the range's top, so that
+// a weight of 2^-35 of the largest still counts.
+template <typename MT> struct Planes;
+template <> struct Planes<bf16_t> {
+  static constexpr float kLag = 8.f, kBias = 32.f;
+  // The planes of two probabilities: the upper halves, then the rest rounded.
+  __device__ static __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+    hi = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
+    lo = f32x2_to_bf16x2_bits(a - __uint_as_float(ua & 0xffff0000u), b - __uint_as_float(ub & 0xffff0000u));
+  }
+};
+template <> struct Planes<f16_t> {
+  static constexpr float kLag = 4.f, kBias = -11.f;
+  __device__ static __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
+    hi = pack2<f16_t>(a, b);
+    float ha, hb;
+    unpack2<f16_t>(hi, ha, hb);
+    lo = pack2<f16_t>(a - ha, b - hb);
+  }
+};
+
+// ---------------------------------------------------------- 4-bit cache ---
+// Of a page and kv head: the codes of `page` tokens, then their scales.  K goes by
+// tokens: codes [token][D / 2 bytes], scales [token][D / 32].  V goes by four
+// tokens, as the lanes of a V^T operand hold them: codes [token / 4][d / 8]
+// [token % 4][4 bytes], scales [token / 4][d / 32][token % 4].
+constexpr int kGroup = 32;                     // values that share a scale
+constexpr int kScaleMin = 2, kScaleMax = 252;  // 2^(s - 127): every value is a normal bf16
+constexpr int kScaleNan = 255;                 // the group held a NaN or an infinity
+
+// A scale byte as the conversions take it.
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+// Codes 2 S, 2 S + 1 of a word as two bf16: exact, and NaN where the scale is kScaleNan.
+template <int S> __device__ __forceinline__ uint32_t codes2(uint32_t w, float scale) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, S));
+}
+// The eight codes of a word.
+__device__ __forceinline__ u32x4 codes8(uint32_t w, float scale) {
+  return u32x4{codes2<0>(w, scale), codes2<1>(w, scale), codes2<2>(w, scale), codes2<3>(w, scale)};
+}
+
+// --------------------------------------------------------------- window ---
+// What the queries at positions p0 .. see: positions from `lo` on (the window of
+// p0), and those before `se` (sinks).  Tiles of `tile` positions are counted by
+// what is seen: `ns` of sinks, then on from tile `fw`.
+struct Seen {
+  int lo, se, ns, fw;
+};
+__host__ __device__ __forceinline__ Seen seen_from(int p0, int window, int sinks, int tile) {
+  Seen s;
+  s.lo = window > 0 && p0 >= window ? p0 - window + 1 : 0;
+  s.se = sinks < s.lo ? sinks : s.lo;
+  s.fw = s.lo / tile;
+  const int t = (s.se + tile - 1) / tile;
+  s.ns = t < s.fw ? t : s.fw;
+  return s;
+}
+// The place of seen tile i among all tiles.
+__host__ __device__ __forceinline__ int seen_tile(const Seen& s, int i) { return i < s.ns ? i : i - s.ns + s.fw; }
+
+// A sum of a part that counts with weight w >= 0: an infinity stays one however
+// small its weight.
+__device__ __forceinline__ float weighted(float v, float w) {
+  return w == 0.f && fabsf(v) == INFINITY ? v : v * w;
+}
+
+__device__ __forceinline__ bool finite16(uint32_t half, bool bf16) {
+  const uint32_t mask = bf16 ? 0x7f80u : 0x7c00u;
+  return (half & mask) != mask;
+}
+
+}  // namespace window
+}  // namespace pl

@@ -1,0 +1,737 @@
+// Decode attention of one query per request over a paged KV cache of 16 or of 4
+// bits per value, under a sliding window with sinks (gfx950).
+//
+// The query of a request of n tokens is at position p = n - 1 and sees
+// t > p - window (window 0: every t) and t < sinks:
+//   o = sum_t p_t v_t / sum_t p_t,  p_t = exp(s q . k_t).
+// A request of no tokens gets o = 0 and lse = -inf.
+//
+// plan_kernel (once per step, for all layers) cuts what the requests see, tiles of
+// 32 tokens, into items of about equal length.  A workgroup takes an item of one kv
+// head for up to 16 heads of its group; its four waves take a quarter of the tiles
+// each, and their states meet in LDS.  merge_kernel joins the items of a request
+// in order.
+//
+// A wave holds its operands in registers: S^T = K Q^T has a query per lane column
+// and four tokens per lane, which are the B operand of O^T += V^T P^T as they lie; of
+// V^T, whose lanes hold eight tokens of one dim, a lane loads D / 16 dims of those
+// tokens and pairs tokens by byte permutes.  Values of 4 bits become bf16 on the way
+// (exact, two per instruction), so that a 4-bit cache is always multiplied in bf16;
+// queries of fp16 go in as two planes (exact).
+//
+// An output that is NaN is looked at again: 0 times an infinity, or the difference of
+// two planes' infinities, is not what the row sees.  The wave's tiles are walked once
+// more with infinities and NaN taken out of V, and their own sum, which all rows
+// share, put in.
+#include "window_common.h"
+
+namespace pl {
+namespace window {
+namespace dec {
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWave * kWaves;
+constexpr int kTile = 32;          // tokens of a step of a wave
+constexpr int kPlanThreads = 1024;
+constexpr int kMagic = 0x57444543;
+constexpr int kMinTiles = 4;       // fewest tiles of an item that is cut: one per wave
+
+// What a plan was made for, then what it holds.
+struct alignas(64) Header {
+  int32_t magic, batch, page_size, window, sinks, indices_capacity, max_items, num_items;
+  int32_t pad[8];
+};
+static_assert(sizeof(Header) == 64, "the plan's header");
+struct Item {
+  int32_t row, kv_len, page_begin, tile_begin, tile_end, slot, parts, pad;
+};
+static_assert(sizeof(Item) == 32, "the plan's record");
+struct Row {
+  int32_t first, parts;
+};
+
+struct Layout {
+  size_t items, rows, indices, bytes;
+};
+inline Layout layout(int batch, int indices_capacity, int max_items) {
+  Layout l;
+  l.items = sizeof(Header);
+  l.rows = l.items + sizeof(Item) * (size_t)max_items;
+  l.indices = align_up(l.rows + sizeof(Row) * (size_t)batch, 64);
+  l.bytes = align_up(l.indices + sizeof(int32_t) * (size_t)indices_capacity, 64);
+  return l;
+}
+
+// Heads of a workgroup: a kv head's group in blocks of 16.
+inline int head_blocks(int hq, int hkv) { return (hq / hkv + 15) / 16; }
+// Items that fill the chip: two workgroups per CU.
+inline int target_items(int hq, int hkv) {
+  const int n = 512 / (hkv * head_blocks(hq, hkv));
+  return n > 1 ? n : 1;
+}
+
+// ------------------------------------------------------------------- plan ---
+struct PlanArgs {
+  const int32_t *indptr, *indices, *last;
+  Header want;
+  Header* header;
+  Item* items;
+  Row* rows;
+  int32_t* ids;
+  int target;
+};
+
+struct Request {
+  int page_begin, len, tiles;
+};
+// Request r, its tables brought into their ranges.
+__device__ __forceinline__ Request read_request(const PlanArgs& A, int r) {
+  Request q;
+  const int cap = A.want.indices_capacity;
+  q.page_begin = min(max(A.indptr[r], 0), cap);
+  const int pages = min(max(A.indptr[r + 1], q.page_begin), cap) - q.page_begin;
+  const int last = min(max(A.last[r], 1), A.want.page_size);
+  const int64_t len = pages > 0 ? (int64_t)(pages - 1) * A.want.page_size + last : 0;
+  q.len = (int)min(len, (int64_t)kMaxLen);
+  const Seen s = seen_from(q.len - 1, A.want.window, A.want.sinks, kTile);
+  q.tiles = s.ns + (q.len + kTile - 1) / kTile - s.fw;
+  return q;
+}
+
+// Workgroup 0 cuts the work; the others copy the page ids.
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs A) {
+  const int tid = threadIdx.x, batch = A.want.batch;
+  if (blockIdx.x > 0) {
+    const int64_t step = (int64_t)(gridDim.x - 1) * kPlanThreads;
+    for (int64_t i = (int64_t)(blockIdx.x - 1) * kPlanThreads + tid; i < A.want.indices_capacity; i += step)
+      A.ids[i] = A.indices[i];
+    return;
+  }
+  __shared__ int64_t s_sum[kPlanThreads / kWave];
+  __shared__ int s_scan[kPlanThreads / kWave];
+  const int lane = tid % kWave, wave = tid / kWave;
+  int64_t sum = 0;
+  for (int r = tid; r < batch; r += kPlanThreads) sum += read_request(A, r).tiles;
+  for (int d = 1; d < kWave; d <<= 1) sum += __shfl_xor(sum, d);
+  if (lane == 0) s_sum[wave] = sum;
+  __syncthreads();
+  int64_t total = 0;
+  for (int w = 0; w < kPlanThreads / kWave; ++w) total += s_sum[w];
+  const int chunk = (int)max((total + A.target - 1) / A.target, (int64_t)kMinTiles);
+  int base = 0;
+  for (int r0 = 0; r0 < batch; r0 += kPlanThreads) {
+    const int r = r0 + tid;
+    const int n = r < batch ? max(1, (read_request(A, r).tiles + chunk - 1) / chunk) : 0;
+    int incl = n;
+    for (int d = 1; d < kWave; d <<= 1) {
+      const int up = __shfl_up(incl, d);
+      incl += lane >= d ? up : 0;
+    }
+    __syncthreads();
+    if (lane == kWave - 1) s_scan[wave] = incl;
+    __syncthreads();
+    int before = base;
+    for (int w = 0; w < kPlanThreads / kWave; ++w) {
+      before += w < wave ? s_scan[w] : 0;
+      base += s_scan[w];
+    }
+    if (r < batch) A.rows[r] = Row{before + incl - n, n};
+  }
+  __syncthreads();
+  const int num = min(base, A.want.max_items);
+  for (int i = tid; i < num; i += kPlanThreads) {
+    int lo = 0, hi = batch;  // the row that holds item i: the last whose first item is <= i
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (A.rows[mid].first <= i) lo = mid; else hi = mid;
+    }
+    const Row row = A.rows[lo];
+    const Request q = read_request(A, lo);
+    const int part = i - row.first;
+    A.items[i] = Item{lo, q.len, q.page_begin, (int)((int64_t)q.tiles * part / row.parts),
+                      (int)((int64_t)q.tiles * (part + 1) / row.parts), i, row.parts, 0};
+  }
+  if (tid == 0) {
+    Header h = A.want;
+    h.num_items = num;
+    *A.header = h;
+  }
+}
+
+// ----------------------------------------------------------------- decode ---
+struct Args {
+  const char *q, *k, *v;
+  char* o;
+  float *lse, *part;
+  const Header* header;
+  const Item* items;
+  const Row* rows;
+  const int32_t* ids;
+  Header want;
+  int64_t q_sb, q_sh, o_sb, o_sh;                        // bytes
+  int64_t page_stride, token_stride, head_stride, num_pages;  // bytes, bytes, bytes (a 4-bit cache has no token stride)
+  int hq, hkv, blocks, page_shift;                       // page_shift: -1 where page_size is no power of two
+  float scale_log2;  // > 0; a negative scale negates q instead
+  uint32_t q_flip;
+};
+
+// Floats of a part: outputs [16][D], then (mu, sum) per head.
+template <int D> constexpr int part_floats() { return 16 * (D + 2); }
+
+__device__ __forceinline__ bool stale(const Header& h, const Header& want) {
+  return h.magic != want.magic || h.batch != want.batch || h.page_size != want.page_size || h.window != want.window ||
+         h.sinks != want.sinks || h.indices_capacity != want.indices_capacity || h.max_items != want.max_items;
+}
+
+template <typename T, bool FOUR, int D, bool PAGE16>
+__global__ __launch_bounds__(kThreads, 2) void decode_kernel(Args A) {
+  using MT = typename std::conditional<FOUR, bf16_t, T>::type;  // what is multiplied
+  using P = Planes<MT>;
+  constexpr bool kBf16 = std::is_same<MT, bf16_t>::value;
+  constexpr int NS = D / 32;                                    // products of a score
+  constexpr int NA = D / 16;                                    // dims of a lane in V
+  constexpr int ND = D / 32;                                    // words of them
+  constexpr int QP = FOUR && std::is_same<T, f16_t>::value ? 2 : 1;  // planes of q
+  constexpr int KW = FOUR ? D / 32 : D / 8;                     // words of a lane's K per block of 16 tokens
+  constexpr int VW = FOUR ? 4 : 4 * ND;                         // words of a lane's V per block
+  __shared__ __align__(16) float s_o[kWaves][16][D];
+  __shared__ float s_m[kWaves][16], s_l[kWaves][16];
+  __shared__ float s_odd[kWaves][D];  // of a second walk: the sums of V's infinities and NaN
+
+  const Header head = *A.header;
+  const Item it = A.items[blockIdx.x];
+  if (stale(head, A.want) || blockIdx.x >= (unsigned)head.num_items) return;
+  const int row = uniform(it.row), len = uniform(it.kv_len), pb = uniform(it.page_begin);
+  if (row < 0 || row >= A.want.batch) return;
+  const int h = blockIdx.y / A.blocks, hb = blockIdx.y % A.blocks;
+  const int g = A.hq / A.hkv, rows = min(g - hb * 16, 16);
+  const int lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave);
+  const int lr = lane % 16, grp = lane / 16;
+  const Seen seen = seen_from(len - 1, A.want.window, A.want.sinks, kTile);
+  const int ps = A.want.page_size;
+  const int32_t* ids = A.ids + pb;
+  const int cap = A.want.indices_capacity - pb;
+
+  // q as the B operand: 4-bit K's lanes hold D / 4 dims in a row, 16-bit K's
+  // eight of every 32
+  u32x4 qb[QP][NS];
+  {
+    const int head_q = h * g + hb * 16 + min(lr, rows - 1);  // columns past the heads repeat the last one
+    const char* qp = A.q + (int64_t)row * A.q_sb + (int64_t)head_q * A.q_sh + (FOUR ? grp * (D / 2) : grp * 16);
+#pragma unroll
+    for (int ks = 0; ks < NS; ++ks) {
+      u32x4 w = *reinterpret_cast<const u32x4*>(qp + ks * (FOUR ? 16 : 64));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] ^= A.q_flip;
+      if constexpr (QP == 2) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float a, b;
+          unpack2<f16_t>(w[e], a, b);
+          const uint32_t hi = f32x2_to_bf16x2_bits(a, b);
+          // (the rest of an infinity is none)
+          const float ra = a - bf16_lo(hi), rb = b - bf16_hi(hi);
+          qb[0][ks][e] = hi;
+          qb[QP - 1][ks][e] = f32x2_to_bf16x2_bits(ra == ra ? ra : 0.f, rb == rb ? rb : 0.f);
+        }
+      } else {
+        qb[0][ks] = w;
+      }
+    }
+  }
+
+  auto page_of = [&](int t) { return A.page_shift >= 0 ? t >> A.page_shift : t / ps; };
+  auto page_at = [&](int page) -> int64_t {
+    const int id = ids[min(page, cap - 1)];
+    return (id < 0 ? 0 : ((int64_t)id >= A.num_pages ? A.num_pages - 1 : (int64_t)id)) * A.page_stride;
+  };
+  const int top = len - 1;  // addresses past the sequence repeat its end's
+
+  struct Raw {
+    uint32_t k[2][KW], v[2][VW], ks[2], vs[2];
+  };
+  const char* kh = A.k + (int64_t)h * A.head_stride;
+  const char* vh = A.v + (int64_t)h * A.head_stride;
+  // the dims' place of a lane in a 4-bit V's codes, and its scale group
+  const int vchunk = D == 64 ? (lr / 2) * 16 : lr * (D / 8), vgroup = lr * NA / kGroup;
+
+  auto load_words = [](const char* p, uint32_t* w, auto count) {
+    constexpr int N = decltype(count)::value;
+    if constexpr (N == 2) {
+      const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p));
+      w[0] = x[0];
+      w[1] = x[1];
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i += 4) {
+        const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p) + i / 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[i + j] = x[j];
+      }
+    }
+  };
+  auto fetch = [&](int i, Raw& raw) {
+    const int t0 = seen_tile(seen, i) * kTile;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      // a block's first token, or where it is past the end the last block's
+      const int tb = min(t0 + 16 * b, top & ~15);
+      int64_t pk, pv[4];
+      int ok, ov[4];
+      if constexpr (PAGE16) {
+        const int page = page_of(tb);
+        pk = page_at(page);
+        ok = tb - page * ps;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) pv[j] = pk, ov[j] = ok + 4 * grp + j;
+        ok += lr;
+      } else {
+        const int tk = min(tb + lr, top);
+        const int page = page_of(tk);
+        pk = page_at(page);
+        ok = tk - page * ps;
+#pragma unroll
+        for (int j = 0; j < (FOUR ? 1 : 4); ++j) {
+          const int tv = FOUR ? min(tb + 4 * grp, top & ~3) : min(tb + 4 * grp + j, top);
+          const int pg = page_of(tv);
+          pv[j] = page_at(pg);
+          ov[j] = tv - pg * ps;
+        }
+      }
+      if constexpr (FOUR) {
+        const char* kp = kh + pk;
+        load_words(kp + (ok * (D / 2) + grp * (D / 8)), raw.k[b], std::integral_constant<int, KW>{});
+        const char* sp = kp + (ps * (D / 2) + ok * (D / 32));
+        raw.ks[b] = *reinterpret_cast<const uint8_t*>(sp + grp * (D / 4) / kGroup);
+        const char* vp = vh + pv[0];
+        const int quad = ov[0] / 4;
+        load_words(vp + (quad * (2 * D) + vchunk), raw.v[b], std::integral_constant<int, VW>{});
+        raw.vs[b] = *reinterpret_cast<const uint32_t*>(vp + (ps * (D / 2) + quad * (D / 8) + vgroup * 4));
+      } else {
+        const char* kp = kh + pk + (int64_t)ok * A.token_stride + grp * 16;
+#pragma unroll
+        for (int ks = 0; ks < NS; ++ks) load_words(kp + ks * 64, raw.k[b] + 4 * ks, std::integral_constant<int, 4>{});
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          load_words(vh + pv[j] + (int64_t)ov[j] * A.token_stride + lr * (2 * NA), raw.v[b] + j * ND,
+                     std::integral_constant<int, ND>{});
+      }
+    }
+  };
+
+  f32x4 acc[NA];
+  float m, l;
+  bool saw_odd = false;
+  const float sc = A.scale_log2;
+
+  auto consume = [&](int i, const Raw& raw, bool again) {
+    const int t0 = seen_tile(seen, i) * kTile;
+    f32x4 s[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      s[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < NS; ++ks) {
+        u32x4 ka;
+        if constexpr (FOUR) {
+          ka = codes8(raw.k[b][ks], scale_of(raw.ks[b]));
+        } else {
+          ka = u32x4{raw.k[b][4 * ks], raw.k[b][4 * ks + 1], raw.k[b][4 * ks + 2], raw.k[b][4 * ks + 3]};
+        }
+#pragma unroll
+        for (int pl = 0; pl < QP; ++pl) s[b] = mfma32<MT>(ka, qb[pl][ks], s[b]);
+      }
+    }
+    // V: words [token 4 grp + j of block b][pairs of dims]
+    uint32_t vt[8][ND];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t* w = vt[4 * b + j];
+        if constexpr (FOUR) {
+          const float scale = scale_of((raw.vs[b] >> (8 * j)) & 255u);
+          if constexpr (D == 64) {
+            const uint32_t x = raw.v[b][j] >> (lr % 2 * 16);
+            w[0] = codes2<0>(x, scale);
+            w[1] = codes2<1>(x, scale);
+          } else {
+            const u32x4 x = codes8(raw.v[b][j], scale);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = x[e];
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < ND; ++e) w[e] = raw.v[b][j * ND + e];
+        }
+      }
+    if (t0 + kTile > len || (t0 < seen.lo && t0 + kTile > seen.se)) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int t = t0 + 16 * b + 4 * grp + j;
+          const bool on = t < len && (t >= seen.lo || t < seen.se);
+          s[b][j] = on ? s[b][j] : -INFINITY;
+#pragma unroll
+          for (int e = 0; e < ND; ++e) vt[4 * b + j][e] = on ? vt[4 * b + j][e] : 0u;  // (0 times what lies there)
+        }
+    }
+    if (again) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int e = 0; e < ND; ++e) {
+          float a, b;
+          unpack2<MT>(vt[j][e], a, b);
+          const bool fa = finite16(vt[j][e] & 0xffffu, kBf16), fb = finite16(vt[j][e] >> 16, kBf16);
+          if (!fa) atomicAdd(&s_odd[wave][lr * NA + 2 * e], a);
+          if (!fb) atomicAdd(&s_odd[wave][lr * NA + 2 * e + 1], b);
+          vt[j][e] &= (fa ? 0xffffu : 0u) | (fb ? 0xffff0000u : 0u);
+        }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mx = fmaxf(mx, s[b][j]);
+    mx *= sc;
+    if (__builtin_amdgcn_ballot_w64(mx > m + P::kLag) != 0) {
+      const float mn = fmaxf(m, column_max(mx));
+      const float alpha = fast_exp2(m - (mn == -INFINITY ? 0.f : mn));
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int a = 0; a < NA; ++a)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[a][j] *= alpha;
+    }
+    const float mu = m == -INFINITY ? 0.f : m + P::kBias;
+    u32x4 pb[2];
+    float ps_ = 0.f;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      float p[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        p[j] = fast_exp2(__builtin_fmaf(s[b][j], sc, -mu));
+        ps_ += p[j];
+      }
+      uint32_t hi0, lo0, hi1, lo1;
+      P::split(p[0], p[1], hi0, lo0);
+      P::split(p[2], p[3], hi1, lo1);
+      pb[0][2 * b] = hi0;
+      pb[0][2 * b + 1] = hi1;
+      pb[1][2 * b] = lo0;
+      pb[1][2 * b + 1] = lo1;
+    }
+    l += ps_;  // per lane; the column's lanes meet after the last tile
+#pragma unroll
+    for (int e = 0; e < ND; ++e) {
+      u32x4 v0, v1;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v0[j] = __builtin_amdgcn_perm(vt[2 * j + 1][e], vt[2 * j][e], 0x05040100u);
+        v1[j] = __builtin_amdgcn_perm(vt[2 * j + 1][e], vt[2 * j][e], 0x07060302u);
+      }
+#pragma unroll
+      for (int pl = 0; pl < 2; ++pl) {
+        acc[2 * e] = mfma32<MT>(v0, pb[pl], acc[2 * e]);
+        acc[2 * e + 1] = mfma32<MT>(v1, pb[pl], acc[2 * e + 1]);
+      }
+    }
+  };
+
+  const int n = it.tile_end - it.tile_begin;
+  const int begin = uniform(it.tile_begin + (int)((int64_t)n * wave / kWaves));
+  const int end = uniform(it.tile_begin + (int)((int64_t)n * (wave + 1) / kWaves));
+  for (bool again = false;; again = true) {
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int a = 0; a < NA; ++a) acc[a] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (begin < end) {
+      Raw r0, r1;
+      fetch(begin, r0);
+      int i = begin;
+      for (; i + 2 <= end; i += 2) {
+        fetch(i + 1, r1);
+        consume(i, r0, again);
+        fetch(min(i + 2, end - 1), r0);
+        consume(i + 1, r1, again);
+      }
+      if (i < end) consume(i, r0, again);
+    }
+    if (again) break;
+    bool odd = false;
+#pragma unroll
+    for (int a = 0; a < NA; ++a)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) odd |= acc[a][j] != acc[a][j];
+    if (__builtin_amdgcn_ballot_w64(odd) == 0) break;
+    for (int d = lane; d < D; d += kWave) s_odd[wave][d] = 0.f;
+    saw_odd = true;
+  }
+  if (saw_odd) {
+    // (of this wave alone: its LDS operations are in order)
+#pragma unroll
+    for (int a = 0; a < NA; ++a)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[a][j] += s_odd[wave][(4 * grp + j) * NA + a];
+  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if (lr < rows) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int a = 0; a < NA; a += 4)
+        *reinterpret_cast<f32x4*>(&s_o[wave][lr][(4 * grp + j) * NA + a]) =
+            f32x4{acc[a][j], acc[a + 1][j], acc[a + 2][j], acc[a + 3][j]};
+    if (grp == 0) {
+      s_m[wave][lr] = m == -INFINITY ? -INFINITY : m + P::kBias;
+      s_l[wave][lr] = l;
+    }
+  }
+  __syncthreads();
+  const int parts = uniform(it.parts);
+  float* part = A.part + ((int64_t)uniform(it.slot) * A.hkv * A.blocks + blockIdx.y) * part_floats<D>();
+  for (int c = threadIdx.x; c < rows * (D / 4); c += kThreads) {
+    const int r = c / (D / 4), d = c % (D / 4) * 4;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, s_m[w][r]);
+    float sum = 0.f;
+    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = s_m[w][r] == -INFINITY ? 0.f : fast_exp2(s_m[w][r] - mx);
+      const f32x4 x = *reinterpret_cast<const f32x4*>(&s_o[w][r][d]);
+      sum += s_l[w][r] * f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += weighted(x[e], f);
+    }
+    if (parts > 1) {
+      *reinterpret_cast<f32x4*>(part + r * D + d) = o;
+      if (d == 0) *reinterpret_cast<f32x2*>(part + 16 * D + 2 * r) = f32x2{mx, sum};
+      continue;
+    }
+    const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+    const int hq = h * g + hb * 16 + r;
+    *reinterpret_cast<u32x2*>(A.o + (int64_t)row * A.o_sb + (int64_t)hq * A.o_sh + d * 2) =
+        u32x2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
+    if (d == 0 && A.lse) A.lse[(int64_t)row * A.hq + hq] = sum > 0.f ? (mx + log2f(sum)) * 0.69314718055994531f : (sum == 0.f ? -INFINITY : sum);
+  }
+}
+
+// One wave per (request, head) of several items: their parts in order, D / 64 dims
+// per lane.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void merge_kernel(Args A) {
+  constexpr int N = D / 64;
+  const Header head = *A.header;
+  if (stale(head, A.want)) return;
+  const int64_t at = (int64_t)blockIdx.x * kWaves + uniform(threadIdx.x / kWave);
+  if (at >= (int64_t)A.want.batch * A.hq) return;
+  const int row = (int)(at / A.hq), hq = (int)(at % A.hq), lane = threadIdx.x % kWave;
+  const Row rec = A.rows[row];
+  const int parts = uniform(rec.parts), first = uniform(rec.first);
+  if (parts <= 1 || first < 0 || first + parts > A.want.max_items) return;
+  const int g = A.hq / A.hkv, h = hq / g, r = hq % g;
+  const float* p = A.part + ((int64_t)first * A.hkv * A.blocks + h * A.blocks + r / 16) * part_floats<D>();
+  const int64_t step = (int64_t)A.hkv * A.blocks * part_floats<D>();
+  const float* ml = p + 16 * D + 2 * (r % 16);
+  float top = -INFINITY;
+  for (int b = lane; b < parts; b += kWave) top = fmaxf(top, ml[b * step]);
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+  float sum = 0.f, o[N] = {};
+  for (int b0 = 0; b0 < parts; b0 += kWave) {
+    const int n = min(parts - b0, kWave);
+    const f32x2 own = lane < n ? *reinterpret_cast<const f32x2*>(ml + (b0 + lane) * step) : f32x2{-INFINITY, 0.f};
+    const float w = own[0] == -INFINITY ? 0.f : fast_exp2(own[0] - top);
+    const float lw = own[1] * w;
+    const float* q = p + b0 * step + (r % 16) * D + lane * N;
+    for (int i0 = 0; i0 < n; i0 += 8) {
+      float v[8][N];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[i][e] = q[min(i0 + i, n - 1) * step + e];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i0 + i >= n) break;
+        const float wi = lane_value(w, i0 + i);
+        sum += lane_value(lw, i0 + i);
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[e] += weighted(v[i][e], wi);
+      }
+    }
+  }
+  const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+  T* op = reinterpret_cast<T*>(A.o + (int64_t)row * A.o_sb + (int64_t)hq * A.o_sh) + lane * N;
+#pragma unroll
+  for (int e = 0; e < N; ++e) op[e] = from_float<T>(o[e] * inv);
+  if (lane == 0 && A.lse) A.lse[(int64_t)row * A.hq + hq] = sum > 0.f ? (top + log2f(sum)) * 0.69314718055994531f : (sum == 0.f ? -INFINITY : sum);
+}
+
+template <typename T, bool FOUR, int D>
+int launch(const Args& a, hipStream_t s) {
+  const dim3 grid((unsigned)a.want.max_items, (unsigned)(a.hkv * a.blocks));
+  if (a.want.page_size % 16 == 0)
+    hipLaunchKernelGGL((decode_kernel<T, FOUR, D, true>), grid, dim3(kThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL((decode_kernel<T, FOUR, D, false>), grid, dim3(kThreads), 0, s, a);
+  PL_LAUNCH_CHECK("window decode_kernel");
+  const int64_t waves = (int64_t)a.want.batch * a.hq;
+  hipLaunchKernelGGL((merge_kernel<T, D>), dim3((unsigned)((waves + kWaves - 1) / kWaves)), dim3(kThreads), 0, s, a);
+  PL_LAUNCH_CHECK("window merge_kernel");
+  return ok();
+}
+
+template <typename T, bool FOUR>
+int launch_d(const Args& a, int d, hipStream_t s) {
+  return d == 64 ? launch<T, FOUR, 64>(a, s) : launch<T, FOUR, 128>(a, s);
+}
+
+}  // namespace dec
+}  // namespace window
+}  // namespace pl
+
+using namespace pl;
+using namespace pl::window;
+using namespace pl::window::dec;
+
+static int check_shape(int batch, int hq, int hkv, int page_size, int window, int sinks) {
+  if (batch < 0 || batch > (1 << 24)) return fail(PL_ERR_INVALID, "batch must be in 0 .. 2^24 (got %d)", batch);
+  if (hkv <= 0 || hq <= 0 || hq % hkv)
+    return fail(PL_ERR_INVALID, "num_qo_heads (%d) must be a multiple of num_kv_heads (%d)", hq, hkv);
+  if ((int64_t)hkv * head_blocks(hq, hkv) > 65535) return fail(PL_ERR_INVALID, "%d kv heads are too many", hkv);
+  if (page_size <= 0 || page_size > kMaxLen) return fail(PL_ERR_INVALID, "page_size must be positive (got %d)", page_size);
+  if (window < 0 || sinks < 0) return fail(PL_ERR_INVALID, "window and sinks must be >= 0");
+  return PL_OK;
+}
+
+static int max_items_of(int batch, int hq, int hkv) { return batch + target_items(hq, hkv); }
+
+extern "C" size_t pl_window_decode_plan_size(int batch, int indices_capacity, int num_qo_heads, int num_kv_heads) {
+  if (check_shape(batch, num_qo_heads, num_kv_heads, 1, 0, 0) != PL_OK || indices_capacity < 0) return 0;
+  return layout(batch, indices_capacity, max_items_of(batch, num_qo_heads, num_kv_heads)).bytes;
+}
+
+extern "C" size_t pl_window_decode_workspace_size(int batch, int num_qo_heads, int num_kv_heads, int head_dim) {
+  if (check_shape(batch, num_qo_heads, num_kv_heads, 1, 0, 0) != PL_OK || head_dim < 0) return 0;
+  return (size_t)max_items_of(batch, num_qo_heads, num_kv_heads) * num_kv_heads *
+         head_blocks(num_qo_heads, num_kv_heads) * 16 * (head_dim + 2) * sizeof(float);
+}
+
+static Header wanted(int batch, int page_size, int window, int sinks, int capacity, int hq, int hkv) {
+  Header h{};
+  h.magic = kMagic ^ (hq << 8) ^ hkv;
+  h.batch = batch;
+  h.page_size = page_size;
+  h.window = window;
+  h.sinks = sinks;
+  h.indices_capacity = capacity;
+  h.max_items = max_items_of(batch, hq, hkv);
+  return h;
+}
+
+extern "C" int pl_window_decode_plan(const int32_t* indptr, const int32_t* indices, int indices_capacity,
+                                     const int32_t* last_page_len, int batch, int num_qo_heads, int num_kv_heads,
+                                     int page_size, int window, int sinks, void* plan, size_t plan_bytes,
+                                     void* stream) {
+  if (int e = check_shape(batch, num_qo_heads, num_kv_heads, page_size, window, sinks)) return e;
+  if (indices_capacity < 0) return fail(PL_ERR_INVALID, "indices_capacity must be >= 0");
+  if (batch == 0) return ok();
+  if (!indptr || !last_page_len || !plan || (indices_capacity > 0 && !indices))
+    return fail(PL_ERR_INVALID, "null pointer argument");
+  if ((uintptr_t)plan % 64) return fail(PL_ERR_INVALID, "the plan must be 64-byte aligned");
+  const Header want = wanted(batch, page_size, window, sinks, indices_capacity, num_qo_heads, num_kv_heads);
+  const Layout l = layout(batch, indices_capacity, want.max_items);
+  if (plan_bytes < l.bytes) return fail(PL_ERR_WORKSPACE, "plan of %zu bytes < %zu needed", plan_bytes, l.bytes);
+  PlanArgs a{};
+  char* p = (char*)plan;
+  a.indptr = indptr;
+  a.indices = indices;
+  a.last = last_page_len;
+  a.want = want;
+  a.header = (Header*)p;
+  a.items = (Item*)(p + l.items);
+  a.rows = (Row*)(p + l.rows);
+  a.ids = (int32_t*)(p + l.indices);
+  a.target = target_items(num_qo_heads, num_kv_heads);
+  const int copies = (indices_capacity + 4 * kPlanThreads - 1) / (4 * kPlanThreads);
+  hipLaunchKernelGGL(plan_kernel, dim3(1 + (copies < 64 ? copies : 64)), dim3(kPlanThreads), 0, (hipStream_t)stream, a);
+  PL_LAUNCH_CHECK("window plan_kernel");
+  return ok();
+}
+
+extern "C" int pl_window_decode_run(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* k_cache,
+                                    const void* v_cache, int64_t page_stride, int64_t token_stride,
+                                    int64_t head_stride, int64_t num_pages, int kv_bits, void* o, int64_t o_stride_b,
+                                    int64_t o_stride_h, float* lse, int batch, int num_qo_heads, int num_kv_heads,
+                                    int head_dim, int page_size, int window, int sinks, float sm_scale, int dtype,
+                                    const void* plan, size_t plan_bytes, int indices_capacity, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  if (int e = check_shape(batch, num_qo_heads, num_kv_heads, page_size, window, sinks)) return e;
+  if (head_dim != 64 && head_dim != 128)
+    return fail(PL_ERR_UNSUPPORTED, "head_dim must be 64 or 128 (got %d)", head_dim);
+  if (dtype != PL_DTYPE_BF16 && dtype != PL_DTYPE_F16)
+    return fail(PL_ERR_UNSUPPORTED, "dtype must be F16 or BF16 (got %d)", dtype);
+  if (kv_bits != 16 && kv_bits != 4) return fail(PL_ERR_UNSUPPORTED, "kv_bits must be 16 or 4 (got %d)", kv_bits);
+  if (kv_bits == 4 && (page_size % 8 || page_size > (1 << 20)))
+    return fail(PL_ERR_INVALID, "pages of a 4-bit cache hold a multiple of 8 tokens, up to 2^20 (got %d)", page_size);
+  if (num_pages <= 0 || indices_capacity < 0) return fail(PL_ERR_INVALID, "num_pages must be positive");
+  if (batch == 0) return ok();
+  if (!q || !k_cache || !v_cache || !o || !plan || !workspace) return fail(PL_ERR_INVALID, "null pointer argument");
+  const int eb = kv_bits == 4 ? 1 : 2;  // a 4-bit cache's strides are bytes
+  const int64_t strides[] = {q_stride_b * 2, q_stride_h * 2, o_stride_b * 2, o_stride_h * 2, page_stride * eb,
+                             kv_bits == 4 ? 0 : token_stride * eb, head_stride * eb};
+  for (int64_t st : strides)
+    if (st % 16) return fail(PL_ERR_INVALID, "strides must be multiples of 16 bytes");
+  const void* ptrs[] = {q, k_cache, v_cache, o, workspace};
+  for (const void* p : ptrs)
+    if ((uintptr_t)p % 16) return fail(PL_ERR_INVALID, "q, o, the caches and workspace must be 16-byte aligned");
+  if ((uintptr_t)plan % 64) return fail(PL_ERR_INVALID, "the plan must be 64-byte aligned");
+  const Header want = wanted(batch, page_size, window, sinks, indices_capacity, num_qo_heads, num_kv_heads);
+  const Layout lay = layout(batch, indices_capacity, want.max_items);
+  if (plan_bytes < lay.bytes) return fail(PL_ERR_WORKSPACE, "plan of %zu bytes < %zu needed", plan_bytes, lay.bytes);
+  const size_t need = pl_window_decode_workspace_size(batch, num_qo_heads, num_kv_heads, head_dim);
+  if (workspace_bytes < need)
+    return fail(PL_ERR_WORKSPACE, "workspace of %zu bytes < %zu needed", workspace_bytes, need);
+  Args a{};
+  const char* p = (const char*)plan;
+  a.q = (const char*)q;
+  a.k = (const char*)k_cache;
+  a.v = (const char*)v_cache;
+  a.o = (char*)o;
+  a.lse = lse;
+  a.part = (float*)workspace;
+  a.header = (const Header*)p;
+  a.items = (const Item*)(p + lay.items);
+  a.rows = (const Row*)(p + lay.rows);
+  a.ids = (const int32_t*)(p + lay.indices);
+  a.want = want;
+  a.q_sb = strides[0];
+  a.q_sh = strides[1];
+  a.o_sb = strides[2];
+  a.o_sh = strides[3];
+  a.page_stride = strides[4];
+  a.token_stride = strides[5];
+  a.head_stride = strides[6];
+  a.num_pages = num_pages;
+  a.hq = num_qo_heads;
+  a.hkv = num_kv_heads;
+  a.blocks = head_blocks(num_qo_heads, num_kv_heads);
+  a.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1;
+  // maxima are taken before scaling: a positive scale (a zero one as one far below
+  // any score's rounding), the sign moved into q
+  const float s2 = sm_scale * 1.44269504088896340736f;
+  a.scale_log2 = fmaxf(fabsf(s2), 1e-30f);
+  a.q_flip = s2 < 0 ? 0x80008000u : 0u;
+  const hipStream_t st = (hipStream_t)stream;
+  if (dtype == PL_DTYPE_BF16)
+    return kv_bits == 4 ? launch_d<bf16_t, true>(a, head_dim, st) : launch_d<bf16_t, false>(a, head_dim, st);
+  return kv_bits == 4 ? launch_d<f16_t, true>(a, head_dim, st) : launch_d<f16_t, false>(a, head_dim, st);
+}

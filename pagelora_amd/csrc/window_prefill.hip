@@ -1,0 +1,783 @@
+// Prefill attention over a paged KV cache of 16 or of 4 bits per value, under a
+// sliding window with sinks (gfx950).
+//
+// Request r's queries are the last qo_len of its kv_len positions; the one at
+// position p sees t <= p with t > p - window (window 0: every one) or t < sinks:
+//   o = sum_t p_t v_t / sum_t p_t,  p_t = exp(s q . k_t).
+//
+// An item is 128 rows (query, head of the GQA group) of a request over a range of
+// the kv tiles, 64 tokens each, that some of its rows see; the host plan cuts the
+// ranges where the rows alone would leave the chip idle, and merge_kernel joins them
+// in order.  Four waves of 32 rows, two columns of 16 each.
+//
+// A tile lies in LDS in 16 bits, two buffers, its 16-byte chunks permuted by the row
+// so that the operand reads are free of bank conflicts.  16-bit pages are loaded
+// straight into it; 4-bit ones are loaded into registers two tiles ahead and become
+// bf16 (exact) on the way in, while the waves work on the tile before.  S^T = K Q^T
+// keeps a query per lane, whose probabilities are the B operand of O^T += V^T P^T as
+// they lie; V^T comes out of LDS transposed.
+//
+// Where an output is NaN (0 times an infinity, or the difference of two planes'
+// infinities, is not what a row sees), the item is worked on once more: V's
+// infinities and NaN are taken out in LDS and added to the rows that see them.
+#include <algorithm>
+#include <vector>
+
+#include "window_common.h"
+
+namespace pl {
+namespace window {
+namespace pre {
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWave * kWaves;
+constexpr int kCols = 2;                    // 16-query columns per wave
+constexpr int kWaveRows = 16 * kCols;
+constexpr int kRows = kWaveRows * kWaves;   // rows per item
+constexpr int kTile = 64;                   // kv tokens per tile
+
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+
+// One work item, or (in the merge list) one row item split into parts.  Tiles are
+// counted by what the item's first row sees on.
+struct Item {
+  int32_t request, row0;
+  int32_t tile_begin, tile_end;
+  int32_t slot;  // first part of the row item; -1: writes the output itself
+  int32_t part, parts;
+  int32_t pad;
+};
+static_assert(sizeof(Item) == 32, "the plan's record");
+
+constexpr int part_floats(int d) { return kRows * (d + 2); }  // outputs [row][dim], then (mu, sum) per row
+
+__device__ __forceinline__ void load_lds16(const char* g, char* l) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
+                                   (__attribute__((address_space(3))) void*)l, 16, 0, 0);
+}
+__device__ __forceinline__ u32x2 read_tr(const char* p) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)p));
+}
+
+struct Args {
+  const char *q, *k, *v;
+  char* o;
+  float* part;
+  const int32_t *qo_indptr, *kv_indptr, *kv_indices, *kv_last;
+  const Item* items;
+  int64_t q_st, q_sh, o_st, o_sh, page_stride, token_stride, head_stride;  // bytes
+  int64_t num_pages;
+  int batch, hq, hkv, page_size, page_shift, window, sinks;
+  float scale_log2;  // > 0; a negative scale negates q instead
+  uint32_t q_flip;
+};
+
+template <typename T, bool FOUR, int D, bool PAGE16>
+__global__ __launch_bounds__(kThreads, 2) void prefill_kernel(Args A) {
+  using MT = typename std::conditional<FOUR, bf16_t, T>::type;  // what is multiplied
+  using P = Planes<MT>;
+  constexpr bool kBf16 = std::is_same<MT, bf16_t>::value;
+  constexpr int QP = FOUR && std::is_same<T, f16_t>::value ? 2 : 1;  // planes of q
+  constexpr int NS = D / 32, NA = D / 16;
+  constexpr int RB = D * 2;              // bytes of a row
+  constexpr int CH = D / 8;              // its 16-byte chunks
+  constexpr int TPL = kWave / CH;        // tokens of a load instruction
+  constexpr int NL = 16 / TPL;           // load instructions of a wave's 16 tokens
+  constexpr int kBuf = kTile * RB;
+  // one object per buffer: writes into one never alias reads of another
+  __shared__ __align__(16) char s_k0[kBuf];
+  __shared__ __align__(16) char s_v0[kBuf];
+  __shared__ __align__(16) char s_k1[kBuf];
+  __shared__ __align__(16) char s_v1[kBuf];
+  __shared__ unsigned int s_odd[4];      // the tile's tokens with infinities or NaN (2 words); whether an output is NaN
+  const int h = blockIdx.x % A.hkv;
+  const Item it = A.items[blockIdx.x / A.hkv];
+  const int r = uniform(it.request), row0 = uniform(it.row0);
+  if (r < 0 || r >= A.batch) return;
+  const int g = A.hq / A.hkv;
+  const int qo_begin = uniform(A.qo_indptr[r]);
+  const int qo_len = uniform(A.qo_indptr[r + 1]) - qo_begin;
+  const int page0 = uniform(A.kv_indptr[r]), n_pages = uniform(A.kv_indptr[r + 1]) - page0;
+  if (n_pages <= 0) return;
+  const int last = min(max(uniform(A.kv_last[r]), 1), A.page_size);
+  const int kv_len = (n_pages - 1) * A.page_size + last;
+  const int n_rows = qo_len * g;
+  const int32_t* ind = A.kv_indices + page0;
+  const int ps = A.page_size;
+
+  const int tid = threadIdx.x, lane = tid % kWave, wave = uniform(tid / kWave);
+  const int lr = lane % 16, grp = lane / 16;
+
+  // what rows see: t <= lim and (t >= lo or t < sinks)
+  const int base = kv_len - qo_len;
+  const Seen seen = seen_from(base + row0 / g, A.window, A.sinks, kTile);
+  auto low = [&](int p) { return A.window > 0 ? max(p - A.window + 1, 0) : 0; };
+  const int wrow = row0 + wave * kWaveRows;
+  const bool wave_on = wrow < n_rows;
+  const int lim_lo = wave_on ? base + wrow / g : -1;
+  const int lim_hi = wave_on ? base + (min(wrow + kWaveRows, n_rows) - 1) / g : -1;
+  const int lo_lo = low(lim_lo), lo_hi = low(lim_hi);
+  int lim[kCols], lo[kCols];
+  u32x4 qb[QP][kCols][NS];
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) {
+    const int row = min(wrow + c * 16 + lr, n_rows - 1);  // rows past the end repeat the last one; not stored
+    const int pos = row / g;
+    lim[c] = base + pos;
+    lo[c] = low(lim[c]);
+    const char* qp = A.q + (int64_t)(qo_begin + pos) * A.q_st + (int64_t)(h * g + row - pos * g) * A.q_sh + grp * 16;
+#pragma unroll
+    for (int ks = 0; ks < NS; ++ks) {
+      u32x4 w = *reinterpret_cast<const u32x4*>(qp + ks * 64);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        w[e] ^= A.q_flip;
+        if constexpr (QP == 2) {
+          float a, b;
+          unpack2<f16_t>(w[e], a, b);
+          w[e] = f32x2_to_bf16x2_bits(a, b);
+          const float ra = a - bf16_lo(w[e]), rb = b - bf16_hi(w[e]);  // (the rest of an infinity is none)
+          qb[QP - 1][c][ks][e] = f32x2_to_bf16x2_bits(ra == ra ? ra : 0.f, rb == rb ? rb : 0.f);
+        }
+      }
+      qb[0][c][ks] = w;
+    }
+  }
+
+  auto page_of = [&](int t) { return A.page_shift >= 0 ? t >> A.page_shift : t / ps; };
+  auto clamp_page = [&](int id) -> int64_t {
+    return (id < 0 ? 0 : ((int64_t)id >= A.num_pages ? A.num_pages - 1 : (int64_t)id)) * A.page_stride;
+  };
+  const int t_begin = uniform(it.tile_begin), t_end = uniform(it.tile_end);
+  // the page of the wave's 16 tokens of a tile (pages of 16 and more)
+  auto wave_page = [&](int t) { return ind[page_of(min(t, kv_len - 1))]; };
+
+  const char* kh = A.k + (int64_t)h * A.head_stride;
+  const char* vh = A.v + (int64_t)h * A.head_stride;
+  // 16 bits: a wave fetches its 16 tokens of a tile, TPL per instruction; lane l of
+  // one token l / CH, chunk (l % CH) permuted by the row
+  auto load_wide = [&](int tile, int id, char* kd, char* vd) {
+    const int t0 = seen_tile(seen, tile) * kTile + wave * 16;
+    kd += wave * 16 * RB;
+    vd += wave * 16 * RB;
+    int64_t page = 0;
+    int in_page = 0;
+    if constexpr (PAGE16) {
+      const int t = min(t0, (kv_len - 1) & ~15);
+      page = clamp_page(id);
+      in_page = t - page_of(t) * ps;
+    }
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+      const int row = j * TPL + lane / CH;
+      int64_t at;
+      if constexpr (PAGE16) {
+        at = page + (int64_t)(in_page + row) * A.token_stride;
+      } else {
+        const int t = min(t0 + row, kv_len - 1), pg = page_of(t);
+        at = clamp_page(ind[pg]) + (int64_t)(t - pg * ps) * A.token_stride;
+      }
+      load_lds16(kh + at + ((lane % CH) ^ (row % CH)) * 16, kd + j * TPL * RB);
+      load_lds16(vh + at + ((lane % CH) ^ (2 * (row % (CH / 2)))) * 16, vd + j * TPL * RB);
+    }
+  };
+  // 4 bits: thread tid holds a quarter of K token tid / 4, and eight dims of V's
+  // tokens 4 q .., q = tid / CH (at head_dim 64 the first half of the threads)
+  constexpr int KQ = D / 32;             // words of a quarter
+  struct Raw {
+    uint32_t k[KQ], ks, vs;
+    u32x4 v;
+  } raw;
+  const int k_tok = tid / 4, v_quad = CH == 16 ? tid / 16 : tid % (16 * CH) / CH, v_chunk = tid % CH;
+  auto load_four = [&](int tile, int id) {
+    const int t0 = seen_tile(seen, tile) * kTile;
+    int64_t pk, pv;
+    int ok, ov;
+    if constexpr (PAGE16) {
+      const int t = min(t0 + wave * 16, (kv_len - 1) & ~15);
+      pk = clamp_page(id);
+      ok = t - page_of(t) * ps + k_tok % 16;
+      if constexpr (D == 128) {
+        pv = pk;
+        ov = t - page_of(t) * ps + v_quad % 4 * 4;
+      }
+    } else {
+      const int t = min(t0 + k_tok, kv_len - 1), pg = page_of(t);
+      pk = clamp_page(ind[pg]);
+      ok = t - pg * ps;
+    }
+    if constexpr (!PAGE16 || D != 128) {
+      const int t = min(t0 + v_quad * 4, (kv_len - 1) & ~3), pg = page_of(t);
+      pv = clamp_page(ind[pg]);
+      ov = t - pg * ps;
+    }
+    const char* kp = kh + pk;
+    if constexpr (KQ == 4) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(kp + ok * (D / 2) + tid % 4 * (D / 8));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) raw.k[e % KQ] = x[e];
+    } else {
+      const u32x2 x = *reinterpret_cast<const u32x2*>(kp + ok * (D / 2) + tid % 4 * (D / 8));
+      raw.k[0] = x[0];
+      raw.k[1] = x[1];
+    }
+    raw.ks = *reinterpret_cast<const uint8_t*>(kp + ps * (D / 2) + ok * (D / kGroup) + tid % 4 * (D / 4) / kGroup);
+    const char* vp = vh + pv;
+    raw.v = *reinterpret_cast<const u32x4*>(vp + ov / 4 * (2 * D) + v_chunk * 16);
+    raw.vs = *reinterpret_cast<const uint32_t*>(vp + ps * (D / 2) + ov / 4 * (D / 8) + v_chunk / 4 * 4);
+  };
+  auto store_four = [&](int tile, char* kd, char* vd) {
+    const int t0 = seen_tile(seen, tile) * kTile;
+    const float ks = scale_of(raw.ks);
+#pragma unroll
+    for (int c = 0; c < KQ; ++c)
+      *reinterpret_cast<u32x4*>(kd + k_tok * RB + (((tid % 4) * KQ + c) ^ (k_tok % CH)) * 16) = codes8(raw.k[c], ks);
+    if (CH == 16 || tid < 16 * CH) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int row = v_quad * 4 + j;
+        u32x4 x = codes8(raw.v[j], scale_of((raw.vs >> (8 * j)) & 255u));
+        if (t0 + row >= kv_len) x = u32x4{0u, 0u, 0u, 0u};  // (0 times what lies there)
+        *reinterpret_cast<u32x4*>(vd + row * RB + (v_chunk ^ (2 * (row % (CH / 2)))) * 16) = x;
+      }
+    }
+  };
+
+  // operand reads: K row blk*16 + lr, chunk 4 ks + grp; V tokens 4 grp + lr/4
+  // (+16 per half, +32 per kc), dims 16 a + 4 (lr % 4)
+  int kaddr[NS], vaddr[NA];
+#pragma unroll
+  for (int ks = 0; ks < NS; ++ks) kaddr[ks] = lr * RB + ((ks * 4 + grp) ^ (lr % CH)) * 16;
+#pragma unroll
+  for (int a = 0; a < NA; ++a) {
+    const int row = grp * 4 + lr / 4;
+    vaddr[a] = row * RB + (((2 * a + (lr % 4) / 2) ^ (2 * (row % (CH / 2)))) * 16) + (lr % 2) * 8;
+  }
+
+  f32x4 acc[kCols][NA];
+  float m[kCols], l[kCols];
+  const float sc = A.scale_log2;
+  int id = 0;  // the page of the tile that is loaded next
+
+  auto body = [&](int tile, const char* kb, char* vb, char* kn, char* vn, bool again) {
+    if constexpr (!FOUR) {
+      // this wave's loads of the tile are done, and past the barrier everyone's
+      // are, and every wave is done with the other buffers
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_waitcnt(0xF70);
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+      if (tile + 1 < t_end) {
+        load_wide(tile + 1, PAGE16 ? uniform(id) : 0, kn, vn);
+        if (PAGE16 && tile + 2 < t_end) id = wave_page(seen_tile(seen, tile + 2) * kTile + wave * 16);
+      }
+    } else {
+      __syncthreads();
+      if (tile + 1 < t_end) {
+        store_four(tile + 1, kn, vn);
+        if (tile + 2 < t_end) {
+          load_four(tile + 2, PAGE16 ? uniform(id) : 0);
+          if (PAGE16 && tile + 3 < t_end) id = wave_page(seen_tile(seen, tile + 3) * kTile + wave * 16);
+        }
+      }
+    }
+    const int t0 = seen_tile(seen, tile) * kTile;
+    if (!FOUR && t0 + kTile > kv_len) {
+      // past the last token the pages hold anything: zero V there (0 * NaN)
+      for (int c = tid; c < kTile * CH; c += kThreads)
+        if (t0 + c / CH >= kv_len) *reinterpret_cast<u32x4*>(vb + c * 16) = u32x4{0u, 0u, 0u, 0u};
+      __syncthreads();
+    }
+    if (again) {
+      if (tid < 2) s_odd[tid] = 0u;
+      __syncthreads();
+      for (int c = tid; c < kTile * CH; c += kThreads) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(vb + c * 16);
+        bool odd = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) odd |= !finite16(x[e] & 0xffffu, kBf16) || !finite16(x[e] >> 16, kBf16);
+        if (odd) atomicOr(&s_odd[c / CH / 32], 1u << (c / CH % 32));
+      }
+      __syncthreads();
+      for (int half = 0; half < 2; ++half)
+        for (unsigned int left = s_odd[half]; left; left &= left - 1) {
+          const int row = half * 32 + __builtin_ctz(left), t = t0 + row;
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) {
+            if (t > lim[c] || (t < lo[c] && t >= A.sinks)) continue;
+#pragma unroll
+            for (int a = 0; a < NA; ++a) {
+              const int d = 16 * a + 4 * grp;
+              const u32x2 x = *reinterpret_cast<const u32x2*>(vb + row * RB + ((d / 8) ^ (2 * (row % (CH / 2)))) * 16 +
+                                                              d % 8 * 2);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                float v[2];
+                unpack2<MT>(x[i / 2], v[0], v[1]);
+                if (!finite16((x[i / 2] >> (16 * (i % 2))) & 0xffffu, kBf16)) acc[c][a][i] += v[i % 2];
+              }
+            }
+          }
+        }
+      __syncthreads();
+      for (int c = tid; c < kTile * CH; c += kThreads) {
+        u32x4 x = *reinterpret_cast<const u32x4*>(vb + c * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          x[e] &= (finite16(x[e] & 0xffffu, kBf16) ? 0xffffu : 0u) | (finite16(x[e] >> 16, kBf16) ? 0xffff0000u : 0u);
+        *reinterpret_cast<u32x4*>(vb + c * 16) = x;
+      }
+      __syncthreads();
+    }
+    // (uniform) no row of the wave sees the tile
+    if (t0 > lim_hi || (t0 + kTile <= lo_lo && t0 >= A.sinks)) return;
+
+    f32x4 s[kCols][4];
+    // four independent accumulations in turn, here and below: an MFMA waits
+    // for the one before it on the same accumulator
+#pragma unroll
+    for (int b0 = 0; b0 < 4; b0 += 2) {
+#pragma unroll
+      for (int c = 0; c < kCols; ++c)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) s[c][b0 + b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < NS; ++ks) {
+        u32x4 ka[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) ka[b] = *reinterpret_cast<const u32x4*>(kb + kaddr[ks] + (b0 + b) * 16 * RB);
+#pragma unroll
+        for (int pl = 0; pl < QP; ++pl)
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) s[c][b0 + b] = mfma32<MT>(ka[b], qb[pl][c][ks], s[c][b0 + b]);
+      }
+    }
+    if (t0 + kTile - 1 > lim_lo || (t0 < lo_hi && t0 + kTile > A.sinks)) {
+      const int t1 = t0 + 4 * grp;
+#pragma unroll
+      for (int c = 0; c < kCols; ++c)
+#pragma unroll
+        for (int blk = 0; blk < 4; ++blk)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int t = t1 + blk * 16 + i;
+            s[c][blk][i] = t <= lim[c] && (t >= lo[c] || t < A.sinks) ? s[c][blk][i] : -INFINITY;
+          }
+    }
+    float mx[kCols];
+    bool rose = false;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      float v = -INFINITY;
+#pragma unroll
+      for (int blk = 0; blk < 4; ++blk)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v = fmaxf(v, s[c][blk][i]);
+      mx[c] = v * sc;
+      rose |= mx[c] > m[c] + P::kLag;
+    }
+    // the columns' maxima are reduced over their lanes, and the sums and
+    // accumulators rescaled, only where some lane saw a score kLag past its
+    // maximum
+    if (__builtin_amdgcn_ballot_w64(rose) != 0) {
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) {
+        const float mn = fmaxf(m[c], column_max(mx[c]));
+        const float alpha = fast_exp2(m[c] - (mn == -INFINITY ? 0.f : mn));
+        m[c] = mn;
+        l[c] *= alpha;
+        if (again) {
+#pragma unroll
+          for (int a = 0; a < NA; ++a)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[c][a][i] = weighted(acc[c][a][i], alpha);
+        } else {
+#pragma unroll
+          for (int a = 0; a < NA; ++a)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[c][a][i] *= alpha;
+        }
+      }
+    }
+    u32x4 pb[kCols][2][2];
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      const float mu = m[c] == -INFINITY ? 0.f : m[c] + P::kBias;
+      float sum = 0.f;
+      // P^T as the B operand: k = 8*grp + e <-> tokens of blocks 2kc (e < 4) and 2kc+1 (e >= 4)
+#pragma unroll
+      for (int blk = 0; blk < 4; ++blk) {
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p[i] = fast_exp2(__builtin_fmaf(s[c][blk][i], sc, -mu));
+          sum += p[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t hi, lo_;
+          P::split(p[2 * i], p[2 * i + 1], hi, lo_);
+          pb[c][blk / 2][0][blk % 2 * 2 + i] = hi;
+          pb[c][blk / 2][1][blk % 2 * 2 + i] = lo_;
+        }
+      }
+      l[c] += sum;  // per lane; the column's lanes meet after the last tile
+    }
+#pragma unroll
+    for (int kc = 0; kc < 2; ++kc)
+#pragma unroll
+      for (int a0 = 0; a0 < NA; a0 += 2) {
+        u32x4 va[2];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+          const u32x2 v0 = read_tr(vb + vaddr[a0 + a] + kc * 32 * RB);
+          const u32x2 v1 = read_tr(vb + vaddr[a0 + a] + (kc * 32 + 16) * RB);
+          va[a] = u32x4{v0[0], v0[1], v1[0], v1[1]};
+        }
+#pragma unroll
+        for (int pl = 0; pl < 2; ++pl)
+#pragma unroll
+          for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) acc[c][a0 + a] = mfma32<MT>(va[a], pb[c][kc][pl], acc[c][a0 + a]);
+      }
+  };
+
+  for (bool again = false;; again = true) {
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      m[c] = -INFINITY;
+      l[c] = 0.f;
+#pragma unroll
+      for (int a = 0; a < NA; ++a) acc[c][a] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    if (tid == 0) s_odd[2] = 0u;
+    if (t_begin < t_end) {
+      auto page_at = [&](int tile) {
+        return PAGE16 && tile < t_end ? wave_page(seen_tile(seen, tile) * kTile + wave * 16) : 0;
+      };
+      if constexpr (FOUR) {
+        load_four(t_begin, uniform(page_at(t_begin)));
+        store_four(t_begin, s_k0, s_v0);
+        if (t_begin + 1 < t_end) load_four(t_begin + 1, uniform(page_at(t_begin + 1)));
+        id = page_at(t_begin + 2);
+      } else {
+        load_wide(t_begin, uniform(page_at(t_begin)), s_k0, s_v0);
+        id = page_at(t_begin + 1);
+      }
+    }
+    int tile = t_begin;
+    for (; tile + 2 <= t_end; tile += 2) {
+      body(tile, s_k0, s_v0, s_k1, s_v1, again);
+      body(tile + 1, s_k1, s_v1, s_k0, s_v0, again);
+    }
+    if (tile < t_end) body(tile, s_k0, s_v0, s_k1, s_v1, again);
+    if (again) break;
+    bool odd = false;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+#pragma unroll
+      for (int a = 0; a < NA; ++a)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) odd |= acc[c][a][i] != acc[c][a][i];
+    __syncthreads();
+    if (odd) s_odd[2] = 1u;
+    __syncthreads();
+    const bool any = s_odd[2] != 0u;
+    __syncthreads();
+    if (!any) break;
+  }
+
+  const int slot = uniform(it.slot);
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) {
+    float sum = l[c];
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    const int row = wrow + c * 16 + lr;
+    if (row >= n_rows) continue;
+    if (slot >= 0) {
+      float* p = A.part + ((int64_t)(slot + it.part) * A.hkv + h) * part_floats(D);
+      const int pr = wave * kWaveRows + c * 16 + lr;
+#pragma unroll
+      for (int a = 0; a < NA; ++a) *reinterpret_cast<f32x4*>(p + pr * D + a * 16 + grp * 4) = acc[c][a];
+      if (grp == 0)
+        *reinterpret_cast<f32x2*>(p + kRows * D + pr * 2) = f32x2{m[c] == -INFINITY ? -INFINITY : m[c] + P::kBias, sum};
+      continue;
+    }
+    const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+    const int pos = row / g;
+    T* op = reinterpret_cast<T*>(A.o + (int64_t)(qo_begin + pos) * A.o_st + (int64_t)(h * g + row - pos * g) * A.o_sh) +
+            grp * 4;
+#pragma unroll
+    for (int a = 0; a < NA; ++a)
+      *reinterpret_cast<u32x2*>(op + a * 16) = u32x2{pack2<T>(acc[c][a][0] * inv, acc[c][a][1] * inv),
+                                                     pack2<T>(acc[c][a][2] * inv, acc[c][a][3] * inv)};
+  }
+}
+
+// One wave per row of a split row item, D / 64 dims per lane: parts in order.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void merge_kernel(Args A, const Item* merges) {
+  constexpr int N = D / 64;
+  const int h = blockIdx.x % A.hkv;
+  const Item it = merges[blockIdx.x / A.hkv];
+  const int r = uniform(it.request);
+  if (r < 0 || r >= A.batch) return;
+  const int g = A.hq / A.hkv;
+  const int qo_begin = uniform(A.qo_indptr[r]);
+  const int n_rows = (uniform(A.qo_indptr[r + 1]) - qo_begin) * g;
+  const int pr = blockIdx.y * kWaves + uniform(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+  const int row = uniform(it.row0) + pr;
+  if (row >= n_rows) return;
+  const int parts = uniform(it.parts);
+  const float* p = A.part + ((int64_t)uniform(it.slot) * A.hkv + h) * part_floats(D);
+  const int64_t step = (int64_t)A.hkv * part_floats(D);
+  // the parts' states one per lane, their outputs eight loads at a time
+  const float* ml = p + kRows * D + pr * 2;
+  float top = -INFINITY;
+  for (int b = lane; b < parts; b += kWave) top = fmaxf(top, ml[b * step]);
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+  float sum = 0.f, o[N] = {};
+  for (int b0 = 0; b0 < parts; b0 += kWave) {
+    const int n = min(parts - b0, kWave);
+    const f32x2 own = lane < n ? *reinterpret_cast<const f32x2*>(ml + (b0 + lane) * step) : f32x2{-INFINITY, 0.f};
+    const float w = own[0] == -INFINITY ? 0.f : fast_exp2(own[0] - top);
+    const float lw = own[1] * w;
+    const float* q = p + b0 * step + pr * D + lane * N;
+    for (int i0 = 0; i0 < n; i0 += 8) {
+      float v[8][N];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[i][e] = q[min(i0 + i, n - 1) * step + e];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i0 + i >= n) break;
+        const float wi = lane_value(w, i0 + i);
+        sum += lane_value(lw, i0 + i);
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[e] += weighted(v[i][e], wi);
+      }
+    }
+  }
+  const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+  const int pos = row / g;
+  T* op = reinterpret_cast<T*>(A.o + (int64_t)(qo_begin + pos) * A.o_st + (int64_t)(h * g + row - pos * g) * A.o_sh) +
+          lane * N;
+#pragma unroll
+  for (int e = 0; e < N; ++e) op[e] = from_float<T>(o[e] * inv);
+}
+
+// ------------------------------------------------------------ host plan ---
+constexpr int kSlots = 512;   // workgroups the chip holds: two per CU
+constexpr int kMinTiles = 4;  // fewest tiles of a part
+
+template <typename T, bool FOUR, int D> int launch(const Args& a, int num_items, int num_merges, hipStream_t s) {
+  const dim3 grid((unsigned)a.hkv * num_items);
+  if (a.page_size % 16 == 0)
+    hipLaunchKernelGGL((prefill_kernel<T, FOUR, D, true>), grid, dim3(kThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL((prefill_kernel<T, FOUR, D, false>), grid, dim3(kThreads), 0, s, a);
+  PL_LAUNCH_CHECK("window prefill_kernel");
+  if (num_merges > 0) {
+    hipLaunchKernelGGL((merge_kernel<T, D>), dim3((unsigned)a.hkv * num_merges, kRows / kWaves), dim3(kThreads), 0, s,
+                       a, a.items + num_items);
+    PL_LAUNCH_CHECK("window prefill merge_kernel");
+  }
+  return ok();
+}
+template <typename T, bool FOUR> int launch_d(const Args& a, int d, int items, int merges, hipStream_t s) {
+  return d == 64 ? launch<T, FOUR, 64>(a, items, merges, s) : launch<T, FOUR, 128>(a, items, merges, s);
+}
+
+// The records of a plan; entry points catch what vectors throw.
+static int make_plan(const int32_t* qo, const int32_t* kv, const int32_t* kv_last, int batch, int hq, int hkv,
+                     int page_size, int window, int sinks, std::vector<Item>& items, std::vector<Item>& merges,
+                     int& slots) {
+  const int g = hq / hkv;
+  struct Rows {
+    int32_t r, row0, tiles;
+  };
+  std::vector<Rows> list;
+  int64_t work = 0;
+  int longest = 0;
+  for (int r = 0; r < batch; ++r) {
+    const int64_t qo_len = (int64_t)qo[r + 1] - qo[r], pages = (int64_t)kv[r + 1] - kv[r];
+    if (qo_len < 0) return fail(PL_ERR_INVALID, "qo_indptr_h must be non-decreasing (row %d)", r);
+    if (pages < 0) return fail(PL_ERR_INVALID, "kv_indptr_h must be non-decreasing (row %d)", r);
+    if (pages > 0 && (kv_last[r] < 1 || kv_last[r] > page_size))
+      return fail(PL_ERR_INVALID, "last_page_len[%d] = %d outside [1, %d]", r, kv_last[r], page_size);
+    const int64_t kv_len = pages > 0 ? (pages - 1) * page_size + kv_last[r] : 0;
+    if (kv_len > kMaxLen) return fail(PL_ERR_INVALID, "row %d: kv_len %lld too large", r, (long long)kv_len);
+    if (qo_len > kv_len)
+      return fail(PL_ERR_INVALID, "row %d: %lld queries exceed its %lld tokens", r, (long long)qo_len,
+                  (long long)kv_len);
+    const int64_t rows = qo_len * g;
+    if (rows > INT32_MAX / 2) return fail(PL_ERR_INVALID, "row %d: %lld query rows too many", r, (long long)rows);
+    for (int64_t r0 = 0; r0 < rows; r0 += kRows) {
+      const int64_t last_row = std::min<int64_t>(r0 + kRows, rows) - 1;
+      const Seen s = seen_from((int)(kv_len - qo_len + r0 / g), window, sinks, kTile);
+      const int tiles = s.ns + (int)((kv_len - qo_len + last_row / g) / kTile) + 1 - s.fw;
+      list.push_back(Rows{r, (int32_t)r0, tiles});
+      work += tiles;
+      longest = std::max(longest, tiles);
+    }
+  }
+  if (list.size() > (size_t)INT32_MAX / 64) return fail(PL_ERR_INVALID, "too many prefill work items");
+  // A part's length: an even share of the work per slot.  Ranges are cut where the
+  // longest row item is more than twice that, and by four tiles more, which the
+  // parts and the merge cost.
+  const int64_t share = std::max<int64_t>(kMinTiles, (work * hkv + kSlots - 1) / kSlots);
+  const int64_t chunk = longest > 2 * share + 4 ? share : INT32_MAX;
+  for (const Rows& e : list) {
+    const int parts = (int)((e.tiles + chunk - 1) / chunk);
+    for (int p = 0; p < parts; ++p)
+      items.push_back(Item{e.r, e.row0, (int32_t)((int64_t)e.tiles * p / parts),
+                           (int32_t)((int64_t)e.tiles * (p + 1) / parts), parts > 1 ? slots : -1, p, parts, 0});
+    if (parts > 1) {
+      merges.push_back(Item{e.r, e.row0, 0, 0, slots, 0, parts, 0});
+      slots += parts;
+    }
+  }
+  // longest first; items of one length by request and kv range, so that the row
+  // items sharing a range run side by side
+  std::stable_sort(items.begin(), items.end(), [](const Item& a, const Item& b) {
+    const int la = a.tile_end - a.tile_begin, lb = b.tile_end - b.tile_begin;
+    if (la != lb) return la > lb;
+    if (a.request != b.request) return a.request < b.request;
+    return a.tile_begin < b.tile_begin;
+  });
+  return PL_OK;
+}
+
+}  // namespace pre
+}  // namespace window
+}  // namespace pl
+
+using namespace pl;
+using namespace pl::window;
+using namespace pl::window::pre;
+
+extern "C" int pl_window_prefill_plan(const int32_t* qo_indptr_h, const int32_t* kv_indptr_h,
+                                      const int32_t* kv_last_page_len_h, int batch, int num_qo_heads,
+                                      int num_kv_heads, int head_dim, int page_size, int window, int sinks,
+                                      int32_t* items_h, int max_records, int* num_items_h, int* num_merges_h,
+                                      size_t* workspace_bytes_h) {
+  if (!num_items_h || !num_merges_h || !workspace_bytes_h)
+    return fail(PL_ERR_INVALID, "num_items_h, num_merges_h and workspace_bytes_h must not be null");
+  *num_items_h = *num_merges_h = 0;
+  *workspace_bytes_h = 0;
+  if (batch < 0) return fail(PL_ERR_INVALID, "batch must be >= 0");
+  if (batch > 0 && (!qo_indptr_h || !kv_indptr_h || !kv_last_page_len_h))
+    return fail(PL_ERR_INVALID, "null table pointer");
+  if (num_kv_heads <= 0 || num_qo_heads <= 0 || num_qo_heads % num_kv_heads)
+    return fail(PL_ERR_INVALID, "num_qo_heads (%d) must be a multiple of num_kv_heads (%d)", num_qo_heads,
+                num_kv_heads);
+  if (head_dim != 64 && head_dim != 128)
+    return fail(PL_ERR_UNSUPPORTED, "head_dim must be 64 or 128 (got %d)", head_dim);
+  if (page_size <= 0) return fail(PL_ERR_INVALID, "page_size must be positive (got %d)", page_size);
+  if (window < 0 || sinks < 0) return fail(PL_ERR_INVALID, "window and sinks must be >= 0");
+  if (batch > 0 && (qo_indptr_h[0] != 0 || kv_indptr_h[0] != 0))
+    return fail(PL_ERR_INVALID, "qo_indptr_h[0] and kv_indptr_h[0] must be 0");
+  try {
+    std::vector<Item> items, merges;
+    int slots = 0;
+    if (int e = make_plan(qo_indptr_h, kv_indptr_h, kv_last_page_len_h, batch, num_qo_heads, num_kv_heads, page_size,
+                          window, sinks, items, merges, slots))
+      return e;
+    *num_items_h = (int)items.size();
+    *num_merges_h = (int)merges.size();
+    *workspace_bytes_h = (size_t)slots * num_kv_heads * part_floats(head_dim) * sizeof(float);
+    if (items_h == nullptr) return ok();
+    if (items.size() + merges.size() > (size_t)std::max(max_records, 0))
+      return fail(PL_ERR_WORKSPACE, "%zu prefill plan records exceed the %d provided", items.size() + merges.size(),
+                  max_records);
+    std::copy(items.begin(), items.end(), reinterpret_cast<Item*>(items_h));
+    std::copy(merges.begin(), merges.end(), reinterpret_cast<Item*>(items_h) + items.size());
+    return ok();
+  } catch (const std::exception&) {
+    return fail(PL_ERR_INVALID, "no host memory for the prefill plan");
+  }
+}
+
+extern "C" int pl_window_prefill_run(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_cache,
+                                     const void* v_cache, int64_t page_stride, int64_t token_stride,
+                                     int64_t head_stride, int64_t num_pages, int kv_bits, const int32_t* qo_indptr,
+                                     const int32_t* kv_indptr, const int32_t* kv_indices,
+                                     const int32_t* kv_last_page_len, const int32_t* items, int num_items,
+                                     int num_merges, void* o, int64_t o_stride_t, int64_t o_stride_h, int batch,
+                                     int num_qo_heads, int num_kv_heads, int head_dim, int page_size, int window,
+                                     int sinks, float sm_scale, int dtype, void* workspace, size_t workspace_bytes,
+                                     size_t plan_workspace_bytes, void* stream) {
+  if (num_items < 0 || num_merges < 0 || batch < 0)
+    return fail(PL_ERR_INVALID, "num_items, num_merges and batch must be >= 0");
+  if (num_kv_heads <= 0 || num_qo_heads <= 0 || num_qo_heads % num_kv_heads)
+    return fail(PL_ERR_INVALID, "num_qo_heads (%d) must be a multiple of num_kv_heads (%d)", num_qo_heads,
+                num_kv_heads);
+  if (head_dim != 64 && head_dim != 128)
+    return fail(PL_ERR_UNSUPPORTED, "head_dim must be 64 or 128 (got %d)", head_dim);
+  if (dtype != PL_DTYPE_BF16 && dtype != PL_DTYPE_F16)
+    return fail(PL_ERR_UNSUPPORTED, "dtype must be F16 or BF16 (got %d)", dtype);
+  if (kv_bits != 16 && kv_bits != 4) return fail(PL_ERR_UNSUPPORTED, "kv_bits must be 16 or 4 (got %d)", kv_bits);
+  if (page_size <= 0 || num_pages <= 0) return fail(PL_ERR_INVALID, "page_size and num_pages must be positive");
+  if (kv_bits == 4 && (page_size % 8 || page_size > (1 << 20)))
+    return fail(PL_ERR_INVALID, "pages of a 4-bit cache hold a multiple of 8 tokens, up to 2^20 (got %d)", page_size);
+  if (window < 0 || sinks < 0) return fail(PL_ERR_INVALID, "window and sinks must be >= 0");
+  if (num_items == 0 || batch == 0) return ok();
+  if (!q || !k_cache || !v_cache || !qo_indptr || !kv_indptr || !kv_indices || !kv_last_page_len || !items || !o)
+    return fail(PL_ERR_INVALID, "null pointer argument");
+  const int eb = kv_bits == 4 ? 1 : 2;  // a 4-bit cache's strides are bytes
+  const int64_t strides[] = {q_stride_t * 2, q_stride_h * 2, o_stride_t * 2, o_stride_h * 2, page_stride * eb,
+                             kv_bits == 4 ? 0 : token_stride * eb, head_stride * eb};
+  for (int64_t st : strides)
+    if (st % 16) return fail(PL_ERR_INVALID, "strides must be multiples of 16 bytes");
+  const void* ptrs[] = {q, k_cache, v_cache, o, items, workspace};
+  for (const void* p : ptrs)
+    if ((uintptr_t)p % 16) return fail(PL_ERR_INVALID, "q, o, the caches, items and workspace must be 16-byte aligned");
+  if ((int64_t)std::max(num_items, num_merges) * num_kv_heads > INT32_MAX)
+    return fail(PL_ERR_INVALID, "grid of %d items x %d heads too large", num_items, num_kv_heads);
+  if (num_merges > 0 && (!workspace || workspace_bytes < plan_workspace_bytes))
+    return fail(PL_ERR_WORKSPACE, "prefill workspace of %zu bytes < %zu needed", workspace_bytes,
+                plan_workspace_bytes);
+  Args a{};
+  a.q = (const char*)q;
+  a.k = (const char*)k_cache;
+  a.v = (const char*)v_cache;
+  a.o = (char*)o;
+  a.part = (float*)workspace;
+  a.qo_indptr = qo_indptr;
+  a.kv_indptr = kv_indptr;
+  a.kv_indices = kv_indices;
+  a.kv_last = kv_last_page_len;
+  a.items = reinterpret_cast<const Item*>(items);
+  a.q_st = strides[0];
+  a.q_sh = strides[1];
+  a.o_st = strides[2];
+  a.o_sh = strides[3];
+  a.page_stride = strides[4];
+  a.token_stride = strides[5];
+  a.head_stride = strides[6];
+  a.num_pages = num_pages;
+  a.batch = batch;
+  a.hq = num_qo_heads;
+  a.hkv = num_kv_heads;
+  a.page_size = page_size;
+  a.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1;
+  a.window = window;
+  a.sinks = sinks;
+  // maxima are taken before scaling: a positive scale (a zero one as one far below
+  // any score's rounding), the sign moved into q
+  const float s2 = sm_scale * 1.44269504088896340736f;
+  a.scale_log2 = std::max(s2 < 0 ? -s2 : s2, 1e-30f);
+  a.q_flip = s2 < 0 ? 0x80008000u : 0u;
+  const hipStream_t st = (hipStream_t)stream;
+  if (dtype == PL_DTYPE_BF16)
+    return kv_bits == 4 ? launch_d<bf16_t, true>(a, head_dim, num_items, num_merges, st)
+                        : launch_d<bf16_t, false>(a, head_dim, num_items, num_merges, st);
+  return kv_bits == 4 ? launch_d<f16_t, true>(a, head_dim, num_items, num_merges, st)
+                      : launch_d<f16_t, false>(a, head_dim, num_items, num_merges, st);
+}

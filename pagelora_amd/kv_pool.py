@@ -34,6 +34,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from .kv4 import kv4_page_shape
 from .page_table import KVBlockSpan, pack_rows
 
 
@@ -41,16 +42,18 @@ def kv_copy_pages(cache: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -
     """Make page ``dst[i]`` a copy of page ``src[i]`` in every layer (``pl_kv_copy_pages``).
 
     ``cache``: the pool [layers, P, 2, page, Hkv, D], or one layer of it, its
-    pages contiguous.  Page ids are host integers.  A source may be listed more
-    than once; a page that is written must not be written twice nor be a
-    source.  Enqueued on the current stream; the lists are read at once.
+    pages contiguous; or a 4-bit one (uint8 [layers, P, 2, Hkv, bytes]).  Page
+    ids are host integers.  A source may be listed more than once; a page that is
+    written must not be written twice nor be a source.  Enqueued on the current stream; the lists are read at once.
     """
 
     shape, strides = cache.shape, cache.stride()
-    if len(shape) == 5:
+    four = cache.dtype == torch.uint8
+    if len(shape) == (4 if four else 5):
         shape, strides = (1, *shape), (0, *strides)
-    if len(shape) != 6 or shape[2] != 2:
-        raise ValueError(f"cache must be [layers, P, 2, page, Hkv, D] or a layer of it, got {tuple(cache.shape)}")
+    if len(shape) != (5 if four else 6) or shape[2] != 2:
+        raise ValueError(f"cache must be [layers, P, 2, page, Hkv, D] or a layer of it, or a 4-bit one (uint8 [layers, P, "
+                         f"2, Hkv, bytes]), got {tuple(cache.shape)}")
     try:
         src, dst = array("i", src), array("i", dst)
     except (TypeError, OverflowError):
@@ -64,13 +67,18 @@ def kv_copy_pages(cache: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -
         raise RuntimeError("kv_copy_pages needs a cache on a ROCm device")
     page = math.prod(shape[2:])
     # (the stride of a dim of one entry says nothing)
-    if any(n > 1 and a != b for n, a, b in zip(shape[2:], strides[2:], (page // 2, shape[4] * shape[5], shape[5], 1))):
+    packed = (page // 2, shape[4], 1) if four else (page // 2, shape[4] * shape[5], shape[5], 1)
+    if any(n > 1 and a != b for n, a, b in zip(shape[2:], strides[2:], packed)):
         raise ValueError("the pages of the KV cache must be contiguous")
+    if four:  # copied in units of two bytes
+        if page % 2 or strides[0] % 2 or strides[1] % 2:
+            raise ValueError("the pages of a 4-bit KV cache must lie at even distances")
+        strides, page = (strides[0] // 2, strides[1] // 2), page // 2
     with _lib.on_device(device):
         _lib.check(_lib.load().pl_kv_copy_pages(
             cache.data_ptr(), strides[0], strides[1], page, shape[0], shape[1], src.buffer_info()[0],
-            dst.buffer_info()[0], len(src), _lib.dtype_code(cache.dtype), _lib.raw_stream(device)),
-            "pl_kv_copy_pages")
+            dst.buffer_info()[0], len(src), _lib.PL_DTYPE_F16 if four else _lib.dtype_code(cache.dtype),
+            _lib.raw_stream(device)), "pl_kv_copy_pages")
 
 
 class PageAllocator:
@@ -167,6 +175,12 @@ class PagedKVPool:
     ``max_pages``: 0 grows without bound (the reference's default), > 0
     grows straight to that many pages and no further, None never grows (an
     exhausted pool raises RuntimeError).
+
+    ``kv_bits`` 4 holds the cache in 4 bits per value, uint8
+    ``[num_layers, pages, 2, num_kv_heads, bytes]`` (:mod:`pagelora_amd.kv4`),
+    for :func:`~pagelora_amd.kv4.kv4_append` and
+    :class:`~pagelora_amd.window_attention.WindowAttention`; ``dtype`` is then
+    that of the tokens appended and is not the cache's.
     """
 
     def __init__(
@@ -180,16 +194,21 @@ class PagedKVPool:
         dtype: torch.dtype,
         device: torch.device | str,
         max_pages: int | None = 0,
+        kv_bits: int = 16,
     ) -> None:
+        if kv_bits not in (16, 4):
+            raise ValueError(f"kv_bits must be 16 or 4, got {kv_bits}")
         if max_pages is not None and max_pages > 0 and max_pages < capacity_pages:
             raise ValueError(f"max_pages {max_pages} < capacity_pages {capacity_pages}")
         self.num_layers = num_layers
         self.page_size = page_size
         self.num_kv_heads = num_kv_heads
         self.head_dim = head_dim
-        self.cache = torch.empty(
-            (num_layers, capacity_pages, 2, page_size, num_kv_heads, head_dim), dtype=dtype, device=device
-        )
+        self.kv_bits = kv_bits
+        page = (2, page_size, num_kv_heads, head_dim) if kv_bits == 16 else kv4_page_shape(
+            num_kv_heads=num_kv_heads, head_dim=head_dim, page_size=page_size)
+        self.cache = torch.empty((num_layers, capacity_pages, *page), dtype=dtype if kv_bits == 16 else torch.uint8,
+                                 device=device)
         self.max_pages = max_pages
         self.version = 0      # bumped whenever the pool tensor moves
         self.grow_count = 0
