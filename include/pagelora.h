@@ -370,9 +370,12 @@ int pl_kv4_read(const void* k_cache, const void* v_cache, int64_t page_stride,
  * one call's at a time.
  */
 size_t pl_window_decode_plan_size(int batch, int indices_capacity,
-                                  int num_qo_heads, int num_kv_heads);
-size_t pl_window_decode_workspace_size(int batch, int num_qo_heads,
-                                       int num_kv_heads, int head_dim);
+                                  int num_qo_heads, int num_kv_heads,
+                                  int page_size, int window, int sinks);
+size_t pl_window_decode_workspace_size(int batch, int indices_capacity,
+                                       int num_qo_heads, int num_kv_heads,
+                                       int head_dim, int page_size, int window,
+                                       int sinks);
 int pl_window_decode_plan(const int32_t* indptr, const int32_t* indices,
                           int indices_capacity, const int32_t* last_page_len,
                           int batch, int num_qo_heads, int num_kv_heads,

@@ -422,8 +422,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             _i32, _vp,                         # dtype, stream
         ],
     ),
-    "pl_window_decode_plan_size": (_sz, [_i32, _i32, _i32, _i32]),
-    "pl_window_decode_workspace_size": (_sz, [_i32, _i32, _i32, _i32]),
+    "pl_window_decode_plan_size": (_sz, [_i32] * 7),
+    "pl_window_decode_workspace_size": (_sz, [_i32] * 8),
     "pl_window_decode_plan": (
         _i32,
         [

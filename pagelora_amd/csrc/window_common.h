@@ -87,6 +87,22 @@ __device__ __forceinline__ u32x4 codes8(uint32_t w, float scale) {
   return u32x4{codes2<0>(w, scale), codes2<1>(w, scale), codes2<2>(w, scale), codes2<3>(w, scale)};
 }
 
+// And as fp16: exact where 2^-14 <= 0.5 scale and 6 scale is in its range.
+template <int S> __device__ __forceinline__ uint32_t halves2(uint32_t w, float scale) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, S));
+}
+__device__ __forceinline__ u32x4 halves8(uint32_t w, float scale) {
+  return u32x4{halves2<0>(w, scale), halves2<1>(w, scale), halves2<2>(w, scale), halves2<3>(w, scale)};
+}
+
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pk_min(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+__device__ __forceinline__ uint32_t pk_max(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+
 // --------------------------------------------------------------- window ---
 // What the queries at positions p0 .. see: positions from `lo` on (the window of
 // p0), and those before `se` (sinks).  Tiles of `tile` positions are counted by

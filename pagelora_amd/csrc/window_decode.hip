@@ -21,8 +21,10 @@
 //
 // An output that is NaN is looked at again: 0 times an infinity, or the difference of
 // two planes' infinities, is not what the row sees.  The wave's tiles are walked once
-// more with infinities and NaN taken out of V, and their own sum, which all rows
-// share, put in.
+// more with infinities and NaN taken out of V, and once with nothing but them, each
+// with weight 1, added to the sums.
+#include <algorithm>
+
 #include "window_common.h"
 
 namespace pl {
@@ -64,10 +66,23 @@ inline Layout layout(int batch, int indices_capacity, int max_items) {
 
 // Heads of a workgroup: a kv head's group in blocks of 16.
 inline int head_blocks(int hq, int hkv) { return (hq / hkv + 15) / 16; }
-// Items that fill the chip: two workgroups per CU.
-inline int target_items(int hq, int hkv) {
-  const int n = 512 / (hkv * head_blocks(hq, hkv));
-  return n > 1 ? n : 1;
+// Items per kv head and head block that the work is cut into: as many as fill the
+// chip with workgroups twice per CU, more where an item then still has kItemTiles, up
+// to four times as many.  us, at 512 / 768 / 1024 / 1536 / 2048 workgroups: 64 x 4096
+// .. 16384 tokens of 4 bits 156 / 151 / 141 / 135 / 133, 1 x 131072 39 / 35 / 38 / 41 /
+// 46, 64 x 1028 of 16 bits (whole rows at 512) 55 / 62 / 62 / 59 / 74.
+constexpr int kItemTiles = 42;
+__host__ __device__ inline int target_items(int64_t tiles, int heads) {
+  const int64_t least = 512 / heads > 1 ? 512 / heads : 1, most = 2048 / heads > 1 ? 2048 / heads : 1;
+  const int64_t n = tiles / kItemTiles;
+  return (int)(n < least ? least : n > most ? most : n);
+}
+// At most so many items: every request's last may be short.
+inline int max_items_of(int batch, int hq, int hkv, int page_size, int window, int sinks, int indices_capacity) {
+  int64_t tiles = (int64_t)indices_capacity * page_size / kTile + batch;
+  if (window > 0) tiles = std::min(tiles, batch * (((int64_t)window + sinks) / kTile + 4));
+  const int64_t cut = std::min((int64_t)target_items(tiles, hkv * head_blocks(hq, hkv)), tiles / kMinTiles + 1);
+  return batch + (int)cut;
 }
 
 // ------------------------------------------------------------------- plan ---
@@ -78,7 +93,7 @@ struct PlanArgs {
   Item* items;
   Row* rows;
   int32_t* ids;
-  int target;
+  int heads;  // kv heads times head blocks
 };
 
 struct Request {
@@ -117,7 +132,9 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs A) {
   __syncthreads();
   int64_t total = 0;
   for (int w = 0; w < kPlanThreads / kWave; ++w) total += s_sum[w];
-  const int chunk = (int)max((total + A.target - 1) / A.target, (int64_t)kMinTiles);
+  // (tables that overlap hold more than any that do not: no more items than there is room for)
+  const int target = min(target_items(total, A.heads), A.want.max_items - batch);
+  const int chunk = (int)max((total + target - 1) / target, (int64_t)kMinTiles);
   int base = 0;
   for (int r0 = 0; r0 < batch; r0 += kPlanThreads) {
     const int r = r0 + tid;
@@ -183,8 +200,13 @@ __device__ __forceinline__ bool stale(const Header& h, const Header& want) {
          h.sinks != want.sinks || h.indices_capacity != want.indices_capacity || h.max_items != want.max_items;
 }
 
+// ln of sum 2^mu; -inf where nothing was seen.
+__device__ __forceinline__ float log_sum(float mu, float sum) {
+  return sum > 0.f ? (mu + log2f(sum)) * 0.69314718055994531f : (sum == 0.f ? -INFINITY : sum);
+}
+
 template <typename T, bool FOUR, int D, bool PAGE16>
-__global__ __launch_bounds__(kThreads, 2) void decode_kernel(Args A) {
+__global__ __launch_bounds__(kThreads, FOUR ? 3 : 2) void decode_kernel(Args A) {
   using MT = typename std::conditional<FOUR, bf16_t, T>::type;  // what is multiplied
   using P = Planes<MT>;
   constexpr bool kBf16 = std::is_same<MT, bf16_t>::value;
@@ -196,7 +218,6 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(Args A) {
   constexpr int VW = FOUR ? 4 : 4 * ND;                         // words of a lane's V per block
   __shared__ __align__(16) float s_o[kWaves][16][D];
   __shared__ float s_m[kWaves][16], s_l[kWaves][16];
-  __shared__ float s_odd[kWaves][D];  // of a second walk: the sums of V's infinities and NaN
 
   const Header head = *A.header;
   const Item it = A.items[blockIdx.x];
@@ -246,6 +267,22 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(Args A) {
     return (id < 0 ? 0 : ((int64_t)id >= A.num_pages ? A.num_pages - 1 : (int64_t)id)) * A.page_stride;
   };
   const int top = len - 1;  // addresses past the sequence repeat its end's
+  const int n_tiles = it.tile_end - it.tile_begin;
+  const int begin = uniform(it.tile_begin + (int)((int64_t)n_tiles * wave / kWaves));
+  const int end = uniform(it.tile_begin + (int)((int64_t)n_tiles * (wave + 1) / kWaves));
+  // Pages of 16 tokens and more: lane l holds where block l % 2 of tile l / 2 of the
+  // next 32 begins, so that no tile's loads wait for its page ids.
+  int64_t places = 0;
+  auto load_places = [&](int i) {
+    const int tb = min(seen_tile(seen, min(i + lane / 2, end - 1)) * kTile + lane % 2 * 16, top & ~15);
+    const int page = page_of(tb);
+    places = page_at(page) + (int64_t)(tb - page * ps) * (FOUR ? (int64_t)(D / 2) : A.token_stride);
+  };
+  auto place = [&](int i, int b) -> int64_t {
+    const int l = (i - begin) % 32 * 2 + b;
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(places >> 32), l) << 32 |
+                     (uint32_t)__builtin_amdgcn_readlane((int)places, l));
+  };
 
   struct Raw {
     uint32_t k[2][KW], v[2][VW], ks[2], vs[2];
@@ -270,61 +307,67 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(Args A) {
       }
     }
   };
+  // the lane's own part of the addresses in a block: K, V, their scales
+  const uint32_t k_own = FOUR ? lr * (D / 2) + grp * (D / 8) : grp * 16, v_own = FOUR ? grp * (2 * D) + vchunk : lr * (2 * NA);
+  const uint32_t ks_own = lr * (D / 32) + grp * (D / 4) / kGroup, vs_own = grp * (D / 8) + vgroup * 4;
   auto fetch = [&](int i, Raw& raw) {
     const int t0 = seen_tile(seen, i) * kTile;
+    if (PAGE16 && (i - begin) % 32 == 0) load_places(i);
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       // a block's first token, or where it is past the end the last block's
       const int tb = min(t0 + 16 * b, top & ~15);
-      int64_t pk, pv[4];
-      int ok, ov[4];
       if constexpr (PAGE16) {
-        const int page = page_of(tb);
-        pk = page_at(page);
-        ok = tb - page * ps;
+        const int64_t at = place(i, b);
+        if constexpr (FOUR) {
+          const int slot = A.page_shift >= 0 ? tb & (ps - 1) : tb % ps;
+          // scales: from the codes' end, D / 32 bytes a token (codes D / 2)
+          const int64_t sat = at + ps * (D / 2) - slot * (D / 2 - D / 32);
+          load_words((kh + at) + k_own, raw.k[b], std::integral_constant<int, KW>{});
+          raw.ks[b] = *reinterpret_cast<const uint8_t*>((kh + sat) + ks_own);
+          load_words((vh + at) + v_own, raw.v[b], std::integral_constant<int, VW>{});
+          raw.vs[b] = *reinterpret_cast<const uint32_t*>((vh + sat) + vs_own);
+        } else {
+          const char* kp = kh + at + ((int64_t)lr * A.token_stride + k_own);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) pv[j] = pk, ov[j] = ok + 4 * grp + j;
-        ok += lr;
-      } else {
-        const int tk = min(tb + lr, top);
-        const int page = page_of(tk);
-        pk = page_at(page);
-        ok = tk - page * ps;
+          for (int ks = 0; ks < NS; ++ks) load_words(kp + ks * 64, raw.k[b] + 4 * ks, std::integral_constant<int, 4>{});
+          const char* vp = vh + at + ((int64_t)(4 * grp) * A.token_stride + v_own);
 #pragma unroll
-        for (int j = 0; j < (FOUR ? 1 : 4); ++j) {
-          const int tv = FOUR ? min(tb + 4 * grp, top & ~3) : min(tb + 4 * grp + j, top);
-          const int pg = page_of(tv);
-          pv[j] = page_at(pg);
-          ov[j] = tv - pg * ps;
+          for (int j = 0; j < 4; ++j)
+            load_words(vp + j * A.token_stride, raw.v[b] + j * ND, std::integral_constant<int, ND>{});
         }
-      }
-      if constexpr (FOUR) {
-        const char* kp = kh + pk;
-        load_words(kp + (ok * (D / 2) + grp * (D / 8)), raw.k[b], std::integral_constant<int, KW>{});
-        const char* sp = kp + (ps * (D / 2) + ok * (D / 32));
-        raw.ks[b] = *reinterpret_cast<const uint8_t*>(sp + grp * (D / 4) / kGroup);
-        const char* vp = vh + pv[0];
-        const int quad = ov[0] / 4;
-        load_words(vp + (quad * (2 * D) + vchunk), raw.v[b], std::integral_constant<int, VW>{});
-        raw.vs[b] = *reinterpret_cast<const uint32_t*>(vp + (ps * (D / 2) + quad * (D / 8) + vgroup * 4));
       } else {
-        const char* kp = kh + pk + (int64_t)ok * A.token_stride + grp * 16;
+        const int tk = min(tb + lr, top), page = page_of(tk), ok = tk - page * ps;
+        const int64_t pk = page_at(page);
+        if constexpr (FOUR) {
+          const char* kp = kh + pk;
+          load_words(kp + ok * (D / 2) + grp * (D / 8), raw.k[b], std::integral_constant<int, KW>{});
+          raw.ks[b] = *reinterpret_cast<const uint8_t*>(kp + ps * (D / 2) + ok * (D / 32) + grp * (D / 4) / kGroup);
+          const int tv = min(tb + 4 * grp, top & ~3), pg = page_of(tv), quad = (tv - pg * ps) / 4;
+          const char* vp = vh + page_at(pg);
+          load_words(vp + quad * (2 * D) + vchunk, raw.v[b], std::integral_constant<int, VW>{});
+          raw.vs[b] = *reinterpret_cast<const uint32_t*>(vp + ps * (D / 2) + quad * (D / 8) + vgroup * 4);
+        } else {
+          const char* kp = kh + pk + (int64_t)ok * A.token_stride + k_own;
 #pragma unroll
-        for (int ks = 0; ks < NS; ++ks) load_words(kp + ks * 64, raw.k[b] + 4 * ks, std::integral_constant<int, 4>{});
+          for (int ks = 0; ks < NS; ++ks) load_words(kp + ks * 64, raw.k[b] + 4 * ks, std::integral_constant<int, 4>{});
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          load_words(vh + pv[j] + (int64_t)ov[j] * A.token_stride + lr * (2 * NA), raw.v[b] + j * ND,
-                     std::integral_constant<int, ND>{});
+          for (int j = 0; j < 4; ++j) {
+            const int tv = min(tb + 4 * grp + j, top), pg = page_of(tv);
+            load_words(vh + page_at(pg) + (int64_t)(tv - pg * ps) * A.token_stride + v_own, raw.v[b] + j * ND,
+                       std::integral_constant<int, ND>{});
+          }
+        }
       }
     }
   };
 
   f32x4 acc[NA];
   float m, l;
-  bool saw_odd = false;
   const float sc = A.scale_log2;
 
-  auto consume = [&](int i, const Raw& raw, bool again) {
+  enum { kAll, kFinite, kOdd };  // what of V a walk takes
+  auto consume = [&](int i, const Raw& raw, int walk) {
     const int t0 = seen_tile(seen, i) * kTile;
     f32x4 s[2];
 #pragma unroll
@@ -377,55 +420,57 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(Args A) {
           for (int e = 0; e < ND; ++e) vt[4 * b + j][e] = on ? vt[4 * b + j][e] : 0u;  // (0 times what lies there)
         }
     }
-    if (again) {
+    if (walk != kAll) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
 #pragma unroll
         for (int e = 0; e < ND; ++e) {
-          float a, b;
-          unpack2<MT>(vt[j][e], a, b);
-          const bool fa = finite16(vt[j][e] & 0xffffu, kBf16), fb = finite16(vt[j][e] >> 16, kBf16);
-          if (!fa) atomicAdd(&s_odd[wave][lr * NA + 2 * e], a);
-          if (!fb) atomicAdd(&s_odd[wave][lr * NA + 2 * e + 1], b);
-          vt[j][e] &= (fa ? 0xffffu : 0u) | (fb ? 0xffff0000u : 0u);
+          const uint32_t held = (finite16(vt[j][e] & 0xffffu, kBf16) ? 0xffffu : 0u) |
+                                (finite16(vt[j][e] >> 16, kBf16) ? 0xffff0000u : 0u);
+          vt[j][e] &= walk == kFinite ? held : ~held;
         }
     }
-    float mx = -INFINITY;
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) mx = fmaxf(mx, s[b][j]);
-    mx *= sc;
-    if (__builtin_amdgcn_ballot_w64(mx > m + P::kLag) != 0) {
-      const float mn = fmaxf(m, column_max(mx));
-      const float alpha = fast_exp2(m - (mn == -INFINITY ? 0.f : mn));
-      m = mn;
-      l *= alpha;
-#pragma unroll
-      for (int a = 0; a < NA; ++a)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[a][j] *= alpha;
-    }
-    const float mu = m == -INFINITY ? 0.f : m + P::kBias;
     u32x4 pb[2];
-    float ps_ = 0.f;
+    if (walk == kOdd) {
+      const uint32_t one = pack2<MT>(1.f, 1.f);
+      pb[0] = pb[1] = u32x4{one, one, one, one};
+    } else {
+      float mx = -INFINITY;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      float p[4];
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        p[j] = fast_exp2(__builtin_fmaf(s[b][j], sc, -mu));
-        ps_ += p[j];
+        for (int j = 0; j < 4; ++j) mx = fmaxf(mx, s[b][j]);
+      mx *= sc;
+      if (__builtin_amdgcn_ballot_w64(mx > m + P::kLag) != 0) {
+        const float mn = fmaxf(m, column_max(mx));
+        const float alpha = fast_exp2(m - (mn == -INFINITY ? 0.f : mn));
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int a = 0; a < NA; ++a)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[a][j] *= alpha;
       }
-      uint32_t hi0, lo0, hi1, lo1;
-      P::split(p[0], p[1], hi0, lo0);
-      P::split(p[2], p[3], hi1, lo1);
-      pb[0][2 * b] = hi0;
-      pb[0][2 * b + 1] = hi1;
-      pb[1][2 * b] = lo0;
-      pb[1][2 * b + 1] = lo1;
+      const float mu = m == -INFINITY ? 0.f : m + P::kBias;
+      float ps_ = 0.f;
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        float p[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          p[j] = fast_exp2(__builtin_fmaf(s[b][j], sc, -mu));
+          ps_ += p[j];
+        }
+        uint32_t hi0, lo0, hi1, lo1;
+        P::split(p[0], p[1], hi0, lo0);
+        P::split(p[2], p[3], hi1, lo1);
+        pb[0][2 * b] = hi0;
+        pb[0][2 * b + 1] = hi1;
+        pb[1][2 * b] = lo0;
+        pb[1][2 * b + 1] = lo1;
+      }
+      l += ps_;  // per lane; the column's lanes meet after the last tile
     }
-    l += ps_;  // per lane; the column's lanes meet after the last tile
 #pragma unroll
     for (int e = 0; e < ND; ++e) {
       u32x4 v0, v1;
@@ -442,42 +487,32 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(Args A) {
     }
   };
 
-  const int n = it.tile_end - it.tile_begin;
-  const int begin = uniform(it.tile_begin + (int)((int64_t)n * wave / kWaves));
-  const int end = uniform(it.tile_begin + (int)((int64_t)n * (wave + 1) / kWaves));
-  for (bool again = false;; again = true) {
-    m = -INFINITY;
-    l = 0.f;
+  for (int walk = kAll;; ++walk) {
+    if (walk != kOdd) {
+      m = -INFINITY;
+      l = 0.f;
 #pragma unroll
-    for (int a = 0; a < NA; ++a) acc[a] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int a = 0; a < NA; ++a) acc[a] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
     if (begin < end) {
       Raw r0, r1;
       fetch(begin, r0);
       int i = begin;
       for (; i + 2 <= end; i += 2) {
         fetch(i + 1, r1);
-        consume(i, r0, again);
+        consume(i, r0, walk);
         fetch(min(i + 2, end - 1), r0);
-        consume(i + 1, r1, again);
+        consume(i + 1, r1, walk);
       }
-      if (i < end) consume(i, r0, again);
+      if (i < end) consume(i, r0, walk);
     }
-    if (again) break;
+    if (walk == kOdd) break;
     bool odd = false;
 #pragma unroll
     for (int a = 0; a < NA; ++a)
 #pragma unroll
       for (int j = 0; j < 4; ++j) odd |= acc[a][j] != acc[a][j];
-    if (__builtin_amdgcn_ballot_w64(odd) == 0) break;
-    for (int d = lane; d < D; d += kWave) s_odd[wave][d] = 0.f;
-    saw_odd = true;
-  }
-  if (saw_odd) {
-    // (of this wave alone: its LDS operations are in order)
-#pragma unroll
-    for (int a = 0; a < NA; ++a)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[a][j] += s_odd[wave][(4 * grp + j) * NA + a];
+    if (walk == kAll && __builtin_amdgcn_ballot_w64(odd) == 0) break;
   }
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
@@ -520,59 +555,79 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(Args A) {
     const int hq = h * g + hb * 16 + r;
     *reinterpret_cast<u32x2*>(A.o + (int64_t)row * A.o_sb + (int64_t)hq * A.o_sh + d * 2) =
         u32x2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
-    if (d == 0 && A.lse) A.lse[(int64_t)row * A.hq + hq] = sum > 0.f ? (mx + log2f(sum)) * 0.69314718055994531f : (sum == 0.f ? -INFINITY : sum);
+    if (d == 0 && A.lse) A.lse[(int64_t)row * A.hq + hq] = log_sum(mx, sum);
   }
 }
 
-// One wave per (request, head) of several items: their parts in order, D / 64 dims
-// per lane.
+// A workgroup per (request, head) of several items: D / 4 lanes take a part, four dims
+// each, and so many parts at a time; what they saw meets in LDS.
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads) void merge_kernel(Args A) {
-  constexpr int N = D / 64;
+  constexpr int kLanes = D / 4, kGroups = kThreads / kLanes, kAhead = 4;
+  __shared__ __align__(16) float s_o[kGroups][D];
+  __shared__ float s_m[kGroups], s_l[kGroups];
+  const int row = blockIdx.x / A.hq, hq = blockIdx.x % A.hq;
   const Header head = *A.header;
-  if (stale(head, A.want)) return;
-  const int64_t at = (int64_t)blockIdx.x * kWaves + uniform(threadIdx.x / kWave);
-  if (at >= (int64_t)A.want.batch * A.hq) return;
-  const int row = (int)(at / A.hq), hq = (int)(at % A.hq), lane = threadIdx.x % kWave;
   const Row rec = A.rows[row];
   const int parts = uniform(rec.parts), first = uniform(rec.first);
-  if (parts <= 1 || first < 0 || first + parts > A.want.max_items) return;
+  if (stale(head, A.want) || parts <= 1 || first < 0 || first + parts > A.want.max_items) return;
   const int g = A.hq / A.hkv, h = hq / g, r = hq % g;
   const float* p = A.part + ((int64_t)first * A.hkv * A.blocks + h * A.blocks + r / 16) * part_floats<D>();
   const int64_t step = (int64_t)A.hkv * A.blocks * part_floats<D>();
-  const float* ml = p + 16 * D + 2 * (r % 16);
-  float top = -INFINITY;
-  for (int b = lane; b < parts; b += kWave) top = fmaxf(top, ml[b * step]);
+  const int group = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
+  float m = -INFINITY, l = 0.f;
+  f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i0 = group; i0 < parts; i0 += kAhead * kGroups) {
+    f32x4 v[kAhead];
+    f32x2 ml[kAhead];
 #pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-  float sum = 0.f, o[N] = {};
-  for (int b0 = 0; b0 < parts; b0 += kWave) {
-    const int n = min(parts - b0, kWave);
-    const f32x2 own = lane < n ? *reinterpret_cast<const f32x2*>(ml + (b0 + lane) * step) : f32x2{-INFINITY, 0.f};
-    const float w = own[0] == -INFINITY ? 0.f : fast_exp2(own[0] - top);
-    const float lw = own[1] * w;
-    const float* q = p + b0 * step + (r % 16) * D + lane * N;
-    for (int i0 = 0; i0 < n; i0 += 8) {
-      float v[8][N];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int e = 0; e < N; ++e) v[i][e] = q[min(i0 + i, n - 1) * step + e];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (i0 + i >= n) break;
-        const float wi = lane_value(w, i0 + i);
-        sum += lane_value(lw, i0 + i);
-#pragma unroll
-        for (int e = 0; e < N; ++e) o[e] += weighted(v[i][e], wi);
-      }
+    for (int i = 0; i < kAhead; ++i) {
+      const float* q = p + min(i0 + i * kGroups, parts - 1) * step;
+      v[i] = *reinterpret_cast<const f32x4*>(q + (r % 16) * D + d);
+      ml[i] = *reinterpret_cast<const f32x2*>(q + 16 * D + 2 * (r % 16));
     }
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (i0 + i * kGroups >= parts) ml[i] = f32x2{-INFINITY, 0.f}, v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      top = fmaxf(top, ml[i][0]);
+    }
+    const float w = m == -INFINITY ? 0.f : fast_exp2(m - top);
+    l *= w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = weighted(o[e], w);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const float wi = ml[i][0] == -INFINITY ? 0.f : fast_exp2(ml[i][0] - top);
+      l += ml[i][1] * wi;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += weighted(v[i][e], wi);
+    }
+    m = top;
+  }
+  *reinterpret_cast<f32x4*>(&s_o[group][d]) = o;
+  if (d == 0) {
+    s_m[group] = m;
+    s_l[group] = l;
+  }
+  __syncthreads();
+  if (group > 0) return;
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kGroups; ++i) top = fmaxf(top, s_m[i]);
+  o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < kGroups; ++i) {
+    const float w = s_m[i] == -INFINITY ? 0.f : fast_exp2(s_m[i] - top);
+    const f32x4 x = *reinterpret_cast<const f32x4*>(&s_o[i][d]);
+    sum += s_l[i] * w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += weighted(x[e], w);
   }
   const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-  T* op = reinterpret_cast<T*>(A.o + (int64_t)row * A.o_sb + (int64_t)hq * A.o_sh) + lane * N;
-#pragma unroll
-  for (int e = 0; e < N; ++e) op[e] = from_float<T>(o[e] * inv);
-  if (lane == 0 && A.lse) A.lse[(int64_t)row * A.hq + hq] = sum > 0.f ? (top + log2f(sum)) * 0.69314718055994531f : (sum == 0.f ? -INFINITY : sum);
+  *reinterpret_cast<u32x2*>(A.o + (int64_t)row * A.o_sb + (int64_t)hq * A.o_sh + d * 2) =
+      u32x2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
+  if (d == 0 && A.lse) A.lse[(int64_t)row * A.hq + hq] = log_sum(top, sum);
 }
 
 template <typename T, bool FOUR, int D>
@@ -583,8 +638,7 @@ int launch(const Args& a, hipStream_t s) {
   else
     hipLaunchKernelGGL((decode_kernel<T, FOUR, D, false>), grid, dim3(kThreads), 0, s, a);
   PL_LAUNCH_CHECK("window decode_kernel");
-  const int64_t waves = (int64_t)a.want.batch * a.hq;
-  hipLaunchKernelGGL((merge_kernel<T, D>), dim3((unsigned)((waves + kWaves - 1) / kWaves)), dim3(kThreads), 0, s, a);
+  hipLaunchKernelGGL((merge_kernel<T, D>), dim3((unsigned)(a.want.batch * a.hq)), dim3(kThreads), 0, s, a);
   PL_LAUNCH_CHECK("window merge_kernel");
   return ok();
 }
@@ -606,23 +660,27 @@ static int check_shape(int batch, int hq, int hkv, int page_size, int window, in
   if (batch < 0 || batch > (1 << 24)) return fail(PL_ERR_INVALID, "batch must be in 0 .. 2^24 (got %d)", batch);
   if (hkv <= 0 || hq <= 0 || hq % hkv)
     return fail(PL_ERR_INVALID, "num_qo_heads (%d) must be a multiple of num_kv_heads (%d)", hq, hkv);
+  if ((int64_t)batch * hq > INT32_MAX) return fail(PL_ERR_INVALID, "%d rows of %d heads are too many", batch, hq);
   if ((int64_t)hkv * head_blocks(hq, hkv) > 65535) return fail(PL_ERR_INVALID, "%d kv heads are too many", hkv);
   if (page_size <= 0 || page_size > kMaxLen) return fail(PL_ERR_INVALID, "page_size must be positive (got %d)", page_size);
   if (window < 0 || sinks < 0) return fail(PL_ERR_INVALID, "window and sinks must be >= 0");
   return PL_OK;
 }
 
-static int max_items_of(int batch, int hq, int hkv) { return batch + target_items(hq, hkv); }
-
-extern "C" size_t pl_window_decode_plan_size(int batch, int indices_capacity, int num_qo_heads, int num_kv_heads) {
-  if (check_shape(batch, num_qo_heads, num_kv_heads, 1, 0, 0) != PL_OK || indices_capacity < 0) return 0;
-  return layout(batch, indices_capacity, max_items_of(batch, num_qo_heads, num_kv_heads)).bytes;
+extern "C" size_t pl_window_decode_plan_size(int batch, int indices_capacity, int num_qo_heads, int num_kv_heads,
+                                             int page_size, int window, int sinks) {
+  if (check_shape(batch, num_qo_heads, num_kv_heads, page_size, window, sinks) != PL_OK) return 0;
+  if (indices_capacity < 0) return fail(PL_ERR_INVALID, "indices_capacity must be >= 0"), 0;
+  return layout(batch, indices_capacity, max_items_of(batch, num_qo_heads, num_kv_heads, page_size, window, sinks,
+                                                      indices_capacity)).bytes;
 }
 
-extern "C" size_t pl_window_decode_workspace_size(int batch, int num_qo_heads, int num_kv_heads, int head_dim) {
-  if (check_shape(batch, num_qo_heads, num_kv_heads, 1, 0, 0) != PL_OK || head_dim < 0) return 0;
-  return (size_t)max_items_of(batch, num_qo_heads, num_kv_heads) * num_kv_heads *
-         head_blocks(num_qo_heads, num_kv_heads) * 16 * (head_dim + 2) * sizeof(float);
+extern "C" size_t pl_window_decode_workspace_size(int batch, int indices_capacity, int num_qo_heads, int num_kv_heads,
+                                                  int head_dim, int page_size, int window, int sinks) {
+  if (check_shape(batch, num_qo_heads, num_kv_heads, page_size, window, sinks) != PL_OK) return 0;
+  if (indices_capacity < 0 || head_dim < 0) return fail(PL_ERR_INVALID, "sizes must be >= 0"), 0;
+  return (size_t)max_items_of(batch, num_qo_heads, num_kv_heads, page_size, window, sinks, indices_capacity) *
+         num_kv_heads * head_blocks(num_qo_heads, num_kv_heads) * 16 * (head_dim + 2) * sizeof(float);
 }
 
 static Header wanted(int batch, int page_size, int window, int sinks, int capacity, int hq, int hkv) {
@@ -633,7 +691,7 @@ static Header wanted(int batch, int page_size, int window, int sinks, int capaci
   h.window = window;
   h.sinks = sinks;
   h.indices_capacity = capacity;
-  h.max_items = max_items_of(batch, hq, hkv);
+  h.max_items = max_items_of(batch, hq, hkv, page_size, window, sinks, capacity);
   return h;
 }
 
@@ -660,7 +718,7 @@ extern "C" int pl_window_decode_plan(const int32_t* indptr, const int32_t* indic
   a.items = (Item*)(p + l.items);
   a.rows = (Row*)(p + l.rows);
   a.ids = (int32_t*)(p + l.indices);
-  a.target = target_items(num_qo_heads, num_kv_heads);
+  a.heads = num_kv_heads * head_blocks(num_qo_heads, num_kv_heads);
   const int copies = (indices_capacity + 4 * kPlanThreads - 1) / (4 * kPlanThreads);
   hipLaunchKernelGGL(plan_kernel, dim3(1 + (copies < 64 ? copies : 64)), dim3(kPlanThreads), 0, (hipStream_t)stream, a);
   PL_LAUNCH_CHECK("window plan_kernel");
@@ -697,7 +755,8 @@ extern "C" int pl_window_decode_run(const void* q, int64_t q_stride_b, int64_t q
   const Header want = wanted(batch, page_size, window, sinks, indices_capacity, num_qo_heads, num_kv_heads);
   const Layout lay = layout(batch, indices_capacity, want.max_items);
   if (plan_bytes < lay.bytes) return fail(PL_ERR_WORKSPACE, "plan of %zu bytes < %zu needed", plan_bytes, lay.bytes);
-  const size_t need = pl_window_decode_workspace_size(batch, num_qo_heads, num_kv_heads, head_dim);
+  const size_t need = pl_window_decode_workspace_size(batch, indices_capacity, num_qo_heads, num_kv_heads,
+                                                      head_dim, page_size, window, sinks);
   if (workspace_bytes < need)
     return fail(PL_ERR_WORKSPACE, "workspace of %zu bytes < %zu needed", workspace_bytes, need);
   Args a{};

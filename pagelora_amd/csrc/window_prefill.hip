@@ -17,9 +17,14 @@
 // keeps a query per lane, whose probabilities are the B operand of O^T += V^T P^T as
 // they lie; V^T comes out of LDS transposed.
 //
+// V of 4 bits is multiplied in fp16 (K too, where q is fp16), which takes fewer planes
+// than bf16: one of the probabilities for bf16 outputs, one of q for fp16 ones.  The
+// values are exact there while their groups' scales are in a range; an item that met
+// others is worked on again in bf16, which holds all of them.
+//
 // Where an output is NaN (0 times an infinity, or the difference of two planes'
-// infinities, is not what a row sees), the item is worked on once more: V's
-// infinities and NaN are taken out in LDS and added to the rows that see them.
+// infinities, is not what a row sees), the item is worked on again: V's infinities and
+// NaN become ones in LDS, kind by kind, to find who sees them, then zeros.
 #include <algorithm>
 #include <vector>
 
@@ -49,6 +54,12 @@ struct Item {
 };
 static_assert(sizeof(Item) == 32, "the plan's record");
 
+// Scales that fp16 holds, V's after 2^kShift: down to the smallest normal number for
+// the smallest code (0.5), up to 6 times a power.
+constexpr uint32_t kShift = 10;
+constexpr uint32_t kKLeast = 127 - 13, kKMost = 127 + 13;
+constexpr uint32_t kVLeast = kKLeast - kShift, kVMost = kKMost - kShift;
+
 constexpr int part_floats(int d) { return kRows * (d + 2); }  // outputs [row][dim], then (mu, sum) per row
 
 __device__ __forceinline__ void load_lds16(const char* g, char* l) {
@@ -72,40 +83,66 @@ struct Args {
   uint32_t q_flip;
 };
 
-template <typename T, bool FOUR, int D, bool PAGE16>
-__global__ __launch_bounds__(kThreads, 2) void prefill_kernel(Args A) {
-  using MT = typename std::conditional<FOUR, bf16_t, T>::type;  // what is multiplied
-  using P = Planes<MT>;
+// Which of V's values a walk over the tiles takes: all, or each kind of those that
+// are not finite by itself (as ones, to find who sees them), or the finite ones.
+enum Walk { kAll, kInf, kMinusInf, kNan, kFinite };
+
+// Two halves of a word of V as `walk` takes them.
+template <typename MT> __device__ __forceinline__ uint32_t taken(uint32_t w, int walk) {
   constexpr bool kBf16 = std::is_same<MT, bf16_t>::value;
-  constexpr int QP = FOUR && std::is_same<T, f16_t>::value ? 2 : 1;  // planes of q
+  constexpr uint32_t kOne = kBf16 ? 0x3f80u : 0x3c00u, kTop = kBf16 ? 0x7f80u : 0x7c00u;
+  uint32_t out = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t x = (w >> (16 * i)) & 0xffffu;
+    const uint32_t y = walk == kFinite     ? (finite16(x, kBf16) ? x : 0u)
+                       : walk == kInf      ? (x == kTop ? kOne : 0u)
+                       : walk == kMinusInf ? (x == (kTop | 0x8000u) ? kOne : 0u)
+                                           : ((x & 0x7fffu) > kTop ? kOne : 0u);
+    out |= y << (16 * i);
+  }
+  return out;
+}
+
+constexpr int buffer_bytes(int d) { return kTile * d * 2; }
+
+// One item's work.  N (narrow, 4 bits alone): in fp16; false where a scale was out of
+// its range, and nothing is written then.  s_k0 .. s_v1: a K and a V buffer each, one
+// object per buffer, so that writes into one never alias reads of another.
+template <typename T, bool FOUR, int D, bool PAGE16, bool N>
+__device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, char* __restrict__ s_v0,
+                                     char* __restrict__ s_k1, char* __restrict__ s_v1) {
+  using KT = typename std::conditional<FOUR && !N, bf16_t, T>::type;  // of K and q as they are multiplied
+  using VT = typename std::conditional<N, f16_t, KT>::type;           // of V and p
+  using P = Planes<VT>;
+  constexpr int QP = FOUR && !N && std::is_same<T, f16_t>::value ? 2 : 1;  // planes of q
+  constexpr int NP = N && std::is_same<T, bf16_t>::value ? 1 : 2;          // planes of p
   constexpr int NS = D / 32, NA = D / 16;
   constexpr int RB = D * 2;              // bytes of a row
   constexpr int CH = D / 8;              // its 16-byte chunks
   constexpr int TPL = kWave / CH;        // tokens of a load instruction
   constexpr int NL = 16 / TPL;           // load instructions of a wave's 16 tokens
-  constexpr int kBuf = kTile * RB;
-  // one object per buffer: writes into one never alias reads of another
-  __shared__ __align__(16) char s_k0[kBuf];
-  __shared__ __align__(16) char s_v0[kBuf];
-  __shared__ __align__(16) char s_k1[kBuf];
-  __shared__ __align__(16) char s_v1[kBuf];
-  __shared__ unsigned int s_odd[4];      // the tile's tokens with infinities or NaN (2 words); whether an output is NaN
+  constexpr bool kHalf = std::is_same<T, f16_t>::value;
   const int h = blockIdx.x % A.hkv;
   const Item it = A.items[blockIdx.x / A.hkv];
   const int r = uniform(it.request), row0 = uniform(it.row0);
-  if (r < 0 || r >= A.batch) return;
+  if (r < 0 || r >= A.batch) return true;
   const int g = A.hq / A.hkv;
   const int qo_begin = uniform(A.qo_indptr[r]);
   const int qo_len = uniform(A.qo_indptr[r + 1]) - qo_begin;
   const int page0 = uniform(A.kv_indptr[r]), n_pages = uniform(A.kv_indptr[r + 1]) - page0;
-  if (n_pages <= 0) return;
+  if (n_pages <= 0) return true;
   const int last = min(max(uniform(A.kv_last[r]), 1), A.page_size);
   const int kv_len = (n_pages - 1) * A.page_size + last;
   const int n_rows = qo_len * g;
   const int32_t* ind = A.kv_indices + page0;
   const int ps = A.page_size;
 
-  const int tid = threadIdx.x, lane = tid % kWave, wave = uniform(tid / kWave);
+  // (not known to be the thread's index, so that nothing is kept in registers from the
+  // narrow work to the other)
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  const int lane = tid % kWave, wave = uniform(tid / kWave);
   const int lr = lane % 16, grp = lane / 16;
 
   // what rows see: t <= lim and (t >= lo or t < sinks)
@@ -117,14 +154,16 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(Args A) {
   const int lim_lo = wave_on ? base + wrow / g : -1;
   const int lim_hi = wave_on ? base + (min(wrow + kWaveRows, n_rows) - 1) / g : -1;
   const int lo_lo = low(lim_lo), lo_hi = low(lim_hi);
-  int lim[kCols], lo[kCols];
+  int lim[kCols];
+#pragma unroll
+  for (int c = 0; c < kCols; ++c)  // rows past the end repeat the last one; not stored
+    lim[c] = base + min(wrow + c * 16 + lr, n_rows - 1) / g;
+
+  // q as the B operand, in the planes of what is multiplied
   u32x4 qb[QP][kCols][NS];
 #pragma unroll
   for (int c = 0; c < kCols; ++c) {
-    const int row = min(wrow + c * 16 + lr, n_rows - 1);  // rows past the end repeat the last one; not stored
-    const int pos = row / g;
-    lim[c] = base + pos;
-    lo[c] = low(lim[c]);
+    const int row = min(wrow + c * 16 + lr, n_rows - 1), pos = row / g;
     const char* qp = A.q + (int64_t)(qo_begin + pos) * A.q_st + (int64_t)(h * g + row - pos * g) * A.q_sh + grp * 16;
 #pragma unroll
     for (int ks = 0; ks < NS; ++ks) {
@@ -149,36 +188,50 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(Args A) {
     return (id < 0 ? 0 : ((int64_t)id >= A.num_pages ? A.num_pages - 1 : (int64_t)id)) * A.page_stride;
   };
   const int t_begin = uniform(it.tile_begin), t_end = uniform(it.tile_end);
-  // the page of the wave's 16 tokens of a tile (pages of 16 and more)
-  auto wave_page = [&](int t) { return ind[page_of(min(t, kv_len - 1))]; };
-
   const char* kh = A.k + (int64_t)h * A.head_stride;
   const char* vh = A.v + (int64_t)h * A.head_stride;
+  // Pages of 16 and more: lane l holds where the wave's 16 tokens of tile l of the
+  // next 64 begin, so that no tile's loads wait for its page id.
+  int64_t places = 0;
+  auto load_places = [&](int tile) __attribute__((always_inline)) {
+    const int t = min(seen_tile(seen, min(tile + lane, t_end - 1)) * kTile + wave * 16, (kv_len - 1) & ~15);
+    const int page = page_of(t);
+    places = clamp_page(ind[page]) + (int64_t)(t - page * ps) * (FOUR ? (int64_t)(D / 2) : A.token_stride);
+  };
+  auto place = [&](int tile) -> int64_t {
+    const int l = (tile - t_begin) % 64;
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(places >> 32), l) << 32 |
+                     (uint32_t)__builtin_amdgcn_readlane((int)places, l));
+  };
   // 16 bits: a wave fetches its 16 tokens of a tile, TPL per instruction; lane l of
   // one token l / CH, chunk (l % CH) permuted by the row
-  auto load_wide = [&](int tile, int id, char* kd, char* vd) {
-    const int t0 = seen_tile(seen, tile) * kTile + wave * 16;
+  uint32_t k_own[NL], v_own[NL];
+#pragma unroll
+  for (int j = 0; j < NL; ++j) {
+    const int row = j * TPL + lane / CH;
+    const uint32_t at = PAGE16 ? (uint32_t)(row * A.token_stride) : 0u;
+    k_own[j] = at + ((lane % CH) ^ (row % CH)) * 16;
+    v_own[j] = at + ((lane % CH) ^ (2 * (row % (CH / 2)))) * 16;
+  }
+  auto load_wide = [&](int tile, char* kd, char* vd) __attribute__((always_inline)) {
     kd += wave * 16 * RB;
     vd += wave * 16 * RB;
-    int64_t page = 0;
-    int in_page = 0;
     if constexpr (PAGE16) {
-      const int t = min(t0, (kv_len - 1) & ~15);
-      page = clamp_page(id);
-      in_page = t - page_of(t) * ps;
-    }
+      const int64_t at = place(tile);
 #pragma unroll
-    for (int j = 0; j < NL; ++j) {
-      const int row = j * TPL + lane / CH;
-      int64_t at;
-      if constexpr (PAGE16) {
-        at = page + (int64_t)(in_page + row) * A.token_stride;
-      } else {
-        const int t = min(t0 + row, kv_len - 1), pg = page_of(t);
-        at = clamp_page(ind[pg]) + (int64_t)(t - pg * ps) * A.token_stride;
+      for (int j = 0; j < NL; ++j) {
+        load_lds16((kh + at) + k_own[j], kd + j * TPL * RB);
+        load_lds16((vh + at) + v_own[j], vd + j * TPL * RB);
       }
-      load_lds16(kh + at + ((lane % CH) ^ (row % CH)) * 16, kd + j * TPL * RB);
-      load_lds16(vh + at + ((lane % CH) ^ (2 * (row % (CH / 2)))) * 16, vd + j * TPL * RB);
+    } else {
+      const int t0 = seen_tile(seen, tile) * kTile + wave * 16;
+#pragma unroll
+      for (int j = 0; j < NL; ++j) {
+        const int t = min(t0 + j * TPL + lane / CH, kv_len - 1), pg = page_of(t);
+        const int64_t at = clamp_page(ind[pg]) + (int64_t)(t - pg * ps) * A.token_stride;
+        load_lds16(kh + at + k_own[j], kd + j * TPL * RB);
+        load_lds16(vh + at + v_own[j], vd + j * TPL * RB);
+      }
     }
   };
   // 4 bits: thread tid holds a quarter of K token tid / 4, and eight dims of V's
@@ -189,56 +242,77 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(Args A) {
     u32x4 v;
   } raw;
   const int k_tok = tid / 4, v_quad = CH == 16 ? tid / 16 : tid % (16 * CH) / CH, v_chunk = tid % CH;
-  auto load_four = [&](int tile, int id) {
+  auto load_four = [&](int tile) __attribute__((always_inline)) {
     const int t0 = seen_tile(seen, tile) * kTile;
-    int64_t pk, pv;
-    int ok, ov;
+    const char *kp, *sp, *vp, *wp;  // K's codes and scale, V's
     if constexpr (PAGE16) {
-      const int t = min(t0 + wave * 16, (kv_len - 1) & ~15);
-      pk = clamp_page(id);
-      ok = t - page_of(t) * ps + k_tok % 16;
-      if constexpr (D == 128) {
-        pv = pk;
-        ov = t - page_of(t) * ps + v_quad % 4 * 4;
-      }
+      const int64_t at = place(tile);
+      const int t = min(t0 + wave * 16, (kv_len - 1) & ~15), slot = A.page_shift >= 0 ? t & (ps - 1) : t % ps;
+      const int64_t sat = at + ps * (D / 2) - slot * (D / 2 - D / 32);  // scales: D / 32 bytes a token, codes D / 2
+      kp = (kh + at) + (uint32_t)(k_tok % 16 * (D / 2) + tid % 4 * (D / 8));
+      sp = (kh + sat) + (uint32_t)(k_tok % 16 * (D / kGroup) + tid % 4 * (D / 4) / kGroup);
+      vp = (vh + at) + (uint32_t)(v_quad % 4 * (2 * D) + v_chunk * 16);
+      wp = (vh + sat) + (uint32_t)(v_quad % 4 * (D / 8) + v_chunk / 4 * 4);
     } else {
-      const int t = min(t0 + k_tok, kv_len - 1), pg = page_of(t);
-      pk = clamp_page(ind[pg]);
-      ok = t - pg * ps;
+      const int t = min(t0 + k_tok, kv_len - 1), pg = page_of(t), ok = t - pg * ps;
+      const char* page = kh + clamp_page(ind[pg]);
+      kp = page + ok * (D / 2) + tid % 4 * (D / 8);
+      sp = page + ps * (D / 2) + ok * (D / kGroup) + tid % 4 * (D / 4) / kGroup;
     }
-    if constexpr (!PAGE16 || D != 128) {
-      const int t = min(t0 + v_quad * 4, (kv_len - 1) & ~3), pg = page_of(t);
-      pv = clamp_page(ind[pg]);
-      ov = t - pg * ps;
+    if constexpr (!PAGE16 || D != 128) {  // (at head_dim 64 V's tokens are not the wave's)
+      const int t = min(t0 + v_quad * 4, (kv_len - 1) & ~3), pg = page_of(t), ov = t - pg * ps;
+      const char* page = vh + clamp_page(ind[pg]);
+      vp = page + ov / 4 * (2 * D) + v_chunk * 16;
+      wp = page + ps * (D / 2) + ov / 4 * (D / 8) + v_chunk / 4 * 4;
     }
-    const char* kp = kh + pk;
     if constexpr (KQ == 4) {
-      const u32x4 x = *reinterpret_cast<const u32x4*>(kp + ok * (D / 2) + tid % 4 * (D / 8));
+      const u32x4 x = *reinterpret_cast<const u32x4*>(kp);
 #pragma unroll
       for (int e = 0; e < 4; ++e) raw.k[e % KQ] = x[e];
     } else {
-      const u32x2 x = *reinterpret_cast<const u32x2*>(kp + ok * (D / 2) + tid % 4 * (D / 8));
+      const u32x2 x = *reinterpret_cast<const u32x2*>(kp);
       raw.k[0] = x[0];
       raw.k[1] = x[1];
     }
-    raw.ks = *reinterpret_cast<const uint8_t*>(kp + ps * (D / 2) + ok * (D / kGroup) + tid % 4 * (D / 4) / kGroup);
-    const char* vp = vh + pv;
-    raw.v = *reinterpret_cast<const u32x4*>(vp + ov / 4 * (2 * D) + v_chunk * 16);
-    raw.vs = *reinterpret_cast<const uint32_t*>(vp + ps * (D / 2) + ov / 4 * (D / 8) + v_chunk / 4 * 4);
+    raw.ks = *reinterpret_cast<const uint8_t*>(sp);
+    raw.v = *reinterpret_cast<const u32x4*>(vp);
+    raw.vs = *reinterpret_cast<const uint32_t*>(wp);
   };
-  auto store_four = [&](int tile, char* kd, char* vd) {
+  // Narrow: K in q's type and V in fp16, times 2^kShift, exact where the scales are in range
+  uint32_t v_least = ~0u, v_most = 0u, k_least = ~0u, k_most = 0u;
+  auto store_four = [&](int tile, char* kd, char* vd) __attribute__((always_inline)) {
     const int t0 = seen_tile(seen, tile) * kTile;
+    if (t0 + k_tok >= kv_len) raw.ks = 127u;  // (what lies there counts for nothing)
     const float ks = scale_of(raw.ks);
+    if constexpr (N && kHalf) {
+      k_least = min(k_least, raw.ks);
+      k_most = max(k_most, raw.ks);
+    }
 #pragma unroll
     for (int c = 0; c < KQ; ++c)
-      *reinterpret_cast<u32x4*>(kd + k_tok * RB + (((tid % 4) * KQ + c) ^ (k_tok % CH)) * 16) = codes8(raw.k[c], ks);
+      *reinterpret_cast<u32x4*>(kd + k_tok * RB + (((tid % 4) * KQ + c) ^ (k_tok % CH)) * 16) =
+          N && kHalf ? halves8(raw.k[c], ks) : codes8(raw.k[c], ks);
     if (CH == 16 || tid < 16 * CH) {
+      if (t0 + kTile > kv_len) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (t0 + v_quad * 4 + j >= kv_len) {  // (0 times what lies there)
+            raw.v[j] = 0u;
+            raw.vs = (raw.vs & ~(255u << (8 * j))) | 127u << (8 * j);
+          }
+      }
+      if constexpr (N) {
+        // the four bytes as two pairs of halves
+        const uint32_t even = raw.vs & 0x00ff00ffu, odd = (raw.vs >> 8) & 0x00ff00ffu;
+        v_least = pk_min(v_least, pk_min(even, odd));
+        v_most = pk_max(v_most, pk_max(even, odd));
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int row = v_quad * 4 + j;
-        u32x4 x = codes8(raw.v[j], scale_of((raw.vs >> (8 * j)) & 255u));
-        if (t0 + row >= kv_len) x = u32x4{0u, 0u, 0u, 0u};  // (0 times what lies there)
-        *reinterpret_cast<u32x4*>(vd + row * RB + (v_chunk ^ (2 * (row % (CH / 2)))) * 16) = x;
+        const uint32_t byte = (raw.vs >> (8 * j)) & 255u;
+        *reinterpret_cast<u32x4*>(vd + row * RB + (v_chunk ^ (2 * (row % (CH / 2)))) * 16) =
+            N ? halves8(raw.v[j], scale_of(byte + kShift)) : codes8(raw.v[j], scale_of(byte));
       }
     }
   };
@@ -257,9 +331,8 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(Args A) {
   f32x4 acc[kCols][NA];
   float m[kCols], l[kCols];
   const float sc = A.scale_log2;
-  int id = 0;  // the page of the tile that is loaded next
 
-  auto body = [&](int tile, const char* kb, char* vb, char* kn, char* vn, bool again) {
+  auto body = [&](int tile, const char* kb, char* vb, char* kn, char* vn, int walk) __attribute__((always_inline)) {
     if constexpr (!FOUR) {
       // this wave's loads of the tile are done, and past the barrier everyone's
       // are, and every wave is done with the other buffers
@@ -268,16 +341,16 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(Args A) {
       __builtin_amdgcn_s_barrier();
       __builtin_amdgcn_sched_barrier(0);
       if (tile + 1 < t_end) {
-        load_wide(tile + 1, PAGE16 ? uniform(id) : 0, kn, vn);
-        if (PAGE16 && tile + 2 < t_end) id = wave_page(seen_tile(seen, tile + 2) * kTile + wave * 16);
+        if (PAGE16 && (tile + 1 - t_begin) % 64 == 0) load_places(tile + 1);
+        load_wide(tile + 1, kn, vn);
       }
     } else {
       __syncthreads();
       if (tile + 1 < t_end) {
         store_four(tile + 1, kn, vn);
         if (tile + 2 < t_end) {
-          load_four(tile + 2, PAGE16 ? uniform(id) : 0);
-          if (PAGE16 && tile + 3 < t_end) id = wave_page(seen_tile(seen, tile + 3) * kTile + wave * 16);
+          if (PAGE16 && (tile + 2 - t_begin) % 64 == 0) load_places(tile + 2);
+          load_four(tile + 2);
         }
       }
     }
@@ -288,43 +361,11 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(Args A) {
         if (t0 + c / CH >= kv_len) *reinterpret_cast<u32x4*>(vb + c * 16) = u32x4{0u, 0u, 0u, 0u};
       __syncthreads();
     }
-    if (again) {
-      if (tid < 2) s_odd[tid] = 0u;
-      __syncthreads();
-      for (int c = tid; c < kTile * CH; c += kThreads) {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(vb + c * 16);
-        bool odd = false;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) odd |= !finite16(x[e] & 0xffffu, kBf16) || !finite16(x[e] >> 16, kBf16);
-        if (odd) atomicOr(&s_odd[c / CH / 32], 1u << (c / CH % 32));
-      }
-      __syncthreads();
-      for (int half = 0; half < 2; ++half)
-        for (unsigned int left = s_odd[half]; left; left &= left - 1) {
-          const int row = half * 32 + __builtin_ctz(left), t = t0 + row;
-#pragma unroll
-          for (int c = 0; c < kCols; ++c) {
-            if (t > lim[c] || (t < lo[c] && t >= A.sinks)) continue;
-#pragma unroll
-            for (int a = 0; a < NA; ++a) {
-              const int d = 16 * a + 4 * grp;
-              const u32x2 x = *reinterpret_cast<const u32x2*>(vb + row * RB + ((d / 8) ^ (2 * (row % (CH / 2)))) * 16 +
-                                                              d % 8 * 2);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                float v[2];
-                unpack2<MT>(x[i / 2], v[0], v[1]);
-                if (!finite16((x[i / 2] >> (16 * (i % 2))) & 0xffffu, kBf16)) acc[c][a][i] += v[i % 2];
-              }
-            }
-          }
-        }
-      __syncthreads();
+    if (!N && walk != kAll) {
       for (int c = tid; c < kTile * CH; c += kThreads) {
         u32x4 x = *reinterpret_cast<const u32x4*>(vb + c * 16);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          x[e] &= (finite16(x[e] & 0xffffu, kBf16) ? 0xffffu : 0u) | (finite16(x[e] >> 16, kBf16) ? 0xffff0000u : 0u);
+        for (int e = 0; e < 4; ++e) x[e] = taken<VT>(x[e], walk);
         *reinterpret_cast<u32x4*>(vb + c * 16) = x;
       }
       __syncthreads();
@@ -351,20 +392,29 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(Args A) {
 #pragma unroll
           for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int c = 0; c < kCols; ++c) s[c][b0 + b] = mfma32<MT>(ka[b], qb[pl][c][ks], s[c][b0 + b]);
+            for (int c = 0; c < kCols; ++c) s[c][b0 + b] = mfma32<KT>(ka[b], qb[pl][c][ks], s[c][b0 + b]);
       }
+    }
+    const bool odd = !N && walk != kAll && walk != kFinite;
+    if (odd) {  // ones for what is seen
+#pragma unroll
+      for (int c = 0; c < kCols; ++c)
+#pragma unroll
+        for (int blk = 0; blk < 4; ++blk) s[c][blk] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     if (t0 + kTile - 1 > lim_lo || (t0 < lo_hi && t0 + kTile > A.sinks)) {
       const int t1 = t0 + 4 * grp;
 #pragma unroll
-      for (int c = 0; c < kCols; ++c)
+      for (int c = 0; c < kCols; ++c) {
+        const int lo = low(lim[c]);
 #pragma unroll
         for (int blk = 0; blk < 4; ++blk)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int t = t1 + blk * 16 + i;
-            s[c][blk][i] = t <= lim[c] && (t >= lo[c] || t < A.sinks) ? s[c][blk][i] : -INFINITY;
+            s[c][blk][i] = t <= lim[c] && (t >= lo || t < A.sinks) ? s[c][blk][i] : -INFINITY;
           }
+      }
     }
     float mx[kCols];
     bool rose = false;
@@ -388,20 +438,13 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(Args A) {
         const float alpha = fast_exp2(m[c] - (mn == -INFINITY ? 0.f : mn));
         m[c] = mn;
         l[c] *= alpha;
-        if (again) {
 #pragma unroll
-          for (int a = 0; a < NA; ++a)
+        for (int a = 0; a < NA; ++a)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[c][a][i] = weighted(acc[c][a][i], alpha);
-        } else {
-#pragma unroll
-          for (int a = 0; a < NA; ++a)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[c][a][i] *= alpha;
-        }
+          for (int i = 0; i < 4; ++i) acc[c][a][i] *= alpha;
       }
     }
-    u32x4 pb[kCols][2][2];
+    u32x4 pb[kCols][2][NP];
 #pragma unroll
     for (int c = 0; c < kCols; ++c) {
       const float mu = m[c] == -INFINITY ? 0.f : m[c] + P::kBias;
@@ -417,10 +460,14 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(Args A) {
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          uint32_t hi, lo_;
-          P::split(p[2 * i], p[2 * i + 1], hi, lo_);
-          pb[c][blk / 2][0][blk % 2 * 2 + i] = hi;
-          pb[c][blk / 2][1][blk % 2 * 2 + i] = lo_;
+          if constexpr (NP == 1) {
+            pb[c][blk / 2][0][blk % 2 * 2 + i] = pack2<VT>(p[2 * i], p[2 * i + 1]);
+          } else {
+            uint32_t hi, lo_;
+            P::split(p[2 * i], p[2 * i + 1], hi, lo_);
+            pb[c][blk / 2][0][blk % 2 * 2 + i] = hi;
+            pb[c][blk / 2][NP - 1][blk % 2 * 2 + i] = lo_;
+          }
         }
       }
       l[c] += sum;  // per lane; the column's lanes meet after the last tile
@@ -437,15 +484,16 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(Args A) {
           va[a] = u32x4{v0[0], v0[1], v1[0], v1[1]};
         }
 #pragma unroll
-        for (int pl = 0; pl < 2; ++pl)
+        for (int pl = 0; pl < NP; ++pl)
 #pragma unroll
           for (int a = 0; a < 2; ++a)
 #pragma unroll
-            for (int c = 0; c < kCols; ++c) acc[c][a0 + a] = mfma32<MT>(va[a], pb[c][kc][pl], acc[c][a0 + a]);
+            for (int c = 0; c < kCols; ++c) acc[c][a0 + a] = mfma32<VT>(va[a], pb[c][kc][pl], acc[c][a0 + a]);
       }
   };
 
-  for (bool again = false;; again = true) {
+  uint32_t who[3][kCols] = {};  // outputs that see each kind of what is not finite
+  for (int walk = kAll;; ++walk) {
 #pragma unroll
     for (int c = 0; c < kCols; ++c) {
       m[c] = -INFINITY;
@@ -453,41 +501,71 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(Args A) {
 #pragma unroll
       for (int a = 0; a < NA; ++a) acc[c][a] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    if (tid == 0) s_odd[2] = 0u;
     if (t_begin < t_end) {
-      auto page_at = [&](int tile) {
-        return PAGE16 && tile < t_end ? wave_page(seen_tile(seen, tile) * kTile + wave * 16) : 0;
-      };
+      if (PAGE16) load_places(t_begin);
       if constexpr (FOUR) {
-        load_four(t_begin, uniform(page_at(t_begin)));
+        load_four(t_begin);
         store_four(t_begin, s_k0, s_v0);
-        if (t_begin + 1 < t_end) load_four(t_begin + 1, uniform(page_at(t_begin + 1)));
-        id = page_at(t_begin + 2);
+        if (t_begin + 1 < t_end) load_four(t_begin + 1);
       } else {
-        load_wide(t_begin, uniform(page_at(t_begin)), s_k0, s_v0);
-        id = page_at(t_begin + 1);
+        load_wide(t_begin, s_k0, s_v0);
       }
     }
     int tile = t_begin;
     for (; tile + 2 <= t_end; tile += 2) {
-      body(tile, s_k0, s_v0, s_k1, s_v1, again);
-      body(tile + 1, s_k1, s_v1, s_k0, s_v0, again);
+      body(tile, s_k0, s_v0, s_k1, s_v1, walk);
+      body(tile + 1, s_k1, s_v1, s_k0, s_v0, walk);
     }
-    if (tile < t_end) body(tile, s_k0, s_v0, s_k1, s_v1, again);
-    if (again) break;
-    bool odd = false;
+    if (tile < t_end) body(tile, s_k0, s_v0, s_k1, s_v1, walk);
+    if constexpr (N) {
+      const uint32_t least = min(v_least & 0xffffu, v_least >> 16), most = max(v_most & 0xffffu, v_most >> 16);
+      if (__syncthreads_or(least < kVLeast || most > kVMost || (kHalf && (k_least < kKLeast || k_most > kKMost))))
+        return false;
+      const float down = __uint_as_float((127u - kShift) << 23);
 #pragma unroll
-    for (int c = 0; c < kCols; ++c)
+      for (int c = 0; c < kCols; ++c)
 #pragma unroll
-      for (int a = 0; a < NA; ++a)
+        for (int a = 0; a < NA; ++a)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) odd |= acc[c][a][i] != acc[c][a][i];
-    __syncthreads();
-    if (odd) s_odd[2] = 1u;
-    __syncthreads();
-    const bool any = s_odd[2] != 0u;
-    __syncthreads();
-    if (!any) break;
+          for (int i = 0; i < 4; ++i) acc[c][a][i] *= down;
+      break;
+    }
+    if (walk == kAll) {
+      bool odd = false;
+#pragma unroll
+      for (int c = 0; c < kCols; ++c)
+#pragma unroll
+        for (int a = 0; a < NA; ++a)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) odd |= acc[c][a][i] != acc[c][a][i];
+      if (!__syncthreads_or(odd)) break;
+    } else if (walk != kFinite) {
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int a = 0; a < NA; ++a)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) bits |= (acc[c][a][i] > 0.f ? 1u : 0u) << (4 * a + i);
+        if (walk == kInf) who[0][c] = bits;
+        if (walk == kMinusInf) who[1][c] = bits;
+        if (walk == kNan) who[2][c] = bits;
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < kCols; ++c)
+#pragma unroll
+        for (int a = 0; a < NA; ++a)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t bit = 1u << (4 * a + i);
+            if ((who[2][c] | (who[0][c] & who[1][c])) & bit) acc[c][a][i] = NAN;
+            else if (who[0][c] & bit) acc[c][a][i] = INFINITY;
+            else if (who[1][c] & bit) acc[c][a][i] = -INFINITY;
+          }
+      break;
+    }
   }
 
   const int slot = uniform(it.slot);
@@ -515,6 +593,18 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(Args A) {
     for (int a = 0; a < NA; ++a)
       *reinterpret_cast<u32x2*>(op + a * 16) = u32x2{pack2<T>(acc[c][a][0] * inv, acc[c][a][1] * inv),
                                                      pack2<T>(acc[c][a][2] * inv, acc[c][a][3] * inv)};
+  }
+  return true;
+}
+
+template <typename T, bool FOUR, int D, bool PAGE16>
+__global__ __launch_bounds__(kThreads, 2) void prefill_kernel(Args A) {
+  __shared__ __align__(16) char s_k0[buffer_bytes(D)];
+  __shared__ __align__(16) char s_v0[buffer_bytes(D)];
+  __shared__ __align__(16) char s_k1[buffer_bytes(D)];
+  __shared__ __align__(16) char s_v1[buffer_bytes(D)];
+  if (!work<T, FOUR, D, PAGE16, FOUR>(A, s_k0, s_v0, s_k1, s_v1)) {
+    if constexpr (FOUR) work<T, true, D, PAGE16, false>(A, s_k0, s_v0, s_k1, s_v1);
   }
 }
 

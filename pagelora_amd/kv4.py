@@ -26,6 +26,7 @@ import torch
 from . import _lib
 
 KV4_GROUP = 32
+_CODES = {torch.bfloat16: _lib.PL_DTYPE_BF16, torch.float16: _lib.PL_DTYPE_F16}
 
 
 def kv4_page_shape(*, num_kv_heads: int, head_dim: int, page_size: int) -> tuple[int, int, int]:
@@ -40,8 +41,9 @@ def kv4_page_shape(*, num_kv_heads: int, head_dim: int, page_size: int) -> tuple
 def kv4_geometry(cache: torch.Tensor, num_kv_heads: int, head_dim: int, page_size: int):
     """A 4-bit layer as numbers: (K and V addresses, page and head stride in bytes, pages, device index)."""
     shape, strides = cache.shape, cache.stride()
-    page = kv4_page_shape(num_kv_heads=num_kv_heads, head_dim=head_dim, page_size=page_size)
-    if cache.dtype != torch.uint8 or len(shape) != 4 or tuple(shape[1:]) != page:
+    if (cache.dtype != torch.uint8 or len(shape) != 4 or page_size < 8 or page_size % 8 or head_dim not in (64, 128)
+            or shape[1:] != (2, num_kv_heads, page_size * (head_dim // 2 + head_dim // KV4_GROUP))):
+        page = kv4_page_shape(num_kv_heads=num_kv_heads, head_dim=head_dim, page_size=page_size)
         raise ValueError(f"4-bit KV cache layer must be uint8 [P, {page[0]}, {page[1]}, {page[2]}], got {cache.dtype} "
                          f"{tuple(shape)}")
     if strides[3] != 1:
@@ -50,15 +52,15 @@ def kv4_geometry(cache: torch.Tensor, num_kv_heads: int, head_dim: int, page_siz
     return k, k + strides[1], strides[0], strides[2], shape[0], cache.get_device()
 
 
-def _places(page_id: torch.Tensor, page_offset: torch.Tensor, tokens: int | None, device: int) -> int:
-    for t in (page_id, page_offset):
-        if t.dtype != torch.int64 or t.dim() != 1 or not t.is_contiguous():
-            raise ValueError("page_id and page_offset must be contiguous 1-D int64 tensors")
-        if t.get_device() != device:
-            raise RuntimeError("page_id and page_offset must be on the cache's device")
-    if page_id.numel() != page_offset.numel() or tokens not in (None, page_id.numel()):
-        raise ValueError("page_id / page_offset must have one entry per token")
-    return page_id.numel()
+def _places(page_id: torch.Tensor, page_offset: torch.Tensor, device: int) -> int:
+    """How many places these are."""
+    n = page_id.shape
+    if (page_id.dtype != torch.int64 or page_offset.dtype != torch.int64 or len(n) != 1 or page_offset.shape != n
+            or not page_id.is_contiguous() or not page_offset.is_contiguous()):
+        raise ValueError("page_id and page_offset must be contiguous 1-D int64 tensors of one length")
+    if page_id.get_device() != device or page_offset.get_device() != device:
+        raise RuntimeError("page_id and page_offset must be on the cache's device")
+    return n[0]
 
 
 def kv4_append(cache_layer: torch.Tensor, k: torch.Tensor, v: torch.Tensor, page_id: torch.Tensor,
@@ -74,23 +76,28 @@ def kv4_append(cache_layer: torch.Tensor, k: torch.Tensor, v: torch.Tensor, page
     k_ptr, v_ptr, page_stride, head_stride, num_pages, device = kv4_geometry(cache_layer, num_kv_heads, head_dim, page_size)
     if device < 0:
         raise RuntimeError("kv4_append needs a cache on a ROCm device")
-    if k.dim() != 3 or k.shape != v.shape or tuple(k.shape[1:]) != (num_kv_heads, head_dim):
+    shape, code = k.shape, _CODES.get(k.dtype)
+    if len(shape) != 3 or shape[1] != num_kv_heads or shape[2] != head_dim or v.shape != shape:
         raise ValueError(f"k and v must be [tokens, {num_kv_heads}, {head_dim}]")
-    if k.dtype != v.dtype or k.dtype not in (torch.bfloat16, torch.float16):
+    if code is None or v.dtype != k.dtype:
         raise NotImplementedError(f"k and v must be both bfloat16 or both float16, got {k.dtype} and {v.dtype}")
     ks, vs = k.stride(), v.stride()
     if ks[2] != 1 or vs[2] != 1:
         raise ValueError("k and v need a contiguous head_dim")
     if k.get_device() != device or v.get_device() != device:
         raise RuntimeError("k and v must be on the cache's device")
-    tokens = _places(page_id, page_offset, k.shape[0], device)
+    tokens = _places(page_id, page_offset, device)
+    if tokens != shape[0]:
+        raise ValueError("page_id / page_offset must have one entry per token")
     if tokens == 0 or num_pages == 0:
         return
     with _lib.on_device(device):
-        _lib.check(_lib.load().pl_kv4_append(
+        status = _lib.load().pl_kv4_append(
             k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1], k_ptr, v_ptr, page_stride, head_stride, num_pages,
-            page_size, page_id.data_ptr(), page_offset.data_ptr(), tokens, num_kv_heads, head_dim,
-            _lib.dtype_code(k.dtype), _lib.raw_stream(device)), "pl_kv4_append")
+            page_size, page_id.data_ptr(), page_offset.data_ptr(), tokens, num_kv_heads, head_dim, code,
+            _lib.raw_stream(device))
+    if status:
+        _lib.check(status, "pl_kv4_append")
 
 
 def kv4_read(cache_layer: torch.Tensor, page_id: torch.Tensor, page_offset: torch.Tensor, *, num_kv_heads: int,
@@ -104,19 +111,21 @@ def kv4_read(cache_layer: torch.Tensor, page_id: torch.Tensor, page_offset: torc
     k_ptr, v_ptr, page_stride, head_stride, num_pages, device = kv4_geometry(cache_layer, num_kv_heads, head_dim, page_size)
     if device < 0:
         raise RuntimeError("kv4_read needs a cache on a ROCm device")
-    if dtype not in (torch.bfloat16, torch.float16):
+    code = _CODES.get(dtype)
+    if code is None:
         raise NotImplementedError(f"dtype must be bfloat16 or float16, got {dtype}")
-    tokens = _places(page_id, page_offset, None, device)
-    k, v = torch.empty((2, tokens, num_kv_heads, head_dim), dtype=dtype, device=cache_layer.device).unbind(0)
+    tokens = _places(page_id, page_offset, device)
+    k = torch.empty((2, tokens, num_kv_heads, head_dim), dtype=dtype, device=cache_layer.device)
     if num_pages == 0:
         k.fill_(float("nan"))
-        v.fill_(float("nan"))
-        return k, v
-    if tokens:
+    elif tokens:
         stride = num_kv_heads * head_dim
+        address = k.data_ptr()
         with _lib.on_device(device):
-            _lib.check(_lib.load().pl_kv4_read(
+            status = _lib.load().pl_kv4_read(
                 k_ptr, v_ptr, page_stride, head_stride, num_pages, page_size, page_id.data_ptr(),
-                page_offset.data_ptr(), tokens, num_kv_heads, head_dim, k.data_ptr(), v.data_ptr(), stride, head_dim,
-                stride, head_dim, _lib.dtype_code(dtype), _lib.raw_stream(device)), "pl_kv4_read")
-    return k, v
+                page_offset.data_ptr(), tokens, num_kv_heads, head_dim, address, address + 2 * tokens * stride, stride,
+                head_dim, stride, head_dim, code, _lib.raw_stream(device))
+        if status:
+            _lib.check(status, "pl_kv4_read")
+    return k.unbind(0)

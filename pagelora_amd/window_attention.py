@@ -25,6 +25,7 @@ from . import _lib
 from .attention_backend import _cache_pointers, _upload_int32, _validate_host_table
 from .kv4 import kv4_geometry
 
+_CODES = {torch.bfloat16: _lib.PL_DTYPE_BF16, torch.float16: _lib.PL_DTYPE_F16}
 
 class WindowAttention:
     """Decode and prefill attention with ``window`` and ``sinks`` (gfx950).
@@ -81,32 +82,39 @@ class WindowAttention:
             raise ValueError(f"page id {max_page} is outside the {num_pages}-page KV pool")
         return k, v, page_stride, token_stride, head_stride, num_pages, bits
 
-    def _check_q(self, q: torch.Tensor, out: torch.Tensor, rows: int, device: int, what: str) -> None:
-        if q.dim() != 3 or tuple(q.shape[1:]) != (self.num_qo_heads, self.head_dim):
-            raise ValueError(f"q must be [{what}, {self.num_qo_heads}, {self.head_dim}], got {tuple(q.shape)}")
-        if q.shape[0] != rows:
-            raise ValueError(f"q has {q.shape[0]} {what} but the plan has {rows}")
-        if q.dtype not in (torch.bfloat16, torch.float16):
-            raise NotImplementedError(f"q must be bfloat16 or float16, got {q.dtype}")
-        if out.shape != q.shape or out.dtype != q.dtype or q.stride(2) != 1 or out.stride(2) != 1:
+    def _queries(self, q: torch.Tensor, out: torch.Tensor, rows: int, device: int, what: str):
+        """(dtype code, q's and out's strides) of packed queries and their output."""
+        shape, dtype = q.shape, q.dtype
+        if len(shape) != 3 or shape[1] != self.num_qo_heads or shape[2] != self.head_dim:
+            raise ValueError(f"q must be [{what}, {self.num_qo_heads}, {self.head_dim}], got {tuple(shape)}")
+        if shape[0] != rows:
+            raise ValueError(f"q has {shape[0]} {what} but the plan has {rows}")
+        code = _CODES.get(dtype)
+        if code is None:
+            raise NotImplementedError(f"q must be bfloat16 or float16, got {dtype}")
+        qs, os_ = q.stride(), out.stride()
+        if out.shape != shape or out.dtype != dtype or qs[2] != 1 or os_[2] != 1:
             raise ValueError("q and out must match in shape/dtype with a contiguous head_dim")
         if q.get_device() != device or out.get_device() != device:
             raise RuntimeError(f"q and out must be on the plan's device (cuda:{device})")
+        return code, qs, os_
 
     def _on_stream(self, plan: dict) -> int:
         """The current stream's handle; the plan's memory and work are ordered with it."""
         stream = _lib.raw_stream(plan["device"])
-        if torch.cuda.is_current_stream_capturing():
-            if not plan["kept"]:
-                plan["kept"] = True
-                self._captured.append(plan)
-        elif plan["captured"]:
-            raise RuntimeError("the plan was captured: it is made when its graph is replayed; plan again for eager runs")
-        elif stream not in plan["streams"]:
-            here = torch.cuda.current_stream(plan["device"])
-            here.wait_event(plan["ready"])
-            plan["memory"].record_stream(here)
-            plan["streams"].add(stream)
+        if not plan["kept"] or plan["captured"] or stream not in plan["streams"]:
+            if torch.cuda.is_current_stream_capturing():
+                if not plan["kept"]:
+                    plan["kept"] = True
+                    self._captured.append(plan)
+            elif plan["captured"]:
+                raise RuntimeError("the plan was captured: it is made when its graph is replayed; plan again for eager "
+                                   "runs")
+            elif stream not in plan["streams"]:
+                here = torch.cuda.current_stream(plan["device"])
+                here.wait_event(plan["ready"])
+                plan["memory"].record_stream(here)
+                plan["streams"].add(stream)
         return stream
 
     # -------------------------------------------------------------- decode
@@ -146,21 +154,21 @@ class WindowAttention:
                     raise ValueError(f"page-table tensors must be on cuda:{device}")
                 tables = [t.contiguous() for t in tables]
             num_indices = tables[1].numel()
-            heads = (self.num_qo_heads, self.num_kv_heads)
-            nbytes = self._lib.pl_window_decode_plan_size(batch, num_indices, *heads)
+            heads, mask = (self.num_qo_heads, self.num_kv_heads), (self.page_size, self.window, self.sinks)
+            nbytes = self._lib.pl_window_decode_plan_size(batch, num_indices, *heads, *mask)
             if nbytes == 0:
                 raise ValueError(f"pl_window_decode_plan_size: {_lib.last_error()}")
             memory = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
             stream = torch.cuda.current_stream(device)
             _lib.check(self._lib.pl_window_decode_plan(
                 tables[0].data_ptr(), tables[1].data_ptr(), num_indices, tables[2].data_ptr(), batch, *heads,
-                self.page_size, self.window, self.sinks, memory.data_ptr(), nbytes, stream.cuda_stream),
-                "pl_window_decode_plan")
+                *mask, memory.data_ptr(), nbytes, stream.cuda_stream), "pl_window_decode_plan")
             self._decode_plan = {
                 "device": device, "batch": batch, "mask": (self.window, self.sinks), "max_page": max_page,
                 "memory": memory,
                 "args": (memory.data_ptr(), nbytes, num_indices),
-                "workspace_bytes": self._lib.pl_window_decode_workspace_size(batch, *heads, self.head_dim),
+                "workspace_bytes": self._lib.pl_window_decode_workspace_size(batch, num_indices, *heads, self.head_dim,
+                                                                             *mask),
                 "captured": captured, "kept": captured, "streams": {stream.cuda_stream},
                 "ready": None if captured else stream.record_event(),
             }
@@ -183,7 +191,7 @@ class WindowAttention:
         if plan is None:
             raise RuntimeError("plan_decode must be called before run_decode")
         device, batch = plan["device"], plan["batch"]
-        self._check_q(q, out, batch, device, "rows")
+        code, qs, os_ = self._queries(q, out, batch, device, "rows")
         k, v, page_stride, token_stride, head_stride, num_pages, bits = self._cache(
             paged_kv_cache_layer, q.dtype, device, plan["max_page"])
         if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous()
@@ -196,13 +204,13 @@ class WindowAttention:
             # per call, from torch's allocator: calls on other streams and graphs share nothing
             nbytes = plan["workspace_bytes"]
             ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-            qs, os_ = q.stride(), out.stride()
-            _lib.check(self._lib.pl_window_decode_run(
+            status = self._lib.pl_window_decode_run(
                 q.data_ptr(), qs[0], qs[1], k, v, page_stride, token_stride, head_stride, num_pages, bits,
                 out.data_ptr(), os_[0], os_[1], lse.data_ptr() if lse is not None else None,
                 batch, self.num_qo_heads, self.num_kv_heads, self.head_dim, self.page_size, *plan["mask"],
-                self.sm_scale, _lib.dtype_code(q.dtype), *plan["args"], ws.data_ptr(), nbytes, stream),
-                "pl_window_decode_run")
+                self.sm_scale, code, *plan["args"], ws.data_ptr(), nbytes, stream)
+            if status:
+                _lib.check(status, "pl_window_decode_run")
         return out
 
     # ------------------------------------------------------------- prefill
@@ -263,7 +271,7 @@ class WindowAttention:
         if plan is None:
             raise RuntimeError("plan_prefill must be called before run_prefill")
         device = plan["device"]
-        self._check_q(q, out, plan["tokens"], device, "tokens")
+        code, qs, os_ = self._queries(q, out, plan["tokens"], device, "tokens")
         k, v, page_stride, token_stride, head_stride, num_pages, bits = self._cache(
             paged_kv_cache_layer, q.dtype, device, plan["max_page"])
         if plan["tokens"] == 0:
@@ -272,10 +280,11 @@ class WindowAttention:
             stream = self._on_stream(plan)
             nbytes = plan["workspace_bytes"]
             ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-            qs, os_ = q.stride(), out.stride()
-            _lib.check(self._lib.pl_window_prefill_run(
+            status = self._lib.pl_window_prefill_run(
                 q.data_ptr(), qs[0], qs[1], k, v, page_stride, token_stride, head_stride, num_pages, bits,
                 *plan["args"], out.data_ptr(), os_[0], os_[1], plan["batch"], self.num_qo_heads, self.num_kv_heads,
-                self.head_dim, self.page_size, *plan["mask"], self.sm_scale, _lib.dtype_code(q.dtype),
-                ws.data_ptr() if nbytes else None, nbytes, nbytes, stream), "pl_window_prefill_run")
+                self.head_dim, self.page_size, *plan["mask"], self.sm_scale, code,
+                ws.data_ptr() if nbytes else None, nbytes, nbytes, stream)
+            if status:
+                _lib.check(status, "pl_window_prefill_run")
         return out

@@ -230,7 +230,7 @@ def test_a_request_from_prompt_to_fork(gpu_device, dtype, window, sinks):
             first += p
         c = {"heads": (hq, hkv), "head_dim": d, "dtype": dtype, "bits": 4, "window": window, "sinks": sinks, "lens": lens,
              "indptr": torch.tensor([0, *np.cumsum(pages)]), "indices": torch.arange(sum(pages)), "cache_host": cache,
-             "qo_indptr": torch.tensor([0, *np.cumsum(new)]), "q_host": q.cpu()}
+             "qo_indptr": torch.tensor([0, *np.cumsum(new)]), "q_host": q.cpu(), "prefill": max(new) > 1}
         check(c, out)
 
     def slots(request, positions):

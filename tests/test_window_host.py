@@ -181,9 +181,13 @@ def test_decode_plan_refuses(kw, status):
 
 def test_decode_sizes():
     lib = _lib.load()
-    assert lib.pl_window_decode_plan_size(-1, 0, 4, 2) == 0 and lib.pl_window_decode_plan_size(1, -1, 4, 2) == 0
-    assert lib.pl_window_decode_plan_size(1, 0, 5, 2) == 0 and lib.pl_window_decode_workspace_size(1, 5, 2, 128) == 0
-    assert lib.pl_window_decode_plan_size(64, 1000, 32, 8) >= 64 + 4000 + 64 * 40
+    good = dict(batch=64, indices=1000, hq=32, hkv=8, ps=16, window=0, sinks=0)
+    for kw in (dict(batch=-1), dict(indices=-1), dict(hq=5), dict(ps=0), dict(window=-1), dict(sinks=-1)):
+        a = {**good, **kw}
+        assert lib.pl_window_decode_plan_size(*a.values()) == 0
+        assert lib.pl_window_decode_workspace_size(*list(a.values())[:4], 128, *list(a.values())[4:]) == 0
+    assert lib.pl_window_decode_plan_size(*good.values()) >= 64 + 4000 + 64 * 40
+    assert lib.pl_window_decode_workspace_size(64, 1000, 32, 8, 128, 16, 0, 0) >= 64 * 8 * 16 * 130 * 4
 
 
 @pytest.mark.parametrize("kw,status", [

@@ -16,7 +16,7 @@ def case(lens, hq, hkv, head_dim, page_size, dtype, device, *, bits=16, new=None
     """Requests of ``lens`` tokens, the last ``new`` of each with queries (default: one, none of an empty request's).
     With ``poison`` all that no query sees is NaN: the tails of pages, unused pages, what a window leaves out."""
     gen = torch.Generator().manual_seed(seed)
-    new = [1] * len(lens) if new is None else new
+    prompts, new = new is not None, [1] * len(lens) if new is None else new
     pages = [-(-n // page_size) for n in lens]
     pool = sum(pages) + extra
     ids = torch.randperm(pool, generator=gen)[: sum(pages)].int()
@@ -33,7 +33,7 @@ def case(lens, hq, hkv, head_dim, page_size, dtype, device, *, bits=16, new=None
         cache[~seen[:, None].expand(-1, 2, -1)] = float("nan")
     out = {"q": q.to(device), "q_host": q, "indptr": indptr, "indices": ids, "last": last, "lens": list(lens), "new": list(new),
            "qo_indptr": torch.tensor([0, *np.cumsum(new)], dtype=torch.int32), "heads": (hq, hkv), "head_dim": head_dim,
-           "page_size": page_size, "dtype": dtype, "bits": bits, "window": window, "sinks": sinks, "device": device}
+           "page_size": page_size, "dtype": dtype, "bits": bits, "window": window, "sinks": sinks, "device": device, "prefill": prompts}
     set_cache(out, cache)
     return out
 
@@ -66,8 +66,8 @@ def reference(c, sm_scale=None, window=None):
     Half a step of the output's type (eps / 2 of the value; below the normal range of fp16, 2^-25), and of the weighted
     mean of |v|: twice (numerator and denominator) what the weights are off by: a score's D products and their sum in
     32 bits, 2^-24 D of sum |q||k| s; its exponent, x up to twice the largest score times log2 e held to 2^-24, and 2^-22
-    of the conversion; the two planes (bf16 2^-7 left, of which 2^-8: 2^-15; fp16 2^-11 twice: 2^-22); the sum over the
-    tokens in 32 bits, 2^-24 each.  And of the largest |v|, per token, what falls below a plane's range: in bf16 weights
+    of the conversion; the two planes (bf16 2^-7 left, of which 2^-8: 2^-15; fp16 2^-11 twice: 2^-22; prompts of bf16 over 4
+    bits have one fp16 plane: 2^-11); the sum over the tokens in 32 bits, 2^-24 each.  And of the largest |v|, per token, what falls below a plane's range: in bf16 weights
     are held with the row's largest at 2^-32 or more, and the second plane ends at the smallest normal number, 2^-126: 2^-94 of
     the largest; in fp16 with the largest at 2^11 or more, and half of 2^-24 is lost: 2^-36.
     """
@@ -85,11 +85,15 @@ def reference(c, sm_scale=None, window=None):
     o, lse, spread, reach = (np.concatenate(x) for x in zip(*outs))
     most = np.nan_to_num(np.abs(c["cache_host"]), nan=0.0, posinf=0.0).max(initial=0.0)
     eps = torch.finfo(c["dtype"]).eps
-    planes = 2.0 ** -22 if c["bits"] == 16 and c["dtype"] == F16 else 2.0 ** -15
+    # past the type's largest by half a step, an output rounds to an infinity
+    with np.errstate(invalid="ignore"):
+        o = np.where(np.abs(o) >= torch.finfo(c["dtype"]).max * (1 + eps / 4), np.copysign(np.inf, o), o)
+    half = c["dtype"] == F16 if c["bits"] == 16 else c.get("prefill", False)  # probabilities in fp16
+    planes = 2.0 ** -15 if not half else 2.0 ** -22 if c["dtype"] == F16 else 2.0 ** -11
     weight = 2 * (2.0 ** -24 * d * reach + 2.0 ** -24 * 2 * 1.4427 * reach + 2.0 ** -22) + planes + 2.0 ** -24 * max(c["lens"], default=0)
     with np.errstate(invalid="ignore"):
         tol = eps / 2 * np.abs(o) + weight[..., None] * spread * (1 + eps) + (2.0 ** -25 if c["dtype"] == F16 else 0)
-        tol += (2.0 ** -36 if planes < 2.0 ** -15 else 2.0 ** -94) * max(c["lens"], default=0) * most
+        tol += (2.0 ** -36 if half else 2.0 ** -94) * max(c["lens"], default=0) * most
     return o, lse, tol, weight
 
 
