@@ -397,9 +397,10 @@ int pl_window_decode_run(const void* q, int64_t q_stride_b, int64_t q_stride_h,
  * Prefill attention under the same mask: request r's queries, rows
  * qo_indptr[r] .. qo_indptr[r+1] of q, are its sequence's last positions.  The
  * plan is made on the host from host tables, and called twice: with items_h null
- * for the numbers of records, then for the records themselves (eight int32 each,
- * num_items work items and then num_merges merges), which the caller uploads
- * together with the tables.  workspace: the plan's bytes (0: may be null).
+ * for the numbers of records, then for the records themselves (16 int32 each,
+ * num_items work items and then num_merges merges), which the caller uploads, 64-byte
+ * aligned, together with the page ids.  workspace: the plan's bytes (0: may be
+ * null).  The plan's records are trusted, page ids clamped to the pool.
  */
 int pl_window_prefill_plan(const int32_t* qo_indptr_h,
                            const int32_t* kv_indptr_h,
@@ -412,11 +413,9 @@ int pl_window_prefill_run(const void* q, int64_t q_stride_t, int64_t q_stride_h,
                           const void* k_cache, const void* v_cache,
                           int64_t page_stride, int64_t token_stride,
                           int64_t head_stride, int64_t num_pages, int kv_bits,
-                          const int32_t* qo_indptr, const int32_t* kv_indptr,
-                          const int32_t* kv_indices,
-                          const int32_t* kv_last_page_len, const int32_t* items,
+                          const int32_t* kv_indices, const int32_t* items,
                           int num_items, int num_merges, void* o,
-                          int64_t o_stride_t, int64_t o_stride_h, int batch,
+                          int64_t o_stride_t, int64_t o_stride_h,
                           int num_qo_heads, int num_kv_heads, int head_dim,
                           int page_size, int window, int sinks, float sm_scale,
                           int dtype, void* workspace, size_t workspace_bytes,

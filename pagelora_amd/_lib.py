@@ -460,10 +460,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             _vp, _i64, _i64,                   # q, strides
             _vp, _vp, _i64, _i64, _i64,        # k/v cache, page/token/head strides
             _i64, _i32,                        # num_pages, kv_bits
-            _vp, _vp, _vp, _vp,                # qo_indptr, kv_indptr, kv_indices, last_page_len
-            _vp, _i32, _i32,                   # items, num_items, num_merges
+            _vp, _vp, _i32, _i32,              # kv_indices, items, num_items, num_merges
             _vp, _i64, _i64,                   # o, strides
-            _i32, _i32, _i32, _i32, _i32,      # batch, hq, hkv, head_dim, page_size
+            _i32, _i32, _i32, _i32,            # hq, hkv, head_dim, page_size
             _i32, _i32, _f32, _i32,            # window, sinks, sm_scale, dtype
             _vp, _sz, _sz, _vp,                # workspace, bytes, the plan's bytes, stream
         ],

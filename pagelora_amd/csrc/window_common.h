@@ -19,6 +19,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // ------------------------------------------------------------ products ---
 template <typename T> __device__ __forceinline__ f32x4 mfma32(u32x4 a, u32x4 b, f32x4 c);
@@ -31,12 +32,34 @@ template <> __device__ __forceinline__ f32x4 mfma32<f16_t>(u32x4 a, u32x4 b, f32
                                                 0);
 }
 
+// 32 x 32 with 16 in the sum: half as many instructions as the above.
+template <typename T> __device__ __forceinline__ f32x16 mfma16(u32x4 a, u32x4 b, f32x16 c);
+template <> __device__ __forceinline__ f32x16 mfma16<bf16_t>(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                 0, 0);
+}
+template <> __device__ __forceinline__ f32x16 mfma16<f16_t>(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                0);
+}
+
+// The larger of the lanes l, l ^ 32.
+__device__ __forceinline__ float pair_max(float v) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+
 // The largest of the four lanes l, l ^ 16, l ^ 32, l ^ 48.
 __device__ __forceinline__ float column_max(float v) {
   auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
   auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// Two floats as fp16, by the packed conversion (to nearest, as pack2's).
+__device__ __forceinline__ uint32_t pack_half(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), half2_t));
 }
 
 // Probabilities are p = 2^(x - mu), mu a constant (kBias) past the running maximum
@@ -59,10 +82,9 @@ template <> struct Planes<bf16_t> {
 template <> struct Planes<f16_t> {
   static constexpr float kLag = 4.f, kBias = -11.f;
   __device__ static __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
-    hi = pack2<f16_t>(a, b);
-    float ha, hb;
-    unpack2<f16_t>(hi, ha, hb);
-    lo = pack2<f16_t>(a - ha, b - hb);
+    const half2_t h = __builtin_convertvector((f32x2{a, b}), half2_t);
+    hi = __builtin_bit_cast(uint32_t, h);
+    lo = pack_half(__builtin_fmaf((float)h.x, -1.f, a), __builtin_fmaf((float)h.y, -1.f, b));
   }
 };
 

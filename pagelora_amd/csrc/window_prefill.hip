@@ -26,6 +26,7 @@
 // infinities, is not what a row sees), the item is worked on again: V's infinities and
 // NaN become ones in LDS, kind by kind, to find who sees them, then zeros.
 #include <algorithm>
+#include <functional>
 #include <vector>
 
 #include "window_common.h"
@@ -43,16 +44,18 @@ constexpr int kTile = 64;                   // kv tokens per tile
 
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 
-// One work item, or (in the merge list) one row item split into parts.  Tiles are
-// counted by what the item's first row sees on.
-struct Item {
-  int32_t request, row0;
+// One work item, or (in the merge list) one row item split into parts: with all that
+// its workgroup needs of its request, so that the page ids are its next load.  Tiles
+// are counted by what the item's first row sees on.
+struct alignas(64) Item {
+  int32_t request, row0, rows;            // rows: all of the request's
+  int32_t qo_begin, kv_len, page_begin;
   int32_t tile_begin, tile_end;
   int32_t slot;  // first part of the row item; -1: writes the output itself
   int32_t part, parts;
-  int32_t pad;
+  int32_t pad[5];
 };
-static_assert(sizeof(Item) == 32, "the plan's record");
+static_assert(sizeof(Item) == 64, "the plan's record: 16 words");
 
 // Scales that fp16 holds, V's after 2^kShift: down to the smallest normal number for
 // the smallest code (0.5), up to 6 times a power.
@@ -74,11 +77,11 @@ struct Args {
   const char *q, *k, *v;
   char* o;
   float* part;
-  const int32_t *qo_indptr, *kv_indptr, *kv_indices, *kv_last;
+  const int32_t* kv_indices;
   const Item* items;
   int64_t q_st, q_sh, o_st, o_sh, page_stride, token_stride, head_stride;  // bytes
   int64_t num_pages;
-  int batch, hq, hkv, page_size, page_shift, window, sinks;
+  int hq, hkv, page_size, page_shift, window, sinks;
   float scale_log2;  // > 0; a negative scale negates q instead
   uint32_t q_flip;
 };
@@ -125,17 +128,9 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
   constexpr bool kHalf = std::is_same<T, f16_t>::value;
   const int h = blockIdx.x % A.hkv;
   const Item it = A.items[blockIdx.x / A.hkv];
-  const int r = uniform(it.request), row0 = uniform(it.row0);
-  if (r < 0 || r >= A.batch) return true;
-  const int g = A.hq / A.hkv;
-  const int qo_begin = uniform(A.qo_indptr[r]);
-  const int qo_len = uniform(A.qo_indptr[r + 1]) - qo_begin;
-  const int page0 = uniform(A.kv_indptr[r]), n_pages = uniform(A.kv_indptr[r + 1]) - page0;
-  if (n_pages <= 0) return true;
-  const int last = min(max(uniform(A.kv_last[r]), 1), A.page_size);
-  const int kv_len = (n_pages - 1) * A.page_size + last;
-  const int n_rows = qo_len * g;
-  const int32_t* ind = A.kv_indices + page0;
+  const int row0 = uniform(it.row0), n_rows = uniform(it.rows);
+  const int g = A.hq / A.hkv, qo_begin = uniform(it.qo_begin), kv_len = uniform(it.kv_len);
+  const int32_t* ind = A.kv_indices + uniform(it.page_begin);
   const int ps = A.page_size;
 
   // (not known to be the thread's index, so that nothing is kept in registers from the
@@ -146,7 +141,7 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
   const int lr = lane % 16, grp = lane / 16;
 
   // what rows see: t <= lim and (t >= lo or t < sinks)
-  const int base = kv_len - qo_len;
+  const int base = kv_len - n_rows / g;
   const Seen seen = seen_from(base + row0 / g, A.window, A.sinks, kTile);
   auto low = [&](int p) { return A.window > 0 ? max(p - A.window + 1, 0) : 0; };
   const int wrow = row0 + wave * kWaveRows;
@@ -317,6 +312,12 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
     }
   };
 
+  auto load_next = [&](int tile) __attribute__((always_inline)) {
+    tile = min(tile, t_end - 1);
+    if (PAGE16 && (tile - t_begin) % 64 == 0) load_places(tile);
+    load_four(tile);
+  };
+
   // operand reads: K row blk*16 + lr, chunk 4 ks + grp; V tokens 4 grp + lr/4
   // (+16 per half, +32 per kc), dims 16 a + 4 (lr % 4)
   int kaddr[NS], vaddr[NA];
@@ -346,13 +347,10 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
       }
     } else {
       __syncthreads();
-      if (tile + 1 < t_end) {
-        store_four(tile + 1, kn, vn);
-        if (tile + 2 < t_end) {
-          if (PAGE16 && (tile + 2 - t_begin) % 64 == 0) load_places(tile + 2);
-          load_four(tile + 2);
-        }
-      }
+      // (without branches past the end, where loads in flight would be waited for: the
+      // last tile is loaded and stored again, into the buffer that is free)
+      store_four(tile + 1, kn, vn);
+      load_next(tile + 2);
     }
     const int t0 = seen_tile(seen, tile) * kTile;
     if (!FOUR && t0 + kTile > kv_len) {
@@ -445,51 +443,61 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
       }
     }
     u32x4 pb[kCols][2][NP];
+    float mu[kCols];
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) {
-      const float mu = m[c] == -INFINITY ? 0.f : m[c] + P::kBias;
-      float sum = 0.f;
-      // P^T as the B operand: k = 8*grp + e <-> tokens of blocks 2kc (e < 4) and 2kc+1 (e >= 4)
+    for (int c = 0; c < kCols; ++c) mu[c] = m[c] == -INFINITY ? 0.f : m[c] + P::kBias;
+    // P^T as the B operand: k = 8*grp + e <-> tokens of blocks 2kc (e < 4) and 2kc+1 (e >= 4)
+    auto weights = [&](int c, int blk) __attribute__((always_inline)) {
+      float p[4];
 #pragma unroll
-      for (int blk = 0; blk < 4; ++blk) {
-        float p[4];
+      for (int i = 0; i < 4; ++i) {
+        p[i] = fast_exp2(__builtin_fmaf(s[c][blk][i], sc, -mu[c]));
+        l[c] += p[i];  // per lane; the column's lanes meet after the last tile
+      }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p[i] = fast_exp2(__builtin_fmaf(s[c][blk][i], sc, -mu));
-          sum += p[i];
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if constexpr (NP == 1) {
-            pb[c][blk / 2][0][blk % 2 * 2 + i] = pack2<VT>(p[2 * i], p[2 * i + 1]);
-          } else {
-            uint32_t hi, lo_;
-            P::split(p[2 * i], p[2 * i + 1], hi, lo_);
-            pb[c][blk / 2][0][blk % 2 * 2 + i] = hi;
-            pb[c][blk / 2][NP - 1][blk % 2 * 2 + i] = lo_;
-          }
+      for (int i = 0; i < 2; ++i) {
+        if constexpr (NP == 1) {
+          pb[c][blk / 2][0][blk % 2 * 2 + i] = pack_half(p[2 * i], p[2 * i + 1]);
+        } else {
+          uint32_t hi, lo_;
+          P::split(p[2 * i], p[2 * i + 1], hi, lo_);
+          pb[c][blk / 2][0][blk % 2 * 2 + i] = hi;
+          pb[c][blk / 2][NP - 1][blk % 2 * 2 + i] = lo_;
         }
       }
-      l[c] += sum;  // per lane; the column's lanes meet after the last tile
+    };
+    // Two 16-dim blocks of V^T for tokens 32 kc ..
+    auto read_v = [&](int step, u32x4 (&va)[2]) __attribute__((always_inline)) {
+      const int kc = step / (NA / 2), a0 = step % (NA / 2) * 2;
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        const u32x2 v0 = read_tr(vb + vaddr[a0 + a] + kc * 32 * RB);
+        const u32x2 v1 = read_tr(vb + vaddr[a0 + a] + (kc * 32 + 16) * RB);
+        va[a] = u32x4{v0[0], v0[1], v1[0], v1[1]};
+      }
+    };
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk) weights(c, blk);
+    u32x4 va[2][2];
+    read_v(0, va[0]);
+#pragma unroll
+    for (int step = 0; step < NA; ++step) {
+      const int kc = step / (NA / 2), a0 = step % (NA / 2) * 2;
+      if (step + 1 < NA) read_v(step + 1, va[(step + 1) % 2]);
+#pragma unroll
+      for (int pl = 0; pl < NP; ++pl)
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) acc[c][a0 + a] = mfma32<VT>(va[step % 2][a], pb[c][kc][pl], acc[c][a0 + a]);
+      if (kc == 0) {  // the other half's weights go between the first half's products
+#pragma unroll
+        for (int i = 0; i < 8 / NA; ++i) weights((step * (8 / NA) + i) / 2, 2 + (step * (8 / NA) + i) % 2);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
-#pragma unroll
-    for (int kc = 0; kc < 2; ++kc)
-#pragma unroll
-      for (int a0 = 0; a0 < NA; a0 += 2) {
-        u32x4 va[2];
-#pragma unroll
-        for (int a = 0; a < 2; ++a) {
-          const u32x2 v0 = read_tr(vb + vaddr[a0 + a] + kc * 32 * RB);
-          const u32x2 v1 = read_tr(vb + vaddr[a0 + a] + (kc * 32 + 16) * RB);
-          va[a] = u32x4{v0[0], v0[1], v1[0], v1[1]};
-        }
-#pragma unroll
-        for (int pl = 0; pl < NP; ++pl)
-#pragma unroll
-          for (int a = 0; a < 2; ++a)
-#pragma unroll
-            for (int c = 0; c < kCols; ++c) acc[c][a0 + a] = mfma32<VT>(va[a], pb[c][kc][pl], acc[c][a0 + a]);
-      }
   };
 
   uint32_t who[3][kCols] = {};  // outputs that see each kind of what is not finite
@@ -506,7 +514,7 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
       if constexpr (FOUR) {
         load_four(t_begin);
         store_four(t_begin, s_k0, s_v0);
-        if (t_begin + 1 < t_end) load_four(t_begin + 1);
+        load_next(t_begin + 1);
       } else {
         load_wide(t_begin, s_k0, s_v0);
       }
@@ -608,62 +616,57 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(Args A) {
   }
 }
 
-// One wave per row of a split row item, D / 64 dims per lane: parts in order.
+// D / 4 lanes per row of a split row item, four dims each, its parts in order.
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads) void merge_kernel(Args A, const Item* merges) {
-  constexpr int N = D / 64;
+  constexpr int kLanes = D / 4, kAhead = 4;
   const int h = blockIdx.x % A.hkv;
   const Item it = merges[blockIdx.x / A.hkv];
-  const int r = uniform(it.request);
-  if (r < 0 || r >= A.batch) return;
-  const int g = A.hq / A.hkv;
-  const int qo_begin = uniform(A.qo_indptr[r]);
-  const int n_rows = (uniform(A.qo_indptr[r + 1]) - qo_begin) * g;
-  const int pr = blockIdx.y * kWaves + uniform(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+  const int g = A.hq / A.hkv, qo_begin = uniform(it.qo_begin), n_rows = uniform(it.rows);
+  const int pr = blockIdx.y * (kThreads / kLanes) + threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
   const int row = uniform(it.row0) + pr;
   if (row >= n_rows) return;
   const int parts = uniform(it.parts);
   const float* p = A.part + ((int64_t)uniform(it.slot) * A.hkv + h) * part_floats(D);
   const int64_t step = (int64_t)A.hkv * part_floats(D);
-  // the parts' states one per lane, their outputs eight loads at a time
-  const float* ml = p + kRows * D + pr * 2;
-  float top = -INFINITY;
-  for (int b = lane; b < parts; b += kWave) top = fmaxf(top, ml[b * step]);
+  float m = -INFINITY, sum = 0.f;
+  f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i0 = 0; i0 < parts; i0 += kAhead) {
+    f32x4 v[kAhead];
+    f32x2 ml[kAhead];
 #pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-  float sum = 0.f, o[N] = {};
-  for (int b0 = 0; b0 < parts; b0 += kWave) {
-    const int n = min(parts - b0, kWave);
-    const f32x2 own = lane < n ? *reinterpret_cast<const f32x2*>(ml + (b0 + lane) * step) : f32x2{-INFINITY, 0.f};
-    const float w = own[0] == -INFINITY ? 0.f : fast_exp2(own[0] - top);
-    const float lw = own[1] * w;
-    const float* q = p + b0 * step + pr * D + lane * N;
-    for (int i0 = 0; i0 < n; i0 += 8) {
-      float v[8][N];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int e = 0; e < N; ++e) v[i][e] = q[min(i0 + i, n - 1) * step + e];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (i0 + i >= n) break;
-        const float wi = lane_value(w, i0 + i);
-        sum += lane_value(lw, i0 + i);
-#pragma unroll
-        for (int e = 0; e < N; ++e) o[e] += weighted(v[i][e], wi);
-      }
+    for (int i = 0; i < kAhead; ++i) {
+      const float* q = p + min(i0 + i, parts - 1) * step;
+      v[i] = *reinterpret_cast<const f32x4*>(q + pr * D + d);
+      ml[i] = *reinterpret_cast<const f32x2*>(q + kRows * D + pr * 2);
     }
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (i0 + i >= parts) ml[i] = f32x2{-INFINITY, 0.f}, v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      top = fmaxf(top, ml[i][0]);
+    }
+    const float w = m == -INFINITY ? 0.f : fast_exp2(m - top);
+    sum *= w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = weighted(o[e], w);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const float wi = ml[i][0] == -INFINITY ? 0.f : fast_exp2(ml[i][0] - top);
+      sum += ml[i][1] * wi;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += weighted(v[i][e], wi);
+    }
+    m = top;
   }
   const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
   const int pos = row / g;
-  T* op = reinterpret_cast<T*>(A.o + (int64_t)(qo_begin + pos) * A.o_st + (int64_t)(h * g + row - pos * g) * A.o_sh) +
-          lane * N;
-#pragma unroll
-  for (int e = 0; e < N; ++e) op[e] = from_float<T>(o[e] * inv);
+  char* op = A.o + (int64_t)(qo_begin + pos) * A.o_st + (int64_t)(h * g + row - pos * g) * A.o_sh + d * 2;
+  *reinterpret_cast<u32x2*>(op) = u32x2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
 }
 
 // ------------------------------------------------------------ host plan ---
-constexpr int kSlots = 512;   // workgroups the chip holds: two per CU
+constexpr int kCus = 256;     // two workgroups run on each at a time, little faster than one after the other
 constexpr int kMinTiles = 4;  // fewest tiles of a part
 
 template <typename T, bool FOUR, int D> int launch(const Args& a, int num_items, int num_merges, hipStream_t s) {
@@ -674,7 +677,7 @@ template <typename T, bool FOUR, int D> int launch(const Args& a, int num_items,
     hipLaunchKernelGGL((prefill_kernel<T, FOUR, D, false>), grid, dim3(kThreads), 0, s, a);
   PL_LAUNCH_CHECK("window prefill_kernel");
   if (num_merges > 0) {
-    hipLaunchKernelGGL((merge_kernel<T, D>), dim3((unsigned)a.hkv * num_merges, kRows / kWaves), dim3(kThreads), 0, s,
+    hipLaunchKernelGGL((merge_kernel<T, D>), dim3((unsigned)a.hkv * num_merges, kRows * D / 4 / kThreads), dim3(kThreads), 0, s,
                        a, a.items + num_items);
     PL_LAUNCH_CHECK("window prefill merge_kernel");
   }
@@ -684,17 +687,99 @@ template <typename T, bool FOUR> int launch_d(const Args& a, int d, int items, i
   return d == 64 ? launch<T, FOUR, 64>(a, items, merges, s) : launch<T, FOUR, 128>(a, items, merges, s);
 }
 
+// The first workgroups go round the CUs twice: so that the longest meets the shortest
+// of them, the second the second shortest, the second round is turned about.
+template <typename I> static void pair_up(std::vector<I>& items, size_t cus) {
+  std::reverse(items.begin() + std::min(items.size(), cus), items.begin() + std::min(items.size(), 2 * cus));
+}
+
+// When the last of these items ends, in tiles of a workgroup that has a CU for itself:
+// two on one are kShared times as fast each.
+static double end_of(const std::vector<int>& items, size_t cus) {
+  constexpr double kShared = 0.6;
+  struct Cu {
+    double at;         // when its items' remaining tiles were counted
+    double left[2];    // < 0: none
+  };
+  std::vector<Cu> cu(cus, Cu{0, {-1, -1}});
+  auto next = [&](const Cu& c) {  // when its first item ends
+    const bool both = c.left[0] >= 0 && c.left[1] >= 0;
+    const double first = both ? std::min(c.left[0], c.left[1]) / kShared : std::max(c.left[0], c.left[1]);
+    return c.at + first;
+  };
+  size_t i = 0;
+  for (int round = 0; round < 2; ++round)
+    for (size_t c = 0; c < cus && i < items.size(); ++c) cu[c].left[round] = items[i++];
+  using Event = std::pair<double, size_t>;
+  std::vector<Event> heap;
+  const auto later = std::greater<Event>();
+  for (size_t c = 0; c < cus; ++c)
+    if (cu[c].left[0] >= 0) heap.push_back(Event{next(cu[c]), c});
+  std::make_heap(heap.begin(), heap.end(), later);
+  double end = 0;
+  while (!heap.empty()) {
+    std::pop_heap(heap.begin(), heap.end(), later);
+    const Event e = heap.back();
+    heap.pop_back();
+    Cu& c = cu[e.second];
+    end = e.first;
+    const bool both = c.left[0] >= 0 && c.left[1] >= 0;
+    const int done = both ? c.left[1] < c.left[0] : c.left[1] >= 0;
+    if (both) c.left[1 - done] -= (e.first - c.at) * kShared;
+    if (both && c.left[1 - done] < 0) c.left[1 - done] = 0;
+    c.at = e.first;
+    c.left[done] = i < items.size() ? items[i++] : -1;
+    if (c.left[0] >= 0 || c.left[1] >= 0) {
+      heap.push_back(Event{next(c), e.second});
+      std::push_heap(heap.begin(), heap.end(), later);
+    }
+  }
+  return end;
+}
+
+// The length at which row items are cut: of those tried, the one whose last item of a
+// head ends first.  An item costs kStart tiles beside its own, a part one more, and the
+// merge kMerge and what the parts' 66 KiB each take.  (In tiles of 2 us.)
+static int chunk_of(const std::vector<int>& lengths, int hkv) {
+  constexpr int kStart = 2, kMerge = 2, kPartsPerTile = 200;
+  constexpr size_t kMost = 4096;  // items past which no cut is needed to fill the chip
+  const int longest = lengths.empty() ? 0 : *std::max_element(lengths.begin(), lengths.end());
+  if (lengths.size() * hkv > kMost || longest < 2 * kMinTiles) return std::max(longest, 1);
+  const size_t cus = std::max(1, kCus / hkv);
+  int best = longest;
+  double least = 0;
+  std::vector<int> items;
+  for (int cut = 1, last = 0; cut <= 4 * (int)cus; cut += 1 + cut / 8) {
+    const int chunk = std::max((longest + cut - 1) / cut, kMinTiles);
+    if (chunk == last) break;
+    last = chunk;
+    items.clear();
+    int64_t parts = 0;
+    for (int t : lengths) {
+      const int n = (t + chunk - 1) / chunk;
+      if (n > 1) parts += n;
+      for (int i = 0; i < n; ++i)
+        items.push_back((int)((int64_t)t * (i + 1) / n - (int64_t)t * i / n) + kStart + (n > 1 ? 1 : 0));
+    }
+    if (cut > 1 && items.size() * hkv > kMost) break;
+    std::sort(items.begin(), items.end(), std::greater<int>());
+    pair_up(items, cus);
+    const double end = end_of(items, cus) + (parts > 0 ? kMerge + (double)parts * hkv / kPartsPerTile : 0.0);
+    if (cut == 1 || end < least) {
+      least = end;
+      best = chunk;
+    }
+  }
+  return best;
+}
+
 // The records of a plan; entry points catch what vectors throw.
 static int make_plan(const int32_t* qo, const int32_t* kv, const int32_t* kv_last, int batch, int hq, int hkv,
                      int page_size, int window, int sinks, std::vector<Item>& items, std::vector<Item>& merges,
                      int& slots) {
   const int g = hq / hkv;
-  struct Rows {
-    int32_t r, row0, tiles;
-  };
-  std::vector<Rows> list;
-  int64_t work = 0;
-  int longest = 0;
+  std::vector<Item> list;  // row items, whole
+  std::vector<int> lengths;
   for (int r = 0; r < batch; ++r) {
     const int64_t qo_len = (int64_t)qo[r + 1] - qo[r], pages = (int64_t)kv[r + 1] - kv[r];
     if (qo_len < 0) return fail(PL_ERR_INVALID, "qo_indptr_h must be non-decreasing (row %d)", r);
@@ -712,24 +797,35 @@ static int make_plan(const int32_t* qo, const int32_t* kv, const int32_t* kv_las
       const int64_t last_row = std::min<int64_t>(r0 + kRows, rows) - 1;
       const Seen s = seen_from((int)(kv_len - qo_len + r0 / g), window, sinks, kTile);
       const int tiles = s.ns + (int)((kv_len - qo_len + last_row / g) / kTile) + 1 - s.fw;
-      list.push_back(Rows{r, (int32_t)r0, tiles});
-      work += tiles;
-      longest = std::max(longest, tiles);
+      Item it{};
+      it.request = r;
+      it.row0 = (int32_t)r0;
+      it.rows = (int32_t)rows;
+      it.qo_begin = qo[r];
+      it.kv_len = (int32_t)kv_len;
+      it.page_begin = kv[r];
+      it.tile_end = tiles;
+      it.slot = -1;
+      it.parts = 1;
+      list.push_back(it);
+      lengths.push_back(tiles);
     }
   }
   if (list.size() > (size_t)INT32_MAX / 64) return fail(PL_ERR_INVALID, "too many prefill work items");
-  // A part's length: an even share of the work per slot.  Ranges are cut where the
-  // longest row item is more than twice that, and by four tiles more, which the
-  // parts and the merge cost.
-  const int64_t share = std::max<int64_t>(kMinTiles, (work * hkv + kSlots - 1) / kSlots);
-  const int64_t chunk = longest > 2 * share + 4 ? share : INT32_MAX;
-  for (const Rows& e : list) {
-    const int parts = (int)((e.tiles + chunk - 1) / chunk);
-    for (int p = 0; p < parts; ++p)
-      items.push_back(Item{e.r, e.row0, (int32_t)((int64_t)e.tiles * p / parts),
-                           (int32_t)((int64_t)e.tiles * (p + 1) / parts), parts > 1 ? slots : -1, p, parts, 0});
+  const int chunk = chunk_of(lengths, hkv);
+  for (const Item& whole : list) {
+    const int tiles = whole.tile_end, parts = (tiles + chunk - 1) / chunk;
+    Item it = whole;
+    it.parts = parts;
+    it.slot = parts > 1 ? slots : -1;
+    for (it.part = 0; it.part < parts; ++it.part) {
+      it.tile_begin = (int32_t)((int64_t)tiles * it.part / parts);
+      it.tile_end = (int32_t)((int64_t)tiles * (it.part + 1) / parts);
+      items.push_back(it);
+    }
     if (parts > 1) {
-      merges.push_back(Item{e.r, e.row0, 0, 0, slots, 0, parts, 0});
+      it.part = it.tile_begin = it.tile_end = 0;
+      merges.push_back(it);
       slots += parts;
     }
   }
@@ -741,6 +837,7 @@ static int make_plan(const int32_t* qo, const int32_t* kv, const int32_t* kv_las
     if (a.request != b.request) return a.request < b.request;
     return a.tile_begin < b.tile_begin;
   });
+  pair_up(items, std::max(1, kCus / hkv));
   return PL_OK;
 }
 
@@ -796,15 +893,12 @@ extern "C" int pl_window_prefill_plan(const int32_t* qo_indptr_h, const int32_t*
 
 extern "C" int pl_window_prefill_run(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_cache,
                                      const void* v_cache, int64_t page_stride, int64_t token_stride,
-                                     int64_t head_stride, int64_t num_pages, int kv_bits, const int32_t* qo_indptr,
-                                     const int32_t* kv_indptr, const int32_t* kv_indices,
-                                     const int32_t* kv_last_page_len, const int32_t* items, int num_items,
-                                     int num_merges, void* o, int64_t o_stride_t, int64_t o_stride_h, int batch,
-                                     int num_qo_heads, int num_kv_heads, int head_dim, int page_size, int window,
-                                     int sinks, float sm_scale, int dtype, void* workspace, size_t workspace_bytes,
-                                     size_t plan_workspace_bytes, void* stream) {
-  if (num_items < 0 || num_merges < 0 || batch < 0)
-    return fail(PL_ERR_INVALID, "num_items, num_merges and batch must be >= 0");
+                                     int64_t head_stride, int64_t num_pages, int kv_bits, const int32_t* kv_indices,
+                                     const int32_t* items, int num_items, int num_merges, void* o, int64_t o_stride_t,
+                                     int64_t o_stride_h, int num_qo_heads, int num_kv_heads, int head_dim,
+                                     int page_size, int window, int sinks, float sm_scale, int dtype, void* workspace,
+                                     size_t workspace_bytes, size_t plan_workspace_bytes, void* stream) {
+  if (num_items < 0 || num_merges < 0) return fail(PL_ERR_INVALID, "num_items and num_merges must be >= 0");
   if (num_kv_heads <= 0 || num_qo_heads <= 0 || num_qo_heads % num_kv_heads)
     return fail(PL_ERR_INVALID, "num_qo_heads (%d) must be a multiple of num_kv_heads (%d)", num_qo_heads,
                 num_kv_heads);
@@ -817,17 +911,18 @@ extern "C" int pl_window_prefill_run(const void* q, int64_t q_stride_t, int64_t 
   if (kv_bits == 4 && (page_size % 8 || page_size > (1 << 20)))
     return fail(PL_ERR_INVALID, "pages of a 4-bit cache hold a multiple of 8 tokens, up to 2^20 (got %d)", page_size);
   if (window < 0 || sinks < 0) return fail(PL_ERR_INVALID, "window and sinks must be >= 0");
-  if (num_items == 0 || batch == 0) return ok();
-  if (!q || !k_cache || !v_cache || !qo_indptr || !kv_indptr || !kv_indices || !kv_last_page_len || !items || !o)
+  if (num_items == 0) return ok();
+  if (!q || !k_cache || !v_cache || !kv_indices || !items || !o)
     return fail(PL_ERR_INVALID, "null pointer argument");
   const int eb = kv_bits == 4 ? 1 : 2;  // a 4-bit cache's strides are bytes
   const int64_t strides[] = {q_stride_t * 2, q_stride_h * 2, o_stride_t * 2, o_stride_h * 2, page_stride * eb,
                              kv_bits == 4 ? 0 : token_stride * eb, head_stride * eb};
   for (int64_t st : strides)
     if (st % 16) return fail(PL_ERR_INVALID, "strides must be multiples of 16 bytes");
-  const void* ptrs[] = {q, k_cache, v_cache, o, items, workspace};
+  const void* ptrs[] = {q, k_cache, v_cache, o, workspace};
   for (const void* p : ptrs)
-    if ((uintptr_t)p % 16) return fail(PL_ERR_INVALID, "q, o, the caches, items and workspace must be 16-byte aligned");
+    if ((uintptr_t)p % 16) return fail(PL_ERR_INVALID, "q, o, the caches and workspace must be 16-byte aligned");
+  if ((uintptr_t)items % 64) return fail(PL_ERR_INVALID, "the plan's records must be 64-byte aligned");
   if ((int64_t)std::max(num_items, num_merges) * num_kv_heads > INT32_MAX)
     return fail(PL_ERR_INVALID, "grid of %d items x %d heads too large", num_items, num_kv_heads);
   if (num_merges > 0 && (!workspace || workspace_bytes < plan_workspace_bytes))
@@ -839,10 +934,7 @@ extern "C" int pl_window_prefill_run(const void* q, int64_t q_stride_t, int64_t 
   a.v = (const char*)v_cache;
   a.o = (char*)o;
   a.part = (float*)workspace;
-  a.qo_indptr = qo_indptr;
-  a.kv_indptr = kv_indptr;
   a.kv_indices = kv_indices;
-  a.kv_last = kv_last_page_len;
   a.items = reinterpret_cast<const Item*>(items);
   a.q_st = strides[0];
   a.q_sh = strides[1];
@@ -852,7 +944,6 @@ extern "C" int pl_window_prefill_run(const void* q, int64_t q_stride_t, int64_t 
   a.token_stride = strides[5];
   a.head_stride = strides[6];
   a.num_pages = num_pages;
-  a.batch = batch;
   a.hq = num_qo_heads;
   a.hkv = num_kv_heads;
   a.page_size = page_size;

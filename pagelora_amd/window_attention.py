@@ -242,20 +242,20 @@ class WindowAttention:
                 self.head_dim, self.page_size, self.window, self.sinks)
         _lib.check(self._lib.pl_window_prefill_plan(*args, None, 0, *counts), "pl_window_prefill_plan")
         records = n.value + merges.value
-        items_h = torch.empty(max(1, 8 * records), dtype=torch.int32)
+        items_h = torch.empty(max(16, 16 * records), dtype=torch.int32)
         _lib.check(self._lib.pl_window_prefill_plan(*args, items_h.data_ptr(), records, *counts),
                    "pl_window_prefill_plan")
         with _lib.on_device(device):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("plan_prefill uploads host tables and cannot be captured")
-            items_d, *tables_d = _upload_int32((items_h, *host), self.device)
+            items_d, ids_d = _upload_int32((items_h, ind_h), self.device)
             stream = torch.cuda.current_stream(device)
             self._prefill_plan = {
-                "device": device, "batch": batch, "tokens": int(qo_h[-1]) if batch else 0,
+                "device": device, "tokens": int(qo_h[-1]) if batch else 0,
                 "mask": (self.window, self.sinks), "max_page": max_page,
-                "memory": items_d,  # one allocation holds every table
-                "args": (*(t.data_ptr() for t in (*tables_d, items_d)), n.value, merges.value),
-                "tables": tables_d, "workspace_bytes": ws_bytes.value,
+                "memory": items_d,  # one allocation holds both
+                "args": (ids_d.data_ptr(), items_d.data_ptr(), n.value, merges.value),
+                "workspace_bytes": ws_bytes.value,
                 "captured": False, "kept": False, "streams": {stream.cuda_stream}, "ready": stream.record_event(),
             }
 
@@ -282,8 +282,8 @@ class WindowAttention:
             ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
             status = self._lib.pl_window_prefill_run(
                 q.data_ptr(), qs[0], qs[1], k, v, page_stride, token_stride, head_stride, num_pages, bits,
-                *plan["args"], out.data_ptr(), os_[0], os_[1], plan["batch"], self.num_qo_heads, self.num_kv_heads,
-                self.head_dim, self.page_size, *plan["mask"], self.sm_scale, code,
+                *plan["args"], out.data_ptr(), os_[0], os_[1], self.num_qo_heads, self.num_kv_heads, self.head_dim,
+                self.page_size, *plan["mask"], self.sm_scale, code,
                 ws.data_ptr() if nbytes else None, nbytes, nbytes, stream)
             if status:
                 _lib.check(status, "pl_window_prefill_run")

@@ -76,7 +76,7 @@ def plan(qo, kv_pages, last, hq=4, hkv=2, head_dim=128, page=16, window=0, sinks
     status = lib.pl_window_prefill_plan(*args, None, 0, *out)
     if status:
         return status, None, None, None
-    records = torch.zeros((n.value + m.value, 8), dtype=torch.int32)
+    records = torch.zeros((n.value + m.value, 16), dtype=torch.int32)
     status = lib.pl_window_prefill_plan(*args, records.data_ptr() if records.numel() else PTR,
                                         records.shape[0] if max_records is None else max_records, *out)
     return status, records[: n.value].tolist(), records[n.value:].tolist(), b.value
@@ -93,7 +93,9 @@ def test_prefill_plan_covers_what_is_seen(window, sinks, hq, hkv):
     assert status == 0
     g = hq // hkv
     blocks = {}
-    for r, row0, begin, end, slot, part, parts, _ in items:
+    starts = np.cumsum([0, *new]), np.cumsum([0, *pages])
+    for r, row0, rows, qo_begin, kv_len, page_begin, begin, end, slot, part, parts, *_ in items:
+        assert (rows, kv_len) == (new[r] * g, lens[r]) and (qo_begin, page_begin) == (starts[0][r], starts[1][r])
         assert begin < end and (slot >= 0) == (parts > 1)
         blocks.setdefault((r, row0), []).append((begin, end, slot, part, parts))
     assert sorted(blocks) == [(r, r0) for r in range(5) for r0 in range(0, new[r] * g, 128)]
@@ -112,7 +114,7 @@ def test_prefill_plan_covers_what_is_seen(window, sinks, hq, hkv):
             assert {t // 64 for t in ow.sees(p, lens[r], window, sinks)} <= set(tiles)
         if cut[0][2] >= 0:
             slots.update(range(cut[0][2], cut[0][2] + len(cut)))
-            assert [r, row0, cut[0][2], len(cut)] in [[m[0], m[1], m[4], m[6]] for m in merges]
+            assert [r, row0, cut[0][2], len(cut)] in [[m[0], m[1], m[8], m[10]] for m in merges]
     assert len(merges) == sum(len(c) > 1 for c in blocks.values())
     assert slots == set(range(len(slots))) and nbytes == len(slots) * hkv * 128 * 130 * 4
 
@@ -138,8 +140,8 @@ def decode_run(**kw):
 
 
 def prefill_run(**kw):
-    a = dict(q=PTR, q_sb=512, q_sh=128, k=PTR, v=PTR, page=4096, token=256, head=128, pages=8, bits=16, qo=PTR, kv=PTR, ind=PTR,
-             last=PTR, items=PTR, n=1, m=1, o=PTR, o_sb=512, o_sh=128, batch=2, hq=4, hkv=2, d=128, ps=16, window=0, sinks=0,
+    a = dict(q=PTR, q_sb=512, q_sh=128, k=PTR, v=PTR, page=4096, token=256, head=128, pages=8, bits=16, ind=PTR,
+             items=PTR, n=1, m=1, o=PTR, o_sb=512, o_sh=128, hq=4, hkv=2, d=128, ps=16, window=0, sinks=0,
              scale=0.1, dtype=2, ws=PTR, ws_bytes=64, need=64, stream=None)
     return _lib.load().pl_window_prefill_run(*{**a, **kw}.values())
 
@@ -147,26 +149,27 @@ def prefill_run(**kw):
 COMMON = [
     (dict(q=None), 1), (dict(k=None), 1), (dict(v=None), 1), (dict(o=None), 1), (dict(q=PTR + 2), 1), (dict(v=PTR + 8), 1),
     (dict(q_sb=514), 1), (dict(o_sh=4), 1), (dict(token=132), 1), (dict(head=4), 1), (dict(page=12), 1), (dict(pages=0), 1),
-    (dict(hq=5), 1), (dict(hkv=0), 1), (dict(ps=0), 1), (dict(window=-1), 1), (dict(sinks=-2), 1), (dict(batch=-1), 1),
+    (dict(hq=5), 1), (dict(hkv=0), 1), (dict(ps=0), 1), (dict(window=-1), 1), (dict(sinks=-2), 1),
     (dict(bits=4, ps=12), 1), (dict(bits=4, ps=1 << 21), 1), (dict(bits=4, head=8), 1), (dict(bits=8), 2), (dict(d=256), 2),
     (dict(dtype=0), 2),
 ]
 
 
-@pytest.mark.parametrize("kw,status", COMMON + [(dict(plan=None), 1), (dict(plan=PTR + 16), 1), (dict(plan_bytes=64), 3),
+@pytest.mark.parametrize("kw,status", COMMON + [(dict(batch=-1), 1), (dict(plan=None), 1), (dict(plan=PTR + 16), 1), (dict(plan_bytes=64), 3),
                                                 (dict(ws_bytes=64), 3), (dict(ws=None), 1), (dict(indices=-1), 1)])
 def test_decode_run_refuses(kw, status):
     assert decode_run(**kw) == status and _lib.last_error()
 
 
 @pytest.mark.parametrize("kw,status", COMMON + [(dict(items=None), 1), (dict(n=-1), 1), (dict(ws=None), 3), (dict(ws_bytes=60), 3),
-                                                (dict(kv=None), 1), (dict(n=1 << 30, hkv=4), 1)])
+                                                (dict(ind=None), 1), (dict(items=PTR + 16), 1), (dict(m=-1), 1),
+                                                (dict(n=1 << 30, hkv=4), 1)])
 def test_prefill_run_refuses(kw, status):
     assert prefill_run(**kw) == status and _lib.last_error()
 
 
 def test_nothing_to_do_launches_nothing():
-    assert decode_run(batch=0) == 0 and prefill_run(batch=0) == 0 and prefill_run(n=0, m=0) == 0
+    assert decode_run(batch=0) == 0 and prefill_run(n=0, m=0) == 0
 
 
 @pytest.mark.parametrize("kw,status", [
