@@ -85,8 +85,11 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Args A) {
   const Place<D> at(A, wave);
   if (at.token >= A.tokens) return;
   const int64_t p = A.page_id[at.token], off = A.offset[at.token];
-  const u32x4 k = *reinterpret_cast<const u32x4*>(A.k + at.token * A.k_st + at.head * A.k_sh + at.chunk * 16);
-  const u32x4 v = *reinterpret_cast<const u32x4*>(A.v + at.token * A.v_st + at.head * A.v_sh + at.chunk * 16);
+  // (read once: kept out of the L2, where pieces of a line from several tokens meet)
+  const u32x4 k = __builtin_nontemporal_load(
+      reinterpret_cast<const u32x4*>(A.k + at.token * A.k_st + at.head * A.k_sh + at.chunk * 16));
+  const u32x4 v = __builtin_nontemporal_load(
+      reinterpret_cast<const u32x4*>(A.v + at.token * A.v_st + at.head * A.v_sh + at.chunk * 16));
   if (p < 0 || p >= A.num_pages || off < 0 || off >= A.page_size) return;  // outside the pool
   const int slot = (int)off;
   const int64_t page = p * A.page_stride + at.head * A.head_stride;
@@ -123,8 +126,8 @@ __global__ __launch_bounds__(kThreads) void read_kernel(Args A) {
     const uint32_t codes = *reinterpret_cast<const uint32_t*>(from + codes_at<D>(i, slot, at.chunk));
     const uint32_t byte = *reinterpret_cast<const uint8_t*>(from + scale_at<D>(i, A.page_size, slot, at.chunk));
     char* to = const_cast<char*>(i ? A.v + at.token * A.v_st + at.head * A.v_sh : A.k + at.token * A.k_st + at.head * A.k_sh);
-    *reinterpret_cast<u32x4*>(to + at.chunk * 16) =
-        from_bf16<T>(codes8(codes, scale_of(held ? byte : (uint32_t)kScaleNan)));
+    __builtin_nontemporal_store(from_bf16<T>(codes8(codes, scale_of(held ? byte : (uint32_t)kScaleNan))),
+                                reinterpret_cast<u32x4*>(to + at.chunk * 16));
   }
 }
 
