@@ -262,26 +262,39 @@ __global__ __launch_bounds__(kThreads, FOUR ? 3 : 2) void decode_kernel(Args A) 
   }
 
   auto page_of = [&](int t) { return A.page_shift >= 0 ? t >> A.page_shift : t / ps; };
-  auto page_at = [&](int page) -> int64_t {
-    const int id = ids[min(page, cap - 1)];
+  auto id_of = [&](int page) { return ids[min(page, cap - 1)]; };
+  auto page_at = [&](int id) -> int64_t {
     return (id < 0 ? 0 : ((int64_t)id >= A.num_pages ? A.num_pages - 1 : (int64_t)id)) * A.page_stride;
   };
   const int top = len - 1;  // addresses past the sequence repeat its end's
   const int n_tiles = it.tile_end - it.tile_begin;
   const int begin = uniform(it.tile_begin + (int)((int64_t)n_tiles * wave / kWaves));
   const int end = uniform(it.tile_begin + (int)((int64_t)n_tiles * (wave + 1) / kWaves));
+  const int64_t unit = FOUR ? (int64_t)(D / 2) : A.token_stride;
   // Pages of 16 tokens and more: lane l holds where block l % 2 of tile l / 2 of the
   // next 32 begins, so that no tile's loads wait for its page ids.
   int64_t places = 0;
   auto load_places = [&](int i) {
     const int tb = min(seen_tile(seen, min(i + lane / 2, end - 1)) * kTile + lane % 2 * 16, top & ~15);
     const int page = page_of(tb);
-    places = page_at(page) + (int64_t)(tb - page * ps) * (FOUR ? (int64_t)(D / 2) : A.token_stride);
+    places = page_at(id_of(page)) + (int64_t)(tb - page * ps) * unit;
   };
   auto place = [&](int i, int b) -> int64_t {
     const int l = (i - begin) % 32 * 2 + b;
     return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(places >> 32), l) << 32 |
                      (uint32_t)__builtin_amdgcn_readlane((int)places, l));
+  };
+
+  // Other pages: lane l holds where token l % 32 of the next tile lies; its page id is
+  // loaded a tile ahead.
+  int id_next = 0, slot_next = 0;
+  auto ask = [&](int i) {
+    const int t = min(seen_tile(seen, i) * kTile + lane % 32, top), page = page_of(t);
+    slot_next = t - page * ps;
+    id_next = id_of(page);
+  };
+  auto from_lane = [&](int64_t x, int l) -> int64_t {
+    return (int64_t)((uint64_t)(uint32_t)__shfl((int)(x >> 32), l) << 32 | (uint32_t)__shfl((int)x, l));
   };
 
   struct Raw {
@@ -312,7 +325,14 @@ __global__ __launch_bounds__(kThreads, FOUR ? 3 : 2) void decode_kernel(Args A) 
   const uint32_t ks_own = lr * (D / 32) + grp * (D / 4) / kGroup, vs_own = grp * (D / 8) + vgroup * 4;
   auto fetch = [&](int i, Raw& raw) {
     const int t0 = seen_tile(seen, i) * kTile;
-    if (PAGE16 && (i - begin) % 32 == 0) load_places(i);
+    int codes = 0;  // of the lane's token: its codes' bytes in the page
+    if constexpr (PAGE16) {
+      if ((i - begin) % 32 == 0) load_places(i);
+    } else {
+      places = page_at(id_next) + slot_next * unit;
+      codes = slot_next * (D / 2);
+      ask(min(i + 1, end - 1));
+    }
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       // a block's first token, or where it is past the end the last block's
@@ -337,26 +357,26 @@ __global__ __launch_bounds__(kThreads, FOUR ? 3 : 2) void decode_kernel(Args A) 
             load_words(vp + j * A.token_stride, raw.v[b] + j * ND, std::integral_constant<int, ND>{});
         }
       } else {
-        const int tk = min(tb + lr, top), page = page_of(tk), ok = tk - page * ps;
-        const int64_t pk = page_at(page);
+        // (tokens past the end are its last one)
         if constexpr (FOUR) {
-          const char* kp = kh + pk;
-          load_words(kp + ok * (D / 2) + grp * (D / 8), raw.k[b], std::integral_constant<int, KW>{});
-          raw.ks[b] = *reinterpret_cast<const uint8_t*>(kp + ps * (D / 2) + ok * (D / 32) + grp * (D / 4) / kGroup);
-          const int tv = min(tb + 4 * grp, top & ~3), pg = page_of(tv), quad = (tv - pg * ps) / 4;
-          const char* vp = vh + page_at(pg);
-          load_words(vp + quad * (2 * D) + vchunk, raw.v[b], std::integral_constant<int, VW>{});
-          raw.vs[b] = *reinterpret_cast<const uint32_t*>(vp + ps * (D / 2) + quad * (D / 8) + vgroup * 4);
+          const int kl = 16 * b + lr, vl = 16 * b + 4 * grp;
+          const char* kp = kh + from_lane(places, kl);
+          load_words(kp + grp * (D / 8), raw.k[b], std::integral_constant<int, KW>{});
+          // scales: from the codes' end, D / 32 bytes a token (codes D / 2)
+          raw.ks[b] = *reinterpret_cast<const uint8_t*>(kp + ps * (D / 2) - __shfl(codes, kl) / 16 * 15 + grp * (D / 4) / kGroup);
+          // V's codes go by four tokens: the last one may be within them
+          const int rest = __shfl(codes, vl) % (2 * D);
+          const char* vp = vh + from_lane(places, vl) - rest;
+          load_words(vp + vchunk, raw.v[b], std::integral_constant<int, VW>{});
+          raw.vs[b] = *reinterpret_cast<const uint32_t*>(vp + ps * (D / 2) - (__shfl(codes, vl) - rest) / 16 * 15 + vgroup * 4);
         } else {
-          const char* kp = kh + pk + (int64_t)ok * A.token_stride + k_own;
+          const char* kp = kh + from_lane(places, 16 * b + lr) + k_own;
 #pragma unroll
           for (int ks = 0; ks < NS; ++ks) load_words(kp + ks * 64, raw.k[b] + 4 * ks, std::integral_constant<int, 4>{});
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int tv = min(tb + 4 * grp + j, top), pg = page_of(tv);
-            load_words(vh + page_at(pg) + (int64_t)(tv - pg * ps) * A.token_stride + v_own, raw.v[b] + j * ND,
+          for (int j = 0; j < 4; ++j)
+            load_words(vh + from_lane(places, 16 * b + 4 * grp + j) + v_own, raw.v[b] + j * ND,
                        std::integral_constant<int, ND>{});
-          }
         }
       }
     }
@@ -496,6 +516,7 @@ __global__ __launch_bounds__(kThreads, FOUR ? 3 : 2) void decode_kernel(Args A) 
     }
     if (begin < end) {
       Raw r0, r1;
+      if (!PAGE16) ask(begin);
       fetch(begin, r0);
       int i = begin;
       for (; i + 2 <= end; i += 2) {
