@@ -160,7 +160,7 @@ int run(const void* k, const void* v, int64_t k_st, int64_t k_sh, int64_t v_st, 
   const void* ptrs[] = {k, v, k_cache, v_cache};
   for (const void* p : ptrs)
     if ((uintptr_t)p % 16) return fail(PL_ERR_INVALID, "k, v and the cache must be 16-byte aligned");
-  if ((head_dim == 64 ? waves_of<64>(tokens, hkv) : waves_of<128>(tokens, hkv)) > ((int64_t)INT32_MAX - 8) * 4)
+  if ((head_dim == 64 ? waves_of<64>(tokens, hkv) : waves_of<128>(tokens, hkv)) >= kMaxGroups * (kThreads / kWave))
     return fail(PL_ERR_INVALID, "%d tokens of %d kv heads exceed a launch", tokens, hkv);
   Args a{};
   a.k = (const char*)k;

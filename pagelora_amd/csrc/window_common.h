@@ -12,6 +12,7 @@ namespace window {
 
 constexpr int kWave = 64;
 constexpr int kMaxLen = 1 << 30;   // tokens of a sequence
+constexpr int64_t kMaxGroups = 1 << 23;  // workgroups of a launch: under 2^32 threads, 256 each
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));

@@ -678,10 +678,10 @@ using namespace pl::window;
 using namespace pl::window::dec;
 
 static int check_shape(int batch, int hq, int hkv, int page_size, int window, int sinks) {
-  if (batch < 0 || batch > (1 << 24)) return fail(PL_ERR_INVALID, "batch must be in 0 .. 2^24 (got %d)", batch);
+  if (batch < 0) return fail(PL_ERR_INVALID, "batch must be >= 0 (got %d)", batch);
   if (hkv <= 0 || hq <= 0 || hq % hkv)
     return fail(PL_ERR_INVALID, "num_qo_heads (%d) must be a multiple of num_kv_heads (%d)", hq, hkv);
-  if ((int64_t)batch * hq > INT32_MAX) return fail(PL_ERR_INVALID, "%d rows of %d heads are too many", batch, hq);
+  if ((int64_t)batch * hq >= kMaxGroups || batch + 2048 >= kMaxGroups) return fail(PL_ERR_INVALID, "%d rows of %d heads are too many", batch, hq);
   if ((int64_t)hkv * head_blocks(hq, hkv) > 65535) return fail(PL_ERR_INVALID, "%d kv heads are too many", hkv);
   if (page_size <= 0 || page_size > kMaxLen) return fail(PL_ERR_INVALID, "page_size must be positive (got %d)", page_size);
   if (window < 0 || sinks < 0) return fail(PL_ERR_INVALID, "window and sinks must be >= 0");

@@ -671,7 +671,8 @@ constexpr int kMinTiles = 4;  // fewest tiles of a part
 
 template <typename T, bool FOUR, int D> int launch(const Args& a, int num_items, int num_merges, hipStream_t s) {
   const dim3 grid((unsigned)a.hkv * num_items);
-  if (a.page_size % 16 == 0)
+  // (16 tokens of a page within 32 bits of each other)
+  if (a.page_size % 16 == 0 && a.token_stride < (1 << 27))
     hipLaunchKernelGGL((prefill_kernel<T, FOUR, D, true>), grid, dim3(kThreads), 0, s, a);
   else
     hipLaunchKernelGGL((prefill_kernel<T, FOUR, D, false>), grid, dim3(kThreads), 0, s, a);
@@ -923,7 +924,7 @@ extern "C" int pl_window_prefill_run(const void* q, int64_t q_stride_t, int64_t 
   for (const void* p : ptrs)
     if ((uintptr_t)p % 16) return fail(PL_ERR_INVALID, "q, o, the caches and workspace must be 16-byte aligned");
   if ((uintptr_t)items % 64) return fail(PL_ERR_INVALID, "the plan's records must be 64-byte aligned");
-  if ((int64_t)std::max(num_items, num_merges) * num_kv_heads > INT32_MAX)
+  if ((int64_t)std::max(num_items, num_merges) * num_kv_heads >= kMaxGroups)
     return fail(PL_ERR_INVALID, "grid of %d items x %d heads too large", num_items, num_kv_heads);
   if (num_merges > 0 && (!workspace || workspace_bytes < plan_workspace_bytes))
     return fail(PL_ERR_WORKSPACE, "prefill workspace of %zu bytes < %zu needed", workspace_bytes,

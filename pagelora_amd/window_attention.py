@@ -9,9 +9,11 @@ held in little memory:
 * a layer's cache is bf16 or fp16 ``[P, 2, page, Hkv, D]`` (NHD) or a ``(k, v)``
   pair, or a 4-bit one (uint8, :mod:`pagelora_amd.kv4`); a run takes either.
 
-``o = softmax(q . K^T / sqrt(D)) . V`` over what the query sees.  A page that no
-query sees is not read: its entry of the page table may name any page.  The
-reference attends every position of a 16-bit cache: it has no counterpart.
+``o = softmax(q . K^T / sqrt(D)) . V`` over what the query sees.  What it does not
+see may hold anything, and a page of which nobody sees a token counts for
+nothing: its entry of the page table may name any page of the pool, such as one
+that was freed.  The reference attends every position of a 16-bit cache: it has
+no counterpart.
 """
 
 from __future__ import annotations

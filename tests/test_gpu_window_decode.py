@@ -157,6 +157,17 @@ def test_pool_past_4_gib(gpu_device, bits):
     check(c, *decode(c))
 
 
+def test_tokens_far_apart(gpu_device):
+    """A page's 16 tokens over more than 4 GiB."""
+    c = case([30], 4, 2, 128, 16, BF16, gpu_device, seed=13, extra=0)
+    apart = 150 << 20  # values
+    memory = torch.empty(16 * apart, dtype=BF16, device=gpu_device)
+    cache = memory.as_strided(c["cache"].shape, (1024, 512, apart, 128, 1))
+    cache.copy_(c["cache"])
+    c["cache"] = cache
+    check(c, *decode(c))
+
+
 @pytest.mark.parametrize("bits", [16, 4])
 def test_pages_that_nobody_sees_may_be_any(gpu_device, bits):
     """Page ids of what the window has left behind are not read: a freed page's, or none's."""

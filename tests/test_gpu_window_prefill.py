@@ -162,6 +162,17 @@ def test_pool_past_4_gib(gpu_device, bits):
     check(c, prefill(c))
 
 
+def test_tokens_far_apart(gpu_device):
+    """A page's 16 tokens over more than 4 GiB."""
+    c = ragged([(30, 20)], 4, 2, 128, 16, BF16, gpu_device, seed=13, extra=0)
+    apart = 150 << 20  # values
+    memory = torch.empty(16 * apart, dtype=BF16, device=gpu_device)
+    cache = memory.as_strided(c["cache"].shape, (1024, 512, apart, 128, 1))
+    cache.copy_(c["cache"])
+    c["cache"] = cache
+    check(c, prefill(c))
+
+
 def test_no_queries(gpu_device):
     for requests in ([], [(5, 0), (0, 0)]):
         c = ragged(requests, 8, 2, 128, 16, BF16, gpu_device, seed=1)

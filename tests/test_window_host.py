@@ -161,6 +161,11 @@ def test_decode_run_refuses(kw, status):
     assert decode_run(**kw) == status and _lib.last_error()
 
 
+def test_launches_of_too_many_workgroups_are_refused():
+    assert decode_run(batch=1 << 21) == 1 and decode_run(batch=2**31 - 1, hq=1, hkv=1) == 1
+    assert prefill_run(n=1 << 22) == 1 and prefill_run(m=1 << 22) == 1
+
+
 @pytest.mark.parametrize("kw,status", COMMON + [(dict(items=None), 1), (dict(n=-1), 1), (dict(ws=None), 3), (dict(ws_bytes=60), 3),
                                                 (dict(ind=None), 1), (dict(items=PTR + 16), 1), (dict(m=-1), 1),
                                                 (dict(n=1 << 30, hkv=4), 1)])
@@ -197,6 +202,7 @@ def test_decode_sizes():
     (dict(tokens=-1), 1), (dict(hkv=0), 1), (dict(d=32), 2), (dict(d=256), 2), (dict(dtype=0), 2), (dict(ps=4), 1), (dict(ps=12), 1),
     (dict(pages=0), 1), (dict(k=None), 1), (dict(kc=None), 1), (dict(ids=None), 1), (dict(k=PTR + 8), 1), (dict(vc=PTR + 4), 1),
     (dict(kt=260), 1), (dict(head=8), 1), (dict(page=100), 1), (dict(tokens=2**31 - 1, hkv=2**16), 1),
+    (dict(tokens=1 << 26), 1),
 ])
 def test_kv4_entries_refuse(kw, status):
     a = dict(k=PTR, v=PTR, kt=256, kh=128, vt=256, vh=128, kc=PTR, vc=PTR, page=4096, head=1088, pages=4, ps=16, ids=PTR, offs=PTR,
