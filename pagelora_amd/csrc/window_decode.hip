@@ -23,6 +23,20 @@
 // two planes' infinities, is not what the row sees.  The wave's tiles are walked once
 // more with infinities and NaN taken out of V, and once with nothing but them, each
 // with weight 1, added to the sums.
+//
+// Measured (head_dim 128; decode_kernel + merge_kernel):
+//   64 x 4096 .. 16384, 4 bits, GQA 4   127.5 + 7.5 us, 5.6 TB/s; the same loads with
+//                                       next to no arithmetic 118.  289 where a
+//                                       tile's loads waited for its page ids; three
+//                                       tiles in flight instead of two 128
+//   1 x 131072, 4 bits, GQA 4           29.5 + 5 us, 4.8 TB/s: ~6 us of start (record,
+//                                       page ids, first tiles), and 24 of stream
+//   64 x 1028 of 8192, 16 bits, GQA 4   51 + 4.5 us, 5.3 TB/s; pages of one token 56 in all
+//   1 x 4112 of 32768, 16 bits, MHA     18.6 + 3.8 us: two tiles per wave, start and end
+//   23 ragged under 1000, 4 bits, GQA 7  10 + 4.2 us, 1 x 2048, 4 bits  5.9 + 4.2 us:
+//                                       dependent round trips and two launches
+// Heads fastest in the grid, so that a page's heads are read together, lost as much
+// (16 bits 52 -> 56 us) as it won (head_dim 64, 16 bits 44 -> 36).
 #include <algorithm>
 
 #include "window_common.h"

@@ -25,6 +25,21 @@
 // Where an output is NaN (0 times an infinity, or the difference of two planes'
 // infinities, is not what a row sees), the item is worked on again: V's infinities and
 // NaN become ones in LDS, kind by kind, to find who sees them, then zeros.
+//
+// Bound by instruction issue: a SIMD issues in 70 (4 bits) to 76 % (16 bits) of its
+// cycles, its matrix unit is busy in 32 to 50 % (bf16's P is two planes, a third of
+// the products).  Measured (head_dim 128, prefill_kernel + merge_kernel):
+//   2048 tokens, 4 bits, GQA 4, bf16       60.5 us (94 in bf16 with two planes of P)
+//   512 behind 16384, 4 bits, GQA 7, fp16  212 + 7 us (377 in bf16 with two planes of q
+//                                          and P, cut for 512 slots instead of by end_of)
+//   8192 under 1024, 16 bits, GQA 4, bf16  205 .. 229 us, 0.76 PFLOP/s with the masked
+//                                          products, 1.1 with the planes (a large bf16
+//                                          product: 1.24)
+//   5 ragged prompts under 512, MHA, fp16  46.5 us
+// A half's weights are formed between the products of the other half: 236 -> 225 us at
+// 8192.  Tried, and not faster: products of 32 x 32 (half as many instructions: 226 us,
+// spills over 4 bits), the conversions of the next tile between the scores' products
+// (spills: 2.3 times as long), a wave priority in the products or by the wave's slot.
 #include <algorithm>
 #include <functional>
 #include <vector>
@@ -666,7 +681,7 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(Args A, const Item* mer
 }
 
 // ------------------------------------------------------------ host plan ---
-constexpr int kCus = 256;     // two workgroups run on each at a time, little faster than one after the other
+constexpr int kCus = 256;     // two workgroups run on each at a time: the first ones i and i + kCus
 constexpr int kMinTiles = 4;  // fewest tiles of a part
 
 template <typename T, bool FOUR, int D> int launch(const Args& a, int num_items, int num_merges, hipStream_t s) {
@@ -694,8 +709,10 @@ template <typename I> static void pair_up(std::vector<I>& items, size_t cus) {
   std::reverse(items.begin() + std::min(items.size(), cus), items.begin() + std::min(items.size(), 2 * cus));
 }
 
-// When the last of these items ends, in tiles of a workgroup that has a CU for itself:
-// two on one are kShared times as fast each.
+// When the last of these items ends, in tiles of a workgroup that has a CU for itself
+// (1.7 .. 2.0 us): two on one are kShared times as fast each (2.1 .. 2.7 us a tile).
+// 512 behind 16384 in 132, 88, 66, 53, 44 and 33 tiles a part: 287, 261, 213, 248, 224
+// and 215 us, 2048 whole 62, in 28 and 16 tiles 58 + 5 and 61 + 10 with the merge.
 static double end_of(const std::vector<int>& items, size_t cus) {
   constexpr double kShared = 0.6;
   struct Cu {

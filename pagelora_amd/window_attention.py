@@ -242,11 +242,15 @@ class WindowAttention:
         counts = (ctypes.byref(n), ctypes.byref(merges), ctypes.byref(ws_bytes))
         args = (qo_h.data_ptr(), kv_h.data_ptr(), last_h.data_ptr(), batch, self.num_qo_heads, self.num_kv_heads,
                 self.head_dim, self.page_size, self.window, self.sinks)
-        _lib.check(self._lib.pl_window_prefill_plan(*args, None, 0, *counts), "pl_window_prefill_plan")
-        records = n.value + merges.value
-        items_h = torch.empty(max(16, 16 * records), dtype=torch.int32)
-        _lib.check(self._lib.pl_window_prefill_plan(*args, items_h.data_ptr(), records, *counts),
-                   "pl_window_prefill_plan")
+        room = 1024  # records, 16 words each; with more, the plan is made again
+        items_h = torch.empty(16 * room, dtype=torch.int32)
+        status = self._lib.pl_window_prefill_plan(*args, items_h.data_ptr(), room, *counts)
+        if status == _lib.PL_ERR_WORKSPACE:
+            room = n.value + merges.value
+            items_h = torch.empty(16 * room, dtype=torch.int32)
+            status = self._lib.pl_window_prefill_plan(*args, items_h.data_ptr(), room, *counts)
+        _lib.check(status, "pl_window_prefill_plan")
+        items_h = items_h[: max(16, 16 * (n.value + merges.value))]
         with _lib.on_device(device):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("plan_prefill uploads host tables and cannot be captured")

@@ -173,6 +173,12 @@ def test_tokens_far_apart(gpu_device):
     check(c, prefill(c))
 
 
+def test_many_requests(gpu_device):
+    """More records than a plan has room for at first."""
+    c = ragged([(3, 1), (20, 2)] * 600, 1, 1, 64, 16, BF16, gpu_device, bits=4, window=9, sinks=1, seed=3)
+    check(c, prefill(c))
+
+
 def test_no_queries(gpu_device):
     for requests in ([], [(5, 0), (0, 0)]):
         c = ragged(requests, 8, 2, 128, 16, BF16, gpu_device, seed=1)
