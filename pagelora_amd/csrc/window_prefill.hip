@@ -26,9 +26,11 @@
 // infinities, is not what a row sees), the item is worked on again: V's infinities and
 // NaN become ones in LDS, kind by kind, to find who sees them, then zeros.
 //
-// Bound by instruction issue: a SIMD issues in 70 (4 bits) to 76 % (16 bits) of its
-// cycles, its matrix unit is busy in 32 to 50 % (bf16's P is two planes, a third of
-// the products).  Measured (head_dim 128, prefill_kernel + merge_kernel):
+// Long items run at the rate of a large library product (1.24 PFLOP/s), P's planes
+// counted: a CU takes 1.33 us for 128 rows by 64 tokens of 16 bits in bf16, 1.21 PFLOP/s
+// (two planes: a third of the products), and 1.04 over 4 bits, 1.03.  Shorter ones are
+// bound by their starts (~6 us) and by the last items, which have a CU for themselves.
+// Measured (head_dim 128, prefill_kernel + merge_kernel):
 //   2048 tokens, 4 bits, GQA 4, bf16       60.5 us (94 in bf16 with two planes of P)
 //   512 behind 16384, 4 bits, GQA 7, fp16  212 + 7 us (377 in bf16 with two planes of q
 //                                          and P, cut for 512 slots instead of by end_of)
@@ -38,8 +40,9 @@
 //   5 ragged prompts under 512, MHA, fp16  46.5 us
 // A half's weights are formed between the products of the other half: 236 -> 225 us at
 // 8192.  Tried, and not faster: products of 32 x 32 (half as many instructions: 226 us,
-// spills over 4 bits), the conversions of the next tile between the scores' products
-// (spills: 2.3 times as long), a wave priority in the products or by the wave's slot.
+// spills over 4 bits), eight waves of 16 rows (twice the waves per SIMD: 270), the
+// conversions of the next tile between the scores' products (spills: 2.3 times as long),
+// a wave priority in the products or by the wave's slot.
 #include <algorithm>
 #include <functional>
 #include <vector>
