@@ -32,8 +32,8 @@
 // bound by their starts (~6 us) and by the last items, which have a CU for themselves.
 // Measured (head_dim 128, prefill_kernel + merge_kernel):
 //   2048 tokens, 4 bits, GQA 4, bf16       60.5 us (94 in bf16 with two planes of P)
-//   512 behind 16384, 4 bits, GQA 7, fp16  212 + 7 us (377 in bf16 with two planes of q
-//                                          and P, cut for 512 slots instead of by end_of)
+//   512 behind 16384, 4 bits, GQA 7, fp16  194 + 8 us (377 in bf16 with two planes of q
+//                                          and P and cut at one length for 512 slots)
 //   8192 under 1024, 16 bits, GQA 4, bf16  205 .. 229 us, 0.76 PFLOP/s with the masked
 //                                          products, 1.1 with the planes (a large bf16
 //                                          product: 1.24)
@@ -714,8 +714,9 @@ template <typename I> static void pair_up(std::vector<I>& items, size_t cus) {
 
 // When the last of these items ends, in tiles of a workgroup that has a CU for itself
 // (1.7 .. 2.0 us): two on one are kShared times as fast each (2.1 .. 2.7 us a tile).
-// 512 behind 16384 in 132, 88, 66, 53, 44 and 33 tiles a part: 287, 261, 213, 248, 224
-// and 215 us, 2048 whole 62, in 28 and 16 tiles 58 + 5 and 61 + 10 with the merge.
+// 512 behind 16384 all in parts of 132, 88, 66, 53, 44 and 33 tiles: 287, 261, 213, 248,
+// 224 and 215 us, in 53 and 66, two parts per CU, 194; 2048 whole 62, in parts of up to
+// 28 and 16 tiles 58 + 5 and 61 + 10 with the merge.
 static double end_of(const std::vector<int>& items, size_t cus) {
   constexpr double kShared = 0.6;
   struct Cu {
@@ -758,37 +759,50 @@ static double end_of(const std::vector<int>& items, size_t cus) {
   return end;
 }
 
-// The length at which row items are cut: of those tried, the one whose last item of a
-// head ends first.  An item costs kStart tiles beside its own, a part one more, and the
-// merge kMerge and what the parts' 66 KiB each take.  (In tiles of 2 us.)
-static int chunk_of(const std::vector<int>& lengths, int hkv) {
+// Into how many parts each row item is cut: of the numbers of parts in all that are
+// tried, dealt out so that the longest part is as short as can be, the one whose last
+// part of a head ends first.  An item costs kStart tiles beside its own, a part one
+// more, and the merge kMerge and what the parts' 66 KiB each take.  (In tiles of 2 us.)
+static std::vector<int> parts_of(const std::vector<int>& lengths, int hkv) {
   constexpr int kStart = 2, kMerge = 2, kPartsPerTile = 200;
   constexpr size_t kMost = 4096;  // items past which no cut is needed to fill the chip
-  const int longest = lengths.empty() ? 0 : *std::max_element(lengths.begin(), lengths.end());
-  if (lengths.size() * hkv > kMost || longest < 2 * kMinTiles) return std::max(longest, 1);
+  std::vector<int> parts(lengths.size(), 1), best = parts;
+  if (lengths.empty() || lengths.size() * hkv > kMost) return best;
   const size_t cus = std::max(1, kCus / hkv);
-  int best = longest;
-  double least = 0;
+  double least = -1;
   std::vector<int> items;
-  for (int cut = 1, last = 0; cut <= 4 * (int)cus; cut += 1 + cut / 8) {
-    const int chunk = std::max((longest + cut - 1) / cut, kMinTiles);
-    if (chunk == last) break;
-    last = chunk;
-    items.clear();
-    int64_t parts = 0;
-    for (int t : lengths) {
-      const int n = (t + chunk - 1) / chunk;
-      if (n > 1) parts += n;
-      for (int i = 0; i < n; ++i)
-        items.push_back((int)((int64_t)t * (i + 1) / n - (int64_t)t * i / n) + kStart + (n > 1 ? 1 : 0));
+  // the longest part first
+  using Part = std::pair<int, size_t>;
+  std::vector<Part> heap;
+  for (size_t i = 0; i < lengths.size(); ++i) heap.push_back(Part{lengths[i], i});
+  std::make_heap(heap.begin(), heap.end());
+  size_t all = lengths.size();
+  for (size_t half = 0; half <= 16; ++half) {  // no cut, then half a part per CU and on
+    const size_t want = half * cus / 2;
+    if (half > 0 && (want <= all || want * hkv > kMost)) continue;
+    while (all < want) {
+      const Part top = heap.front();
+      if (lengths[top.second] < (parts[top.second] + 1) * kMinTiles) break;
+      std::pop_heap(heap.begin(), heap.end());
+      ++parts[top.second];
+      heap.back().first = (lengths[top.second] + parts[top.second] - 1) / parts[top.second];
+      std::push_heap(heap.begin(), heap.end());
+      ++all;
     }
-    if (cut > 1 && items.size() * hkv > kMost) break;
+    items.clear();
+    int64_t cut = 0;
+    for (size_t i = 0; i < lengths.size(); ++i) {
+      const int t = lengths[i], n = parts[i];
+      if (n > 1) cut += n;
+      for (int j = 0; j < n; ++j)
+        items.push_back((int)((int64_t)t * (j + 1) / n - (int64_t)t * j / n) + kStart + (n > 1 ? 1 : 0));
+    }
     std::sort(items.begin(), items.end(), std::greater<int>());
     pair_up(items, cus);
-    const double end = end_of(items, cus) + (parts > 0 ? kMerge + (double)parts * hkv / kPartsPerTile : 0.0);
-    if (cut == 1 || end < least) {
+    const double end = end_of(items, cus) + (cut > 0 ? kMerge + (double)cut * hkv / kPartsPerTile : 0.0);
+    if (least < 0 || end < least) {
       least = end;
-      best = chunk;
+      best = parts;
     }
   }
   return best;
@@ -833,10 +847,10 @@ static int make_plan(const int32_t* qo, const int32_t* kv, const int32_t* kv_las
     }
   }
   if (list.size() > (size_t)INT32_MAX / 64) return fail(PL_ERR_INVALID, "too many prefill work items");
-  const int chunk = chunk_of(lengths, hkv);
-  for (const Item& whole : list) {
-    const int tiles = whole.tile_end, parts = (tiles + chunk - 1) / chunk;
-    Item it = whole;
+  const std::vector<int> cuts = parts_of(lengths, hkv);
+  for (size_t i = 0; i < list.size(); ++i) {
+    const int tiles = list[i].tile_end, parts = cuts[i];
+    Item it = list[i];
     it.parts = parts;
     it.slot = parts > 1 ? slots : -1;
     for (it.part = 0; it.part < parts; ++it.part) {
