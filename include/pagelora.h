@@ -325,8 +325,9 @@ int pl_prefill_split_run(const void* q, int64_t q_stride_t, int64_t q_stride_h,
  * power of two 2^(s - 127): the least at which the largest magnitude is at most
  * 6, s in 2 .. 252 (values below fall to 0, values above end at the largest).
  * A value is an e2m1 code of it (sign, 0 0.5 1 1.5 2 3 4 6), the nearest,
- * halfway to the one of even mantissa; lower nibble, lower dim.  A group that
- * holds a NaN or an infinity gets s = 255 and reads back as NaN.
+ * halfway to the one of even mantissa; lower nibble, lower dim.  A group of
+ * zeros gets s = 127; one that holds a NaN or an infinity gets s = 255 and reads
+ * back as NaN.
  *   K: codes [token][head_dim / 2], scales [token][head_dim / 32];
  *   V: codes [token / 4][d / 8][token % 4][4], scales [token / 4][d / 32][token % 4].
  *

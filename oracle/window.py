@@ -21,7 +21,7 @@ def quantize(x):
     top = np.abs(g).max(-1)
     held = np.isfinite(top)
     with np.errstate(divide="ignore", invalid="ignore"):
-        e = np.where(held & (top > 0), np.ceil(np.log2(np.where(held, top, 1.0) / 6.0)), -125.0)
+        e = np.where(held & (top > 0), np.ceil(np.log2(np.where(held, top, 1.0) / 6.0)), 0.0)
     e = np.clip(e, -125, 125)
     y = np.where(held[..., None], g, 0.0) / np.exp2(e)[..., None]
     a = np.minimum(np.abs(y), 6.0)

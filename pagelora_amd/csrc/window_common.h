@@ -20,7 +20,6 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // ------------------------------------------------------------ products ---
 template <typename T> __device__ __forceinline__ f32x4 mfma32(u32x4 a, u32x4 b, f32x4 c);
@@ -31,23 +30,6 @@ template <> __device__ __forceinline__ f32x4 mfma32<bf16_t>(u32x4 a, u32x4 b, f3
 template <> __device__ __forceinline__ f32x4 mfma32<f16_t>(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
                                                 0);
-}
-
-// 32 x 32 with 16 in the sum: half as many instructions as the above.
-template <typename T> __device__ __forceinline__ f32x16 mfma16(u32x4 a, u32x4 b, f32x16 c);
-template <> __device__ __forceinline__ f32x16 mfma16<bf16_t>(u32x4 a, u32x4 b, f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
-                                                 0, 0);
-}
-template <> __device__ __forceinline__ f32x16 mfma16<f16_t>(u32x4 a, u32x4 b, f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
-                                                0);
-}
-
-// The larger of the lanes l, l ^ 32.
-__device__ __forceinline__ float pair_max(float v) {
-  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
 }
 
 // The largest of the four lanes l, l ^ 16, l ^ 32, l ^ 48.
@@ -96,6 +78,7 @@ template <> struct Planes<f16_t> {
 // [token % 4][4 bytes], scales [token / 4][d / 32][token % 4].
 constexpr int kGroup = 32;                     // values that share a scale
 constexpr int kScaleMin = 2, kScaleMax = 252;  // 2^(s - 127): every value is a normal bf16
+constexpr int kScaleZero = 127;                // every value is 0: a scale that any product's type holds
 constexpr int kScaleNan = 255;                 // the group held a NaN or an infinity
 
 // A scale byte as the conversions take it.

@@ -6,8 +6,8 @@ scales.  Each 32 values of a token along head_dim share a power of two
 ``2^(s - 127)``, one byte ``s``: the least at which the largest magnitude is at
 most 6.  A value is a code of 4 bits times it (e2m1: a sign and 0, 0.5, 1, 1.5,
 2, 3, 4 or 6), the nearest one, halfway to the one with an even mantissa: 4.25
-bits per value.  ``s`` lies in 2 .. 252; 255 marks a group that held a NaN or an
-infinity, and reads back as NaN.
+bits per value.  ``s`` lies in 2 .. 252, and is 127 in a group of zeros; 255 marks
+a group that held a NaN or an infinity, and reads back as NaN.
 
 * K: codes ``[token][D / 2 bytes]``, scales ``[token][D / 32]``;
 * V: codes ``[token / 4][d / 8][token % 4][4 bytes]``, scales

@@ -109,6 +109,21 @@ def test_error_of_a_value(gpu_device, dtype):
     assert (off <= groups.abs() / 5)[groups.abs() * 3 >= top].all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_groups_of_zeros(gpu_device, dtype):
+    """Scale 127, that of 4 to 6, whatever stands beside them."""
+    x = torch.randn((9, 2, 64), generator=torch.Generator().manual_seed(8)).to(dtype)
+    x[..., 32:] = 0.0
+    x[1, :, 40] = -0.0
+    where = places(9, 2, 8, 5)
+    layer, back = run(x, x, *where, 8, 2, gpu_device, fill=0xA5)
+    scales = torch.from_numpy(layer)[..., 8 * 32:]
+    k = scales[:, 0].unflatten(2, (8, 2))[where[0], :, where[1]]
+    v = scales[:, 1].unflatten(2, (2, 2, 4))[where[0], :, where[1] // 4, :, where[1] % 4]
+    assert (k[..., 1] == 127).all() and (v[..., 1] == 127).all() and (k[..., 0] != 127).any()
+    assert torch.equal(back[0][..., 32:], x[..., 32:]) and torch.equal(back[1][..., 32:], x[..., 32:])
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_what_is_not_finite_marks_its_group(gpu_device, dtype, bad):

@@ -102,6 +102,19 @@ def test_scales_of_a_4_bit_cache(gpu_device, dtype, requests, k_power, v_power):
     check(c, prefill(c))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_head_dims_that_only_pad(gpu_device, dtype):
+    """96 dims in 128: groups of zeros in q, K and V, and a V token of zeros."""
+    c = ragged([(200, 150), (2000, 6)], 4, 2, 128, 16, dtype, gpu_device, bits=4, seed=6, poison=False)
+    cache = torch.randn((c["indices"].numel() + 3, 2, 16, 2, 128), generator=torch.Generator().manual_seed(1))
+    cache[..., 96:] = 0.0
+    cache[int(c["indices"][2]), 1, 3] = 0.0
+    set_cache(c, cache.to(BF16))
+    out = prefill(c)
+    check(c, out)
+    assert (out[..., 96:] == 0).all()
+
+
 @pytest.mark.parametrize("window,sinks", [(0, 0), (30, 2)])
 def test_nan_groups_of_a_4_bit_cache(gpu_device, window, sinks):
     c = ragged([(200, 150)], 4, 2, 128, 16, BF16, gpu_device, bits=4, window=window, sinks=sinks, seed=5, poison=False)
