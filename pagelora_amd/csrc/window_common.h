@@ -45,29 +45,36 @@ __device__ __forceinline__ uint32_t pack_half(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), half2_t));
 }
 
-// Probabilities are p = 2^(x - mu), mu a constant (kBias) past the running maximum
-// that the row's sums are held at, which follows only scores more than kLag above
-// it.  They enter the product with V in two planes of its type, so that 16 bits of
-// each (bf16) or 22 (fp16) do: off by 2^-15 and 2^-22 of the weight, under the 2^-8
-// and 2^-11 of the output's rounding.  bf16: p <= 2^-24, so that the sums over 2^24
-// tokens of the largest V are finite.  fp16: p <= 2^15, near the range's top, so that
-// a weight of 2^-35 of the largest still counts.
+// Probabilities are p = kScale 2^(x - m), m the running maximum that the row's sums are
+// held at, which follows only scores more than kLag above it.  (The factor is a product
+// of its own: in the exponent, 32 would take 5 bits of it.)  They enter the product with V in planes of its type, each what the one before
+// left: three of bf16, cut, hold the 24 bits of fp32, two of fp16, rounded to nearest,
+// 22 of them, as in the other attention kernels.  Two planes of bf16 leave 2^-16,
+// which is past an output's rounding where the terms cancel to 2^-8 of themselves.
+// bf16: p <= 2^-24, so that the sums over 2^24 tokens of the largest V are finite;
+// the planes end at 2^-126, 2^-94 of the row's largest weight or less.  fp16: p <= 2^15,
+// near the range's top; the planes end at 2^-25, 2^-36 of the largest weight or less.
 template <typename MT> struct Planes;
 template <> struct Planes<bf16_t> {
-  static constexpr float kLag = 8.f, kBias = 32.f;
-  // The planes of two probabilities: the upper halves, then the rest rounded.
-  __device__ static __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
-    const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
-    hi = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
-    lo = f32x2_to_bf16x2_bits(a - __uint_as_float(ua & 0xffff0000u), b - __uint_as_float(ub & 0xffff0000u));
+  static constexpr int kPlanes = 3;
+  static constexpr float kLag = 8.f, kShift = -32.f, kScale = 0x1p-32f;
+  __device__ static __forceinline__ void split(float a, float b, uint32_t (&w)[kPlanes]) {
+#pragma unroll
+    for (int i = 0; i < kPlanes; ++i) {
+      const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+      w[i] = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
+      a -= __uint_as_float(ua & 0xffff0000u);
+      b -= __uint_as_float(ub & 0xffff0000u);
+    }
   }
 };
 template <> struct Planes<f16_t> {
-  static constexpr float kLag = 4.f, kBias = -11.f;
-  __device__ static __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
+  static constexpr int kPlanes = 2;
+  static constexpr float kLag = 4.f, kShift = 11.f, kScale = 0x1p11f;
+  __device__ static __forceinline__ void split(float a, float b, uint32_t (&w)[kPlanes]) {
     const half2_t h = __builtin_convertvector((f32x2{a, b}), half2_t);
-    hi = __builtin_bit_cast(uint32_t, h);
-    lo = pack_half(__builtin_fmaf((float)h.x, -1.f, a), __builtin_fmaf((float)h.y, -1.f, b));
+    w[0] = __builtin_bit_cast(uint32_t, h);
+    w[1] = pack_half(__builtin_fmaf((float)h.x, -1.f, a), __builtin_fmaf((float)h.y, -1.f, b));
   }
 };
 

@@ -206,7 +206,7 @@ struct Args {
   uint32_t q_flip;
 };
 
-// Floats of a part: outputs [16][D], then (mu, sum) per head.
+// Floats of a part: outputs [16][D], then (m, sum) per head.
 template <int D> constexpr int part_floats() { return 16 * (D + 2); }
 
 __device__ __forceinline__ bool stale(const Header& h, const Header& want) {
@@ -214,9 +214,9 @@ __device__ __forceinline__ bool stale(const Header& h, const Header& want) {
          h.sinks != want.sinks || h.indices_capacity != want.indices_capacity || h.max_items != want.max_items;
 }
 
-// ln of sum 2^mu; -inf where nothing was seen.
-__device__ __forceinline__ float log_sum(float mu, float sum) {
-  return sum > 0.f ? (mu + log2f(sum)) * 0.69314718055994531f : (sum == 0.f ? -INFINITY : sum);
+// ln of sum 2^(m - shift); -inf where nothing was seen.
+__device__ __forceinline__ float log_sum(float m, float sum, float shift) {
+  return sum > 0.f ? (m + (log2f(sum) - shift)) * 0.69314718055994531f : (sum == 0.f ? -INFINITY : sum);
 }
 
 template <typename T, bool FOUR, int D, bool PAGE16>
@@ -464,10 +464,11 @@ __global__ __launch_bounds__(kThreads, FOUR ? 3 : 2) void decode_kernel(Args A) 
           vt[j][e] &= walk == kFinite ? held : ~held;
         }
     }
-    u32x4 pb[2];
+    u32x4 pb[P::kPlanes];
     if (walk == kOdd) {
       const uint32_t one = pack2<MT>(1.f, 1.f);
-      pb[0] = pb[1] = u32x4{one, one, one, one};
+#pragma unroll
+      for (int pl = 0; pl < P::kPlanes; ++pl) pb[pl] = u32x4{one, one, one, one};
     } else {
       float mx = -INFINITY;
 #pragma unroll
@@ -485,23 +486,23 @@ __global__ __launch_bounds__(kThreads, FOUR ? 3 : 2) void decode_kernel(Args A) 
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[a][j] *= alpha;
       }
-      const float mu = m == -INFINITY ? 0.f : m + P::kBias;
+      const float mu = m == -INFINITY ? 0.f : m;
       float ps_ = 0.f;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         float p[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          p[j] = fast_exp2(__builtin_fmaf(s[b][j], sc, -mu));
+          p[j] = fast_exp2(__builtin_fmaf(s[b][j], sc, -mu)) * P::kScale;
           ps_ += p[j];
         }
-        uint32_t hi0, lo0, hi1, lo1;
-        P::split(p[0], p[1], hi0, lo0);
-        P::split(p[2], p[3], hi1, lo1);
-        pb[0][2 * b] = hi0;
-        pb[0][2 * b + 1] = hi1;
-        pb[1][2 * b] = lo0;
-        pb[1][2 * b + 1] = lo1;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t w[P::kPlanes];
+          P::split(p[2 * i], p[2 * i + 1], w);
+#pragma unroll
+          for (int pl = 0; pl < P::kPlanes; ++pl) pb[pl][2 * b + i] = w[pl];
+        }
       }
       l += ps_;  // per lane; the column's lanes meet after the last tile
     }
@@ -514,7 +515,7 @@ __global__ __launch_bounds__(kThreads, FOUR ? 3 : 2) void decode_kernel(Args A) 
         v1[j] = __builtin_amdgcn_perm(vt[2 * j + 1][e], vt[2 * j][e], 0x07060302u);
       }
 #pragma unroll
-      for (int pl = 0; pl < 2; ++pl) {
+      for (int pl = 0; pl < P::kPlanes; ++pl) {
         acc[2 * e] = mfma32<MT>(v0, pb[pl], acc[2 * e]);
         acc[2 * e + 1] = mfma32<MT>(v1, pb[pl], acc[2 * e + 1]);
       }
@@ -559,7 +560,7 @@ __global__ __launch_bounds__(kThreads, FOUR ? 3 : 2) void decode_kernel(Args A) 
         *reinterpret_cast<f32x4*>(&s_o[wave][lr][(4 * grp + j) * NA + a]) =
             f32x4{acc[a][j], acc[a + 1][j], acc[a + 2][j], acc[a + 3][j]};
     if (grp == 0) {
-      s_m[wave][lr] = m == -INFINITY ? -INFINITY : m + P::kBias;
+      s_m[wave][lr] = m;
       s_l[wave][lr] = l;
     }
   }
@@ -590,14 +591,15 @@ __global__ __launch_bounds__(kThreads, FOUR ? 3 : 2) void decode_kernel(Args A) 
     const int hq = h * g + hb * 16 + r;
     *reinterpret_cast<u32x2*>(A.o + (int64_t)row * A.o_sb + (int64_t)hq * A.o_sh + d * 2) =
         u32x2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
-    if (d == 0 && A.lse) A.lse[(int64_t)row * A.hq + hq] = log_sum(mx, sum);
+    if (d == 0 && A.lse) A.lse[(int64_t)row * A.hq + hq] = log_sum(mx, sum, P::kShift);
   }
 }
 
 // A workgroup per (request, head) of several items: D / 4 lanes take a part, four dims
 // each, and so many parts at a time; what they saw meets in LDS.
-template <typename T, int D>
+template <typename T, bool FOUR, int D>
 __global__ __launch_bounds__(kThreads) void merge_kernel(Args A) {
+  using P = Planes<typename std::conditional<FOUR, bf16_t, T>::type>;
   constexpr int kLanes = D / 4, kGroups = kThreads / kLanes, kAhead = 4;
   __shared__ __align__(16) float s_o[kGroups][D];
   __shared__ float s_m[kGroups], s_l[kGroups];
@@ -662,7 +664,7 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(Args A) {
   const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
   *reinterpret_cast<u32x2*>(A.o + (int64_t)row * A.o_sb + (int64_t)hq * A.o_sh + d * 2) =
       u32x2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
-  if (d == 0 && A.lse) A.lse[(int64_t)row * A.hq + hq] = log_sum(top, sum);
+  if (d == 0 && A.lse) A.lse[(int64_t)row * A.hq + hq] = log_sum(top, sum, P::kShift);
 }
 
 template <typename T, bool FOUR, int D>
@@ -673,7 +675,7 @@ int launch(const Args& a, hipStream_t s) {
   else
     hipLaunchKernelGGL((decode_kernel<T, FOUR, D, false>), grid, dim3(kThreads), 0, s, a);
   PL_LAUNCH_CHECK("window decode_kernel");
-  hipLaunchKernelGGL((merge_kernel<T, D>), dim3((unsigned)(a.want.batch * a.hq)), dim3(kThreads), 0, s, a);
+  hipLaunchKernelGGL((merge_kernel<T, FOUR, D>), dim3((unsigned)(a.want.batch * a.hq)), dim3(kThreads), 0, s, a);
   PL_LAUNCH_CHECK("window merge_kernel");
   return ok();
 }

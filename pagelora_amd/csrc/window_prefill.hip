@@ -17,10 +17,12 @@
 // keeps a query per lane, whose probabilities are the B operand of O^T += V^T P^T as
 // they lie; V^T comes out of LDS transposed.
 //
-// V of 4 bits is multiplied in fp16 (K too, where q is fp16), which takes fewer planes
-// than bf16: one of the probabilities for bf16 outputs, one of q for fp16 ones.  The
-// values are exact there while their groups' scales are in a range; an item that met
-// others is worked on again in bf16, which holds all of them.
+// For queries of fp16, K and V of 4 bits are multiplied in fp16, which takes fewer
+// planes than bf16: one of q, two of the probabilities.  The values are exact there
+// while their groups' scales are in a range; an item that met others is worked on again
+// in bf16, which holds all of them.  For bf16 queries they are multiplied in bf16: a
+// weight that fp16 cannot hold, under 2^-36 of the row's largest, counts in an output
+// of bf16 where the larger ones meet zeros.
 //
 // Where an output is NaN (0 times an infinity, or the difference of two planes'
 // infinities, is not what a row sees), the item is worked on again: V's infinities and
@@ -81,7 +83,7 @@ constexpr uint32_t kShift = 10;
 constexpr uint32_t kKLeast = 127 - 13, kKMost = 127 + 13;
 constexpr uint32_t kVLeast = kKLeast - kShift, kVMost = kKMost - kShift;
 
-constexpr int part_floats(int d) { return kRows * (d + 2); }  // outputs [row][dim], then (mu, sum) per row
+constexpr int part_floats(int d) { return kRows * (d + 2); }  // outputs [row][dim], then (m, sum) per row
 
 __device__ __forceinline__ void load_lds16(const char* g, char* l) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
@@ -127,23 +129,23 @@ template <typename MT> __device__ __forceinline__ uint32_t taken(uint32_t w, int
 
 constexpr int buffer_bytes(int d) { return kTile * d * 2; }
 
-// One item's work.  N (narrow, 4 bits alone): in fp16; false where a scale was out of
+// One item's work.  N (narrow, fp16 over 4 bits): in fp16; false where a scale was out of
 // its range, and nothing is written then.  s_k0 .. s_v1: a K and a V buffer each, one
 // object per buffer, so that writes into one never alias reads of another.
 template <typename T, bool FOUR, int D, bool PAGE16, bool N>
 __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, char* __restrict__ s_v0,
                                      char* __restrict__ s_k1, char* __restrict__ s_v1) {
-  using KT = typename std::conditional<FOUR && !N, bf16_t, T>::type;  // of K and q as they are multiplied
-  using VT = typename std::conditional<N, f16_t, KT>::type;           // of V and p
-  using P = Planes<VT>;
-  constexpr int QP = FOUR && !N && std::is_same<T, f16_t>::value ? 2 : 1;  // planes of q
-  constexpr int NP = N && std::is_same<T, bf16_t>::value ? 1 : 2;          // planes of p
+  constexpr bool kHalf = std::is_same<T, f16_t>::value;
+  static_assert(!N || (FOUR && kHalf), "narrow: fp16 over 4 bits");
+  using MT = typename std::conditional<FOUR && !N, bf16_t, T>::type;  // what is multiplied
+  using P = Planes<MT>;
+  constexpr int QP = FOUR && !N && kHalf ? 2 : 1;  // planes of q
+  constexpr int NP = P::kPlanes;                   // planes of p
   constexpr int NS = D / 32, NA = D / 16;
   constexpr int RB = D * 2;              // bytes of a row
   constexpr int CH = D / 8;              // its 16-byte chunks
   constexpr int TPL = kWave / CH;        // tokens of a load instruction
   constexpr int NL = 16 / TPL;           // load instructions of a wave's 16 tokens
-  constexpr bool kHalf = std::is_same<T, f16_t>::value;
   const int h = blockIdx.x % A.hkv;
   const Item it = A.items[blockIdx.x / A.hkv];
   const int row0 = uniform(it.row0), n_rows = uniform(it.rows);
@@ -291,20 +293,20 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
     raw.v = *reinterpret_cast<const u32x4*>(vp);
     raw.vs = *reinterpret_cast<const uint32_t*>(wp);
   };
-  // Narrow: K in q's type and V in fp16, times 2^kShift, exact where the scales are in range
+  // Narrow: K in fp16, and V times 2^kShift, exact where the scales are in range
   uint32_t v_least = ~0u, v_most = 0u, k_least = ~0u, k_most = 0u;
   auto store_four = [&](int tile, char* kd, char* vd) __attribute__((always_inline)) {
     const int t0 = seen_tile(seen, tile) * kTile;
     if (t0 + k_tok >= kv_len) raw.ks = 127u;  // (what lies there counts for nothing)
     const float ks = scale_of(raw.ks);
-    if constexpr (N && kHalf) {
+    if constexpr (N) {
       k_least = min(k_least, raw.ks);
       k_most = max(k_most, raw.ks);
     }
 #pragma unroll
     for (int c = 0; c < KQ; ++c)
       *reinterpret_cast<u32x4*>(kd + k_tok * RB + (((tid % 4) * KQ + c) ^ (k_tok % CH)) * 16) =
-          N && kHalf ? halves8(raw.k[c], ks) : codes8(raw.k[c], ks);
+          N ? halves8(raw.k[c], ks) : codes8(raw.k[c], ks);
     if (CH == 16 || tid < 16 * CH) {
       if (t0 + kTile > kv_len) {
 #pragma unroll
@@ -381,7 +383,7 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
       for (int c = tid; c < kTile * CH; c += kThreads) {
         u32x4 x = *reinterpret_cast<const u32x4*>(vb + c * 16);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = taken<VT>(x[e], walk);
+        for (int e = 0; e < 4; ++e) x[e] = taken<MT>(x[e], walk);
         *reinterpret_cast<u32x4*>(vb + c * 16) = x;
       }
       __syncthreads();
@@ -408,7 +410,7 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
 #pragma unroll
           for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int c = 0; c < kCols; ++c) s[c][b0 + b] = mfma32<KT>(ka[b], qb[pl][c][ks], s[c][b0 + b]);
+            for (int c = 0; c < kCols; ++c) s[c][b0 + b] = mfma32<MT>(ka[b], qb[pl][c][ks], s[c][b0 + b]);
       }
     }
     const bool odd = !N && walk != kAll && walk != kFinite;
@@ -463,25 +465,21 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
     u32x4 pb[kCols][2][NP];
     float mu[kCols];
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) mu[c] = m[c] == -INFINITY ? 0.f : m[c] + P::kBias;
+    for (int c = 0; c < kCols; ++c) mu[c] = m[c] == -INFINITY ? 0.f : m[c];
     // P^T as the B operand: k = 8*grp + e <-> tokens of blocks 2kc (e < 4) and 2kc+1 (e >= 4)
     auto weights = [&](int c, int blk) __attribute__((always_inline)) {
       float p[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        p[i] = fast_exp2(__builtin_fmaf(s[c][blk][i], sc, -mu[c]));
+        p[i] = fast_exp2(__builtin_fmaf(s[c][blk][i], sc, -mu[c])) * P::kScale;
         l[c] += p[i];  // per lane; the column's lanes meet after the last tile
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        if constexpr (NP == 1) {
-          pb[c][blk / 2][0][blk % 2 * 2 + i] = pack_half(p[2 * i], p[2 * i + 1]);
-        } else {
-          uint32_t hi, lo_;
-          P::split(p[2 * i], p[2 * i + 1], hi, lo_);
-          pb[c][blk / 2][0][blk % 2 * 2 + i] = hi;
-          pb[c][blk / 2][NP - 1][blk % 2 * 2 + i] = lo_;
-        }
+        uint32_t w[NP];
+        P::split(p[2 * i], p[2 * i + 1], w);
+#pragma unroll
+        for (int pl = 0; pl < NP; ++pl) pb[c][blk / 2][pl][blk % 2 * 2 + i] = w[pl];
       }
     };
     // Two 16-dim blocks of V^T for tokens 32 kc ..
@@ -509,7 +507,7 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
 #pragma unroll
         for (int a = 0; a < 2; ++a)
 #pragma unroll
-          for (int c = 0; c < kCols; ++c) acc[c][a0 + a] = mfma32<VT>(va[step % 2][a], pb[c][kc][pl], acc[c][a0 + a]);
+          for (int c = 0; c < kCols; ++c) acc[c][a0 + a] = mfma32<MT>(va[step % 2][a], pb[c][kc][pl], acc[c][a0 + a]);
       if (kc == 0) {  // the other half's weights go between the first half's products
 #pragma unroll
         for (int i = 0; i < 8 / NA; ++i) weights((step * (8 / NA) + i) / 2, 2 + (step * (8 / NA) + i) % 2);
@@ -545,15 +543,19 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
     if (tile < t_end) body(tile, s_k0, s_v0, s_k1, s_v1, walk);
     if constexpr (N) {
       const uint32_t least = min(v_least & 0xffffu, v_least >> 16), most = max(v_most & 0xffffu, v_most >> 16);
-      if (__syncthreads_or(least < kVLeast || most > kVMost || (kHalf && (k_least < kKLeast || k_most > kKMost))))
+      if (__syncthreads_or(least < kVLeast || most > kVMost || k_least < kKLeast || k_most > kKMost))
         return false;
-      const float down = __uint_as_float((127u - kShift) << 23);
+      // as the sums of bf16 are held, since a row's other parts may be worked on in it
+      constexpr float kDown = Planes<bf16_t>::kScale / P::kScale;
+      const float down = __uint_as_float((127u - kShift) << 23) * kDown;
 #pragma unroll
-      for (int c = 0; c < kCols; ++c)
+      for (int c = 0; c < kCols; ++c) {
+        l[c] *= kDown;
 #pragma unroll
         for (int a = 0; a < NA; ++a)
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[c][a][i] *= down;
+      }
       break;
     }
     if (walk == kAll) {
@@ -608,7 +610,7 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
 #pragma unroll
       for (int a = 0; a < NA; ++a) *reinterpret_cast<f32x4*>(p + pr * D + a * 16 + grp * 4) = acc[c][a];
       if (grp == 0)
-        *reinterpret_cast<f32x2*>(p + kRows * D + pr * 2) = f32x2{m[c] == -INFINITY ? -INFINITY : m[c] + P::kBias, sum};
+        *reinterpret_cast<f32x2*>(p + kRows * D + pr * 2) = f32x2{m[c], sum};
       continue;
     }
     const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
@@ -629,8 +631,9 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(Args A) {
   __shared__ __align__(16) char s_v0[buffer_bytes(D)];
   __shared__ __align__(16) char s_k1[buffer_bytes(D)];
   __shared__ __align__(16) char s_v1[buffer_bytes(D)];
-  if (!work<T, FOUR, D, PAGE16, FOUR>(A, s_k0, s_v0, s_k1, s_v1)) {
-    if constexpr (FOUR) work<T, true, D, PAGE16, false>(A, s_k0, s_v0, s_k1, s_v1);
+  constexpr bool kNarrow = FOUR && std::is_same<T, f16_t>::value;
+  if (!work<T, FOUR, D, PAGE16, kNarrow>(A, s_k0, s_v0, s_k1, s_v1)) {
+    if constexpr (kNarrow) work<T, true, D, PAGE16, false>(A, s_k0, s_v0, s_k1, s_v1);
   }
 }
 
