@@ -45,12 +45,16 @@ __device__ __forceinline__ uint32_t pack_half(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), half2_t));
 }
 
-// Probabilities are p = kScale 2^(x - m), m the running maximum that the row's sums are
-// held at, which follows only scores more than kLag above it.  (The factor is a product
-// of its own: in the exponent, 32 would take 5 bits of it.)  They enter the product with V in planes of its type, each what the one before
-// left: three of bf16, cut, hold the 24 bits of fp32, two of fp16, rounded to nearest,
-// 22 of them, as in the other attention kernels.  Two planes of bf16 leave 2^-16,
-// which is past an output's rounding where the terms cancel to 2^-8 of themselves.
+// Probabilities are p = kScale 2^(sc (s - m)), m the running maximum of the products
+// q . k themselves that the row's sums are held at, which follows only scores more than
+// kLag above it.  The differences s - m come out of the matrix products, whose
+// accumulators begin at -m: of a maximum that is scaled and rounded, products of
+// thousands are whole powers of two away, and a subtraction per score costs 4 % of a
+// prompt over 16 bits and 20 % over 4.  They enter the product with V in
+// planes of its type, each what the one before left: three of bf16, cut, hold the 24
+// bits of fp32, two of fp16, rounded to nearest, 22 of them, as in the other attention
+// kernels.  Two planes of bf16 leave 2^-16, which is past an output's rounding where
+// the terms cancel to 2^-8 of themselves.
 // bf16: p <= 2^-24, so that the sums over 2^24 tokens of the largest V are finite;
 // the planes end at 2^-126, 2^-94 of the row's largest weight or less.  fp16: p <= 2^15,
 // near the range's top; the planes end at 2^-25, 2^-36 of the largest weight or less.
@@ -58,6 +62,8 @@ template <typename MT> struct Planes;
 template <> struct Planes<bf16_t> {
   static constexpr int kPlanes = 3;
   static constexpr float kLag = 8.f, kShift = -32.f, kScale = 0x1p-32f;
+  // (the factor is a product of its own: in the exponent, 32 would take 5 of the bits)
+  __device__ static __forceinline__ float weight(float s, float sc) { return fast_exp2(s * sc) * kScale; }
   __device__ static __forceinline__ void split(float a, float b, uint32_t (&w)[kPlanes]) {
 #pragma unroll
     for (int i = 0; i < kPlanes; ++i) {
@@ -71,12 +77,34 @@ template <> struct Planes<bf16_t> {
 template <> struct Planes<f16_t> {
   static constexpr int kPlanes = 2;
   static constexpr float kLag = 4.f, kShift = 11.f, kScale = 0x1p11f;
+  // (in the exponent, which 11 leaves off by 2^-21 at most, no more than the planes are)
+  __device__ static __forceinline__ float weight(float s, float sc) { return fast_exp2(__builtin_fmaf(s, sc, kShift)); }
   __device__ static __forceinline__ void split(float a, float b, uint32_t (&w)[kPlanes]) {
     const half2_t h = __builtin_convertvector((f32x2{a, b}), half2_t);
     w[0] = __builtin_bit_cast(uint32_t, h);
     w[1] = pack_half(__builtin_fmaf((float)h.x, -1.f, a), __builtin_fmaf((float)h.y, -1.f, b));
   }
 };
+
+// What sums held at the maximum m count for at the maximum `top` >= m: nothing where
+// nothing was seen (m of -inf, which `top` may be too).
+__device__ __forceinline__ float weight(float m, float top, float sc) {
+  return m == -INFINITY ? 0.f : fast_exp2((m - top) * sc);
+}
+
+// A row's maximum follows the differences of its scores from it, whose largest is
+// `top`: they go down by `up` (so that the largest is 0, whatever m + up rounds to),
+// sums by alpha.
+struct Rise {
+  float up, alpha;
+};
+__device__ __forceinline__ Rise rise_to(float top, float& m, float sc) {
+  const bool first = m == -INFINITY;  // nothing was seen yet: the differences are from 0
+  const float up = first ? (top == -INFINITY ? 0.f : top) : fmaxf(top, 0.f);
+  const Rise r{up, first ? 0.f : fast_exp2(-up * sc)};
+  m = first ? top : m + up;
+  return r;
+}
 
 // ---------------------------------------------------------- 4-bit cache ---
 // Of a page and kv head: the codes of `page` tokens, then their scales.  K goes by

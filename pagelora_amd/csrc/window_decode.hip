@@ -214,9 +214,9 @@ __device__ __forceinline__ bool stale(const Header& h, const Header& want) {
          h.sinks != want.sinks || h.indices_capacity != want.indices_capacity || h.max_items != want.max_items;
 }
 
-// ln of sum 2^(m - shift); -inf where nothing was seen.
-__device__ __forceinline__ float log_sum(float m, float sum, float shift) {
-  return sum > 0.f ? (m + (log2f(sum) - shift)) * 0.69314718055994531f : (sum == 0.f ? -INFINITY : sum);
+// ln of sum 2^(m sc - shift); -inf where nothing was seen.
+__device__ __forceinline__ float log_sum(float m, float sc, float sum, float shift) {
+  return sum > 0.f ? __builtin_fmaf(m, sc, log2f(sum) - shift) * 0.69314718055994531f : (sum == 0.f ? -INFINITY : sum);
 }
 
 template <typename T, bool FOUR, int D, bool PAGE16>
@@ -398,15 +398,16 @@ __global__ __launch_bounds__(kThreads, FOUR ? 3 : 2) void decode_kernel(Args A) 
 
   f32x4 acc[NA];
   float m, l;
-  const float sc = A.scale_log2;
+  const float sc = A.scale_log2, lag = P::kLag / sc;
 
   enum { kAll, kFinite, kOdd };  // what of V a walk takes
   auto consume = [&](int i, const Raw& raw, int walk) {
     const int t0 = seen_tile(seen, i) * kTile;
     f32x4 s[2];
+    const float from = m == -INFINITY ? 0.f : -m;  // scores begin at -m, so that they come out as the differences
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      s[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+      s[b] = f32x4{from, from, from, from};
 #pragma unroll
       for (int ks = 0; ks < NS; ++ks) {
         u32x4 ka;
@@ -475,25 +476,26 @@ __global__ __launch_bounds__(kThreads, FOUR ? 3 : 2) void decode_kernel(Args A) 
       for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int j = 0; j < 4; ++j) mx = fmaxf(mx, s[b][j]);
-      mx *= sc;
-      if (__builtin_amdgcn_ballot_w64(mx > m + P::kLag) != 0) {
-        const float mn = fmaxf(m, column_max(mx));
-        const float alpha = fast_exp2(m - (mn == -INFINITY ? 0.f : mn));
-        m = mn;
+      if (__builtin_amdgcn_ballot_w64(mx > (m == -INFINITY ? -INFINITY : lag)) != 0) {
+        const Rise rise = rise_to(column_max(mx), m, sc);
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[b][j] -= rise.up;
+        const float alpha = rise.alpha;
         l *= alpha;
 #pragma unroll
         for (int a = 0; a < NA; ++a)
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[a][j] *= alpha;
       }
-      const float mu = m == -INFINITY ? 0.f : m;
       float ps_ = 0.f;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         float p[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          p[j] = fast_exp2(__builtin_fmaf(s[b][j], sc, -mu)) * P::kScale;
+          p[j] = P::weight(s[b][j], sc);
           ps_ += p[j];
         }
 #pragma unroll
@@ -576,7 +578,7 @@ __global__ __launch_bounds__(kThreads, FOUR ? 3 : 2) void decode_kernel(Args A) 
     f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const float f = s_m[w][r] == -INFINITY ? 0.f : fast_exp2(s_m[w][r] - mx);
+      const float f = weight(s_m[w][r], mx, A.scale_log2);
       const f32x4 x = *reinterpret_cast<const f32x4*>(&s_o[w][r][d]);
       sum += s_l[w][r] * f;
 #pragma unroll
@@ -591,7 +593,7 @@ __global__ __launch_bounds__(kThreads, FOUR ? 3 : 2) void decode_kernel(Args A) 
     const int hq = h * g + hb * 16 + r;
     *reinterpret_cast<u32x2*>(A.o + (int64_t)row * A.o_sb + (int64_t)hq * A.o_sh + d * 2) =
         u32x2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
-    if (d == 0 && A.lse) A.lse[(int64_t)row * A.hq + hq] = log_sum(mx, sum, P::kShift);
+    if (d == 0 && A.lse) A.lse[(int64_t)row * A.hq + hq] = log_sum(mx, A.scale_log2, sum, P::kShift);
   }
 }
 
@@ -629,13 +631,13 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(Args A) {
       if (i0 + i * kGroups >= parts) ml[i] = f32x2{-INFINITY, 0.f}, v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
       top = fmaxf(top, ml[i][0]);
     }
-    const float w = m == -INFINITY ? 0.f : fast_exp2(m - top);
+    const float w = weight(m, top, A.scale_log2);
     l *= w;
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = weighted(o[e], w);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const float wi = ml[i][0] == -INFINITY ? 0.f : fast_exp2(ml[i][0] - top);
+      const float wi = weight(ml[i][0], top, A.scale_log2);
       l += ml[i][1] * wi;
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] += weighted(v[i][e], wi);
@@ -655,7 +657,7 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(Args A) {
   o = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < kGroups; ++i) {
-    const float w = s_m[i] == -INFINITY ? 0.f : fast_exp2(s_m[i] - top);
+    const float w = weight(s_m[i], top, A.scale_log2);
     const f32x4 x = *reinterpret_cast<const f32x4*>(&s_o[i][d]);
     sum += s_l[i] * w;
 #pragma unroll
@@ -664,7 +666,7 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(Args A) {
   const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
   *reinterpret_cast<u32x2*>(A.o + (int64_t)row * A.o_sb + (int64_t)hq * A.o_sh + d * 2) =
       u32x2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
-  if (d == 0 && A.lse) A.lse[(int64_t)row * A.hq + hq] = log_sum(top, sum, P::kShift);
+  if (d == 0 && A.lse) A.lse[(int64_t)row * A.hq + hq] = log_sum(top, A.scale_log2, sum, P::kShift);
 }
 
 template <typename T, bool FOUR, int D>

@@ -351,7 +351,7 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
 
   f32x4 acc[kCols][NA];
   float m[kCols], l[kCols];
-  const float sc = A.scale_log2;
+  const float sc = A.scale_log2, lag = P::kLag / sc;
 
   auto body = [&](int tile, const char* kb, char* vb, char* kn, char* vn, int walk) __attribute__((always_inline)) {
     if constexpr (!FOUR) {
@@ -391,7 +391,12 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
     // (uniform) no row of the wave sees the tile
     if (t0 > lim_hi || (t0 + kTile <= lo_lo && t0 >= A.sinks)) return;
 
-    f32x4 s[kCols][4];
+    f32x4 s[kCols][4], from[kCols];  // scores begin at -m, so that they come out as the differences
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      const float f = m[c] == -INFINITY ? 0.f : -m[c];
+      from[c] = f32x4{f, f, f, f};
+    }
     // four independent accumulations in turn, here and below: an MFMA waits
     // for the one before it on the same accumulator
 #pragma unroll
@@ -399,7 +404,7 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
 #pragma unroll
       for (int c = 0; c < kCols; ++c)
 #pragma unroll
-        for (int b = 0; b < 2; ++b) s[c][b0 + b] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int b = 0; b < 2; ++b) s[c][b0 + b] = from[c];
 #pragma unroll
       for (int ks = 0; ks < NS; ++ks) {
         u32x4 ka[2];
@@ -443,8 +448,8 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
       for (int blk = 0; blk < 4; ++blk)
 #pragma unroll
         for (int i = 0; i < 4; ++i) v = fmaxf(v, s[c][blk][i]);
-      mx[c] = v * sc;
-      rose |= mx[c] > m[c] + P::kLag;
+      mx[c] = v;
+      rose |= v > (m[c] == -INFINITY ? -INFINITY : lag);
     }
     // the columns' maxima are reduced over their lanes, and the sums and
     // accumulators rescaled, only where some lane saw a score kLag past its
@@ -452,9 +457,12 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
     if (__builtin_amdgcn_ballot_w64(rose) != 0) {
 #pragma unroll
       for (int c = 0; c < kCols; ++c) {
-        const float mn = fmaxf(m[c], column_max(mx[c]));
-        const float alpha = fast_exp2(m[c] - (mn == -INFINITY ? 0.f : mn));
-        m[c] = mn;
+        const Rise rise = rise_to(column_max(mx[c]), m[c], sc);
+        const float alpha = rise.alpha;
+#pragma unroll
+        for (int blk = 0; blk < 4; ++blk)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[c][blk][i] -= rise.up;
         l[c] *= alpha;
 #pragma unroll
         for (int a = 0; a < NA; ++a)
@@ -463,15 +471,12 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
       }
     }
     u32x4 pb[kCols][2][NP];
-    float mu[kCols];
-#pragma unroll
-    for (int c = 0; c < kCols; ++c) mu[c] = m[c] == -INFINITY ? 0.f : m[c];
     // P^T as the B operand: k = 8*grp + e <-> tokens of blocks 2kc (e < 4) and 2kc+1 (e >= 4)
     auto weights = [&](int c, int blk) __attribute__((always_inline)) {
       float p[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        p[i] = fast_exp2(__builtin_fmaf(s[c][blk][i], sc, -mu[c])) * P::kScale;
+        p[i] = P::weight(s[c][blk][i], sc);
         l[c] += p[i];  // per lane; the column's lanes meet after the last tile
       }
 #pragma unroll
@@ -667,13 +672,13 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(Args A, const Item* mer
       if (i0 + i >= parts) ml[i] = f32x2{-INFINITY, 0.f}, v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
       top = fmaxf(top, ml[i][0]);
     }
-    const float w = m == -INFINITY ? 0.f : fast_exp2(m - top);
+    const float w = weight(m, top, A.scale_log2);
     sum *= w;
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = weighted(o[e], w);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const float wi = ml[i][0] == -INFINITY ? 0.f : fast_exp2(ml[i][0] - top);
+      const float wi = weight(ml[i][0], top, A.scale_log2);
       sum += ml[i][1] * wi;
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] += weighted(v[i][e], wi);

@@ -32,9 +32,9 @@ def test_terms_that_cancel(gpu_device, dtype, bits, heads, head_dim, how):
     a 4-bit cache holds, alike over the 32 dims of a group but for their sign.
 
     Of a weight, in units of 2^-24: the exponent, under 2 in size, 2.8 (its scale's two roundings) and 1.4 (its own), the
-    exponential 2, and in fp16 4 of the planes (2^-11 of 2^-11): 6.2 and 10.2.  A sum of n terms in k planes is n k additions,
-    each off by 2 of the largest partial sum (cut off, not rounded).  Two planes of bf16 leave 256 of a weight, one of fp16
-    8192.  The store rounds to half a step; q k is one product, exact."""
+    exponential 2, and in fp16 4 of the planes (2^-11 of 2^-11) and 5.5 of the 11 in the exponent (2^-21 ln 2): 6.2 and 15.7.
+    A sum of n terms in k planes is n k additions, each off by 2 of the largest partial sum (cut off, not rounded).  Two planes
+    of bf16 leave 256 of a weight, one of fp16 8192.  The store rounds to half a step; q k is one product, exact."""
     requests, rng = 24, np.random.default_rng(head_dim + heads[0])
     c, cache = one_query([8] * requests, heads, head_dim, dtype, bits, gpu_device, 1, how)
     c["q_host"][..., 0] = torch.as_tensor(rng.uniform(0.5, 0.9, (requests, 1)) * math.sqrt(head_dim)).to(dtype)
@@ -62,7 +62,7 @@ def test_terms_that_cancel(gpu_device, dtype, bits, heads, head_dim, how):
                 sign = rng.choice([-1.0, 1.0], 32)
                 cache[page, 1, :8, h, d: d + 32] = torch.as_tensor(v[:, None] * sign).to(dtype)
                 g = heads[0] // heads[1]
-                units = (6.2 if planes == 3 else 10.2) * size + n * planes * 2 * max(top, 1.0)
+                units = (6.2 if planes == 3 else 15.7) * size + n * planes * 2 * max(top, 1.0)
                 bound[r, h * g: h * g + g, d: d + 32] = units * 2.0**-24 / p.sum()
     set_cache(c, cache)
     got, o = run(c, how), reference(c)[0]
