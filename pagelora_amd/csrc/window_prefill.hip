@@ -164,6 +164,10 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
   const int base = kv_len - n_rows / g;
   const Seen seen = seen_from(base + row0 / g, A.window, A.sinks, kTile);
   auto low = [&](int p) { return A.window > 0 ? max(p - A.window + 1, 0) : 0; };
+  // 4 bits: what no row of the item sees becomes zeros, so that it neither takes the item
+  // out of fp16 nor through the tiles again for its NaN.
+  const int last = base + (min(row0 + kRows, n_rows) - 1) / g;
+  auto unseen = [&](int t) { return t > last || (t >= seen.se && t < seen.lo); };
   const int wrow = row0 + wave * kWaveRows;
   const bool wave_on = wrow < n_rows;
   const int lim_lo = wave_on ? base + wrow / g : -1;
@@ -296,8 +300,8 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
   // Narrow: K in fp16, and V times 2^kShift, exact where the scales are in range
   uint32_t v_least = ~0u, v_most = 0u, k_least = ~0u, k_most = 0u;
   auto store_four = [&](int tile, char* kd, char* vd) __attribute__((always_inline)) {
-    const int t0 = seen_tile(seen, tile) * kTile;
-    if (t0 + k_tok >= kv_len) raw.ks = 127u;  // (what lies there counts for nothing)
+    const int t0 = seen_tile(seen, min(tile, t_end - 1)) * kTile;
+    if (N && unseen(t0 + k_tok)) raw.ks = kScaleZero;
     const float ks = scale_of(raw.ks);
     if constexpr (N) {
       k_least = min(k_least, raw.ks);
@@ -308,12 +312,12 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
       *reinterpret_cast<u32x4*>(kd + k_tok * RB + (((tid % 4) * KQ + c) ^ (k_tok % CH)) * 16) =
           N ? halves8(raw.k[c], ks) : codes8(raw.k[c], ks);
     if (CH == 16 || tid < 16 * CH) {
-      if (t0 + kTile > kv_len) {
+      if (t0 + kTile > last + 1 || (t0 < seen.lo && t0 + kTile > seen.se)) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (t0 + v_quad * 4 + j >= kv_len) {  // (0 times what lies there)
+          if (unseen(t0 + v_quad * 4 + j)) {
             raw.v[j] = 0u;
-            raw.vs = (raw.vs & ~(255u << (8 * j))) | 127u << (8 * j);
+            raw.vs = (raw.vs & ~(255u << (8 * j))) | (uint32_t)kScaleZero << (8 * j);
           }
       }
       if constexpr (N) {
@@ -374,7 +378,8 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
     }
     const int t0 = seen_tile(seen, tile) * kTile;
     if (!FOUR && t0 + kTile > kv_len) {
-      // past the last token the pages hold anything: zero V there (0 * NaN)
+      // past the last token the pages hold anything: zero V there (0 * NaN; before the
+      // window it is left to the walks, since a barrier per item cost 2 to 4 %)
       for (int c = tid; c < kTile * CH; c += kThreads)
         if (t0 + c / CH >= kv_len) *reinterpret_cast<u32x4*>(vb + c * 16) = u32x4{0u, 0u, 0u, 0u};
       __syncthreads();
@@ -630,6 +635,17 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
   return true;
 }
 
+// The other work over 4 bits for an item that fp16 does not hold.  A function of its own,
+// so that its registers are none of the narrow work's: a load of one that was put aside
+// waits for the tiles' loads in flight (512 behind 16384, fp16: 175 .. 226 us with both in
+// one body, 171 so).
+typedef __attribute__((address_space(3))) char* Lds;
+template <typename T, int D, bool PAGE16>
+__device__ __attribute__((noinline)) void wide_work(const __attribute__((address_space(4))) Args* A, Lds s_k0, Lds s_v0, Lds s_k1,
+                                                    Lds s_v1) {
+  work<T, true, D, PAGE16, false>(*(const Args*)A, (char*)s_k0, (char*)s_v0, (char*)s_k1, (char*)s_v1);
+}
+
 template <typename T, bool FOUR, int D, bool PAGE16>
 __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(Args A) {
   __shared__ __align__(16) char s_k0[buffer_bytes(D)];
@@ -638,7 +654,9 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(Args A) {
   __shared__ __align__(16) char s_v1[buffer_bytes(D)];
   constexpr bool kNarrow = FOUR && std::is_same<T, f16_t>::value;
   if (!work<T, FOUR, D, PAGE16, kNarrow>(A, s_k0, s_v0, s_k1, s_v1)) {
-    if constexpr (kNarrow) work<T, true, D, PAGE16, false>(A, s_k0, s_v0, s_k1, s_v1);
+    if constexpr (kNarrow)
+      wide_work<T, D, PAGE16>((const __attribute__((address_space(4))) Args*)__builtin_amdgcn_kernarg_segment_ptr(), (Lds)s_k0,
+                              (Lds)s_v0, (Lds)s_k1, (Lds)s_v1);
   }
 }
 
