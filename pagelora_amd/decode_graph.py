@@ -56,6 +56,7 @@ class BatchDecodeGraphRunner:
 
     def __init__(self, weights: DecoderWeights, pool: PagedKVPool, backend: PagedDecodeAttention,
                  max_entries: int = 32) -> None:
+        pool.need_16_bits("BatchDecodeGraphRunner")
         self.weights = weights
         self.pool = pool
         self.backend = backend

@@ -752,6 +752,7 @@ def decode_step_static(weights: DecoderWeights, pool: PagedKVPool, backend: Page
 
     Returns the logits [B, vocab] (graph-owned under capture).
     """
+    pool.need_16_bits("decode_step_static")
     cfg = weights.cfg
     hidden = F.embedding(ctx.tokens, weights.embed)
     if folded_qkv_decode(cfg, weights.dtype):
@@ -809,6 +810,7 @@ def prefill(weights: DecoderWeights, pool: PagedKVPool, request: Request, tokens
     causal) shared by all layers; per layer q/k-norm + RoPE + KV append into
     the pages, then causal paged attention over them.
     """
+    pool.need_16_bits("prefill")
     cfg = weights.cfg
     ps = pool.page_size
     start = request.length - tokens.numel()

@@ -125,6 +125,7 @@ class BatchGenerator:
 
     def __init__(self, weights: DecoderWeights, pool: PagedKVPool, *, workspace_mb: int = 128,
                  use_graph: bool = True) -> None:
+        pool.need_16_bits("BatchGenerator")
         cfg = weights.cfg
         self.weights = weights
         self.pool = pool
@@ -429,6 +430,7 @@ def prefill_requests(weights: DecoderWeights, pool: PagedKVPool, prompts: list[t
     The shared prefix must fill whole pages so rows can list its pages
     read-only (paged_kvcache_manager.py:324-333).
     """
+    pool.need_16_bits("prefill_requests")
     dev = pool.cache.device
     ps = pool.page_size
     adapters = adapters or [0] * len(prompts)

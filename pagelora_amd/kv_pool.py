@@ -180,7 +180,8 @@ class PagedKVPool:
     ``[num_layers, pages, 2, num_kv_heads, bytes]`` (:mod:`pagelora_amd.kv4`),
     for :func:`~pagelora_amd.kv4.kv4_append` and
     :class:`~pagelora_amd.window_attention.WindowAttention`; ``dtype`` is then
-    that of the tokens appended and is not the cache's.
+    that of the tokens appended and is not the cache's.  The decoder and the
+    generators take pools of 16 bits and refuse others.
     """
 
     def __init__(
@@ -238,6 +239,12 @@ class PagedKVPool:
     @property
     def capacity_pages(self) -> int:
         return self.cache.shape[1]
+
+    def need_16_bits(self, what: str) -> None:
+        """Raises where a path that reads and appends 16 bits is handed a pool of 4."""
+        if self.kv_bits != 16:
+            raise NotImplementedError(f"{what} needs a KV pool of 16 bits per value, got kv_bits={self.kv_bits} (for kv4_append "
+                                      "and WindowAttention)")
 
     def layer_cache(self, layer: int) -> torch.Tensor:
         return self.cache[layer]
