@@ -41,6 +41,10 @@ const char* pl_last_error(void);
 /* Library ABI version: (major << 16) | minor. */
 int pl_version(void);
 
+/* The number of the capture into a graph that `stream` is in, one for all of its
+ * streams and no other capture's.  An error outside a capture. */
+int pl_capture_id(void* stream, unsigned long long* id_h);
+
 /* ------------------------------------------------------------------------ */
 /* Paged decode attention                                                    */
 /* ------------------------------------------------------------------------ */

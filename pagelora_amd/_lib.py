@@ -147,6 +147,7 @@ _sz = ctypes.c_size_t
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "pl_last_error": (ctypes.c_char_p, []),
     "pl_version": (_i32, []),
+    "pl_capture_id": (_i32, [_vp, ctypes.POINTER(ctypes.c_ulonglong)]),
     "pl_decode_workspace_size": (_sz, [_i32, _i32, _i32, _i32]),
     "pl_decode_plan": (_i32, [_vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _sz, _vp]),
     "pl_decode_workspace_size_shared": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32]),
@@ -573,3 +574,11 @@ def raw_stream(index: int) -> int:
 
     get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
     return get(index) if get is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def capture_id(stream: int) -> int:
+    """Which capture into a graph this stream, one that is captured, is in (``pl_capture_id``)."""
+
+    number = ctypes.c_ulonglong(0)
+    check(load().pl_capture_id(stream, ctypes.byref(number)), "pl_capture_id")
+    return number.value

@@ -58,7 +58,7 @@ class WindowAttention:
         self._lib = _lib.load() if self.device.type == "cuda" else None
         self._decode_plan: dict | None = None
         self._prefill_plan: dict | None = None
-        self._captured: list = []  # what captured graphs read, kept as long as this object
+        self._captured: list = []  # plans that graphs read and do not hold themselves
 
     # -------------------------------------------------------------- shared
     def _need_device(self, what: str) -> int:
@@ -106,7 +106,12 @@ class WindowAttention:
         stream = _lib.raw_stream(plan["device"])
         if not plan["kept"] or plan["captured"] or stream not in plan["streams"]:
             if torch.cuda.is_current_stream_capturing():
-                if not plan["kept"]:
+                if plan["captured"] == (_lib.capture_id(stream),):
+                    # the plan's memory is its graph's, which holds what it captured
+                    if stream not in plan["streams"]:
+                        plan["memory"].record_stream(torch.cuda.current_stream(plan["device"]))
+                        plan["streams"].add(stream)
+                elif not plan["kept"]:
                     plan["kept"] = True
                     self._captured.append(plan)
             elif plan["captured"]:
@@ -119,6 +124,17 @@ class WindowAttention:
                 plan["streams"].add(stream)
         return stream
 
+    def release_captured(self) -> None:
+        """Let go of the plans that captured runs read, for when their graphs are gone.
+
+        A run that is captured without its plan replays on memory that this
+        object keeps until then; a graph that holds both needs no keeping.
+        """
+
+        for plan in self._captured:
+            plan["kept"] = False
+        self._captured.clear()
+
     # -------------------------------------------------------------- decode
     def plan_decode(self, *, paged_kv_indptr: torch.Tensor, paged_kv_indices: torch.Tensor,
                     paged_kv_last_page_len: torch.Tensor) -> None:
@@ -127,9 +143,10 @@ class WindowAttention:
         int32 tables, all on the host (validated, uploaded) or all on the device
         (trusted: the kernels clamp every index into its buffer).  With device
         tables it may be captured, together with the runs on it: the replays
-        then follow the tables as they are.  A run captured on a plan made
-        before the capture replays on that plan, which is kept.  A request of no
-        tokens is allowed.
+        then follow the tables as they are, and the graph holds the plan.  A run
+        captured on a plan made before its capture replays on that plan, which
+        this object keeps until :meth:`release_captured`.  A request of no tokens
+        is allowed.
         """
 
         tables = (paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len)
@@ -146,9 +163,9 @@ class WindowAttention:
         max_page = _validate_host_table(*tables, self.page_size) if host else None
         device = self._need_device("plan_decode")
         with _lib.on_device(device):
-            captured = torch.cuda.is_current_stream_capturing()
+            capturing = torch.cuda.is_current_stream_capturing()
             if host:
-                if captured:
+                if capturing:
                     raise RuntimeError("plan_decode with host tables uploads them and cannot be captured")
                 tables = _upload_int32(tables, self.device)
             else:
@@ -162,6 +179,7 @@ class WindowAttention:
                 raise ValueError(f"pl_window_decode_plan_size: {_lib.last_error()}")
             memory = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
             stream = torch.cuda.current_stream(device)
+            captured = capturing and (_lib.capture_id(stream.cuda_stream),)  # (true whatever the number)
             _lib.check(self._lib.pl_window_decode_plan(
                 tables[0].data_ptr(), tables[1].data_ptr(), num_indices, tables[2].data_ptr(), batch, *heads,
                 *mask, memory.data_ptr(), nbytes, stream.cuda_stream), "pl_window_decode_plan")
@@ -171,11 +189,9 @@ class WindowAttention:
                 "args": (memory.data_ptr(), nbytes, num_indices),
                 "workspace_bytes": self._lib.pl_window_decode_workspace_size(batch, num_indices, *heads, self.head_dim,
                                                                              *mask),
-                "captured": captured, "kept": captured, "streams": {stream.cuda_stream},
+                "captured": captured, "kept": False, "streams": {stream.cuda_stream},
                 "ready": None if captured else stream.record_event(),
             }
-            if captured:
-                self._captured.append(self._decode_plan)
 
     def run_decode(self, q: torch.Tensor, paged_kv_cache_layer) -> torch.Tensor:
         """One layer of decode attention: ``q`` is ``[B, Hq, D]`` or ``[B, Hq, 1, D]``; returns its shape."""
@@ -223,7 +239,8 @@ class WindowAttention:
         Request r owns query rows ``qo_indptr[r] .. qo_indptr[r+1]``, the last
         positions of its paged sequence.  int32 tables on the host or the device
         (read on the host; the work list is uploaded).  Cannot be captured; a run
-        can, and replays on the plan it was captured with.
+        can, and replays on the plan it was captured with, which this object keeps
+        until :meth:`release_captured`.
         """
 
         tables = (qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len)
