@@ -63,7 +63,7 @@ struct Item {
 };
 static_assert(sizeof(Item) == 32, "the plan's record");
 struct Row {
-  int32_t first, parts;
+  int32_t first, parts, slot;  // its items, and where their parts lie if it is cut
 };
 
 struct Layout {
@@ -97,6 +97,14 @@ inline int max_items_of(int batch, int hq, int hkv, int page_size, int window, i
   if (window > 0) tiles = std::min(tiles, batch * (((int64_t)window + sinks) / kTile + 4));
   const int64_t cut = std::min((int64_t)target_items(tiles, hkv * head_blocks(hq, hkv)), tiles / kMinTiles + 1);
   return batch + (int)cut;
+}
+
+// Parts of the rows that are cut: a row of n > 1 parts has more than n - 1 chunks of
+// tiles, n / 2 or more, and all rows together no more chunks than the work is cut into.
+// (A part for every row's item took 1.1 GB for 4096 rows of 32 kv heads, so 34 MB.)
+__host__ __device__ inline int max_slots_of(int batch, int max_items) {
+  const int cut = max_items - batch;
+  return 2 * cut < max_items ? 2 * cut : max_items;
 }
 
 // ------------------------------------------------------------------- plan ---
@@ -137,7 +145,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs A) {
     return;
   }
   __shared__ int64_t s_sum[kPlanThreads / kWave];
-  __shared__ int s_scan[kPlanThreads / kWave];
+  __shared__ int64_t s_scan[kPlanThreads / kWave];
   const int lane = tid % kWave, wave = tid / kWave;
   int64_t sum = 0;
   for (int r = tid; r < batch; r += kPlanThreads) sum += read_request(A, r).tiles;
@@ -149,27 +157,28 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs A) {
   // (tables that overlap hold more than any that do not: no more items than there is room for)
   const int target = min(target_items(total, A.heads), A.want.max_items - batch);
   const int chunk = (int)max((total + target - 1) / target, (int64_t)kMinTiles);
-  int base = 0;
+  int64_t base = 0;  // items before, and the parts among them in the upper half
   for (int r0 = 0; r0 < batch; r0 += kPlanThreads) {
     const int r = r0 + tid;
     const int n = r < batch ? max(1, (read_request(A, r).tiles + chunk - 1) / chunk) : 0;
-    int incl = n;
+    const int64_t own = n | (int64_t)(n > 1 ? n : 0) << 32;
+    int64_t incl = own;
     for (int d = 1; d < kWave; d <<= 1) {
-      const int up = __shfl_up(incl, d);
+      const int64_t up = __shfl_up(incl, d);
       incl += lane >= d ? up : 0;
     }
     __syncthreads();
     if (lane == kWave - 1) s_scan[wave] = incl;
     __syncthreads();
-    int before = base;
+    int64_t before = base;
     for (int w = 0; w < kPlanThreads / kWave; ++w) {
       before += w < wave ? s_scan[w] : 0;
       base += s_scan[w];
     }
-    if (r < batch) A.rows[r] = Row{before + incl - n, n};
+    if (r < batch) A.rows[r] = Row{(int)(before + incl - own), n, (int)((before + incl - own) >> 32)};
   }
   __syncthreads();
-  const int num = min(base, A.want.max_items);
+  const int num = min((int)base, A.want.max_items);
   for (int i = tid; i < num; i += kPlanThreads) {
     int lo = 0, hi = batch;  // the row that holds item i: the last whose first item is <= i
     while (hi - lo > 1) {
@@ -180,7 +189,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs A) {
     const Request q = read_request(A, lo);
     const int part = i - row.first;
     A.items[i] = Item{lo, q.len, q.page_begin, (int)((int64_t)q.tiles * part / row.parts),
-                      (int)((int64_t)q.tiles * (part + 1) / row.parts), i, row.parts, 0};
+                      (int)((int64_t)q.tiles * (part + 1) / row.parts), row.slot + part, row.parts, 0};
   }
   if (tid == 0) {
     Header h = A.want;
@@ -568,6 +577,7 @@ __global__ __launch_bounds__(kThreads, FOUR ? 3 : 2) void decode_kernel(Args A) 
   }
   __syncthreads();
   const int parts = uniform(it.parts);
+  if (parts > 1 && (unsigned)it.slot >= (unsigned)max_slots_of(A.want.batch, A.want.max_items)) return;
   float* part = A.part + ((int64_t)uniform(it.slot) * A.hkv * A.blocks + blockIdx.y) * part_floats<D>();
   for (int c = threadIdx.x; c < rows * (D / 4); c += kThreads) {
     const int r = c / (D / 4), d = c % (D / 4) * 4;
@@ -608,8 +618,8 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(Args A) {
   const int row = blockIdx.x / A.hq, hq = blockIdx.x % A.hq;
   const Header head = *A.header;
   const Row rec = A.rows[row];
-  const int parts = uniform(rec.parts), first = uniform(rec.first);
-  if (stale(head, A.want) || parts <= 1 || first < 0 || first + parts > A.want.max_items) return;
+  const int parts = uniform(rec.parts), first = uniform(rec.slot);
+  if (stale(head, A.want) || parts <= 1 || first < 0 || first + parts > max_slots_of(A.want.batch, A.want.max_items)) return;
   const int g = A.hq / A.hkv, h = hq / g, r = hq % g;
   const float* p = A.part + ((int64_t)first * A.hkv * A.blocks + h * A.blocks + r / 16) * part_floats<D>();
   const int64_t step = (int64_t)A.hkv * A.blocks * part_floats<D>();
@@ -718,8 +728,9 @@ extern "C" size_t pl_window_decode_workspace_size(int batch, int indices_capacit
                                                   int head_dim, int page_size, int window, int sinks) {
   if (check_shape(batch, num_qo_heads, num_kv_heads, page_size, window, sinks) != PL_OK) return 0;
   if (indices_capacity < 0 || head_dim < 0) return fail(PL_ERR_INVALID, "sizes must be >= 0"), 0;
-  return (size_t)max_items_of(batch, num_qo_heads, num_kv_heads, page_size, window, sinks, indices_capacity) *
-         num_kv_heads * head_blocks(num_qo_heads, num_kv_heads) * 16 * (head_dim + 2) * sizeof(float);
+  const int items = max_items_of(batch, num_qo_heads, num_kv_heads, page_size, window, sinks, indices_capacity);
+  return (size_t)max_slots_of(batch, items) * num_kv_heads * head_blocks(num_qo_heads, num_kv_heads) * 16 *
+         (head_dim + 2) * sizeof(float);
 }
 
 static Header wanted(int batch, int page_size, int window, int sinks, int capacity, int hq, int hkv) {
