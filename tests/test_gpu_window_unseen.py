@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from tests.window_cases import BF16, F16, attention, case, check, prefill, tables
+from tests.window_cases import BF16, F16, attention, case, check, prefill, set_cache, tables
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +47,21 @@ def test_pages_that_no_query_sees_may_be_any(gpu_device, dtype, bits, window, si
     assert moved > 100
     attn.plan_prefill(qo_indptr=c["qo_indptr"], **{**tables(c), "paged_kv_indices": ids})
     assert torch.equal(attn.run_prefill(c["q"], c["cache"]), want)
+
+
+@pytest.mark.parametrize("dtype,bits", [(BF16, 16), (F16, 16), (BF16, 4), (F16, 4)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 3)])
+def test_nan_in_k_and_q(gpu_device, dtype, bits, window, sinks):
+    """A NaN score makes a row NaN, and no row that does not see it."""
+    c = case([200, 60], 4, 2, 128, 16, dtype, gpu_device, bits=bits, new=[150, 60], window=window, sinks=sinks, seed=5, poison=False)
+    cache = torch.randn((c["indices"].numel() + 3, 2, 16, 2, 128), generator=torch.Generator().manual_seed(1)).to(dtype)
+    cache[int(c["indices"][5]), 0, 5, 1, 9] = float("nan")  # position 85 of the first request, kv head 1
+    set_cache(c, cache)
+    c["q_host"][160, 1, 3] = float("nan")
+    c["q"] = c["q_host"].to(gpu_device)
+    want = torch.zeros(210, 4, dtype=torch.bool)
+    rows = torch.arange(50, 200)
+    want[:150, 2:] = ((rows >= 85) & ((rows < 85 + window) if window else True))[:, None]
+    want[160, 1] = True
+    nan = prefill(c).isnan().cpu()
+    assert (nan.all(2) == want).all() and (nan.any(2) == want).all()
