@@ -24,17 +24,20 @@
 // more with infinities and NaN taken out of V, and once with nothing but them, each
 // with weight 1, added to the sums.
 //
-// Measured (head_dim 128; decode_kernel + merge_kernel):
-//   64 x 4096 .. 16384, 4 bits, GQA 4   127.5 + 7.5 us, 5.6 TB/s; the same loads with
-//                                       next to no arithmetic 118.  289 where a
-//                                       tile's loads waited for its page ids; three
-//                                       tiles in flight instead of two 128
-//   1 x 131072, 4 bits, GQA 4           29.5 + 5 us, 4.8 TB/s: ~6 us of start (record,
-//                                       page ids, first tiles), and 24 of stream
-//   64 x 1028 of 8192, 16 bits, GQA 4   51 + 4.5 us, 5.3 TB/s; pages of one token 56 in all
-//   1 x 4112 of 32768, 16 bits, MHA     18.6 + 3.8 us: two tiles per wave, start and end
-//   23 ragged under 1000, 4 bits, GQA 7  10 + 4.2 us, 1 x 2048, 4 bits  5.9 + 4.2 us:
-//                                       dependent round trips and two launches
+// Measured (head_dim 128; us of a pass, decode_kernel and merge_kernel, of which the
+// second 3.8 .. 8):
+//   64 x 4096 .. 16384, 4 bits, GQA 4   137, 5.2 TB/s, issue in 98 % of the cycles; the
+//                                       same loads with next to no arithmetic 118 + 7.
+//                                       131 with two planes of P for three; with two,
+//                                       the kernel 289 where a tile's loads waited for
+//                                       its page ids (128), and three tiles in flight
+//                                       no faster than two
+//   1 x 131072, 4 bits, GQA 4           35, 4.1 TB/s: ~6 us of start (record, page ids,
+//                                       first tiles), 24 of stream, 5 of the merge
+//   64 x 1028 of 8192, 16 bits, GQA 4   53.4, 5.1 TB/s; pages of one token 56
+//   1 x 4112 of 32768, 16 bits, MHA     22.2: two tiles per wave, start and end
+//   23 ragged under 1000, 4 bits, GQA 7  14.1, 1 x 2048, 4 bits  12.1 (6 + 4 in the
+//                                       kernels): dependent round trips, two launches
 // Heads fastest in the grid, so that a page's heads are read together, lost as much
 // (16 bits 52 -> 56 us) as it won (head_dim 64, 16 bits 44 -> 36).
 #include <algorithm>
@@ -82,7 +85,7 @@ inline Layout layout(int batch, int indices_capacity, int max_items) {
 inline int head_blocks(int hq, int hkv) { return (hq / hkv + 15) / 16; }
 // Items per kv head and head block that the work is cut into: as many as fill the
 // chip with workgroups twice per CU, more where an item then still has kItemTiles, up
-// to four times as many.  us, at 512 / 768 / 1024 / 1536 / 2048 workgroups: 64 x 4096
+// to four times as many.  us (two planes of P), at 512 / 768 / 1024 / 1536 / 2048 workgroups: 64 x 4096
 // .. 16384 tokens of 4 bits 156 / 151 / 141 / 135 / 133, 1 x 131072 39 / 35 / 38 / 41 /
 // 46, 64 x 1028 of 16 bits (whole rows at 512) 55 / 62 / 62 / 59 / 74.
 constexpr int kItemTiles = 42;

@@ -28,23 +28,25 @@
 // infinities, is not what a row sees), the item is worked on again: V's infinities and
 // NaN become ones in LDS, kind by kind, to find who sees them, then zeros.
 //
-// Long items run at the rate of a large library product (1.24 PFLOP/s), P's planes
-// counted: a CU takes 1.33 us for 128 rows by 64 tokens of 16 bits in bf16, 1.21 PFLOP/s
-// (two planes: a third of the products), and 1.04 over 4 bits, 1.03.  Shorter ones are
-// bound by their starts (~6 us) and by the last items, which have a CU for themselves.
-// Measured (head_dim 128, prefill_kernel + merge_kernel):
-//   2048 tokens, 4 bits, GQA 4, bf16       60.5 us (94 in bf16 with two planes of P)
-//   512 behind 16384, 4 bits, GQA 7, fp16  194 + 8 us (377 in bf16 with two planes of q
-//                                          and P and cut at one length for 512 slots)
-//   8192 under 1024, 16 bits, GQA 4, bf16  205 .. 229 us, 0.76 PFLOP/s with the masked
-//                                          products, 1.1 with the planes (a large bf16
-//                                          product: 1.24)
-//   5 ragged prompts under 512, MHA, fp16  46.5 us
-// A half's weights are formed between the products of the other half: 236 -> 225 us at
-// 8192.  Tried, and not faster: products of 32 x 32 (half as many instructions: 226 us,
-// spills over 4 bits), eight waves of 16 rows (twice the waves per SIMD: 270), the
-// conversions of the next tile between the scores' products (spills: 2.3 times as long),
-// a wave priority in the products or by the wave's slot.
+// Long items run at the rate of a large library product (1.24 PFLOP/s in bf16, 1.19 in
+// fp16), P's planes counted: two workgroups on a CU take 1.65 us for 128 rows by 64
+// tokens in bf16, 1.30 PFLOP/s (three planes: half of the products), and 1.33 in fp16,
+// 1.21, over 16 bits and over 4 alike.  Shorter ones are bound by their starts (~6 us)
+// and by the last items, which have a CU for themselves.
+// Measured (head_dim 128; us of a pass, with the merge's 8 where ranges are cut):
+//   2048 tokens, 4 bits, GQA 4, bf16       86 (94 .. 97 after pauses, at lower clocks; 55
+//                                          with one plane of P in fp16, 11 bits)
+//   512 behind 16384, 4 bits, GQA 7, fp16  171 (both in bf16, with two planes of q and P
+//                                          and cut at one length for 512 slots 377)
+//   8192 under 1024, 16 bits, GQA 4, bf16  249, 1.15 PFLOP/s with the masked products
+//                                          and the planes (205 with two of them)
+//   5 ragged prompts under 512, MHA, fp16  44.5
+// Those after this with two planes of P in bf16.  A half's weights are formed between
+// the products of the other half: 236 -> 225 us at 8192.  Tried, and not faster:
+// products of 32 x 32 (half as many instructions: 226 us, spills over 4 bits), eight
+// waves of 16 rows (twice the waves per SIMD: 270), the conversions of the next tile
+// between the scores' products (spills: 2.3 times as long), a wave priority in the
+// products or by the wave's slot.
 #include <algorithm>
 #include <functional>
 #include <vector>
@@ -637,8 +639,8 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
 
 // The other work over 4 bits for an item that fp16 does not hold.  A function of its own,
 // so that its registers are none of the narrow work's: a load of one that was put aside
-// waits for the tiles' loads in flight (512 behind 16384, fp16: 175 .. 226 us with both in
-// one body, 171 so).
+// waits for the tiles' loads in flight (512 behind 16384, fp16: 226 us with both in one
+// body, 180 so; 2048 tokens whose V it takes twice 198, 77 without).
 typedef __attribute__((address_space(3))) char* Lds;
 template <typename T, int D, bool PAGE16>
 __device__ __attribute__((noinline)) void wide_work(const __attribute__((address_space(4))) Args* A, Lds s_k0, Lds s_v0, Lds s_k1,
@@ -739,7 +741,8 @@ template <typename I> static void pair_up(std::vector<I>& items, size_t cus) {
 }
 
 // When the last of these items ends, in tiles of a workgroup that has a CU for itself
-// (1.7 .. 2.0 us): two on one are kShared times as fast each (2.1 .. 2.7 us a tile).
+// (1.7 us in fp16, 2.0 .. 2.3 in bf16): two on one are kShared times as fast each (2.7
+// and 3.3 us a tile).  (fp16, and bf16 with one plane of P:)
 // 512 behind 16384 all in parts of 132, 88, 66, 53, 44 and 33 tiles: 287, 261, 213, 248,
 // 224 and 215 us, in 53 and 66, two parts per CU, 194; 2048 whole 62, in parts of up to
 // 28 and 16 tiles 58 + 5 and 61 + 10 with the merge.
@@ -788,7 +791,7 @@ static double end_of(const std::vector<int>& items, size_t cus) {
 // Into how many parts each row item is cut: of the numbers of parts in all that are
 // tried, dealt out so that the longest part is as short as can be, the one whose last
 // part of a head ends first.  An item costs kStart tiles beside its own, a part one
-// more, and the merge kMerge and what the parts' 66 KiB each take.  (In tiles of 2 us.)
+// more, and the merge kMerge and what the parts' 66 KiB each take.  (In tiles of ~2 us.)
 static std::vector<int> parts_of(const std::vector<int>& lengths, int hkv) {
   constexpr int kStart = 2, kMerge = 2, kPartsPerTile = 200;
   constexpr size_t kMost = 4096;  // items past which no cut is needed to fill the chip
