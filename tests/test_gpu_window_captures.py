@@ -5,7 +5,7 @@ import gc
 import pytest
 import torch
 
-from tests.window_cases import BF16, attention, case, check, tables
+from tests.window_cases import BF16, F16, attention, case, check, set_cache, tables
 
 pytestmark = pytest.mark.gpu
 
@@ -134,3 +134,25 @@ def test_captured_runs_of_eager_plans_are_released(gpu_device, how):
         before = before or held()
     assert held() - before < 4 * ROOM
     check(c, getattr(attn, "run_" + how)(c["q"], c["cache"]))  # (the plan at hand stays)
+
+
+@pytest.mark.parametrize("fits", [True, False])
+def test_captured_prompts_of_fp16_over_4_bits(gpu_device, fits):
+    """Both ways of an item, by what fp16 holds, replayed with eager prompts in between."""
+    c = case([300, 1500], 4, 2, 128, 16, F16, gpu_device, bits=4, new=[130, 40], window=200, sinks=5, seed=9)
+    if not fits:
+        cache = torch.randn((c["indices"].numel() + 3, 2, 16, 2, 128), generator=torch.Generator().manual_seed(1))
+        cache[:, 1, :, 1, 32:64] *= 2.0**-30
+        set_cache(c, cache)
+    attn = attention(c)
+    attn.plan_prefill(qo_indptr=c["qo_indptr"], **tables(c))
+    want = attn.run_prefill(c["q"], c["cache"])
+    torch.cuda.synchronize()
+    check(c, want)
+    graph, out = captured(lambda: attn.run_prefill(c["q"], c["cache"]))
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(attn.run_prefill(c["q"], c["cache"]), want)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
