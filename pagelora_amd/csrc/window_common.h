@@ -48,13 +48,14 @@ __device__ __forceinline__ uint32_t pack_half(float a, float b) {
 // Probabilities are p = kScale 2^(sc (s - m)), m the running maximum of the products
 // q . k themselves that the row's sums are held at, which follows only scores more than
 // kLag above it.  The differences s - m come out of the matrix products, whose
-// accumulators begin at -m: of a maximum that is scaled and rounded, products of
-// thousands are whole powers of two away, and a subtraction per score costs 4 % of a
-// prompt over 16 bits and 20 % over 4.  They enter the product with V in
-// planes of its type, each what the one before left: three of bf16, cut, hold the 24
-// bits of fp32, two of fp16, rounded to nearest, 22 of them, as in the other attention
-// kernels.  Two planes of bf16 leave 2^-16, which is past an output's rounding where
-// the terms cancel to 2^-8 of themselves.
+// accumulators begin at -m: from a maximum that is scaled and rounded, products of
+// millions are whole powers of two away, and a subtraction per score costs 3 % of a
+// prompt over 16 bits (256 us, not 250) and, with its registers, a fifth over 4 (212,
+// not 173).
+// They enter the product with V in planes of its type, each what the one before left:
+// three of bf16, cut, hold the 24 bits of fp32, two of fp16, rounded to nearest, 22 of
+// them, as in decode and tree attention.  Two planes of bf16 leave 2^-16, which is past
+// an output's rounding where the terms cancel to 2^-8 of themselves.
 // bf16: p <= 2^-24, so that the sums over 2^24 tokens of the largest V are finite;
 // the planes end at 2^-126, 2^-94 of the row's largest weight or less.  fp16: p <= 2^15,
 // near the range's top; the planes end at 2^-25, 2^-36 of the largest weight or less.

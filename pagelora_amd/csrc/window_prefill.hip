@@ -29,7 +29,7 @@
 // NaN become ones in LDS, kind by kind, to find who sees them, then zeros.
 //
 // Long items run at the rate of a large library product (1.24 PFLOP/s in bf16, 1.19 in
-// fp16), P's planes counted: two workgroups on a CU take 1.65 us for 128 rows by 64
+// fp16), P's planes counted: a CU with two workgroups takes 1.65 us per 128 rows by 64
 // tokens in bf16, 1.30 PFLOP/s (three planes: half of the products), and 1.33 in fp16,
 // 1.21, over 16 bits and over 4 alike.  Shorter ones are bound by their starts (~6 us)
 // and by the last items, which have a CU for themselves.
@@ -643,8 +643,8 @@ __device__ __forceinline__ bool work(const Args& A, char* __restrict__ s_k0, cha
 // body, 180 so; 2048 tokens whose V it takes twice 198, 77 without).
 typedef __attribute__((address_space(3))) char* Lds;
 template <typename T, int D, bool PAGE16>
-__device__ __attribute__((noinline)) void wide_work(const __attribute__((address_space(4))) Args* A, Lds s_k0, Lds s_v0, Lds s_k1,
-                                                    Lds s_v1) {
+__device__ __attribute__((noinline)) void wide_work(const __attribute__((address_space(4))) Args* A, Lds s_k0, Lds s_v0,
+                                                    Lds s_k1, Lds s_v1) {
   work<T, true, D, PAGE16, false>(*(const Args*)A, (char*)s_k0, (char*)s_v0, (char*)s_k1, (char*)s_v1);
 }
 
